@@ -14,13 +14,16 @@ import torch
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libfovi_hip.so")
 
-ABI_VERSION = 36
+ABI_VERSION = 37
 F32, BF16, F8E4M3 = 0, 1, 2
 NEAREST, BILINEAR = 0, 1
 PAD_ZEROS, PAD_BORDER = 0, 1
 ACT_NONE, ACT_RELU = 0, 1
 W_ROWS, W_MFMA, W_IMG = 0, 1, 2
 POOL_MAX, POOL_AVG, POOL_SUM, POOL_GAUSSIAN = 0, 1, 2, 3
+PAIR_HALF, PAIR_ADJACENT = 0, 1
+ROTARY_MAX_AXES = 4
+MASK_NONE, MASK_KEEP, MASK_BIAS = 0, 1, 2
 
 _DTYPE_CODE = {torch.float32: F32, torch.bfloat16: BF16, torch.float8_e4m3fn: F8E4M3}
 
@@ -32,7 +35,10 @@ EXPORTED = ("fovi_abi_version", "fovi_last_error", "fovi_sampler_fwd", "fovi_knn
             "fovi_knnconv_dw", "fovi_knnpool_bwd", "fovi_knnconv_last_path",
             "fovi_knnconv_fwd_noalloc", "fovi_knnconv_wide_tiles", "fovi_knnconv_weight_img_elems",
             "fovi_knnconv_pack_weight_img", "fovi_knnconv_img_tables", "fovi_knnconv_dw_few",
-            "fovi_knnconv_dw_few_workspace_bytes", "fovi_knnconv_dw_few_us")
+            "fovi_knnconv_dw_few_workspace_bytes", "fovi_knnconv_dw_few_us",
+            "fovi_layer_norm_fwd", "fovi_layer_norm_workspace_bytes", "fovi_layer_norm_bwd", "fovi_rotary",
+            "fovi_attention_fwd_workspace_bytes", "fovi_attention_fwd", "fovi_attention_bwd_workspace_bytes",
+            "fovi_attention_bwd")
 
 
 class SamplerArgs(C.Structure):
@@ -206,6 +212,57 @@ class KnnConvDwFewArgs(C.Structure):
     ]
 
 
+class LayerNormArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("dtype", C.c_int32), ("p_dtype", C.c_int32),
+        ("rows0", C.c_int64), ("rows1", C.c_int64), ("channels", C.c_int64),
+        ("x_stride", C.c_int64 * 2),
+        ("weight", C.c_void_p), ("bias", C.c_void_p),
+        ("eps", C.c_float), ("reserved0", C.c_int32),
+        ("y", C.c_void_p), ("y_stride", C.c_int64 * 2),
+        ("mean", C.c_void_p), ("rstd", C.c_void_p),
+        ("dy", C.c_void_p), ("dy_stride", C.c_int64 * 2),
+        ("dx", C.c_void_p), ("dx_stride", C.c_int64 * 2),
+        ("dweight", C.c_void_p), ("dbias", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+    ]
+
+
+class RotaryArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("dtype", C.c_int32), ("pairing", C.c_int32),
+        ("batch", C.c_int64), ("length", C.c_int64), ("heads", C.c_int64), ("head_dim", C.c_int64),
+        ("x_stride", C.c_int64 * 3),
+        ("positions", C.c_void_p), ("pos_stride", C.c_int64 * 2),
+        ("freqs", C.c_void_p), ("n_axes", C.c_int32), ("inverse", C.c_int32),
+        ("section_end", C.c_int32 * ROTARY_MAX_AXES),
+        ("y", C.c_void_p), ("y_stride", C.c_int64 * 3),
+    ]
+
+
+class AttentionArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+        ("dtype", C.c_int32), ("mask_kind", C.c_int32),
+        ("batch", C.c_int64), ("q_len", C.c_int64), ("kv_len", C.c_int64),
+        ("heads", C.c_int64), ("kv_heads", C.c_int64), ("head_dim", C.c_int64),
+        ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3),
+        ("mask", C.c_void_p), ("mask_stride", C.c_int64 * 4),
+        ("kv_lengths", C.c_void_p), ("scale", C.c_float), ("reserved0", C.c_int32),
+        ("out", C.c_void_p), ("out_stride", C.c_int64 * 3), ("stats", C.c_void_p), ("out_rest", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+    ]
+
+
+class AttentionBwdArgs(C.Structure):
+    _fields_ = [
+        ("fwd", AttentionArgs),
+        ("dout", C.c_void_p), ("dout_stride", C.c_int64 * 3),
+        ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p),
+        ("dq_stride", C.c_int64 * 3), ("dk_stride", C.c_int64 * 3), ("dv_stride", C.c_int64 * 3),
+    ]
+
+
 _lib = None
 
 
@@ -273,6 +330,20 @@ def load(path: str = LIB_PATH):
     lib.fovi_knnpool_bwd.restype = C.c_int
     lib.fovi_knnconv_wide_tiles.argtypes = [C.c_int64] + [C.c_int32] * 5 + [C.POINTER(C.c_int64)]
     lib.fovi_knnconv_wide_tiles.restype = C.c_int
+    for name in ("fovi_layer_norm_fwd", "fovi_layer_norm_bwd"):
+        getattr(lib, name).argtypes = [C.POINTER(LayerNormArgs), C.c_void_p]
+        getattr(lib, name).restype = C.c_int
+    lib.fovi_layer_norm_workspace_bytes.argtypes = [C.c_int64, C.c_int64, C.c_int32]
+    lib.fovi_layer_norm_workspace_bytes.restype = C.c_int64
+    lib.fovi_rotary.argtypes = [C.POINTER(RotaryArgs), C.c_void_p]
+    lib.fovi_rotary.restype = C.c_int
+    for name in ("fovi_attention_fwd_workspace_bytes", "fovi_attention_bwd_workspace_bytes"):
+        getattr(lib, name).argtypes = [C.c_int64] * 6 + [C.c_int32]
+        getattr(lib, name).restype = C.c_int64
+    lib.fovi_attention_fwd.argtypes = [C.POINTER(AttentionArgs), C.c_void_p]
+    lib.fovi_attention_fwd.restype = C.c_int
+    lib.fovi_attention_bwd.argtypes = [C.POINTER(AttentionBwdArgs), C.c_void_p]
+    lib.fovi_attention_bwd.restype = C.c_int
     got = lib.fovi_abi_version()
     if got != ABI_VERSION:
         raise RuntimeError(f"{path}: ABI version {got}, expected {ABI_VERSION}")

@@ -23,7 +23,7 @@
 extern "C" {
 #endif
 
-#define FOVI_ABI_VERSION 36
+#define FOVI_ABI_VERSION 37
 
 enum fovi_dtype { FOVI_F32 = 0, FOVI_BF16 = 1, FOVI_F8E4M3 = 2 };
 enum fovi_interp { FOVI_NEAREST = 0, FOVI_BILINEAR = 1 };
@@ -748,6 +748,142 @@ int fovi_knnconv_dw_few(const fovi_knnconv_dw_few_args* args, void* stream);
  * block where that is largest. */
 double fovi_knnconv_dw_few_us(int64_t batch, int64_t c_in, int64_t c_out, int64_t n_in, int64_t n_out, int64_t n_ref,
                               int32_t x_dtype, double rounds);
+
+/*
+ * Layer norm over the last dimension of token rows (no counterpart among the replaced ATen sites;
+ * the reference's norms over [B, C, N] are fovi/arch/norm.py:125-157):
+ *   h = (x - mean(x)) * rstd, rstd = 1 / sqrt(mean((x - mean(x))^2) + eps), y = h * weight + bias
+ * Rows are indexed (i0, i1); strides are [i0, i1] with the channels adjacent. x, y, dy, dx share
+ * one dtype (F32 or BF16); weight, bias and their gradients share p_dtype. Statistics and sums are
+ * fp32, one rounding at the output. weight and bias may be NULL (1 and 0).
+ * forward: y, and mean / rstd [rows0 * rows1] unless NULL.
+ * backward: from x, dy, mean, rstd: dx (unless NULL), dweight and dbias (each unless NULL); the
+ * weight gradients need a workspace of fovi_layer_norm_workspace_bytes, 16-byte aligned.
+ */
+typedef struct fovi_layer_norm_args {
+  const void* x;
+  int32_t dtype;
+  int32_t p_dtype;
+  int64_t rows0, rows1, channels;
+  int64_t x_stride[2];
+  const void* weight;
+  const void* bias;
+  float eps;
+  int32_t reserved0;
+  void* y;
+  int64_t y_stride[2];
+  float* mean;
+  float* rstd;
+  const void* dy;             /* backward only, from here on */
+  int64_t dy_stride[2];
+  void* dx;
+  int64_t dx_stride[2];
+  void* dweight;
+  void* dbias;
+  void* workspace;
+  int64_t workspace_bytes;
+} fovi_layer_norm_args;
+
+int fovi_layer_norm_fwd(const fovi_layer_norm_args* args, void* stream);
+int64_t fovi_layer_norm_workspace_bytes(int64_t rows, int64_t channels, int32_t dtype);
+int fovi_layer_norm_bwd(const fovi_layer_norm_args* args, void* stream);
+
+/*
+ * Rotary positions on several axes. Pair j of a head (of axis a, section_end[a - 1] <= j <
+ * section_end[a], n_pairs in all) turns by the angle positions[b, l, a] * freqs[j]:
+ *   (u, v) -> (u cos - v sin, v cos + u sin)
+ * pairing FOVI_PAIR_HALF: elements (j, j + n_pairs); FOVI_PAIR_ADJACENT: (2j, 2j + 1). Elements
+ * from 2 * n_pairs on are copied. inverse != 0 turns by the negative angle (the gradient). The
+ * angle is reduced in fp64, so that it keeps fp32 accuracy at any position.
+ * x and y: F32 or BF16, strides [batch, token, head], head elements adjacent. positions: fp32,
+ * strides [batch, token], axes adjacent.
+ */
+enum fovi_pairing { FOVI_PAIR_HALF = 0, FOVI_PAIR_ADJACENT = 1 };
+#define FOVI_ROTARY_MAX_AXES 4
+
+typedef struct fovi_rotary_args {
+  const void* x;
+  int32_t dtype;
+  int32_t pairing;
+  int64_t batch, length, heads, head_dim;
+  int64_t x_stride[3];
+  const float* positions;
+  int64_t pos_stride[2];
+  const float* freqs;         /* [n_pairs] */
+  int32_t n_axes;
+  int32_t inverse;
+  int32_t section_end[FOVI_ROTARY_MAX_AXES];
+  void* y;
+  int64_t y_stride[3];
+} fovi_rotary_args;
+
+int fovi_rotary(const fovi_rotary_args* args, void* stream);
+
+/*
+ * Attention of q_len queries to kv_len states. Query head h reads key head h / (heads / kv_heads).
+ *   s_ij = scale * q_i . k_j (+ bias_ij),  p = softmax over the states that row i keeps,
+ *   out_i = sum_j p_ij v_j
+ * A state is left out of a row where j >= kv_lengths[b], where a boolean mask holds 0, or where the
+ * score is -inf; a row that keeps nothing gives zeros, and no gradient. Values in places that a mask
+ * or a length leaves out have no effect, infinities and NaN included.
+ * mask_kind: FOVI_MASK_NONE; FOVI_MASK_KEEP, bytes, 0 = left out; FOVI_MASK_BIAS, fp32 added to the
+ * scores. mask strides [batch, head, query, state], 0 where it is broadcast. kv_lengths: int32
+ * [batch] on the device, NULL for kv_len; taken as within [0, kv_len].
+ * dtype F32 or BF16 for q, k, v, out and the gradients; strides [batch, token, head], head elements
+ * adjacent; head_dim 1 to 128; scale > 0. Scores, statistics and sums are fp32.
+ * stats [2, batch, heads, q_len]: each row's largest score and its sum of exponentials below it (units
+ * of the library's own; apart, because the log of the sum vanishes beside a bias of the type's lowest
+ * value); NULL if no backward follows. out_rest (BF16; NULL if no backward follows): what the rounding of out took
+ * away, in bf16 and out's strides. The backward subtracts dout . out from nearly equal numbers where
+ * a row reads mostly one state; with out alone its rounding would be a large part of the difference.
+ * The workspace (fovi_attention_fwd_workspace_bytes, may be 0; 16-byte aligned) holds partial results
+ * where the states are split over workgroups.
+ */
+enum fovi_mask_kind { FOVI_MASK_NONE = 0, FOVI_MASK_KEEP = 1, FOVI_MASK_BIAS = 2 };
+
+typedef struct fovi_attention_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  int32_t dtype;
+  int32_t mask_kind;
+  int64_t batch, q_len, kv_len, heads, kv_heads, head_dim;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  const void* mask;
+  int64_t mask_stride[4];
+  const int32_t* kv_lengths;
+  float scale;
+  int32_t reserved0;
+  void* out;
+  int64_t out_stride[3];
+  float* stats;
+  void* out_rest;
+  void* workspace;
+  int64_t workspace_bytes;
+} fovi_attention_args;
+
+int64_t fovi_attention_fwd_workspace_bytes(int64_t batch, int64_t q_len, int64_t kv_len, int64_t heads,
+                                           int64_t kv_heads, int64_t head_dim, int32_t dtype);
+int fovi_attention_fwd(const fovi_attention_args* args, void* stream);
+
+/*
+ * Its gradients, from the forward's out, out_rest and stats (fwd.workspace is the backward's, of
+ * fovi_attention_bwd_workspace_bytes). dq, dk and dv are written whole (zeros where a state is
+ * left out by every row), dk and dv summed over the heads that share a key head.
+ */
+typedef struct fovi_attention_bwd_args {
+  fovi_attention_args fwd;
+  const void* dout;
+  int64_t dout_stride[3];
+  void* dq;
+  void* dk;
+  void* dv;
+  int64_t dq_stride[3], dk_stride[3], dv_stride[3];
+} fovi_attention_bwd_args;
+
+int64_t fovi_attention_bwd_workspace_bytes(int64_t batch, int64_t q_len, int64_t kv_len, int64_t heads,
+                                           int64_t kv_heads, int64_t head_dim, int32_t dtype);
+int fovi_attention_bwd(const fovi_attention_bwd_args* args, void* stream);
 
 #ifdef __cplusplus
 }

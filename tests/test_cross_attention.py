@@ -1,0 +1,446 @@
+"""Cross attention forward and backward against float64, over lengths, heads, layouts, masks and types.
+
+Tolerances, from the arithmetic. fp32: a score is a sum of D products (error about sqrt(D) 2^-24 of
+|q||k| scale, 1e-6 absolute at the spreads used here), which the exponential turns into a relative
+error; with the sums over the states and the gradients' differences 1e-5 relative is allowed. bf16:
+probabilities (and score gradients) enter the second product rounded to bf16, at most 2^-9 each, and
+the result is rounded once more; independent roundings add to at most 2^-9 (1 + a) with a <= 2 the
+ratio of sum p|v| to |sum p v| over these random inputs: 6e-3. A score gradient is the difference
+p (do.v - do.o), which may cancel (one state, equal values): its terms' roundings, 2^-21 of
+p (|do.v| + |do.o|) in fp32 and 2^-16 in bf16 (o is kept to 2^-18 there), come on top in dq and dk.
+"""
+import math
+
+import pytest
+import torch
+
+from fovi_amd import _lib
+
+TOL = {torch.float32: 1e-5, torch.bfloat16: 6e-3}
+TERMS = {torch.float32: 2.0 ** -21, torch.bfloat16: 2.0 ** -16}
+INF = math.inf
+
+
+def _reference(q, k, v, lengths=None, mask=None, scale=None, dout=None):
+    """out, dq, dk, dv in float64 on the CPU, pair by pair (what is left out is never multiplied), and the
+    norms of what dq and dk are with the terms of the score gradients taken absolutely."""
+    q, k, v = (t.detach().double().cpu() for t in (q, k, v))
+    b, lq, hq, d = q.shape
+    lk, hk = k.shape[1:3]
+    scale = d ** -0.5 if scale is None else scale
+    keep = torch.ones(b, hq, lq, lk, dtype=torch.bool)
+    bias = torch.zeros(b, hq, lq, lk, dtype=torch.float64)
+    if lengths is not None:
+        keep &= torch.arange(lk) < lengths.cpu()[:, None, None, None]
+    if mask is not None:
+        m = mask.cpu().expand(b, hq, lq, lk)
+        if m.dtype == torch.bool:
+            keep &= m
+        else:
+            bias = m.double()
+            keep &= bias != -INF
+    out = torch.zeros(b, lq, hq, d, dtype=torch.float64)
+    dq, dk, dv = torch.zeros_like(out), torch.zeros_like(k), torch.zeros_like(v)
+    tq, tk = torch.zeros_like(out), torch.zeros_like(k)
+    for i in range(b):
+        for h in range(hq):
+            j = h * hk // hq
+            for r in range(lq):
+                at = keep[i, h, r].nonzero()[:, 0]
+                if len(at) == 0:
+                    continue
+                kk, vv = k[i, at, j], v[i, at, j]
+                p = torch.softmax(kk @ q[i, r, h] * scale + bias[i, h, r, at], 0)
+                out[i, r, h] = p @ vv
+                if dout is not None:
+                    g = dout[i, r, h].double().cpu()
+                    ds = p * (vv @ g - g @ out[i, r, h])
+                    terms = p * ((vv @ g).abs() + (g @ out[i, r, h]).abs())
+                    tq[i, r, h] = scale * (terms @ kk.abs())
+                    tk[i, at, j] += scale * terms[:, None] * q[i, r, h].abs()
+                    dq[i, r, h] = scale * (ds @ kk)
+                    dk[i, at, j] += scale * ds[:, None] * q[i, r, h]
+                    dv[i, at, j] += p[:, None] * g
+    return out, dq, dk, dv, tq.norm(), tk.norm()
+
+
+def _close(got, want, tol, what, terms=0.0):
+    got = got.detach().double().cpu()
+    assert got.shape == want.shape and torch.isfinite(got).all(), what
+    err, most = (got - want).norm(), tol * want.norm() + terms
+    assert err <= most, f"{what}: off by {err:.2e} of {want.norm():.2e}, {most:.2e} allowed"
+
+
+def _inputs(b, lq, lk, hq, hk, d, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    q = (1.3 * torch.randn(b, lq, hq, d, generator=g)).to(dtype).cuda()
+    k, v = (torch.randn(b, lk, hk, d, generator=g).to(dtype).cuda() for _ in range(2))
+    return q, k, v, torch.randn(b, lq, hq, d, generator=g).to(dtype).cuda(), g
+
+
+def _check(q, k, v, dout, tol=None, **kw):
+    """Forward without and with gradients, and the gradients, against the reference."""
+    from fovi_amd.arch.attention import cross_attention
+    tol = TOL[q.dtype] if tol is None else tol
+    plain = cross_attention(q, k, v, **kw)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    out = cross_attention(*leaves, **kw)
+    grads = torch.autograd.grad(out, leaves, dout)
+    want = _reference(q, k, v, kw.get("kv_lengths"), kw.get("mask"), kw.get("scale"), dout)
+    _close(plain, want[0], tol, "out without gradients")
+    _close(out, want[0], tol, "out")
+    for name, got, ref, terms in zip(("dq", "dk", "dv"), grads, want[1:4], (want[4], want[5], 0.0)):
+        _close(got, ref, tol, name, TERMS[q.dtype] * terms)
+    again = torch.autograd.grad(cross_attention(*leaves, **kw), leaves, dout)
+    assert all(torch.equal(x, y) for x, y in zip(grads, again))        # sums in a fixed order
+    return out, grads
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("b,lq,lk,hq,hk,d", [
+    (1, 1, 1, 1, 1, 64), (1, 1, 64, 6, 6, 64), (2, 3, 65, 4, 2, 32), (1, 33, 31, 2, 2, 64), (2, 70, 129, 4, 1, 64),
+    (1, 128, 128, 2, 2, 128), (1, 5, 300, 8, 2, 80), (1, 257, 40, 1, 1, 96), (2, 31, 33, 3, 3, 16), (1, 2, 2, 2, 1, 8),
+    (1, 130, 200, 2, 1, 40), (1, 64, 1, 3, 3, 64), (1, 1, 700, 16, 2, 128), (3, 17, 90, 6, 2, 64),
+    (1, 9, 20, 2, 2, 1), (1, 12, 50, 2, 1, 33), (2, 8, 70, 1, 1, 127), (1, 40, 77, 2, 2, 5)])
+def test_sizes(b, lq, lk, hq, hk, d, dtype):
+    _check(*_inputs(b, lq, lk, hq, hk, d, dtype)[:4])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("layout", ["heads_first", "kv_pair", "padded", "odd_offset", "element_stride", "expanded", "mixed"])
+def test_layouts(layout, dtype):
+    b, lq, lk, h, d = 2, 37, 75, 3, 32
+    q, k, v, dout, g = _inputs(b, lq, lk, h, h, d, dtype, seed=1)
+
+    def randn(*shape):
+        return torch.randn(shape, generator=g).to(dtype).cuda()
+
+    if layout in ("heads_first", "mixed"):
+        q = randn(b, h, lq, d).transpose(1, 2)
+        if layout == "heads_first":
+            k, v = randn(b, h, lk, d).transpose(1, 2), randn(b, h, lk, d).transpose(1, 2)
+    elif layout == "kv_pair":
+        kv = randn(b, lk, 2, h, d)
+        k, v = kv[:, :, 0], kv[:, :, 1]
+    elif layout == "padded":
+        q, k, v = randn(b, lq, h, d + 8)[..., :d], randn(b, lk + 5, h, d)[:, 5:], randn(b, lk, h + 2, d)[:, :, 1:-1]
+    elif layout == "odd_offset":
+        q, k, v = (randn(b, n, h, d + 3)[..., 3:] for n in (lq, lk, lk))
+    elif layout == "element_stride":
+        q, k, v = (randn(b, n, d, h).transpose(2, 3) for n in (lq, lk, lk))
+        dout = randn(b, lq, d, h).transpose(2, 3)
+    elif layout == "expanded":
+        k, v = randn(1, lk, 1, d).expand(b, lk, h, d), randn(b, 1, h, d).expand(b, lk, h, d)
+        dout = randn(b, lq, 1, 1).expand(b, lq, h, d)
+    out, _ = _check(q, k, v, dout)
+    if layout == "heads_first":
+        assert out.stride() == q.stride()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lq", [1, 4, 45])
+@pytest.mark.parametrize("hq,hk,d", [(4, 2, 64), (2, 2, 128), (1, 1, 32)])
+def test_lengths(lq, hq, hk, d, dtype):
+    """Images with no state, one, a few, all; beyond the tensor and below zero. What lies behind a
+    length is NaN."""
+    q, k, v, dout, _ = _inputs(7, lq, 100, hq, hk, d, dtype, seed=2)
+    lengths = torch.tensor([0, 1, 33, 64, 100, 1000, -3])
+    for i, n in enumerate(lengths.clamp(0, 100).tolist()):
+        k[i, n:], v[i, n:] = float("nan"), float("inf")
+    out, (_, dk, dv) = _check(q, k, v, dout, kv_lengths=lengths.int().cuda())
+    assert not out[0].any() and not dk[0].any() and not dv[1, 1:].any()
+    _check(q, k, v, dout, kv_lengths=lengths.cuda())
+    from fovi_amd.arch.attention import cross_attention
+    assert not cross_attention(q, k, v, kv_lengths=torch.zeros(7, dtype=torch.int32, device="cuda")).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", ["pairs", "heads", "keys", "full", "rows", "strided"])
+@pytest.mark.parametrize("lq,lk,d", [(37, 77, 64), (3, 150, 32), (1, 40, 128)])
+def test_boolean_masks(shape, lq, lk, d, dtype):
+    b, hq, hk = 2, 4, 2
+    q, k, v, dout, g = _inputs(b, lq, lk, hq, hk, d, dtype, seed=3)
+
+    def rand(*size):
+        return (torch.rand(size, generator=g) < 0.6).cuda()
+
+    mask = {"pairs": lambda: rand(lq, lk), "heads": lambda: rand(1, hq, lq, lk), "keys": lambda: rand(b, 1, 1, lk),
+            "full": lambda: rand(b, hq, lq, lk), "rows": lambda: rand(b, 1, lq, 1),
+            "strided": lambda: rand(lk, lq, b).permute(2, 1, 0)[:, None]}[shape]()
+    mask = mask.clone(memory_format=torch.preserve_format)
+    if shape in ("pairs", "full", "strided"):
+        mask[..., ::3, :] = False                       # rows that keep nothing
+    out, (dq, _, _) = _check(q, k, v, dout, mask=mask)
+    empty = ~mask.expand(b, hq, lq, lk).any(-1).transpose(1, 2)
+    assert not out[empty].any() and not dq[empty].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lq,lk", [(21, 70), (2, 130)])
+def test_bias_masks(lq, lk, dtype):
+    """A float bias: ordinary values, the type's lowest value, -inf, a row of each alone."""
+    b, h, d = 2, 2, 64
+    q, k, v, dout, g = _inputs(b, lq, lk, h, h, d, dtype, seed=4)
+    bias = torch.randn(b, 1, lq, lk, generator=g)
+    bias[:, :, :, 5::7] = -INF
+    bias[:, :, :, 3::5] = torch.finfo(torch.float32).min
+    bias[0, :, 0] = -INF
+    bias[1, :, 1] = torch.finfo(torch.float32).min       # the lowest value alone: every state the same
+    bias = bias.cuda()
+    out, _ = _check(q, k, v, dout, mask=bias)
+    assert not out[0, 0].any()
+    assert ((out[1, 1].double() - v[1].double().mean(0)).norm() / v[1].double().mean(0).norm()) < TOL[dtype]
+    half = bias[:, :, :1].bfloat16()
+    _check(q, k, v, dout, mask=half)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lq,lk,d", [(40, 100, 64), (2, 300, 64), (33, 70, 128), (70, 40, 32)])
+@pytest.mark.parametrize("kind", ["bool", "bias"])
+def test_non_finite_values_in_masked_places(lq, lk, d, kind, dtype):
+    """NaN and infinities in states that no row keeps, in states that some rows leave out, and in
+    queries (and their incoming gradients) that keep nothing."""
+    b, h = 2, 2
+    q, k, v, dout, g = _inputs(b, lq, lk, h, h, d, dtype, seed=5)
+    keep = torch.rand(b, 1, lq, lk, generator=g) < 0.7
+    keep[:, :, 1] = False
+    q[:, 1], dout[:, 1] = float("nan"), float("inf")      # a padded query
+    keep[:, :, :, 7] = False
+    k[:, 7], v[:, 7] = float("inf"), float("nan")
+    mask = keep.cuda() if kind == "bool" else torch.zeros(keep.shape).masked_fill(~keep, -INF).cuda()
+    _check(q, k, v, dout, mask=mask)
+    # a state whose value is not finite, read by the first row alone: the other rows do not see it
+    from fovi_amd.arch.attention import cross_attention
+    keep[:, :, :, 9] = False
+    keep[:, :, 0, 9] = True
+    mask = keep.cuda() if kind == "bool" else torch.zeros(keep.shape).masked_fill(~keep, -INF).cuda()
+    clean = v.clone()
+    clean[:, 9] = 0
+    v[:, 9, :, 0], v[:, 9, :, 1], v[:, 9, :, 2] = float("nan"), INF, -INF
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    out = cross_attention(*leaves, mask=mask)
+    dout[:, 0] = 0
+    dq, dk, dv = torch.autograd.grad(out, leaves, dout)
+    assert out[:, 0, :, 0].isnan().all() and (out[:, 0, :, 1] == INF).all() and (out[:, 0, :, 2] == -INF).all()
+    want = _reference(q, k, clean, None, mask, None, dout)
+    _close(out[:, 1:], want[0][:, 1:], TOL[dtype], "out of the other rows")
+    _close(dq[:, 1:], want[1][:, 1:], TOL[dtype], "dq of the other rows")
+    other = [i for i in range(lk) if not bool(keep[:, :, 0, i].any())]
+    _close(dv[:, other], want[3][:, other], TOL[dtype], "dv of states that row does not read")
+    _close(dk[:, other], want[2][:, other], TOL[dtype], "dk of states that row does not read")
+
+
+@pytest.mark.gpu
+def test_infinite_keys_poison_their_readers_only():
+    """A key of infinities (kept) in one image: the other image and the other heads do not change."""
+    from fovi_amd.arch.attention import cross_attention
+    q, k, v, _, _ = _inputs(2, 20, 50, 2, 2, 64, torch.float32, seed=6)
+    want = cross_attention(q, k, v)
+    k[0, 3, 1, 0] = INF
+    out = cross_attention(q, k, v)
+    assert torch.equal(out[1], want[1]) and torch.equal(out[0, :, 0], want[0, :, 0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_large_scores(dtype):
+    """Scores to about +-400: the running maximum, no overflow; rows that read one state. fp32 scores of
+    400 are off by 400 * 2^-24 * a few, so 2e-4 is allowed there; bf16 products are exact in fp32."""
+    q, k, v, dout, _ = _inputs(1, 40, 130, 2, 2, 64, dtype, seed=7)
+    _check(12 * q, k, v, dout, tol=2e-4 if dtype == torch.float32 else 6e-3, scale=0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lq,hq,hk", [(1, 6, 6), (4, 16, 4), (1, 1, 1), (50, 2, 2)])
+def test_many_states(lq, hq, hk, dtype):
+    """20000 states: the sums over the states, in parts, against float64 on the GPU."""
+    from fovi_amd.arch.attention import cross_attention
+    q, k, v, dout, _ = _inputs(1, lq, 20000, hq, hk, 64, dtype, seed=8)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    out = cross_attention(*leaves)
+    grads = torch.autograd.grad(out, leaves, dout)
+    ref = [t.detach().double().requires_grad_(True) for t in (q, k, v)]
+    kk, vv = (t.repeat_interleave(hq // hk, 2).transpose(1, 2) for t in ref[1:])
+    want = (torch.softmax(ref[0].transpose(1, 2) @ kk.transpose(2, 3) / 8, -1) @ vv).transpose(1, 2)
+    rgrads = torch.autograd.grad(want, ref, dout.double())
+    _close(out, want.detach().cpu(), TOL[dtype], "out")
+    _close(cross_attention(q, k, v), want.detach().cpu(), TOL[dtype], "out without gradients")
+    for name, a, b in zip(("dq", "dk", "dv"), grads, rgrads):
+        _close(a, b.cpu(), TOL[dtype], name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_many_queries_over_few_states(dtype):
+    """5000 queries over 70 states: the sums of dk and dv over the queries."""
+    from fovi_amd.arch.attention import cross_attention
+    q, k, v, dout, _ = _inputs(1, 5000, 70, 2, 1, 32, dtype, seed=9)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    grads = torch.autograd.grad(cross_attention(*leaves), leaves, dout)
+    ref = [t.detach().double().requires_grad_(True) for t in (q, k, v)]
+    kk, vv = (t.repeat_interleave(2, 2).transpose(1, 2) for t in ref[1:])
+    want = (torch.softmax(ref[0].transpose(1, 2) @ kk.transpose(2, 3) * 32 ** -0.5, -1) @ vv).transpose(1, 2)
+    for name, a, b in zip(("dq", "dk", "dv"), grads, torch.autograd.grad(want, ref, dout.double())):
+        _close(a, b.cpu(), TOL[dtype], name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_almost_one_state(dtype):
+    """Two states, one of them read nearly alone: dq and dk are small differences. The forward's output
+    enters them before its rounding."""
+    g = torch.Generator().manual_seed(10)
+    q = torch.randn(1, 200, 1, 64, generator=g).to(dtype)
+    k = torch.cat([q.mean(1, keepdim=True) * 0, 0.5 * torch.randn(1, 1, 1, 64, generator=g).to(dtype)], 1)
+    v, dout = (torch.randn(1, n, 1, 64, generator=g).to(dtype) for n in (2, 200))
+    _check(q.cuda(), k.cuda(), v.cuda(), dout.cuda(), scale=1.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lq", [1, 40])
+def test_offsets_beyond_32_bits(lq):
+    """States so far apart that their element offsets pass 2^31."""
+    from fovi_amd.arch.attention import cross_attention
+    q, k, v, dout, _ = _inputs(1, lq, 9, 1, 1, 32, torch.bfloat16, seed=11)
+    step = (1 << 28) + 8
+    room = torch.empty(8 * step + 64, dtype=torch.bfloat16, device="cuda")
+    far = torch.as_strided(room, (1, 9, 1, 32), (0, step, 32, 1))
+    far.copy_(k)
+    assert torch.equal(cross_attention(q, far, v), cross_attention(q, k, v))
+    far.copy_(v)
+    assert torch.equal(cross_attention(q, k, far), cross_attention(q, k, v))
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    want = torch.autograd.grad(cross_attention(*leaves), leaves, dout)
+    far_v = far.detach().requires_grad_(True)
+    got = torch.autograd.grad(cross_attention(leaves[0], leaves[1], far_v), leaves[:2], dout)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
+def test_gradients_against_differences():
+    """Central differences in fp32 with step 2e-2: the second-order error is step^2 / 6 times third
+    derivatives of order 1 (7e-5), the rounding 2^-24 * 10 / 4e-2 (2e-5) times a few."""
+    from fovi_amd.arch.attention import cross_attention
+    q, k, v, dout, _ = _inputs(2, 3, 5, 2, 1, 8, torch.float32, seed=12)
+    mask = torch.ones(2, 1, 3, 5, dtype=torch.bool, device="cuda")
+    mask[0, 0, 1], mask[1, 0, 0, 2] = False, False
+    leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, v)]
+    grads = torch.autograd.grad(cross_attention(*leaves, mask=mask), leaves, dout)
+
+    def f():
+        with torch.no_grad():
+            return (cross_attention(*leaves, mask=mask).double() * dout.double()).sum().item()
+
+    for t, gt in zip(leaves, grads):
+        flat = t.detach().reshape(-1)
+        for i in range(0, flat.numel(), 7):
+            x = flat[i].item()
+            flat[i] = x + 2e-2
+            up = f()
+            flat[i] = x - 2e-2
+            down = f()
+            flat[i] = x
+            assert abs((up - down) / 4e-2 - gt.reshape(-1)[i].item()) < 1e-3
+
+
+@pytest.mark.gpu
+def test_empty_tensors():
+    from fovi_amd.arch.attention import cross_attention
+    def z(b, n, h):
+        return torch.randn(b, n, h, 16, device="cuda", requires_grad=True)
+    for b, lq, lk in ((0, 3, 4), (2, 0, 4), (2, 3, 0), (0, 0, 0)):
+        q, k, v = z(b, lq, 2), z(b, lk, 1), z(b, lk, 1)
+        out = cross_attention(q, k, v)
+        assert out.shape == (b, lq, 2, 16) and not out.any()
+        for g, t in zip(torch.autograd.grad(out, (q, k, v), torch.ones_like(out)), (q, k, v)):
+            assert g.shape == t.shape and not g.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lq", [1, 50])
+def test_streams_and_capture(lq):
+    """On a side stream; and captured, replayed with new inputs and with work of its own between."""
+    from fovi_amd.arch.attention import cross_attention
+    q, k, v, _, g = _inputs(2, lq, 3000, 4, 2, 64, torch.bfloat16, seed=13)
+    want = cross_attention(q, k, v)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = cross_attention(q, k, v)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got, want)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = cross_attention(q, k, v)
+    for i in range(4):
+        q.copy_(torch.randn(q.shape, generator=g).cuda())
+        want = cross_attention(q, k, v)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), i
+
+
+@pytest.mark.gpu
+def test_autocast_takes_bf16():
+    from fovi_amd.arch.attention import cross_attention
+    q, k, v, _, _ = _inputs(1, 9, 33, 2, 2, 32, torch.float32, seed=14)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        out = cross_attention(q, k, v)
+    assert out.dtype == torch.bfloat16
+    assert torch.equal(out, cross_attention(q.bfloat16(), k.bfloat16(), v.bfloat16()))
+
+
+@pytest.mark.gpu
+def test_refusals():
+    from fovi_amd.arch.attention import cross_attention
+    q, k, v, _, _ = _inputs(2, 5, 7, 4, 2, 16, torch.float32)
+    lengths = torch.tensor([3, 7], device="cuda")
+    cross_attention(q, k, v, kv_lengths=lengths)
+    big = torch.zeros(2, 5, 4, 136, device="cuda")
+    mask = torch.ones(5, 7, dtype=torch.bool, device="cuda")
+    for args, kw, kind, match in [
+            ((q.cpu(), k, v), {}, RuntimeError, "no CPU fallback"), ((q[0], k, v), {}, ValueError, "expected"),
+            ((q, k, v[:, :6]), {}, ValueError, "do not fit"), ((q, k[..., :8], v[..., :8]), {}, ValueError, "do not fit"),
+            ((q[:, :, :3], k, v), {}, ValueError, "heads"), ((big, big, big), {}, ValueError, "128"),
+            ((q.half(), k.half(), v.half()), {}, TypeError, "dtypes"), ((q.bfloat16(), k, v), {}, TypeError, "dtypes"),
+            ((q, k, v), {"scale": 0.0}, ValueError, "scale"), ((q, k, v), {"scale": INF}, ValueError, "scale"),
+            ((q, k, v), {"kv_lengths": lengths[:1]}, ValueError, "kv_lengths"),
+            ((q, k, v), {"kv_lengths": lengths.float()}, ValueError, "kv_lengths"),
+            ((q, k, v), {"mask": mask[:, :6]}, ValueError, "mask of shape"),
+            ((q, k, v), {"mask": mask.to(torch.uint8)}, TypeError, "mask dtype"),
+            ((q, k, v), {"mask": mask.float().requires_grad_(True)}, ValueError, "no gradient"),
+            ((q, k, v), {"mask": mask.cpu()}, RuntimeError, "no CPU fallback")]:
+        with pytest.raises(kind, match=match):
+            cross_attention(*args, **kw)
+
+
+def test_c_arguments_are_refused():
+    lib = _lib.load()
+    a = _lib.AttentionArgs()
+    assert lib.fovi_attention_fwd(a, None) != 0 and b"null pointer" in lib.fovi_last_error()
+    a.q = a.k = a.v = a.out = 16
+    a.dtype = 9
+    assert lib.fovi_attention_fwd(a, None) != 0 and b"dtype" in lib.fovi_last_error()
+    a.dtype = _lib.BF16
+    assert lib.fovi_attention_fwd(a, None) != 0 and b"bad sizes" in lib.fovi_last_error()
+    a.batch, a.q_len, a.kv_len, a.heads, a.kv_heads, a.head_dim = 1, 4, 4, 3, 2, 64
+    assert lib.fovi_attention_fwd(a, None) != 0 and b"multiple" in lib.fovi_last_error()
+    a.heads, a.head_dim = 4, 129
+    assert lib.fovi_attention_fwd(a, None) != 0 and b"head_dim" in lib.fovi_last_error()
+    a.head_dim = 64
+    assert lib.fovi_attention_fwd(a, None) != 0 and b"scale" in lib.fovi_last_error()
+    a.scale, a.mask_kind = 1.0, 3
+    assert lib.fovi_attention_fwd(a, None) != 0 and b"mask_kind" in lib.fovi_last_error()
+    a.mask_kind = _lib.MASK_KEEP
+    assert lib.fovi_attention_fwd(a, None) != 0 and b"null mask" in lib.fovi_last_error()
+    b = _lib.AttentionBwdArgs()
+    assert lib.fovi_attention_bwd(b, None) != 0 and b"null pointer" in lib.fovi_last_error()
