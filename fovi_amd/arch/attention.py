@@ -17,14 +17,30 @@ from .. import _lib
 __all__ = ["cross_attention"]
 
 
-def _unit(t):
-    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
+def _strides(t):
+    """Strides of batch, token and head, 0 along dimensions of one."""
+    return tuple(s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride()[:3]))
+
+
+def _pieces(t):
+    """``t`` as the kernels read it: heads of whole 16-byte pieces at aligned addresses. Other layouts
+    are copied, heads padded with zeros to the next piece (which no score or sum notices)."""
+    per = 16 // t.element_size()
+    extra = -t.shape[3] % per
+    if extra:
+        return torch.nn.functional.pad(t, (0, extra))
+    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and not any(s % per for s in _strides(t)):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _like(t):
-    """An output of ``t``'s shape, in its layout where that is dense with head elements adjacent."""
+    """An output of ``t``'s shape, in its layout where that is dense."""
     y = torch.empty_like(t)
-    return y if y.stride(3) == 1 or y.shape[3] == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    per = 16 // t.element_size()
+    if y.stride(3) == 1 and not any(s % per for s in _strides(y)):
+        return y
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _args(a, q, k, v, kv_lengths, mask, scale):
@@ -32,7 +48,7 @@ def _args(a, q, k, v, kv_lengths, mask, scale):
     a.dtype = _lib.dtype_code(q.dtype)
     a.batch, a.q_len, a.heads, a.head_dim = q.shape
     a.kv_len, a.kv_heads = k.shape[1], k.shape[2]
-    a.q_stride[:], a.k_stride[:], a.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
+    a.q_stride[:], a.k_stride[:], a.v_stride[:] = _strides(q), _strides(k), _strides(v)
     if mask is not None:
         a.mask_kind = _lib.MASK_KEEP if mask.dtype == torch.bool else _lib.MASK_BIAS
         a.mask = mask.data_ptr()
@@ -66,7 +82,7 @@ def _forward(q, k, v, kv_lengths, mask, scale, keep):
     a = _lib.AttentionArgs()
     _args(a, q, k, v, kv_lengths, mask, scale)
     a.out = out.data_ptr()
-    a.out_stride[:] = out.stride()[:3]
+    a.out_stride[:] = _strides(out)
     if keep:
         a.stats = stats.data_ptr()
         if rest is not None:
@@ -94,7 +110,7 @@ class _CrossAttentionFn(torch.autograd.Function):
         dq, dk, dv = _like(q), _like(k), _like(v)
         if q.numel() == 0:
             return dq, dk.zero_(), dv.zero_(), None, None, None
-        dout = _unit(dout.to(q.dtype))
+        dout = _pieces(dout.to(q.dtype))
         lib = _lib.load()
         a = _lib.AttentionBwdArgs()
         _args(a.fwd, q, k, v, kv_lengths, mask, ctx.scale)
@@ -102,8 +118,8 @@ class _CrossAttentionFn(torch.autograd.Function):
         if rest is not None:
             a.fwd.out_rest = rest.data_ptr()
         a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-        a.fwd.out_stride[:], a.dout_stride[:] = out.stride()[:3], dout.stride()[:3]
-        a.dq_stride[:], a.dk_stride[:], a.dv_stride[:] = dq.stride()[:3], dk.stride()[:3], dv.stride()[:3]
+        a.fwd.out_stride[:], a.dout_stride[:] = _strides(out), _strides(dout)
+        a.dq_stride[:], a.dk_stride[:], a.dv_stride[:] = _strides(dq), _strides(dk), _strides(dv)
         work = _workspace(a.fwd, lib.fovi_attention_bwd_workspace_bytes, q.device)
         _lib.check(lib.fovi_attention_bwd(a, _lib.stream_handle(q.device)), "fovi_attention_bwd")
         del work
@@ -114,8 +130,8 @@ def cross_attention(q, k, v, kv_lengths=None, mask=None, scale=None):
     """``softmax(scale q k^T + mask) v``, in the type and layout of ``q [B, Lq, Hq, D]``.
 
     ``k, v [B, Lk, Hk, D]``, Hq a multiple of Hk (query head h reads key head h // (Hq / Hk)), D up
-    to 128, fp32 or bf16 (under bf16 autocast fp32 inputs are taken in bf16). Any strides; head
-    elements that are not adjacent are copied first.
+    to 128, fp32 or bf16 (under bf16 autocast fp32 inputs are taken in bf16). Any strides: heads of
+    whole 16-byte pieces at aligned addresses are read where they are (broadcast ones too), others copied.
 
     ``kv_lengths [B]`` (integers on the device): image b has only its first ``kv_lengths[b]`` states.
     ``mask``, broadcastable to ``[B, Hq, Lq, Lk]``: boolean, True where a row may read a state, or a
@@ -163,7 +179,9 @@ def cross_attention(q, k, v, kv_lengths=None, mask=None, scale=None):
             mask = mask.expand(b, hq, lq, lk)
         except RuntimeError:
             raise ValueError(f"cross_attention: mask of shape {tuple(mask.shape)} for {(b, hq, lq, lk)}") from None
-    q, k, v = _unit(q), _unit(k), _unit(v)
+    q, k, v = _pieces(q), _pieces(k), _pieces(v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _CrossAttentionFn.apply(q, k, v, kv_lengths, mask, scale)
-    return _forward(q, k, v, kv_lengths, mask, scale, False)[0]
+        out = _CrossAttentionFn.apply(q, k, v, kv_lengths, mask, scale)
+    else:
+        out = _forward(q, k, v, kv_lengths, mask, scale, False)[0]
+    return out if out.shape[3] == d else out[..., :d]

@@ -1,0 +1,433 @@
+// Attention backward (see attention.h for the block layout).
+//
+//   p_ij = exp(s_ij - max_i) / sum_i, ds_ij = p_ij (do_i.v_j - delta_i), delta_i = do_i.o_i
+//   dq_i = scale sum_j ds_ij k_j, dk_j = scale sum_i ds_ij q_i, dv_j = sum_i p_ij do_i
+//
+// Three launches: delta; dq, whose workgroups own query rows and walk the states; dk and dv, whose
+// workgroups own states and walk the query rows of all heads that share the key head. The scores
+// are formed twice (7 products instead of 5), and in return every gradient is summed by one
+// workgroup in a fixed order, without atomics and without a score matrix in memory. Where the owned
+// axis is short, the walked one is split over workgroups and the partial sums join in a last launch.
+#include "attention.h"
+
+namespace fovi {
+
+// delta of four rows per wave: 16 lanes each
+template <typename T>
+__global__ __launch_bounds__(256) void attn_delta_kernel(AttnParams p) {
+  constexpr int N = Chunk<T>::N;
+  const int64_t rows = p.B * p.H * p.Lq, x = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
+  float sum = 0;
+  if (x < rows) {
+    const int64_t bh = x / p.Lq, i = x - bh * p.Lq, b = bh / p.H, h = bh - b * p.H;
+    const T* g = static_cast<const T*>(p.dout) + b * p.dos[0] + i * p.dos[1] + h * p.dos[2];
+    const int64_t off = b * p.os[0] + i * p.os[1] + h * p.os[2];
+    for (int c = threadIdx.x & 15; c * N < p.D; c += 16) {
+      T a[N], o[N], r[N];
+      const uint4 ga = load_chunk<T>(g, c, p.D), oa = load_chunk<T>(static_cast<const T*>(p.o) + off, c, p.D);
+      const uint4 ra = p.rest ? load_chunk<T>(static_cast<const T*>(p.rest) + off, c, p.D) : make_uint4(0, 0, 0, 0);
+      __builtin_memcpy(a, &ga, 16);
+      __builtin_memcpy(o, &oa, 16);
+      __builtin_memcpy(r, &ra, 16);
+#pragma unroll
+      for (int e = 0; e < N; ++e) sum = fmaf(Elem<T>::load(a + e), Elem<T>::load(o + e) + Elem<T>::load(r + e), sum);
+    }
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+  if (x < rows && (threadIdx.x & 15) == 0) p.delta[x] = sum;
+}
+
+// What a row's probabilities need: exp2(t - shift) * factor. Without a bias the log of the sum goes
+// into the shift (factor 1). A row that keeps nothing has shift +inf: probabilities 0.
+struct RowStat { float shift, factor, delta; };
+template <int KIND>
+__device__ __forceinline__ RowStat row_stat(const AttnParams& p, int64_t at) {
+  const float m = p.stats[at], sum = p.stats[p.B * p.H * p.Lq + at];
+  RowStat r;
+  r.shift = sum == 0 ? __builtin_inff() : KIND ? m : m + log2f(sum);
+  r.factor = KIND ? (sum == 0 ? 0.0f : 1.0f / sum) : 1.0f;
+  r.delta = p.delta[at];
+  return r;
+}
+
+// Probability and score gradient of one pair; KIND 1: t is the masked score, left-out pairs become kLeftOut.
+template <int KIND>
+__device__ __forceinline__ void pair_grad(float t, float c, float shift, float factor, float delta, float dp, float& e, float& ds) {
+  if (KIND) {
+    const bool out = t == kNegInf || shift == __builtin_inff();
+    e = exp2_fast(t - shift) * factor;
+    ds = out ? kLeftOut : e * (dp - delta);
+    e = out ? kLeftOut : e;
+  } else {
+    e = exp2_fast(fmaf(t, c, -shift));
+    ds = e * (dp - delta);
+  }
+}
+
+template <typename T, int DP, int QT, int KIND>
+__global__ __launch_bounds__(256) void attn_dq_kernel(AttnParams p) {
+  constexpr int LP = DP == 96 ? 128 : DP, KB = sizeof(T) == 2 ? 2 : 1, KT = 32 * KB, DT = DP / 32, STEPS = DP / (2 * Chunk<T>::N);
+  __shared__ __attribute__((aligned(16))) char tiles[2][2][KT * LP * sizeof(T)];
+  __shared__ int bad_tile[2];
+  const int64_t all = p.tiles * p.B * p.Hk, id = xcd_tile(blockIdx.x, gridDim.x);
+  if (id >= all) return;
+  const int64_t bh = id / p.tiles, b = bh / p.Hk;
+  const int hk = static_cast<int>(bh - b * p.Hk), split = blockIdx.y, l = threadIdx.x & 63;
+  const int64_t len = attn_len(p, b), j0 = split * p.chunk, n = len < j0 + p.chunk ? len : j0 + p.chunk;
+  if (split && n <= j0) return;
+  const int64_t r0 = (id - bh * p.tiles) * (128 * QT) + (threadIdx.x >> 6) * (32 * QT);
+  uint4 q[QT][STEPS], g[QT][STEPS];
+  f32x16 dq[QT][DT] = {};
+  RowStat st[QT];
+  const void* mrow[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int64_t r = r0 + 32 * t + (l & 31);
+    const int64_t gr = r < p.R ? r / p.Lq : 0, i = r < p.R ? r - gr * p.Lq : 0, h = hk * p.G + gr;
+    const T* qr = static_cast<const T*>(p.q) + b * p.qs[0] + i * p.qs[1] + h * p.qs[2];
+    const T* gg = static_cast<const T*>(p.dout) + b * p.dos[0] + i * p.dos[1] + h * p.dos[2];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      q[t][s] = load_chunk<T>(qr, 2 * s + (l >> 5), r < p.R ? p.D : 0);
+      g[t][s] = load_chunk<T>(gg, 2 * s + (l >> 5), r < p.R ? p.D : 0);
+    }
+    st[t] = row_stat<KIND>(p, (b * p.H + h) * p.Lq + i);
+    mrow[t] = KIND ? mask_row(p, b, h, i) : nullptr;
+  }
+  const T* k = static_cast<const T*>(p.k) + b * p.ks[0] + hk * p.ks[2];
+  const T* v = static_cast<const T*>(p.v) + b * p.vs[0] + hk * p.vs[2];
+  Staged<T, DP, LP, KT, 256> kr, vr;
+  if (KIND && threadIdx.x < 2) bad_tile[threadIdx.x] = -1;
+  if (KIND) __syncthreads();
+  int at = 0;
+  auto put = [&](int buf, int tile) {
+    kr.store(tiles[buf][0], threadIdx.x);
+    vr.store(tiles[buf][1], threadIdx.x);
+    if (KIND && kr.bad()) bad_tile[buf] = tile;
+  };
+  if (j0 < n) {
+    kr.load(k + j0 * p.ks[1], p.ks[1], n - j0, p.D, threadIdx.x);
+    vr.load(v + j0 * p.vs[1], p.vs[1], n - j0, p.D, threadIdx.x);
+    put(0, 0);
+  }
+  for (int64_t j = j0; j < n; j += KT, ++at) {
+    const int64_t next = j + KT;
+    if (next < n) {
+      kr.load(k + next * p.ks[1], p.ks[1], n - next, p.D, threadIdx.x);
+      vr.load(v + next * p.vs[1], p.vs[1], n - next, p.D, threadIdx.x);
+    }
+    __syncthreads();
+    const char* kt = tiles[at & 1][0];
+    const char* vt = tiles[at & 1][1];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      f32x16 s[QT] = {}, dp[QT] = {};
+#pragma unroll
+      for (int t = 0; t < STEPS; ++t) {
+        const int off = kb * 32 * LP * static_cast<int>(sizeof(T)) + tile_at<T, LP>(l & 31, 2 * t + (l >> 5));
+        const uint4 ka = *reinterpret_cast<const uint4*>(kt + off), va = *reinterpret_cast<const uint4*>(vt + off);
+#pragma unroll
+        for (int x = 0; x < QT; ++x) {
+          s[x] = mma_step(T(), ka, q[x][t], s[x]);
+          dp[x] = mma_step(T(), va, g[x][t], dp[x]);
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < QT; ++x) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int64_t col = j + kb * 32 + 8 * (i / 4) + 4 * (l >> 5) + i % 4;
+          float t = s[x][i], e, ds;
+          if (KIND) t = col < n ? masked_score(p, mrow[x], col, t) : kNegInf;
+          else if (j + kb * 32 + 32 > n) t = col < n ? t : kNegInf;
+          pair_grad<KIND>(t, p.c, st[x].shift, st[x].factor, st[x].delta, dp[x][i], e, ds);
+          s[x][i] = ds;
+        }
+        if (KIND && bad_tile[at & 1] == at) {
+          slow_second<T, LP, DT>(kt, kb * 32, s[x], dq[x]);
+        } else {
+          const Block<T> ds(s[x]);
+#pragma unroll
+          for (int d = 0; d < DT; ++d) dq[x][d] = mma_second<LP>(T(), kt, kb * 32, d, ds, dq[x][d]);
+        }
+      }
+    }
+    if (next < n) put((at + 1) & 1, at + 1);
+  }
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int64_t r = r0 + 32 * t + (l & 31);
+    if (r >= p.R) continue;
+    const int64_t gr = r / p.Lq, i = r - gr * p.Lq;
+    T* out = static_cast<T*>(p.dq) + b * p.dqs[0] + i * p.dqs[1] + (hk * p.G + gr) * p.dqs[2];
+    float* part = p.part + ((split * p.B * p.Hk + bh) * p.R + r) * p.D;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const int at_d = d * 32 + 2 * e + 4 * (l >> 5);
+        const float a = dq[t][d][e] * p.scale, bb = dq[t][d][e + 1] * p.scale, c = dq[t][d][e + 2] * p.scale, f = dq[t][d][e + 3] * p.scale;
+        if (p.splits > 1) store_run(part, at_d, p.D, a, bb, c, f);
+        else store_run(out, at_d, p.D, a, bb, c, f);
+      }
+  }
+}
+
+template <typename T, int DP, int KIND>
+__global__ __launch_bounds__(256) void attn_dkv_kernel(AttnParams p) {
+  constexpr int LP = DP == 96 ? 128 : DP, DT = DP / 32, STEPS = DP / (2 * Chunk<T>::N);
+  __shared__ __attribute__((aligned(16))) char tiles[2][2][32 * LP * sizeof(T)];
+  __shared__ __attribute__((aligned(16))) float stats[2][3][32];
+  __shared__ int bad_tile[2][2];
+  const int64_t all = p.tiles * p.B * p.Hk, id = xcd_tile(blockIdx.x, gridDim.x);
+  if (id >= all) return;
+  const int64_t bh = id / p.tiles, b = bh / p.Hk;
+  const int hk = static_cast<int>(bh - b * p.Hk), split = blockIdx.y, l = threadIdx.x & 63;
+  const int64_t n = attn_len(p, b), w0 = (id - bh * p.tiles) * 128, j = w0 + (threadIdx.x >> 6) * 32 + (l & 31);
+  const T* kp = static_cast<const T*>(p.k) + b * p.ks[0] + j * p.ks[1] + hk * p.ks[2];
+  const T* vp = static_cast<const T*>(p.v) + b * p.vs[0] + j * p.vs[1] + hk * p.vs[2];
+  uint4 k[STEPS], v[STEPS];
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    k[s] = load_chunk<T>(kp, 2 * s + (l >> 5), j < n ? p.D : 0);
+    v[s] = load_chunk<T>(vp, 2 * s + (l >> 5), j < n ? p.D : 0);
+  }
+  f32x16 dk[DT] = {}, dv[DT] = {};
+  // tiles of 32 rows, head by head: tile x is rows 32 (x % per) .. of head x / per of the group
+  const int64_t per = (p.Lq + 31) / 32, end = per * p.G;
+  int64_t x = split * p.chunk;
+  const int64_t x1 = w0 >= n ? x : end < x + p.chunk ? end : x + p.chunk;
+  Staged<T, DP, LP, 32, 256> qr, gr;
+  RowStat sr;
+  if (KIND && threadIdx.x < 4) bad_tile[threadIdx.x >> 1][threadIdx.x & 1] = -1;
+  if (KIND) __syncthreads();
+  auto fetch = [&](int64_t tile) {
+    const int64_t h = hk * p.G + tile / per, i = tile % per * 32;
+    qr.load(static_cast<const T*>(p.q) + b * p.qs[0] + i * p.qs[1] + h * p.qs[2], p.qs[1], p.Lq - i, p.D, threadIdx.x);
+    gr.load(static_cast<const T*>(p.dout) + b * p.dos[0] + i * p.dos[1] + h * p.dos[2], p.dos[1], p.Lq - i, p.D, threadIdx.x);
+    if (threadIdx.x < 32) {
+      if (i + threadIdx.x < p.Lq) sr = row_stat<KIND>(p, (b * p.H + h) * p.Lq + i + threadIdx.x);
+      else sr = {__builtin_inff(), 0.0f, 0.0f};
+    }
+  };
+  auto put = [&](int buf, int tile) {
+    qr.store(tiles[buf][0], threadIdx.x);
+    gr.store(tiles[buf][1], threadIdx.x);
+    if (threadIdx.x < 32) {
+      stats[buf][0][threadIdx.x] = sr.shift;
+      stats[buf][1][threadIdx.x] = sr.factor;
+      stats[buf][2][threadIdx.x] = sr.delta;
+    }
+    if (KIND && qr.bad()) bad_tile[buf][0] = tile;
+    if (KIND && gr.bad()) bad_tile[buf][1] = tile;
+  };
+  int at = 0;
+  if (x < x1) {
+    fetch(x);
+    put(0, 0);
+  }
+  for (; x < x1; ++x, ++at) {
+    if (x + 1 < x1) fetch(x + 1);
+    __syncthreads();
+    const char* qt = tiles[at & 1][0];
+    const char* gt = tiles[at & 1][1];
+    f32x16 s = {}, dp = {};
+#pragma unroll
+    for (int t = 0; t < STEPS; ++t) {
+      const int off = tile_at<T, LP>(l & 31, 2 * t + (l >> 5));
+      s = mma_step(T(), *reinterpret_cast<const uint4*>(qt + off), k[t], s);
+      dp = mma_step(T(), *reinterpret_cast<const uint4*>(gt + off), v[t], dp);
+    }
+    const int64_t h = hk * p.G + x / per, i0 = x % per * 32;
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const int r = 2 * i + 4 * (l >> 5);
+      const f32x4 shift = *reinterpret_cast<const f32x4*>(&stats[at & 1][0][r]), delta = *reinterpret_cast<const f32x4*>(&stats[at & 1][2][r]);
+      f32x4 factor;
+      if (KIND) factor = *reinterpret_cast<const f32x4*>(&stats[at & 1][1][r]);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        float t = s[i + y], e, ds;
+        if (KIND) t = j < n && i0 + r + y < p.Lq ? masked_score(p, mask_row(p, b, h, i0 + r + y), j, t) : kNegInf;
+        pair_grad<KIND>(t, p.c, shift[y], KIND ? factor[y] : 1.0f, delta[y], dp[i + y], e, ds);
+        s[i + y] = e;
+        dp[i + y] = ds;
+      }
+    }
+    if (KIND && bad_tile[at & 1][1] == at) {
+      slow_second<T, LP, DT>(gt, 0, s, dv);
+    } else {
+      const Block<T> e(s);
+#pragma unroll
+      for (int d = 0; d < DT; ++d) dv[d] = mma_second<LP>(T(), gt, 0, d, e, dv[d]);
+    }
+    if (KIND && bad_tile[at & 1][0] == at) {
+      slow_second<T, LP, DT>(qt, 0, dp, dk);
+    } else {
+      const Block<T> ds(dp);
+#pragma unroll
+      for (int d = 0; d < DT; ++d) dk[d] = mma_second<LP>(T(), qt, 0, d, ds, dk[d]);
+    }
+    if (x + 1 < x1) put((at + 1) & 1, at + 1);
+  }
+  if (j >= p.Lk) return;
+  T* dko = static_cast<T*>(p.dk) + b * p.dks[0] + j * p.dks[1] + hk * p.dks[2];
+  T* dvo = static_cast<T*>(p.dv) + b * p.dvs[0] + j * p.dvs[1] + hk * p.dvs[2];
+  float* part = p.part + ((split * p.B * p.Hk + bh) * p.Lk + j) * 2 * p.D;
+  const float keep = j < n ? 1.0f : 0.0f;          // (columns behind the length never met a value: 0 or NaN)
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const int at_d = d * 32 + 2 * e + 4 * (l >> 5);
+      float a[4], c[4];
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        a[y] = keep != 0 ? dk[d][e + y] * p.scale : 0.0f;
+        c[y] = keep != 0 ? dv[d][e + y] : 0.0f;
+      }
+      if (p.splits > 1) {
+        store_run(part, at_d, p.D, a[0], a[1], a[2], a[3]);
+        store_run(part + p.D, at_d, p.D, c[0], c[1], c[2], c[3]);
+      } else {
+        store_run(dko, at_d, p.D, a[0], a[1], a[2], a[3]);
+        store_run(dvo, at_d, p.D, c[0], c[1], c[2], c[3]);
+      }
+    }
+}
+
+// Partial sums added up in the order of the splits, four elements a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_dq_join_kernel(AttnParams p) {
+  const int per = p.D / 4;
+  const int64_t rows = p.B * p.Hk * p.R, x = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (x >= rows * per) return;
+  const int64_t row = x / per, d = (x - row * per) * 4, bh = row / p.R, r = row - bh * p.R, b = bh / p.Hk, g = r / p.Lq;
+  int64_t used = (attn_len(p, b) + p.chunk - 1) / p.chunk;
+  if (used < 1) used = 1;
+  f32x4 sum = {};
+  for (int64_t s = 0; s < used; ++s) sum += *reinterpret_cast<const f32x4*>(p.part + (s * rows + row) * p.D + d);
+  T* out = static_cast<T*>(p.dq) + b * p.dqs[0] + (r - g * p.Lq) * p.dqs[1] + ((bh - b * p.Hk) * p.G + g) * p.dqs[2];
+  store_run(out, static_cast<int>(d), p.D, sum[0], sum[1], sum[2], sum[3]);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void attn_dkv_join_kernel(AttnParams p) {
+  const int per = p.D / 4;
+  const int64_t rows = p.B * p.Hk * p.Lk, x = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (x >= rows * 2 * per) return;
+  const int64_t row = x / (2 * per), y = x - row * 2 * per, d = y % per * 4, bh = row / p.Lk, j = row - bh * p.Lk, b = bh / p.Hk;
+  f32x4 sum = {};
+  for (int64_t s = 0; s < p.splits; ++s) sum += *reinterpret_cast<const f32x4*>(p.part + (s * rows + row) * 2 * p.D + y * 4);
+  T* out = y >= per ? static_cast<T*>(p.dv) + b * p.dvs[0] + j * p.dvs[1] + (bh - b * p.Hk) * p.dvs[2]
+                    : static_cast<T*>(p.dk) + b * p.dks[0] + j * p.dks[1] + (bh - b * p.Hk) * p.dks[2];
+  store_run(out, static_cast<int>(d), p.D, sum[0], sum[1], sum[2], sum[3]);
+}
+
+struct BwdPlan {
+  int qt, q_splits, k_splits;
+  int64_t q_tiles, q_chunk, k_tiles, k_chunk;
+};
+
+static BwdPlan bwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t D) {
+  BwdPlan f;
+  const int64_t R = H / Hk * Lq;
+  f.qt = D <= 64 && R > 128 ? 2 : 1;
+  f.q_tiles = (R + 128 * f.qt - 1) / (128 * f.qt);
+  f.k_tiles = (Lk + 127) / 128;
+  // splits for two workgroups a compute unit, each with at least 256 states or 256 rows to walk
+  const int64_t gq = B * Hk * f.q_tiles, gk = B * Hk * f.k_tiles, row_tiles = H / Hk * ((Lq + 31) / 32);
+  int64_t s = gq > 0 ? 512 / gq : 1;
+  if (s > Lk / 256) s = Lk / 256;
+  if (s < 1) s = 1;
+  f.q_chunk = ((Lk + s - 1) / s + 127) / 128 * 128;
+  if (f.q_chunk < 128) f.q_chunk = 128;
+  f.q_splits = static_cast<int>(Lk ? (Lk + f.q_chunk - 1) / f.q_chunk : 1);
+  s = gk > 0 ? 512 / gk : 1;
+  if (s > row_tiles / 8) s = row_tiles / 8;
+  if (s < 1) s = 1;
+  f.k_chunk = (row_tiles + s - 1) / s;
+  if (f.k_chunk < 1) f.k_chunk = 1;
+  f.k_splits = static_cast<int>(row_tiles ? (row_tiles + f.k_chunk - 1) / f.k_chunk : 1);
+  return f;
+}
+
+static int64_t align16(int64_t n) { return (n + 15) / 16 * 16; }
+
+int64_t attn_bwd_workspace(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t D, int dtype) {
+  (void)dtype;
+  const BwdPlan f = bwd_plan(B, Lq, Lk, H, Hk, D);
+  // delta, then the partial sums of dq, later those of dk and dv in their place
+  const int64_t q = f.q_splits > 1 ? f.q_splits * B * H * Lq * D * 4 : 0, k = f.k_splits > 1 ? f.k_splits * B * Hk * Lk * 2 * D * 4 : 0;
+  return align16(B * H * Lq * 4) + (q > k ? q : k);
+}
+
+template <typename T, int DP, int KIND>
+static void bwd_dq(const AttnParams& p, int qt, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>((p.B * p.Hk * p.tiles + 7) / 8 * 8), static_cast<unsigned>(p.splits));
+  if (qt == 1) attn_dq_kernel<T, DP, 1, KIND><<<grid, 256, 0, s>>>(p);
+  else if constexpr (DP <= 64) attn_dq_kernel<T, DP, 2, KIND><<<grid, 256, 0, s>>>(p);
+}
+
+template <typename T, int DP, int KIND>
+static void bwd_dkv(const AttnParams& p, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>((p.B * p.Hk * p.tiles + 7) / 8 * 8), static_cast<unsigned>(p.splits));
+  attn_dkv_kernel<T, DP, KIND><<<grid, 256, 0, s>>>(p);
+}
+
+template <typename T>
+static int bwd_type(AttnParams& p, hipStream_t s) {
+  const BwdPlan f = bwd_plan(p.B, p.Lq, p.Lk, p.H, p.Hk, p.D);
+  p.delta = p.part;
+  p.part = reinterpret_cast<float*>(reinterpret_cast<char*>(p.part) + align16(p.B * p.H * p.Lq * 4));
+  const int64_t rows = p.B * p.H * p.Lq;
+  if (rows) {
+    attn_delta_kernel<T><<<static_cast<unsigned>((rows + 15) / 16), 256, 0, s>>>(p);
+    if (check_launch("fovi_attention_bwd")) return 1;
+    p.tiles = f.q_tiles; p.splits = f.q_splits; p.chunk = f.q_chunk;
+    const int dp = p.D <= 32 ? 32 : p.D <= 64 ? 64 : p.D <= 96 ? 96 : 128;
+    if (p.kind) {
+      if (dp == 32) bwd_dq<T, 32, 1>(p, f.qt, s);
+      else if (dp == 64) bwd_dq<T, 64, 1>(p, f.qt, s);
+      else if (dp == 96) bwd_dq<T, 96, 1>(p, f.qt, s);
+      else bwd_dq<T, 128, 1>(p, f.qt, s);
+    } else {
+      if (dp == 32) bwd_dq<T, 32, 0>(p, f.qt, s);
+      else if (dp == 64) bwd_dq<T, 64, 0>(p, f.qt, s);
+      else if (dp == 96) bwd_dq<T, 96, 0>(p, f.qt, s);
+      else bwd_dq<T, 128, 0>(p, f.qt, s);
+    }
+    if (check_launch("fovi_attention_bwd")) return 1;
+    if (f.q_splits > 1) {
+      attn_dq_join_kernel<T><<<static_cast<unsigned>((rows * (p.D / 4) + 255) / 256), 256, 0, s>>>(p);
+      if (check_launch("fovi_attention_bwd")) return 1;
+    }
+  }
+  if (p.Lk == 0 || p.B == 0) return 0;
+  p.tiles = f.k_tiles; p.splits = f.k_splits; p.chunk = f.k_chunk;
+  if (p.kind) {
+    if (p.D <= 32) bwd_dkv<T, 32, 1>(p, s);
+    else if (p.D <= 64) bwd_dkv<T, 64, 1>(p, s);
+    else if (p.D <= 96) bwd_dkv<T, 96, 1>(p, s);
+    else bwd_dkv<T, 128, 1>(p, s);
+  } else {
+    if (p.D <= 32) bwd_dkv<T, 32, 0>(p, s);
+    else if (p.D <= 64) bwd_dkv<T, 64, 0>(p, s);
+    else if (p.D <= 96) bwd_dkv<T, 96, 0>(p, s);
+    else bwd_dkv<T, 128, 0>(p, s);
+  }
+  if (check_launch("fovi_attention_bwd")) return 1;
+  if (f.k_splits > 1) {
+    const int64_t n = p.B * p.Hk * p.Lk * 2 * (p.D / 4);
+    attn_dkv_join_kernel<T><<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(p);
+    return check_launch("fovi_attention_bwd");
+  }
+  return 0;
+}
+
+int attn_bwd_launch(AttnParams& p, int dtype, hipStream_t s) {
+  return dtype == FOVI_BF16 ? bwd_type<uint16_t>(p, s) : bwd_type<float>(p, s);
+}
+
+}  // namespace fovi

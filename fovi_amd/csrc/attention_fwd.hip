@@ -1,0 +1,419 @@
+// Attention forward: out = softmax(scale q k^T + mask) v, one pass over the states with the running
+// maximum and sum of every row (see attention.h for the block layout).
+//
+//  * tile kernel: a workgroup owns 4 * 32 * QT query rows of one key head (the rows of the query heads
+//    that share it, in one sequence) and walks the states in tiles that all four waves read from
+//    LDS; the next tile is on its way in registers meanwhile.
+//  * few-row kernel: up to 32 * QT rows in all. Every wave of the workgroup has all the rows and its own
+//    states: keys straight from memory as matrix operands, values through an LDS tile of the
+//    wave's own (only the transposing read needs it), no barrier until the four waves' results join.
+//
+// Where rows are few, the states are split over workgroups too; a second launch joins the partial
+// results in a fixed order.
+#include "attention.h"
+
+namespace fovi {
+
+template <typename T, int DP, int QT>
+struct RowState {
+  static constexpr int DT = DP / 32, STEPS = DP / (2 * Chunk<T>::N);
+  uint4 q[QT][STEPS];
+  f32x16 o[QT][DT];
+  float m[QT], l[QT];         // the row's maximum so far; the lane's share of the sum
+  const void* mrow[QT];
+};
+
+// The rows r0 + 32 t + lane of key head (b, hk): queries as B operands, statistics cleared.
+template <typename T, int DP, int QT>
+__device__ __forceinline__ void init_rows(const AttnParams& p, RowState<T, DP, QT>& st, int64_t b, int hk, int64_t r0) {
+  const int l = threadIdx.x & 63;
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int64_t r = r0 + 32 * t + (l & 31);
+    const int64_t g = r < p.R ? r / p.Lq : 0, i = r < p.R ? r - g * p.Lq : 0, h = hk * p.G + g;
+    const T* q = static_cast<const T*>(p.q) + b * p.qs[0] + i * p.qs[1] + h * p.qs[2];
+#pragma unroll
+    for (int s = 0; s < RowState<T, DP, QT>::STEPS; ++s)
+      st.q[t][s] = r < p.R ? load_chunk<T>(q, 2 * s + (l >> 5), p.D) : make_uint4(0, 0, 0, 0);
+    st.m[t] = kNegInf;
+    st.l[t] = 0;
+    st.mrow[t] = p.kind ? mask_row(p, b, h, i) : nullptr;
+#pragma unroll
+    for (int d = 0; d < RowState<T, DP, QT>::DT; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) st.o[t][d][e] = 0;
+  }
+}
+
+// Scores of KB blocks of 32 states (j .. n valid) into probabilities; the running statistics of
+// rows t and the outputs' scale follow. KIND 1: the mask is applied, pairs that are left out become kLeftOut.
+template <typename T, int DP, int QT, int KIND, int KB>
+__device__ __forceinline__ void softmax_blocks(const AttnParams& p, RowState<T, DP, QT>& st, int t, f32x16 (&s)[KB], Block<T> (&e)[KB],
+                                               int64_t j, int64_t n) {
+  const int h = (threadIdx.x & 63) >> 5;
+  const float c = KIND ? 1.0f : p.c;
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb) {
+    if (KIND) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int64_t at = j + kb * 32 + 8 * (i / 4) + 4 * h + i % 4;
+        s[kb][i] = at < n ? masked_score(p, st.mrow[t], at, s[kb][i]) : kNegInf;
+      }
+    } else if (j + kb * 32 + 32 > n) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (j + kb * 32 + 8 * (i / 4) + 4 * h + i % 4 >= n) s[kb][i] = kNegInf;
+    }
+  }
+  float top = st.m[t];
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][i]);
+  top = fmaxf(top, __shfl_xor(top, 32));
+  const float at = top == kNegInf ? 0.0f : top;
+  if (__any(top != st.m[t])) {                 // the maxima settle after the first tiles
+    const float keep = exp2_fast((st.m[t] - at) * c);
+    st.l[t] *= keep;
+#pragma unroll
+    for (int d = 0; d < RowState<T, DP, QT>::DT; ++d) st.o[t][d] *= keep;
+    st.m[t] = top;
+  }
+  const float mc = at * c;
+  float sum = 0;
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float x = exp2_fast(fmaf(s[kb][i], c, -mc));
+      s[kb][i] = KIND && s[kb][i] == kNegInf ? kLeftOut : x;
+    }
+    e[kb] = Block<T>(s[kb]);
+    sum = e[kb].sum(sum);
+  }
+  st.l[t] += sum;
+}
+
+__device__ __forceinline__ int64_t stat_at(const AttnParams& p, int64_t b, int hk, int64_t r) {
+  return (b * p.H + static_cast<int64_t>(hk) * p.G) * p.Lq + r;      // row (b, head, query) of the statistics
+}
+
+template <typename T, int DP, int QT, int KIND>
+__global__ __launch_bounds__(256) void attn_fwd_tile_kernel(AttnParams p) {
+  constexpr int LP = DP == 96 ? 128 : DP, KB = sizeof(T) == 2 ? 2 : 1, KT = 32 * KB, DT = DP / 32;
+  constexpr int STEPS = RowState<T, DP, QT>::STEPS;
+  __shared__ __attribute__((aligned(16))) char tiles[2][2][KT * LP * sizeof(T)];
+  __shared__ int bad_tile[2];
+  const int64_t all = p.tiles * p.B * p.Hk, id = xcd_tile(blockIdx.x, gridDim.x);
+  if (id >= all) return;
+  const int64_t bh = id / p.tiles, b = bh / p.Hk;
+  const int hk = static_cast<int>(bh - b * p.Hk), split = blockIdx.y;
+  const int64_t len = attn_len(p, b), j0 = split * p.chunk, n = len < j0 + p.chunk ? len : j0 + p.chunk;
+  if (split && n <= j0) return;                        // (split 0 writes the rows of images without states)
+  const int64_t r0 = (id - bh * p.tiles) * (128 * QT) + (threadIdx.x >> 6) * (32 * QT);
+  RowState<T, DP, QT> st;
+  init_rows<T, DP, QT>(p, st, b, hk, r0);
+  const T* k = static_cast<const T*>(p.k) + b * p.ks[0] + hk * p.ks[2];
+  const T* v = static_cast<const T*>(p.v) + b * p.vs[0] + hk * p.vs[2];
+  Staged<T, DP, LP, KT, 256> kr, vr;
+  if (KIND && threadIdx.x < 2) bad_tile[threadIdx.x] = -1;
+  if (KIND) __syncthreads();
+  int at = 0;
+  auto put = [&](int buf, int tile) {
+    kr.store(tiles[buf][0], threadIdx.x);
+    vr.store(tiles[buf][1], threadIdx.x);
+    if (KIND && vr.bad()) bad_tile[buf] = tile;
+  };
+  if (j0 < n) {
+    kr.load(k + j0 * p.ks[1], p.ks[1], n - j0, p.D, threadIdx.x);
+    vr.load(v + j0 * p.vs[1], p.vs[1], n - j0, p.D, threadIdx.x);
+    put(0, 0);
+  }
+  for (int64_t j = j0; j < n; j += KT, ++at) {
+    const int64_t next = j + KT;
+    if (next < n) {
+      kr.load(k + next * p.ks[1], p.ks[1], n - next, p.D, threadIdx.x);
+      vr.load(v + next * p.vs[1], p.vs[1], n - next, p.D, threadIdx.x);
+    }
+    __syncthreads();                                   // tile `at` is in LDS, tile at - 1 is done with
+    const char* kt = tiles[at & 1][0];
+    const char* vt = tiles[at & 1][1];
+    const int l = threadIdx.x & 63;
+    f32x16 s[QT][KB] = {};
+    Block<T> e[QT][KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int t = 0; t < STEPS; ++t) {
+        const uint4 a = *reinterpret_cast<const uint4*>(kt + kb * 32 * LP * sizeof(T) + tile_at<T, LP>(l & 31, 2 * t + (l >> 5)));
+#pragma unroll
+        for (int q = 0; q < QT; ++q) s[q][kb] = mma_step(T(), a, st.q[q][t], s[q][kb]);
+      }
+#pragma unroll
+    for (int q = 0; q < QT; ++q) softmax_blocks<T, DP, QT, KIND, KB>(p, st, q, s[q], e[q], j, n);
+    if (KIND && bad_tile[at & 1] == at) {
+#pragma unroll
+      for (int q = 0; q < QT; ++q)
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) slow_second<T, LP, DT>(vt, kb * 32, s[q][kb], st.o[q]);
+    } else {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int q = 0; q < QT; ++q)
+#pragma unroll
+          for (int d = 0; d < DT; ++d) st.o[q][d] = mma_second<LP>(T(), vt, kb * 32, d, e[q][kb], st.o[q][d]);
+    }
+    if (next < n) put((at + 1) & 1, at + 1);
+  }
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int q = 0; q < QT; ++q) {
+    const int64_t r = r0 + 32 * q + (lane & 31);
+    const float sum = st.l[q] + __shfl_xor(st.l[q], 32), m = KIND ? st.m[q] : st.m[q] * p.c;
+    if (r >= p.R) continue;
+    if (p.splits > 1) {
+      float* out = p.part + ((split * p.B * p.Hk + bh) * p.R + r) * (p.D + 2);
+      if (lane < 32) { out[p.D] = m; out[p.D + 1] = sum; }
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int at_d = d * 32 + 8 * (e / 4) + 4 * (lane >> 5) + e % 4;
+          if (at_d < p.D) out[at_d] = st.o[q][d][e];
+        }
+      continue;
+    }
+    const int64_t g = r / p.Lq, i = r - g * p.Lq, off = b * p.os[0] + i * p.os[1] + (hk * p.G + g) * p.os[2];
+    T* out = static_cast<T*>(p.o) + off;
+    const float inv = sum == 0 ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const int at_d = d * 32 + 2 * e + 4 * (lane >> 5);
+        float y[4], rest[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          y[x] = st.o[q][d][e + x] * inv;
+          rest[x] = y[x] - bf16_bits_to_f32(f32_to_bf16_bits(y[x]));
+        }
+        store_run(out, at_d, p.D, y[0], y[1], y[2], y[3]);
+        if (p.rest) store_run(static_cast<T*>(p.rest) + off, at_d, p.D, rest[0], rest[1], rest[2], rest[3]);
+      }
+    if (p.stats && lane < 32) {
+      const int64_t w = stat_at(p, b, hk, r);
+      p.stats[w] = m;
+      p.stats[p.B * p.H * p.Lq + w] = sum;
+    }
+  }
+}
+
+// Element d of row r (key head (b, hk)) from its sum, maximum and unscaled value.
+template <typename T>
+__device__ __forceinline__ void put_row(const AttnParams& p, int64_t b, int hk, int64_t r, int d, float value, float m, float sum) {
+  const int64_t g = r / p.Lq, i = r - g * p.Lq, off = b * p.os[0] + i * p.os[1] + (hk * p.G + g) * p.os[2] + d;
+  const float y = sum == 0 ? 0.0f : value / sum;
+  Elem<T>::store(static_cast<T*>(p.o) + off, y);
+  if (p.rest) Elem<T>::store(static_cast<T*>(p.rest) + off, y - Elem<T>::load(static_cast<const T*>(p.o) + off));
+  if (p.stats && d == 0) {
+    const int64_t w = stat_at(p, b, hk, r);
+    p.stats[w] = m;
+    p.stats[p.B * p.H * p.Lq + w] = sum;
+  }
+}
+
+template <typename T, int DP, int QT, int KIND>
+__global__ __launch_bounds__(256) void attn_fwd_few_kernel(AttnParams p) {
+  constexpr int LP = DP == 96 ? 128 : DP, DT = DP / 32, STEPS = RowState<T, DP, QT>::STEPS;
+  constexpr int TILE = 32 * LP * static_cast<int>(sizeof(T)), JOIN = 32 * (DP + 1) * 4;
+  __shared__ __attribute__((aligned(16))) char lds[4 * (TILE > JOIN ? TILE : JOIN)];
+  __shared__ float wm[4][32], wl[4][32];
+  const int64_t bh = blockIdx.x, b = bh / p.Hk;
+  const int hk = static_cast<int>(bh - b * p.Hk), split = blockIdx.y, w = threadIdx.x >> 6, l = threadIdx.x & 63;
+  const int64_t len = attn_len(p, b), j0 = split * p.chunk, n = len < j0 + p.chunk ? len : j0 + p.chunk;
+  if (split && n <= j0) return;
+  RowState<T, DP, QT> st;
+  init_rows<T, DP, QT>(p, st, b, hk, 0);
+  const T* k = static_cast<const T*>(p.k) + b * p.ks[0] + hk * p.ks[2];
+  const T* v = static_cast<const T*>(p.v) + b * p.vs[0] + hk * p.vs[2];
+  char* vt = lds + w * TILE;
+  uint4 ka[STEPS];
+  Staged<T, DP, LP, 32, 64> vr;
+  auto fetch = [&](int64_t j) {
+    const T* row = k + (j + (l & 31)) * p.ks[1];
+#pragma unroll
+    for (int t = 0; t < STEPS; ++t)
+      ka[t] = j + (l & 31) < n ? load_chunk<T>(row, 2 * t + (l >> 5), p.D) : make_uint4(0, 0, 0, 0);
+    vr.load(v + j * p.vs[1], p.vs[1], n - j, p.D, l);
+  };
+  if (j0 + 32 * w < n) fetch(j0 + 32 * w);
+  for (int64_t j = j0 + 32 * w; j < n; j += 128) {
+    f32x16 s[QT][1] = {};
+    Block<T> e[QT][1];
+#pragma unroll
+    for (int t = 0; t < STEPS; ++t)
+#pragma unroll
+      for (int q = 0; q < QT; ++q) s[q][0] = mma_step(T(), ka[t], st.q[q][t], s[q][0]);
+    vr.store(vt, l);                       // the wave's own tile: LDS serves a wave's accesses in order
+    __builtin_amdgcn_wave_barrier();
+    const bool bad = KIND && __any(vr.bad());
+    if (j + 128 < n) fetch(j + 128);
+#pragma unroll
+    for (int q = 0; q < QT; ++q) softmax_blocks<T, DP, QT, KIND, 1>(p, st, q, s[q], e[q], j, n);
+#pragma unroll
+    for (int q = 0; q < QT; ++q) {
+      if (bad) {
+        slow_second<T, LP, DT>(vt, 0, s[q][0], st.o[q]);
+      } else {
+#pragma unroll
+        for (int d = 0; d < DT; ++d) st.o[q][d] = mma_second<LP>(T(), vt, 0, d, e[q][0], st.o[q][d]);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+  float* join = reinterpret_cast<float*>(lds) + w * (JOIN / 4);
+#pragma unroll
+  for (int q = 0; q < QT; ++q) {
+    if (q * 32 >= p.R) break;
+    __syncthreads();
+    const float sum = st.l[q] + __shfl_xor(st.l[q], 32);
+    if (l < 32) { wm[w][l] = KIND ? st.m[q] : st.m[q] * p.c; wl[w][l] = sum; }
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) join[(l & 31) * (DP + 1) + d * 32 + 8 * (e / 4) + 4 * (l >> 5) + e % 4] = st.o[q][d][e];
+    __syncthreads();
+    const int rows = static_cast<int>(p.R - q * 32 < 32 ? p.R - q * 32 : 32);
+    for (int x = threadIdx.x; x < rows * p.D; x += 256) {
+      const int r = x / p.D, d = x - r * p.D;
+      const float m = fmaxf(fmaxf(wm[0][r], wm[1][r]), fmaxf(wm[2][r], wm[3][r])), at = m == kNegInf ? 0.0f : m;
+      float value = 0, total = 0;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const float f = exp2_fast(wm[y][r] - at);
+        total = fmaf(wl[y][r], f, total);
+        value = fmaf(reinterpret_cast<const float*>(lds)[y * (JOIN / 4) + r * (DP + 1) + d], f, value);
+      }
+      const int64_t row = q * 32 + r;
+      if (p.splits > 1) {
+        float* out = p.part + ((split * p.B * p.Hk + bh) * p.R + row) * (p.D + 2);
+        out[d] = value;
+        if (d == 0) { out[p.D] = m; out[p.D + 1] = total; }
+      } else {
+        put_row<T>(p, b, hk, row, d, value, m, total);
+      }
+    }
+  }
+}
+
+// The partial results of a row's splits added up; one wave per row.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_fwd_join_kernel(AttnParams p) {
+  const int64_t rows = p.B * p.Hk * p.R, x = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (x >= rows) return;
+  const int l = threadIdx.x & 63;
+  const int64_t bh = x / p.R, b = bh / p.Hk, len = attn_len(p, b), step = rows * (p.D + 2);
+  int64_t used = (len + p.chunk - 1) / p.chunk;
+  if (used < 1) used = 1;
+  const float* part = p.part + x * (p.D + 2);
+  float m = kNegInf;
+  for (int64_t s = l; s < used; s += 64) m = fmaxf(m, part[s * step + p.D]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  const float at = m == kNegInf ? 0.0f : m;
+  float sum = 0, y[2] = {0, 0};
+  for (int64_t s = 0; s < used; ++s) {
+    const float* row = part + s * step;
+    const float f = exp2_fast(row[p.D] - at);
+    sum = fmaf(row[p.D + 1], f, sum);
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+      if (l + 64 * c < p.D) y[c] = fmaf(row[l + 64 * c], f, y[c]);
+  }
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+    if (l + 64 * c < p.D) put_row<T>(p, b, static_cast<int>(bh - b * p.Hk), x - bh * p.R, l + 64 * c, y[c], m, sum);
+}
+
+// How a call is laid out. Few rows: every workgroup has them all. Else tiles of 128 or 256 rows.
+struct FwdPlan {
+  bool few;
+  int qt, splits;
+  int64_t tiles, chunk;
+};
+
+static FwdPlan fwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t D, int dtype) {
+  FwdPlan f;
+  const int64_t R = H / Hk * Lq;
+  f.few = R <= (dtype == FOVI_BF16 && D <= 64 ? 64 : 32);      // (two blocks of rows need too many registers else)
+  if (f.few) {
+    f.qt = R <= 32 ? 1 : 2;
+    f.tiles = 1;
+  } else {
+    f.qt = D <= 64 && R > 128 ? 2 : 1;
+    f.tiles = (R + 128 * f.qt - 1) / (128 * f.qt);
+  }
+  // about four workgroups a compute unit (few rows), two (tiles), each with at least 256 states
+  const int64_t groups = B * Hk * f.tiles, want = f.few ? 1024 : 512;
+  int64_t splits = groups > 0 ? want / groups : 1;
+  if (splits > (Lk + 255) / 256) splits = (Lk + 255) / 256;
+  if (splits > 1024) splits = 1024;
+  if (splits < 1) splits = 1;
+  f.chunk = ((Lk + splits - 1) / splits + 127) / 128 * 128;
+  if (f.chunk < 128) f.chunk = 128;
+  f.splits = static_cast<int>(Lk ? (Lk + f.chunk - 1) / f.chunk : 1);
+  return f;
+}
+
+int64_t attn_fwd_workspace(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t D, int dtype) {
+  const FwdPlan f = fwd_plan(B, Lq, Lk, H, Hk, D, dtype);
+  return f.splits > 1 ? f.splits * B * H * Lq * (D + 2) * 4 : 0;
+}
+
+template <typename T, int DP, int KIND>
+static void fwd_launch(const AttnParams& p, const FwdPlan& f, hipStream_t s) {
+  const int64_t all = p.B * p.Hk * f.tiles;
+  if (f.few) {
+    const dim3 grid(static_cast<unsigned>(all), static_cast<unsigned>(f.splits));
+    if (f.qt == 1) attn_fwd_few_kernel<T, DP, 1, KIND><<<grid, 256, 0, s>>>(p);
+    else if constexpr (DP <= 64 && sizeof(T) == 2) attn_fwd_few_kernel<T, DP, 2, KIND><<<grid, 256, 0, s>>>(p);
+  } else {
+    const dim3 grid(static_cast<unsigned>((all + 7) / 8 * 8), static_cast<unsigned>(f.splits));
+    if (f.qt == 1) attn_fwd_tile_kernel<T, DP, 1, KIND><<<grid, 256, 0, s>>>(p);
+    else if constexpr (DP <= 64) attn_fwd_tile_kernel<T, DP, 2, KIND><<<grid, 256, 0, s>>>(p);
+  }
+}
+
+template <typename T>
+static int fwd_type(AttnParams& p, hipStream_t s) {
+  const FwdPlan f = fwd_plan(p.B, p.Lq, p.Lk, p.H, p.Hk, p.D, sizeof(T) == 2 ? FOVI_BF16 : FOVI_F32);
+  p.splits = f.splits;
+  p.chunk = f.chunk;
+  p.tiles = f.tiles;
+  if (p.kind) {
+    if (p.D <= 32) fwd_launch<T, 32, 1>(p, f, s);
+    else if (p.D <= 64) fwd_launch<T, 64, 1>(p, f, s);
+    else if (p.D <= 96) fwd_launch<T, 96, 1>(p, f, s);
+    else fwd_launch<T, 128, 1>(p, f, s);
+  } else {
+    if (p.D <= 32) fwd_launch<T, 32, 0>(p, f, s);
+    else if (p.D <= 64) fwd_launch<T, 64, 0>(p, f, s);
+    else if (p.D <= 96) fwd_launch<T, 96, 0>(p, f, s);
+    else fwd_launch<T, 128, 0>(p, f, s);
+  }
+  if (check_launch("fovi_attention_fwd")) return 1;
+  if (f.splits > 1) {
+    const int64_t rows = p.B * p.Hk * p.R;
+    attn_fwd_join_kernel<T><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, s>>>(p);
+    return check_launch("fovi_attention_fwd");
+  }
+  return 0;
+}
+
+int attn_fwd_launch(AttnParams& p, int dtype, hipStream_t s) {
+  return dtype == FOVI_BF16 ? fwd_type<uint16_t>(p, s) : fwd_type<float>(p, s);
+}
+
+}  // namespace fovi
