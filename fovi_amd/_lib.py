@@ -382,6 +382,12 @@ def stream_handle(device=None):
     return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+def stream_of(t):
+    """The current stream of a GPU tensor's device as an integer handle: what ``stream_handle`` gives,
+    without the Stream object (2 us of a small call's 10)."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
 def check(rc: int, what: str):
     if rc != 0:
         msg = load().fovi_last_error().decode(errors="replace")
@@ -393,3 +399,14 @@ def require_device(*tensors):
         if t is not None and not t.is_cuda:
             raise RuntimeError("fovi_amd HIP kernels need GPU tensors (got a CPU tensor); "
                                "there is no CPU fallback")
+
+
+@torch.autograd.function.once_differentiable
+def _once(ctx, backward, *grads):
+    return backward(ctx, *grads)
+
+
+def differentiated_once(backward, ctx, *grads):
+    """``backward(ctx, *grads)`` of an autograd function whose gradients have none: a second
+    differentiation raises. The guard that does it is left out where no graph is being made."""
+    return _once(ctx, backward, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)

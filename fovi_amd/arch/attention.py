@@ -19,35 +19,42 @@ __all__ = ["cross_attention"]
 
 def _strides(t):
     """Strides of batch, token and head, 0 along dimensions of one."""
+    s0, s1, s2, _ = t.stride()
+    if (s0 | s1 | s2) & 7 == 0:
+        return s0, s1, s2
     return tuple(s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride()[:3]))
 
 
+def _whole(t):
+    """Whether the kernels can read (or write) ``t`` where it is: heads of whole 16-byte pieces at
+    aligned addresses."""
+    rest = (7 if t.dtype == torch.bfloat16 else 3)
+    s0, s1, s2 = _strides(t)
+    return t.stride(3) == 1 and (s0 | s1 | s2 | t.shape[3]) & rest == 0 and t.data_ptr() & 15 == 0
+
+
 def _pieces(t):
-    """``t`` as the kernels read it: heads of whole 16-byte pieces at aligned addresses. Other layouts
-    are copied, heads padded with zeros to the next piece (which no score or sum notices)."""
-    per = 16 // t.element_size()
-    extra = -t.shape[3] % per
+    """``t`` as the kernels read it. Other layouts are copied, heads padded with zeros to the next
+    piece (which no score or sum notices)."""
+    if _whole(t):
+        return t
+    extra = -t.shape[3] % (16 // t.element_size())
     if extra:
         return torch.nn.functional.pad(t, (0, extra))
-    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and not any(s % per for s in _strides(t)):
-        return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
 def _like(t):
     """An output of ``t``'s shape, in its layout where that is dense."""
     y = torch.empty_like(t)
-    per = 16 // t.element_size()
-    if y.stride(3) == 1 and not any(s % per for s in _strides(y)):
-        return y
-    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    return y if _whole(y) else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _args(a, q, k, v, kv_lengths, mask, scale):
     a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
     a.dtype = _lib.dtype_code(q.dtype)
     a.batch, a.q_len, a.heads, a.head_dim = q.shape
-    a.kv_len, a.kv_heads = k.shape[1], k.shape[2]
+    _, a.kv_len, a.kv_heads, _ = k.shape
     a.q_stride[:], a.k_stride[:], a.v_stride[:] = _strides(q), _strides(k), _strides(v)
     if mask is not None:
         a.mask_kind = _lib.MASK_KEEP if mask.dtype == torch.bool else _lib.MASK_BIAS
@@ -61,8 +68,6 @@ def _args(a, q, k, v, kv_lengths, mask, scale):
 def _workspace(a, size, device):
     """The call's workspace, kept alive by the caller until the launch."""
     n = size(a.batch, a.q_len, a.kv_len, a.heads, a.kv_heads, a.head_dim, a.dtype)
-    if n < 0:
-        raise RuntimeError("cross_attention: " + _lib.load().fovi_last_error().decode())
     if n == 0:
         return None
     work = torch.empty(n, dtype=torch.uint8, device=device)
@@ -71,12 +76,15 @@ def _workspace(a, size, device):
 
 
 def _forward(q, k, v, kv_lengths, mask, scale, keep):
-    out = _like(q)
-    stats = torch.empty(2, q.shape[0], q.shape[2], q.shape[1], dtype=torch.float32, device=q.device) if keep else None
-    # what the rounding of a bf16 output takes away, for the backward's differences
-    rest = torch.empty_strided(out.shape, out.stride(), dtype=out.dtype, device=q.device) \
-        if keep and q.dtype == torch.bfloat16 else None
-    if out.numel() == 0:
+    """The output, and with ``keep`` what the backward needs: the rows' statistics and what the
+    rounding of a bf16 output takes away."""
+    out, stats, rest = _like(q), None, None
+    b, n, h, _ = q.shape
+    if keep:
+        stats = torch.empty(2, b, h, n, dtype=torch.float32, device=q.device)
+        if q.dtype == torch.bfloat16:
+            rest = torch.empty_strided(out.shape, out.stride(), dtype=out.dtype, device=q.device)
+    if b * n == 0:
         return out, stats, rest
     lib = _lib.load()
     a = _lib.AttentionArgs()
@@ -88,9 +96,31 @@ def _forward(q, k, v, kv_lengths, mask, scale, keep):
         if rest is not None:
             a.out_rest = rest.data_ptr()
     work = _workspace(a, lib.fovi_attention_fwd_workspace_bytes, q.device)
-    _lib.check(lib.fovi_attention_fwd(a, _lib.stream_handle(q.device)), "fovi_attention_fwd")
+    _lib.check(lib.fovi_attention_fwd(a, _lib.stream_of(q)), "fovi_attention_fwd")
     del work
     return out, stats, rest
+
+
+def _backward(ctx, dout):
+    q, k, v, kv_lengths, mask, out, stats, rest = ctx.saved_tensors
+    dq, dk, dv = _like(q), _like(k), _like(v)
+    if q.numel() == 0:
+        return dq, dk.zero_(), dv.zero_(), None, None, None
+    dout = _pieces(dout if dout.dtype == q.dtype else dout.to(q.dtype))
+    lib = _lib.load()
+    a = _lib.AttentionBwdArgs()
+    f = a.fwd
+    _args(f, q, k, v, kv_lengths, mask, ctx.scale)
+    f.out, f.stats, a.dout = out.data_ptr(), stats.data_ptr(), dout.data_ptr()
+    if rest is not None:
+        f.out_rest = rest.data_ptr()
+    a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+    f.out_stride[:], a.dout_stride[:] = _strides(out), _strides(dout)
+    a.dq_stride[:], a.dk_stride[:], a.dv_stride[:] = _strides(dq), _strides(dk), _strides(dv)
+    work = _workspace(f, lib.fovi_attention_bwd_workspace_bytes, q.device)
+    _lib.check(lib.fovi_attention_bwd(a, _lib.stream_of(q)), "fovi_attention_bwd")
+    del work
+    return dq, dk, dv, None, None, None
 
 
 class _CrossAttentionFn(torch.autograd.Function):
@@ -104,26 +134,8 @@ class _CrossAttentionFn(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, kv_lengths, mask, out, stats, rest = ctx.saved_tensors
-        dq, dk, dv = _like(q), _like(k), _like(v)
-        if q.numel() == 0:
-            return dq, dk.zero_(), dv.zero_(), None, None, None
-        dout = _pieces(dout.to(q.dtype))
-        lib = _lib.load()
-        a = _lib.AttentionBwdArgs()
-        _args(a.fwd, q, k, v, kv_lengths, mask, ctx.scale)
-        a.fwd.out, a.fwd.stats, a.dout = out.data_ptr(), stats.data_ptr(), dout.data_ptr()
-        if rest is not None:
-            a.fwd.out_rest = rest.data_ptr()
-        a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-        a.fwd.out_stride[:], a.dout_stride[:] = _strides(out), _strides(dout)
-        a.dq_stride[:], a.dk_stride[:], a.dv_stride[:] = _strides(dq), _strides(dk), _strides(dv)
-        work = _workspace(a.fwd, lib.fovi_attention_bwd_workspace_bytes, q.device)
-        _lib.check(lib.fovi_attention_bwd(a, _lib.stream_handle(q.device)), "fovi_attention_bwd")
-        del work
-        return dq, dk, dv, None, None, None
+        return _lib.differentiated_once(_backward, ctx, dout)
 
 
 def cross_attention(q, k, v, kv_lengths=None, mask=None, scale=None):
@@ -165,7 +177,8 @@ def cross_attention(q, k, v, kv_lengths=None, mask=None, scale=None):
             raise ValueError("cross_attention: kv_lengths must be on the device of q")
         if kv_lengths.dtype != torch.int32:
             kv_lengths = kv_lengths.clamp(0, lk).to(torch.int32)
-        kv_lengths = kv_lengths.contiguous()
+        if kv_lengths.stride(0) != 1:
+            kv_lengths = kv_lengths.contiguous()
     if mask is not None:
         if mask.requires_grad:
             raise ValueError("cross_attention: no gradient for the mask")

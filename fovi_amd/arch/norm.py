@@ -19,9 +19,10 @@ __all__ = ["layer_norm", "LayerNorm"]
 def _rows(x):
     """``(x, rows0, rows1, stride0, stride1)``: the leading dimensions as two, ``x`` copied where
     its channels are not adjacent or more than two row strides remain."""
-    if x.dim() == 2 and x.stride(1) == 1:
-        return x, 1, x.shape[0], 0, x.stride(0)
-    if x.stride(-1) == 1 or x.shape[-1] == 1:
+    c = x.shape[-1]
+    if x.is_contiguous():
+        return x, 1, x.numel() // c, 0, c
+    if x.stride(-1) == 1 or c == 1:
         dims = []
         for n, s in zip(x.shape[:-1], x.stride()[:-1]):
             if n == 1:
@@ -33,84 +34,86 @@ def _rows(x):
         if len(dims) <= 2:
             (n0, s0), (n1, s1) = ([[1, 0]] * (2 - len(dims)) + dims)
             return x, n0, n1, s0, s1
-    x = x.contiguous()
+    return x.contiguous(), 1, x.numel() // c, 0, c
+
+
+def _forward(x, weight, bias, eps, stats):
+    xr, n0, n1, s0, s1 = _rows(x)
     c = x.shape[-1]
-    return x, 1, x.numel() // c, 0, c
-
-
-def _args(x, weight, bias, eps):
-    x, n0, n1, s0, s1 = _rows(x)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     a = _lib.LayerNormArgs()
-    a.x, a.dtype = x.data_ptr(), _lib.dtype_code(x.dtype)
-    a.rows0, a.rows1, a.channels = n0, n1, x.shape[-1]
+    a.x, a.dtype, a.rows0, a.rows1, a.channels, a.eps = xr.data_ptr(), _lib.dtype_code(x.dtype), n0, n1, c, eps
     a.x_stride[:] = (s0, s1)
-    param = weight if weight is not None else bias
-    a.p_dtype = _lib.F32 if param is None else _lib.dtype_code(param.dtype)
     if weight is not None:
-        a.weight = weight.data_ptr()
+        a.weight, a.p_dtype = weight.data_ptr(), _lib.dtype_code(weight.dtype)
     if bias is not None:
-        a.bias = bias.data_ptr()
-    a.eps = eps
-    return a, x
+        a.bias, a.p_dtype = bias.data_ptr(), _lib.dtype_code(bias.dtype)
+    a.y = y.data_ptr()
+    a.y_stride[:] = (n1 * c, c)
+    if stats is not None:
+        a.mean, a.rstd = stats.data_ptr(), stats.data_ptr() + 4 * n0 * n1
+    lib = _lib.load()
+    _lib.check(lib.fovi_layer_norm_fwd(a, _lib.stream_of(x)), "fovi_layer_norm_fwd")
+    return y
+
+
+def _backward(ctx, dy):
+    x, weight, bias, stats = ctx.saved_tensors
+    need_x, need_w, need_b = ctx.needs_input_grad[:3]
+    c = x.shape[-1]
+    xr, n0, n1, s0, s1 = _rows(x)
+    if dy.dtype != x.dtype:
+        dy = dy.to(x.dtype)
+    dyr, m0, m1, t0, t1 = _rows(dy)
+    if (m0, m1) != (n0, n1):            # rows of x and dy in the same two levels; one splits into any two
+        if m0 == 1:
+            t0 = n1 * t1
+        elif n0 == 1:
+            n0, n1, s0 = m0, m1, m1 * s1
+        else:
+            dyr, t0, t1 = dy.contiguous(), n1 * c, c
+    a = _lib.LayerNormArgs()
+    a.x, a.dtype, a.rows0, a.rows1, a.channels, a.eps = xr.data_ptr(), _lib.dtype_code(x.dtype), n0, n1, c, ctx.eps
+    a.x_stride[:] = (s0, s1)
+    a.dy = dyr.data_ptr()
+    a.dy_stride[:] = (t0, t1)
+    a.mean, a.rstd = stats.data_ptr(), stats.data_ptr() + 4 * n0 * n1
+    dx = dw = db = work = None
+    lib = _lib.load()
+    if need_x:
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        a.dx = dx.data_ptr()
+        a.dx_stride[:] = (n1 * c, c)
+    if weight is not None:
+        a.weight, a.p_dtype = weight.data_ptr(), _lib.dtype_code(weight.dtype)
+        if need_w:
+            dw = torch.empty_like(weight)
+            a.dweight = dw.data_ptr()
+    if need_b:
+        db = torch.empty_like(bias)
+        a.dbias, a.p_dtype = db.data_ptr(), _lib.dtype_code(bias.dtype)
+    if need_w or need_b:
+        nbytes = lib.fovi_layer_norm_workspace_bytes(n0 * n1, c, a.dtype)
+        work = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        a.workspace, a.workspace_bytes = work.data_ptr(), nbytes
+    _lib.check(lib.fovi_layer_norm_bwd(a, _lib.stream_of(x)), "fovi_layer_norm_bwd")
+    return dx, dw, db, None
 
 
 class _LayerNormFn(torch.autograd.Function):
     """Forward ``fovi_layer_norm_fwd`` with the rows' statistics kept; backward ``fovi_layer_norm_bwd``."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, eps, keep):
-        a, xr = _args(x, weight, bias, eps)
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        c = x.shape[-1]
-        a.y = y.data_ptr()
-        a.y_stride[:] = (a.rows1 * c, c)
-        if keep:
-            stats = torch.empty(2, a.rows0 * a.rows1, dtype=torch.float32, device=x.device)
-            a.mean, a.rstd = stats.data_ptr(), stats.data_ptr() + 4 * stats.shape[1]
-            ctx.save_for_backward(x, weight, bias, stats)
-            ctx.eps = eps
-        _lib.check(_lib.load().fovi_layer_norm_fwd(a, _lib.stream_handle(x.device)), "fovi_layer_norm_fwd")
+    def forward(ctx, x, weight, bias, eps):
+        stats = torch.empty(2, x.numel() // x.shape[-1], dtype=torch.float32, device=x.device)
+        y = _forward(x, weight, bias, eps, stats)
+        ctx.save_for_backward(x, weight, bias, stats)
+        ctx.eps = eps
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, bias, stats = ctx.saved_tensors
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        a, xr = _args(x, weight, bias, ctx.eps)
-        # rows of x and dy in the same two levels; the statistics are in row order
-        dy = dy.to(x.dtype)
-        dyr, n0, n1, s0, s1 = _rows(dy)
-        if (n0, n1) != (a.rows0, a.rows1):
-            if n0 == 1:                              # one level splits into any two
-                n0, n1, s0 = a.rows0, a.rows1, a.rows1 * s1
-            elif a.rows0 == 1:
-                a.rows0, a.rows1 = n0, n1
-                a.x_stride[0] = n1 * a.x_stride[1]
-            else:
-                dyr = dy.contiguous()
-                n0, n1, s0, s1 = a.rows0, a.rows1, a.rows1 * x.shape[-1], x.shape[-1]
-        a.dy = dyr.data_ptr()
-        a.dy_stride[:] = (s0, s1)
-        a.mean, a.rstd = stats.data_ptr(), stats.data_ptr() + 4 * stats.shape[1]
-        dx = dw = db = None
-        lib = _lib.load()
-        if need_x:
-            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            a.dx = dx.data_ptr()
-            a.dx_stride[:] = (n1 * x.shape[-1], x.shape[-1])
-        if need_w:
-            dw = torch.empty_like(weight, memory_format=torch.contiguous_format)
-            a.dweight = dw.data_ptr()
-        if need_b:
-            db = torch.empty_like(bias, memory_format=torch.contiguous_format)
-            a.dbias = db.data_ptr()
-        if need_w or need_b:
-            nbytes = lib.fovi_layer_norm_workspace_bytes(n0 * n1, x.shape[-1], a.dtype)
-            work = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-            a.workspace, a.workspace_bytes = work.data_ptr(), nbytes
-        _lib.check(lib.fovi_layer_norm_bwd(a, _lib.stream_handle(x.device)), "fovi_layer_norm_bwd")
-        return dx, dw, db, None, None
+        return _lib.differentiated_once(_backward, ctx, dy)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
@@ -144,9 +147,10 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
         return y
     weight = weight if weight is None else weight.contiguous()
     bias = bias if bias is None else bias.contiguous()
-    keep = torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                        or (bias is not None and bias.requires_grad))
-    return _LayerNormFn.apply(x, weight, bias, float(eps), keep)
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
+        return _LayerNormFn.apply(x, weight, bias, float(eps))
+    return _forward(x, weight, bias, eps, None)
 
 
 class LayerNorm(nn.Module):

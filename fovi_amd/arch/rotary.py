@@ -22,26 +22,35 @@ _PAIRINGS = {"half": _lib.PAIR_HALF, "adjacent": _lib.PAIR_ADJACENT}
 
 
 def _launch(x, positions, freqs, ends, pairing, inverse):
-    if x.stride(3) != 1 and x.shape[3] != 1:
+    b, n, h, d = x.shape
+    x0, x1, x2, x3 = x.stride()
+    if x3 != 1:
         x = x.contiguous()
+        x0, x1, x2, _ = x.stride()
     y = torch.empty_like(x)              # a dense layout of x is kept (heads before tokens, say)
-    if y.numel() == 0:
+    if b * n * h == 0:
         return y
-    if y.stride(3) != 1:
+    y0, y1, y2, y3 = y.stride()
+    if y3 != 1:
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        y0, y1, y2, _ = y.stride()
     a = _lib.RotaryArgs()
     a.x, a.dtype, a.pairing = x.data_ptr(), _lib.dtype_code(x.dtype), pairing
-    a.batch, a.length, a.heads, a.head_dim = x.shape
-    a.x_stride[:] = x.stride()[:3]
+    a.batch, a.length, a.heads, a.head_dim = b, n, h, d
+    a.x_stride[:] = (x0, x1, x2)
     a.positions, a.freqs = positions.data_ptr(), freqs.data_ptr()
     a.pos_stride[:] = positions.stride()[:2] if positions.dim() == 3 else (0, positions.stride(0))
     a.n_axes, a.inverse = len(ends), inverse
-    for i, e in enumerate(ends):
-        a.section_end[i] = e
+    a.section_end[:len(ends)] = ends
     a.y = y.data_ptr()
-    a.y_stride[:] = y.stride()[:3]
-    _lib.check(_lib.load().fovi_rotary(a, _lib.stream_handle(x.device)), "fovi_rotary")
+    a.y_stride[:] = (y0, y1, y2)
+    _lib.check(_lib.load().fovi_rotary(a, _lib.stream_of(x)), "fovi_rotary")
     return y
+
+
+def _backward(ctx, dy):
+    positions, freqs = ctx.saved_tensors
+    return _launch(dy, positions, freqs, ctx.ends, ctx.pairing, 1), None, None, None, None
 
 
 class _RotaryFn(torch.autograd.Function):
@@ -54,10 +63,8 @@ class _RotaryFn(torch.autograd.Function):
         return _launch(x, positions, freqs, ends, pairing, 0)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        positions, freqs = ctx.saved_tensors
-        return _launch(dy, positions, freqs, ctx.ends, ctx.pairing, 1), None, None, None, None
+        return _lib.differentiated_once(_backward, ctx, dy)
 
 
 def rotary(x, positions, freqs, sections, pairing="half"):
