@@ -3,10 +3,13 @@
 //   h = (x - mean) * rstd, y = h * w + b
 //   dx = rstd * (g - mean(g) - h * mean(g * h)), g = dy * w; dw = sum dy * h; db = sum dy
 //
-// One workgroup per row; the row is read once for the mean, once for the centred squares (no
-// cancellation between large sums) and once to write. The weight gradients are summed by columns:
-// a workgroup takes 64 columns of a chunk of rows into fp32 partial sums, which a second launch
-// adds in a fixed order, so results do not change from run to run.
+// Bound by memory. A row is read once into the registers of a group of lanes (16, 64 or 256), which
+// takes the mean and then the centred squares from there (no cancellation between large sums), and
+// writes from there too. Groups walk the rows with the parameters in registers. The backward keeps
+// the sums of dy * h and dy of its channels over all its rows in registers as well, so that x and dy
+// are read once for all three gradients; each workgroup leaves one row of partial sums, and a second
+// launch adds those in a fixed order (no atomics: results do not change from run to run).
+// Rows too wide for registers go through kernels of a workgroup per row that read them again.
 #include "common.h"
 
 namespace fovi {
@@ -34,6 +37,185 @@ __device__ __forceinline__ float block_sum(float v, float* sh) {
   if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
   __syncthreads();
   return (sh[0] + sh[1]) + (sh[2] + sh[3]);
+}
+
+// VEC adjacent channels from c on as floats; zeros from C on. VEC > 1: 16 bytes, C a multiple of VEC.
+template <typename T, int VEC>
+__device__ __forceinline__ void norm_load(const T* row, int64_t c, int64_t C, float (&v)[VEC]) {
+  if (VEC == 1) {
+    v[0] = c < C ? Elem<T>::load(row + c) : 0.0f;
+    return;
+  }
+  const uint4 u = c < C ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
+  T e[16 / sizeof(T)];
+  __builtin_memcpy(e, &u, 16);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) v[i] = Elem<T>::load(e + i);
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void norm_store(T* row, int64_t c, int64_t C, const float (&v)[VEC]) {
+  if (c >= C) return;
+  if (VEC == 1) {
+    Elem<T>::store(row + c, v[0]);
+    return;
+  }
+  T e[16 / sizeof(T)];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) Elem<T>::store(e + i, v[i]);
+  uint4 u;
+  __builtin_memcpy(&u, e, 16);
+  *reinterpret_cast<uint4*>(row + c) = u;
+}
+
+// Sum over a group of LANES; every lane gets the result.
+template <int LANES>
+__device__ __forceinline__ float group_sum(float v, float* sh) {
+  if (LANES == 256) return block_sum(v, sh);
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+
+template <typename T, int VEC, int LANES, int NV>
+__global__ __launch_bounds__(256) void norm_fwd_rows_kernel(NormParams p) {
+  __shared__ float sh[4];
+  const int lane = threadIdx.x % LANES;
+  float w[NV][VEC], b[NV][VEC];
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const int64_t c = static_cast<int64_t>(lane + k * LANES) * VEC + i;
+      w[k][i] = c < p.C ? norm_param(p.w, c, p.p_bf16, 1.0f) : 0.0f;
+      b[k][i] = c < p.C ? norm_param(p.b, c, p.p_bf16, 0.0f) : 0.0f;
+    }
+  const float n = 1.0f / static_cast<float>(p.C);
+  const int64_t rows = p.rows0 * p.rows1, step = static_cast<int64_t>(gridDim.x) * (256 / LANES);
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES; row < rows; row += step) {
+    const int64_t i0 = p.rows0 == 1 ? 0 : row / p.rows1, i1 = row - i0 * p.rows1;
+    const T* xr = static_cast<const T*>(p.x) + i0 * p.xs[0] + i1 * p.xs[1];
+    T* yr = static_cast<T*>(p.y) + i0 * p.ys[0] + i1 * p.ys[1];
+    float x[NV][VEC], s = 0;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) norm_load<T, VEC>(xr, static_cast<int64_t>(lane + k * LANES) * VEC, p.C, x[k]);
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) s += x[k][i];
+    const float mean = group_sum<LANES>(s, sh) * n;
+    s = 0;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const bool in = static_cast<int64_t>(lane + k * LANES) * VEC < p.C;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        x[k][i] = in ? x[k][i] - mean : 0.0f;
+        s = fmaf(x[k][i], x[k][i], s);
+      }
+    }
+    const float rstd = 1.0f / sqrtf(group_sum<LANES>(s, sh) * n + p.eps);
+    if (lane == 0 && p.mean) { p.mean[row] = mean; p.rstd[row] = rstd; }
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      float y[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) y[i] = fmaf(x[k][i] * rstd, w[k][i], b[k][i]);
+      norm_store<T, VEC>(yr, static_cast<int64_t>(lane + k * LANES) * VEC, p.C, y);
+    }
+  }
+}
+
+// dx of the rows and, with `partial`, the workgroup's sums of dy * h and dy: partial[(block * 2 + {0, 1}) * C + c].
+template <typename T, int VEC, int LANES, int NV>
+__global__ __launch_bounds__(256) void norm_bwd_rows_kernel(NormParams p, float* partial) {
+  __shared__ float sh[4];
+  const int lane = threadIdx.x % LANES;
+  float w[NV][VEC], dw[NV][VEC], db[NV][VEC];
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const int64_t c = static_cast<int64_t>(lane + k * LANES) * VEC + i;
+      w[k][i] = c < p.C ? norm_param(p.w, c, p.p_bf16, 1.0f) : 0.0f;
+      dw[k][i] = db[k][i] = 0;
+    }
+  const float n = 1.0f / static_cast<float>(p.C);
+  const int64_t rows = p.rows0 * p.rows1, step = static_cast<int64_t>(gridDim.x) * (256 / LANES);
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES; row < rows; row += step) {
+    const int64_t i0 = p.rows0 == 1 ? 0 : row / p.rows1, i1 = row - i0 * p.rows1;
+    const T* xr = static_cast<const T*>(p.x) + i0 * p.xs[0] + i1 * p.xs[1];
+    const T* gr = static_cast<const T*>(p.dy) + i0 * p.dys[0] + i1 * p.dys[1];
+    const float mean = p.mean[row], rstd = p.rstd[row];
+    float h[NV][VEC], g[NV][VEC], sg = 0, sgh = 0;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int64_t c = static_cast<int64_t>(lane + k * LANES) * VEC;
+      norm_load<T, VEC>(xr, c, p.C, h[k]);
+      norm_load<T, VEC>(gr, c, p.C, g[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const bool in = static_cast<int64_t>(lane + k * LANES) * VEC < p.C;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        h[k][i] = in ? (h[k][i] - mean) * rstd : 0.0f;
+        dw[k][i] = fmaf(g[k][i], h[k][i], dw[k][i]);
+        db[k][i] += g[k][i];
+        g[k][i] *= w[k][i];
+        sg += g[k][i];
+        sgh = fmaf(g[k][i], h[k][i], sgh);
+      }
+    }
+    if (!p.dx) continue;
+    sg = group_sum<LANES>(sg, sh) * n;
+    sgh = group_sum<LANES>(sgh, sh) * n;
+    T* dxr = static_cast<T*>(p.dx) + i0 * p.dxs[0] + i1 * p.dxs[1];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      float dx[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) dx[i] = rstd * (g[k][i] - sg - h[k][i] * sgh);
+      norm_store<T, VEC>(dxr, static_cast<int64_t>(lane + k * LANES) * VEC, p.C, dx);
+    }
+  }
+  if (!partial) return;
+  float* out = partial + static_cast<int64_t>(blockIdx.x) * 2 * p.C;
+  if (LANES == 256) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int64_t c = static_cast<int64_t>(lane + k * LANES) * VEC;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (c + i < p.C) { out[c + i] = dw[k][i]; out[p.C + c + i] = db[k][i]; }
+    }
+    return;
+  }
+  // the groups of a wave by shuffles, the waves through LDS
+  constexpr int WIDTH = LANES * NV * VEC;
+  extern __shared__ float sums[];                    // [4][2][WIDTH]
+  const int wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      float a = dw[k][i], c = db[k][i];
+#pragma unroll
+      for (int o = 32; o >= LANES; o >>= 1) {
+        a += __shfl_xor(a, o);
+        c += __shfl_xor(c, o);
+      }
+      const int at = (lane + k * LANES) * VEC + i;
+      if ((threadIdx.x & 63) < LANES) {
+        sums[(wave * 2) * WIDTH + at] = a;
+        sums[(wave * 2 + 1) * WIDTH + at] = c;
+      }
+    }
+  __syncthreads();
+  for (int x = threadIdx.x; x < 2 * WIDTH; x += 256) {
+    const int which = x / WIDTH, at = x - which * WIDTH;
+    if (at < p.C)
+      out[which * p.C + at] = (sums[x] + sums[2 * WIDTH + x]) + (sums[4 * WIDTH + x] + sums[6 * WIDTH + x]);
+  }
 }
 
 template <typename T>
@@ -111,24 +293,54 @@ __global__ __launch_bounds__(256) void norm_dw_kernel(NormParams p, int64_t per,
   }
 }
 
-// dweight[c], dbias[c]: the partial sums added up; workgroup: 16 columns by 16 chunks at a time
+// dweight[c], dbias[c]: the partial sums added up; workgroup: 8 columns by 32 partial rows at a time
 __global__ __launch_bounds__(256) void norm_dw_join_kernel(const float* partial, int64_t chunks, int64_t C, void* dw,
                                                            void* db, int p_bf16) {
-  __shared__ float sh[256];
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x & 15);
+  __shared__ float sh[4][8];
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x & 7);
   void* out = blockIdx.y ? db : dw;
   if (!out) return;
   float s = 0;
-  if (c < C)
-    for (int64_t q = threadIdx.x >> 4; q < chunks; q += 16) s += partial[(q * 2 + blockIdx.y) * C + c];
-  sh[threadIdx.x] = s;
-  __syncthreads();
-  if (threadIdx.x >= 16 || c >= C) return;
-  float t = 0;
+  if (c < C) {
+#pragma unroll 4
+    for (int64_t q = threadIdx.x >> 3; q < chunks; q += 32) s += partial[(q * 2 + blockIdx.y) * C + c];
+  }
 #pragma unroll
-  for (int i = 0; i < 16; ++i) t += sh[threadIdx.x + 16 * i];
+  for (int o = 32; o >= 8; o >>= 1) s += __shfl_xor(s, o);
+  if ((threadIdx.x & 63) < 8) sh[threadIdx.x >> 6][threadIdx.x & 7] = s;
+  __syncthreads();
+  if (threadIdx.x >= 8 || c >= C) return;
+  const float t = (sh[0][threadIdx.x] + sh[1][threadIdx.x]) + (sh[2][threadIdx.x] + sh[3][threadIdx.x]);
   if (p_bf16) static_cast<uint16_t*>(out)[c] = f32_to_bf16_bits(t);
   else static_cast<float*>(out)[c] = t;
+}
+
+// The shape of a call: VEC channels a load (16 bytes, or one where rows or widths are not whole
+// pieces), the lanes of a row and the loads a lane holds; nv 0: too wide for registers. Rows of up to 64
+// pieces take 16 lanes (4 rows a wave: a shorter reduction, no idle lanes at 48 pieces), unless
+// there are too few rows to fill the card that way.
+struct NormPlan { bool vec; int lanes, nv; };
+
+static NormPlan norm_plan(int64_t rows, int64_t C, int es, bool aligned) {
+  NormPlan f;
+  f.vec = aligned && C * es % 16 == 0;
+  const int64_t n = f.vec ? C * es / 16 : C;
+  if (n <= 64) {
+    f.lanes = rows >= 4096 || !f.vec ? 16 : 64;
+    f.nv = static_cast<int>((n + f.lanes - 1) / f.lanes);
+  } else if (f.vec) {
+    f.lanes = n <= 256 ? 64 : 256;
+    f.nv = n <= 1024 ? static_cast<int>((n + f.lanes - 1) / f.lanes) : 0;
+  } else {
+    f.lanes = n <= 1024 ? 64 : 256;
+    f.nv = n <= 128 ? 2 : n <= 256 ? 4 : n <= 512 ? 8 : n <= 1024 ? 16 : n <= 2048 ? 8 : n <= 4096 ? 16 : 0;
+  }
+  return f;
+}
+
+static int64_t norm_groups(int64_t rows, const NormPlan& f, int64_t most) {
+  const int64_t per = 256 / f.lanes, n = (rows + per - 1) / per;
+  return n < most ? n : most;
 }
 
 static int64_t norm_chunks(int64_t rows, int64_t C) {
@@ -136,6 +348,65 @@ static int64_t norm_chunks(int64_t rows, int64_t C) {
   int64_t chunks = (1024 + cols - 1) / cols;        // about four workgroups a compute unit
   if (chunks > (rows + 15) / 16) chunks = (rows + 15) / 16;
   return chunks < 1 ? 1 : chunks;
+}
+
+// Calls fn<T, VEC, LANES, NV>; false where the plan has no such kernel.
+#define FOVI_NORM_CASES(CALL)                                                                        \
+  if (f.vec) {                                                                                       \
+    constexpr int V = 16 / sizeof(T);                                                                \
+    if (f.lanes == 16) {                                                                             \
+      if (f.nv == 1) CALL(V, 16, 1) else if (f.nv == 2) CALL(V, 16, 2) else if (f.nv == 3) CALL(V, 16, 3) else CALL(V, 16, 4) \
+    } else if (f.lanes == 64) {                                                                      \
+      if (f.nv == 1) CALL(V, 64, 1) else if (f.nv == 2) CALL(V, 64, 2) else if (f.nv == 3) CALL(V, 64, 3) else CALL(V, 64, 4) \
+    } else {                                                                                         \
+      if (f.nv == 2) CALL(V, 256, 2) else if (f.nv == 3) CALL(V, 256, 3) else CALL(V, 256, 4)        \
+    }                                                                                                \
+  } else if (f.lanes == 16) {                                                                        \
+    if (f.nv == 1) CALL(1, 16, 1) else if (f.nv == 2) CALL(1, 16, 2) else if (f.nv == 3) CALL(1, 16, 3) else CALL(1, 16, 4) \
+  } else if (f.lanes == 64) {                                                                        \
+    if (f.nv == 2) CALL(1, 64, 2) else if (f.nv == 4) CALL(1, 64, 4) else if (f.nv == 8) CALL(1, 64, 8) else CALL(1, 64, 16) \
+  } else {                                                                                           \
+    if (f.nv == 8) CALL(1, 256, 8) else CALL(1, 256, 16)                                             \
+  }
+
+template <typename T>
+static void norm_fwd_launch(const NormParams& p, bool aligned, hipStream_t s) {
+  const int64_t rows = p.rows0 * p.rows1;
+  const NormPlan f = norm_plan(rows, p.C, sizeof(T), aligned);
+  if (f.nv == 0) {
+    norm_fwd_kernel<T><<<static_cast<unsigned>(rows < (1 << 16) ? rows : (1 << 16)), 256, 0, s>>>(p);
+    return;
+  }
+  const unsigned grid = static_cast<unsigned>(norm_groups(rows, f, 2048));
+#define CALL(V, L, N) norm_fwd_rows_kernel<T, V, L, N><<<grid, 256, 0, s>>>(p);
+  FOVI_NORM_CASES(CALL)
+#undef CALL
+}
+
+constexpr int64_t kNormBlocks = 512;                 // workgroups of the backward: rows of partial sums
+
+template <typename T>
+static int64_t norm_bwd_launch(const NormParams& p, bool aligned, float* partial, hipStream_t s) {
+  const int64_t rows = p.rows0 * p.rows1;
+  const NormPlan f = norm_plan(rows, p.C, sizeof(T), aligned);
+  if (f.nv == 0) {
+    if (p.dx) norm_dx_kernel<T><<<static_cast<unsigned>(rows < (1 << 16) ? rows : (1 << 16)), 256, 0, s>>>(p);
+    if (!partial) return 0;
+    const int64_t chunks = norm_chunks(rows, p.C), per = (rows + chunks - 1) / chunks;
+    norm_dw_kernel<T><<<dim3(static_cast<unsigned>((p.C + 63) / 64), static_cast<unsigned>(chunks)), 256, 0, s>>>(p, per, partial);
+    return chunks;
+  }
+  const int64_t groups = norm_groups(rows, f, kNormBlocks);
+  const unsigned grid = static_cast<unsigned>(groups);
+#define CALL(V, L, N) \
+  norm_bwd_rows_kernel<T, V, L, N><<<grid, 256, partial && L < 256 ? 4 * 2 * L * N * V * 4 : 0, s>>>(p, partial);
+  FOVI_NORM_CASES(CALL)
+#undef CALL
+  return groups;
+}
+
+static bool norm_aligned(const void* p, const int64_t* stride, int es) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride[0] * es % 16 == 0 && stride[1] * es % 16 == 0;
 }
 
 static int norm_check(const fovi_layer_norm_args* a, const char* what) {
@@ -174,17 +445,19 @@ extern "C" int fovi_layer_norm_fwd(const fovi_layer_norm_args* a, void* stream) 
   const int64_t rows = a->rows0 * a->rows1;
   if (rows == 0) return 0;
   const NormParams p = norm_params(a);
-  const unsigned grid = static_cast<unsigned>(rows < (1 << 16) ? rows : (1 << 16));
+  const int es = a->dtype == FOVI_BF16 ? 2 : 4;
+  const bool aligned = norm_aligned(p.x, p.xs, es) && norm_aligned(p.y, p.ys, es);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (a->dtype == FOVI_BF16) norm_fwd_kernel<uint16_t><<<grid, 256, 0, s>>>(p);
-  else norm_fwd_kernel<float><<<grid, 256, 0, s>>>(p);
+  if (a->dtype == FOVI_BF16) norm_fwd_launch<uint16_t>(p, aligned, s);
+  else norm_fwd_launch<float>(p, aligned, s);
   return check_launch("fovi_layer_norm_fwd");
 }
 
 extern "C" int64_t fovi_layer_norm_workspace_bytes(int64_t rows, int64_t channels, int32_t dtype) {
   (void)dtype;
   if (rows < 1 || channels < 1) return 0;
-  return norm_chunks(rows, channels) * 2 * channels * 4;
+  const int64_t chunks = norm_chunks(rows, channels), blocks = rows < kNormBlocks ? rows : kNormBlocks;
+  return (chunks > blocks ? chunks : blocks) * 2 * channels * 4;
 }
 
 extern "C" int fovi_layer_norm_bwd(const fovi_layer_norm_args* a, void* stream) {
@@ -200,23 +473,16 @@ extern "C" int fovi_layer_norm_bwd(const fovi_layer_norm_args* a, void* stream) 
   }
   const NormParams p = norm_params(a);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (a->dx && rows) {
-    const unsigned grid = static_cast<unsigned>(rows < (1 << 16) ? rows : (1 << 16));
-    if (a->dtype == FOVI_BF16) norm_dx_kernel<uint16_t><<<grid, 256, 0, s>>>(p);
-    else norm_dx_kernel<float><<<grid, 256, 0, s>>>(p);
+  int64_t chunks = 0;
+  float* partial = params ? static_cast<float*>(a->workspace) : nullptr;
+  if (rows) {
+    const int es = a->dtype == FOVI_BF16 ? 2 : 4;
+    const bool aligned = norm_aligned(p.x, p.xs, es) && norm_aligned(p.dy, p.dys, es) && (!p.dx || norm_aligned(p.dx, p.dxs, es));
+    chunks = a->dtype == FOVI_BF16 ? norm_bwd_launch<uint16_t>(p, aligned, partial, s) : norm_bwd_launch<float>(p, aligned, partial, s);
     if (check_launch("fovi_layer_norm_bwd")) return 1;
   }
   if (!params) return 0;
-  const int64_t chunks = rows ? norm_chunks(rows, p.C) : 0;
-  float* partial = static_cast<float*>(a->workspace);
-  if (chunks) {
-    const dim3 grid(static_cast<unsigned>((p.C + 63) / 64), static_cast<unsigned>(chunks));
-    const int64_t per = (rows + chunks - 1) / chunks;
-    if (a->dtype == FOVI_BF16) norm_dw_kernel<uint16_t><<<grid, 256, 0, s>>>(p, per, partial);
-    else norm_dw_kernel<float><<<grid, 256, 0, s>>>(p, per, partial);
-    if (check_launch("fovi_layer_norm_bwd")) return 1;
-  }
-  norm_dw_join_kernel<<<dim3(static_cast<unsigned>((p.C + 15) / 16), 2), 256, 0, s>>>(partial, chunks, p.C, a->dweight,
-                                                                                    a->dbias, p.p_bf16);
+  norm_dw_join_kernel<<<dim3(static_cast<unsigned>((p.C + 7) / 8), 2), 256, 0, s>>>(partial, chunks, p.C, a->dweight, a->dbias,
+                                                                                    p.p_bf16);
   return check_launch("fovi_layer_norm_bwd");
 }

@@ -33,14 +33,73 @@ __device__ __forceinline__ float2 rotary_angle(const RotaryParams& p, int64_t to
   return make_float2(c, p.inverse ? -s : s);
 }
 
-template <typename T>
+// N adjacent elements in one access (N * sizeof(T) is 2 to 16 bytes, aligned).
+template <typename T, int N> struct alignas(N * sizeof(T)) Run { T e[N]; };
+
+// VEC: elements of an access. Half pairing: a unit is VEC pairs (j .. j + VEC, and n_pairs further on),
+// then come units of VEC copied elements; VEC divides n_pairs and head_dim. Adjacent pairing: a unit
+// is VEC elements, VEC / 2 pairs, turned or copied; VEC divides head_dim. A thread keeps its unit of a
+// token's row and goes from token to token.
+template <typename T, int VEC, bool ADJACENT>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p) {
+  __shared__ __attribute__((aligned(16))) float2 table[kRotaryTable];
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.tokens, all = p.B * p.L;
+  const int n = static_cast<int>(all - t0 < p.tokens ? all - t0 : p.tokens);
+  for (int i = threadIdx.x; i < n * p.P; i += 256) table[i] = rotary_angle(p, t0 + i / p.P, i % p.P);
+  __syncthreads();
+  const int per = ADJACENT ? p.D / VEC : (p.D - p.P) / VEC, units = p.H * per, at_once = units < 256 ? 256 / units : 1;
+  const int64_t b0 = t0 / p.L, l0 = t0 - b0 * p.L;
+  for (int t = threadIdx.x / units; t < n; t += at_once) {
+    if (units < 256 && threadIdx.x >= static_cast<unsigned>(units * at_once)) break;
+    int64_t b = b0, l = l0 + t;
+    if (l >= p.L) { b += l / p.L; l %= p.L; }
+    const T* xt = static_cast<const T*>(p.x) + b * p.xs[0] + l * p.xs[1];
+    T* yt = static_cast<T*>(p.y) + b * p.ys[0] + l * p.ys[1];
+    const float2* turn = table + t * p.P;
+    for (int u = units < 256 ? threadIdx.x % units : threadIdx.x; u < units; u += 256) {
+      const int h = u / per, j = (u - h * per) * VEC;
+      const T* x = xt + h * p.xs[2] + j;
+      T* y = yt + h * p.ys[2] + j;
+      if (ADJACENT) {
+        const Run<T, VEC> a = *reinterpret_cast<const Run<T, VEC>*>(x);
+        Run<T, VEC> o = a;
+#pragma unroll
+        for (int i = 0; i + 1 < VEC; i += 2)
+          if (j + i < 2 * p.P) {
+            const float2 cs = turn[(j + i) / 2];
+            const float u0 = Elem<T>::load(&a.e[i]), v0 = Elem<T>::load(&a.e[i + 1]);
+            Elem<T>::store(&o.e[i], u0 * cs.x - v0 * cs.y);
+            Elem<T>::store(&o.e[i + 1], v0 * cs.x + u0 * cs.y);
+          }
+        *reinterpret_cast<Run<T, VEC>*>(y) = o;
+      } else if (j >= p.P) {
+        *reinterpret_cast<Run<T, VEC>*>(y + p.P) = *reinterpret_cast<const Run<T, VEC>*>(x + p.P);
+      } else {
+        const Run<T, VEC> a = *reinterpret_cast<const Run<T, VEC>*>(x), c = *reinterpret_cast<const Run<T, VEC>*>(x + p.P);
+        Run<T, VEC> ao, co;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float2 cs = turn[j + i];
+          const float u0 = Elem<T>::load(&a.e[i]), v0 = Elem<T>::load(&c.e[i]);
+          Elem<T>::store(&ao.e[i], u0 * cs.x - v0 * cs.y);
+          Elem<T>::store(&co.e[i], v0 * cs.x + u0 * cs.y);
+        }
+        *reinterpret_cast<Run<T, VEC>*>(y) = ao;
+        *reinterpret_cast<Run<T, VEC>*>(y + p.P) = co;
+      }
+    }
+  }
+}
+
+// Adjacent pairs of heads of an odd size, or at odd addresses: element by element.
+template <typename T>
+__global__ __launch_bounds__(256) void rotary_pairs_kernel(RotaryParams p) {
   __shared__ float2 table[kRotaryTable];
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.tokens, all = p.B * p.L;
   const int n = static_cast<int>(all - t0 < p.tokens ? all - t0 : p.tokens);
   for (int i = threadIdx.x; i < n * p.P; i += 256) table[i] = rotary_angle(p, t0 + i / p.P, i % p.P);
   __syncthreads();
-  const int rest = p.D - 2 * p.P, per = p.P + rest;     // a head's work: its pairs, then the copied elements
+  const int per = p.D - p.P;                            // a head's pairs, then its copied elements
   for (int i = threadIdx.x; i < n * p.H * per; i += 256) {
     const int t = i / (p.H * per), r = i - t * p.H * per, h = r / per, j = r - h * per;
     const int64_t b = (t0 + t) / p.L, l = t0 + t - b * p.L;
@@ -50,11 +109,39 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p) {
       y[p.P + j] = x[p.P + j];
       continue;
     }
-    const int iu = p.adjacent ? 2 * j : j, iv = p.adjacent ? 2 * j + 1 : j + p.P;
     const float2 cs = table[t * p.P + j];
-    const float u = Elem<T>::load(x + iu), v = Elem<T>::load(x + iv);
-    Elem<T>::store(y + iu, u * cs.x - v * cs.y);
-    Elem<T>::store(y + iv, v * cs.x + u * cs.y);
+    const float u = Elem<T>::load(x + 2 * j), v = Elem<T>::load(x + 2 * j + 1);
+    Elem<T>::store(y + 2 * j, u * cs.x - v * cs.y);
+    Elem<T>::store(y + 2 * j + 1, v * cs.x + u * cs.y);
+  }
+}
+
+// Largest access of 2^k elements, up to 16 bytes, that sizes, strides and addresses allow.
+static int rotary_vec(const RotaryParams& p, int es) {
+  int64_t all = p.D * es;
+  if (!p.adjacent) all |= p.P * es;
+  for (int i = 0; i < 3; ++i) all |= p.xs[i] * es | p.ys[i] * es;
+  all |= static_cast<int64_t>(reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.y));
+  int bytes = 16;
+  while (all % bytes) bytes /= 2;
+  return bytes / es;
+}
+
+template <typename T>
+static void rotary_launch(const RotaryParams& p, unsigned grid, hipStream_t s) {
+  const int vec = rotary_vec(p, sizeof(T));
+  if (p.adjacent) {
+    if constexpr (sizeof(T) == 2)
+      if (vec == 8) { rotary_kernel<T, 8, true><<<grid, 256, 0, s>>>(p); return; }
+    if (vec >= 4) rotary_kernel<T, 4, true><<<grid, 256, 0, s>>>(p);
+    else if (vec == 2) rotary_kernel<T, 2, true><<<grid, 256, 0, s>>>(p);
+    else rotary_pairs_kernel<T><<<grid, 256, 0, s>>>(p);
+  } else {
+    if constexpr (sizeof(T) == 2)
+      if (vec == 8) { rotary_kernel<T, 8, false><<<grid, 256, 0, s>>>(p); return; }
+    if (vec >= 4) rotary_kernel<T, 4, false><<<grid, 256, 0, s>>>(p);
+    else if (vec == 2) rotary_kernel<T, 2, false><<<grid, 256, 0, s>>>(p);
+    else rotary_kernel<T, 1, false><<<grid, 256, 0, s>>>(p);
   }
 }
 
@@ -99,7 +186,7 @@ extern "C" int fovi_rotary(const fovi_rotary_args* a, void* stream) {
   const int64_t grid = (tokens + per - 1) / per;
   if (grid > 0x7fffffff) { set_error("fovi_rotary: too many tokens"); return 1; }
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (a->dtype == FOVI_BF16) rotary_kernel<uint16_t><<<static_cast<unsigned>(grid), 256, 0, s>>>(p);
-  else rotary_kernel<float><<<static_cast<unsigned>(grid), 256, 0, s>>>(p);
+  if (a->dtype == FOVI_BF16) rotary_launch<uint16_t>(p, static_cast<unsigned>(grid), s);
+  else rotary_launch<float>(p, static_cast<unsigned>(grid), s);
   return check_launch("fovi_rotary");
 }
