@@ -29,6 +29,22 @@ __device__ __forceinline__ float norm_param(const void* p, int64_t c, int bf16, 
   return bf16 ? bf16_bits_to_f32(static_cast<const uint16_t*>(p)[c]) : static_cast<const float*>(p)[c];
 }
 
+// VEC parameters from channel c on (wide loads: a workgroup's first work), `none` without any.
+template <int VEC>
+__device__ __forceinline__ void norm_params_at(const void* p, int64_t c, int64_t C, int bf16, float none, float (&v)[VEC]) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) v[i] = none;
+  if (!p || c >= C) return;
+  if (bf16) {
+    uint16_t e[VEC];
+    __builtin_memcpy(e, static_cast<const uint16_t*>(p) + c, sizeof(e));
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = bf16_bits_to_f32(e[i]);
+  } else {
+    __builtin_memcpy(v, static_cast<const float*>(p) + c, sizeof(v));
+  }
+}
+
 // Sum over the workgroup of 256; every thread gets the result.
 __device__ __forceinline__ float block_sum(float v, float* sh) {
 #pragma unroll
@@ -82,13 +98,10 @@ __global__ __launch_bounds__(256) void norm_fwd_rows_kernel(NormParams p) {
   const int lane = threadIdx.x % LANES;
   float w[NV][VEC], b[NV][VEC];
 #pragma unroll
-  for (int k = 0; k < NV; ++k)
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const int64_t c = static_cast<int64_t>(lane + k * LANES) * VEC + i;
-      w[k][i] = c < p.C ? norm_param(p.w, c, p.p_bf16, 1.0f) : 0.0f;
-      b[k][i] = c < p.C ? norm_param(p.b, c, p.p_bf16, 0.0f) : 0.0f;
-    }
+  for (int k = 0; k < NV; ++k) {
+    norm_params_at<VEC>(p.w, static_cast<int64_t>(lane + k * LANES) * VEC, p.C, p.p_bf16, 1.0f, w[k]);
+    norm_params_at<VEC>(p.b, static_cast<int64_t>(lane + k * LANES) * VEC, p.C, p.p_bf16, 0.0f, b[k]);
+  }
   const float n = 1.0f / static_cast<float>(p.C);
   const int64_t rows = p.rows0 * p.rows1, step = static_cast<int64_t>(gridDim.x) * (256 / LANES);
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES; row < rows; row += step) {
@@ -132,13 +145,11 @@ __global__ __launch_bounds__(256) void norm_bwd_rows_kernel(NormParams p, float*
   const int lane = threadIdx.x % LANES;
   float w[NV][VEC], dw[NV][VEC], db[NV][VEC];
 #pragma unroll
-  for (int k = 0; k < NV; ++k)
+  for (int k = 0; k < NV; ++k) {
+    norm_params_at<VEC>(p.w, static_cast<int64_t>(lane + k * LANES) * VEC, p.C, p.p_bf16, 1.0f, w[k]);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const int64_t c = static_cast<int64_t>(lane + k * LANES) * VEC + i;
-      w[k][i] = c < p.C ? norm_param(p.w, c, p.p_bf16, 1.0f) : 0.0f;
-      dw[k][i] = db[k][i] = 0;
-    }
+    for (int i = 0; i < VEC; ++i) dw[k][i] = db[k][i] = 0;
+  }
   const float n = 1.0f / static_cast<float>(p.C);
   const int64_t rows = p.rows0 * p.rows1, step = static_cast<int64_t>(gridDim.x) * (256 / LANES);
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES; row < rows; row += step) {
