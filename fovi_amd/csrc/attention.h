@@ -224,15 +224,68 @@ struct Staged {
   }
 };
 
+// The other half's value (lane l and l ^ 32), by a swap of register halves: no trip through LDS.
+__device__ __forceinline__ float other_half(float x) {
+  const uint32_t u = __float_as_uint(x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// The mask at (row, state j): the score in units of log2, -inf where the pair is left out.
-__device__ __forceinline__ float masked_score(const AttnParams& p, const void* row, int64_t j, float s) {
-  const int64_t at = j * p.ms[3];
-  if (p.kind == FOVI_MASK_KEEP) return static_cast<const uint8_t*>(row)[at] ? s * p.c : kNegInf;
-  const float bias = static_cast<const float*>(row)[at];
-  // (the type's lowest value times log2(e) is still a number: rows of nothing else read all alike)
-  return bias == kNegInf ? kNegInf : fmaf(s, p.c, fmaxf(bias * kLog2e, -3.402823466e38f));
+// The mask over a lane's 16 pairs of a block whose columns are query rows: states j0 + 8 (i / 4) + i % 4
+// of its row (j0 holds the lane's half; n states in all). Scores in units of log2, -inf where a pair
+// is left out. Where the mask's states are adjacent, bytes come four at a time.
+__device__ __forceinline__ void mask_block(const AttnParams& p, const void* row, int64_t j0, int64_t n, f32x16& s) {
+  const int64_t step = p.ms[3];
+  if (p.kind == FOVI_MASK_KEEP) {
+    const uint8_t* m = static_cast<const uint8_t*>(row) + j0 * step;
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      uint32_t keep = 0;
+      if (step == 1 && j0 + 2 * i + 4 <= n) {
+        __builtin_memcpy(&keep, m + 2 * i, 4);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (j0 + 2 * i + e < n) keep |= static_cast<uint32_t>(m[(2 * i + e) * step]) << (8 * e);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[i + e] = (keep >> (8 * e)) & 0xff ? s[i + e] * p.c : kNegInf;
+    }
+  } else {
+    const float* m = static_cast<const float*>(row) + j0 * step;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int at = 8 * (i / 4) + i % 4;
+      const float bias = j0 + at < n ? m[at * step] : kNegInf;
+      // (the type's lowest value times log2(e) is still a number: rows of nothing else read all alike)
+      s[i] = bias == kNegInf ? kNegInf : fmaf(s[i], p.c, fmaxf(bias * kLog2e, -3.402823466e38f));
+    }
+  }
+}
+
+// The same where the columns are states: 16 rows i0 + 8 (i / 4) + i % 4 (n in all) of one state, `col` its
+// place in row 0's mask.
+__device__ __forceinline__ void mask_column(const AttnParams& p, const void* col, int64_t i0, int64_t n, f32x16& s) {
+  const int64_t step = p.ms[2];
+  if (p.kind == FOVI_MASK_KEEP) {
+    const uint8_t* m = static_cast<const uint8_t*>(col) + i0 * step;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int at = 8 * (i / 4) + i % 4;
+      const bool keep = i0 + at < n && m[at * step] != 0;
+      s[i] = keep ? s[i] * p.c : kNegInf;
+    }
+  } else {
+    const float* m = static_cast<const float*>(col) + i0 * step;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int at = 8 * (i / 4) + i % 4;
+      const float bias = i0 + at < n ? m[at * step] : kNegInf;
+      s[i] = bias == kNegInf ? kNegInf : fmaf(s[i], p.c, fmaxf(bias * kLog2e, -3.402823466e38f));
+    }
+  }
 }
 __device__ __forceinline__ const void* mask_row(const AttnParams& p, int64_t b, int64_t h, int64_t i) {
   return static_cast<const char*>(p.mask) + (b * p.ms[0] + h * p.ms[1] + i * p.ms[2]) * (p.kind == FOVI_MASK_KEEP ? 1 : 4);

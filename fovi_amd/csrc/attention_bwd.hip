@@ -65,8 +65,16 @@ __device__ __forceinline__ void pair_grad(float t, float c, float shift, float f
   }
 }
 
+// Waves a SIMD shall hold: two wherever a kernel fits 256 registers without spilling much.
+template <typename T> constexpr int dq_waves(int DP, int KIND) {
+  return sizeof(T) == 2 ? (KIND && DP == 128 ? 1 : 2) : DP >= 96 ? 1 : 2;
+}
+template <typename T> constexpr int dkv_waves(int DP, int KIND) {
+  return sizeof(T) == 2 ? (KIND && DP >= 96 ? 1 : 2) : DP >= 96 || (KIND && DP == 64) ? 1 : 2;
+}
+
 template <typename T, int DP, int QT, int KIND>
-__global__ __launch_bounds__(256) void attn_dq_kernel(AttnParams p) {
+__global__ __launch_bounds__(256, dq_waves<T>(DP, KIND)) void attn_dq_kernel(AttnParams p) {
   constexpr int LP = DP == 96 ? 128 : DP, KB = sizeof(T) == 2 ? 2 : 1, KT = 32 * KB, DT = DP / 32, STEPS = DP / (2 * Chunk<T>::N);
   __shared__ __attribute__((aligned(16))) char tiles[2][2][KT * LP * sizeof(T)];
   __shared__ int bad_tile[2];
@@ -135,12 +143,11 @@ __global__ __launch_bounds__(256) void attn_dq_kernel(AttnParams p) {
       }
 #pragma unroll
       for (int x = 0; x < QT; ++x) {
+        if (KIND) mask_block(p, mrow[x], j + kb * 32 + 4 * (l >> 5), n, s[x]);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const int64_t col = j + kb * 32 + 8 * (i / 4) + 4 * (l >> 5) + i % 4;
           float t = s[x][i], e, ds;
-          if (KIND) t = col < n ? masked_score(p, mrow[x], col, t) : kNegInf;
-          else if (j + kb * 32 + 32 > n) t = col < n ? t : kNegInf;
+          if (!KIND && j + kb * 32 + 32 > n) t = j + kb * 32 + 8 * (i / 4) + 4 * (l >> 5) + i % 4 < n ? t : kNegInf;
           pair_grad<KIND>(t, p.c, st[x].shift, st[x].factor, st[x].delta, dp[x][i], e, ds);
           s[x][i] = ds;
         }
@@ -175,7 +182,7 @@ __global__ __launch_bounds__(256) void attn_dq_kernel(AttnParams p) {
 }
 
 template <typename T, int DP, int KIND>
-__global__ __launch_bounds__(256) void attn_dkv_kernel(AttnParams p) {
+__global__ __launch_bounds__(256, dkv_waves<T>(DP, KIND)) void attn_dkv_kernel(AttnParams p) {
   constexpr int LP = DP == 96 ? 128 : DP, DT = DP / 32, STEPS = DP / (2 * Chunk<T>::N);
   __shared__ __attribute__((aligned(16))) char tiles[2][2][32 * LP * sizeof(T)];
   __shared__ __attribute__((aligned(16))) float stats[2][3][32];
@@ -239,7 +246,11 @@ __global__ __launch_bounds__(256) void attn_dkv_kernel(AttnParams p) {
       s = mma_step(T(), *reinterpret_cast<const uint4*>(qt + off), k[t], s);
       dp = mma_step(T(), *reinterpret_cast<const uint4*>(gt + off), v[t], dp);
     }
-    const int64_t h = hk * p.G + x / per, i0 = x % per * 32;
+    if (KIND) {
+      const int64_t h = hk * p.G + x / per, i0 = x % per * 32 + 4 * (l >> 5);
+      const char* col = static_cast<const char*>(mask_row(p, b, h, 0)) + (j < n ? j : 0) * p.ms[3] * (p.kind == FOVI_MASK_KEEP ? 1 : 4);
+      mask_column(p, col, i0, j < n ? p.Lq : 0, s);
+    }
 #pragma unroll
     for (int i = 0; i < 16; i += 4) {
       const int r = 2 * i + 4 * (l >> 5);
@@ -249,7 +260,6 @@ __global__ __launch_bounds__(256) void attn_dkv_kernel(AttnParams p) {
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
         float t = s[i + y], e, ds;
-        if (KIND) t = j < n && i0 + r + y < p.Lq ? masked_score(p, mask_row(p, b, h, i0 + r + y), j, t) : kNegInf;
         pair_grad<KIND>(t, p.c, shift[y], KIND ? factor[y] : 1.0f, delta[y], dp[i + y], e, ds);
         s[i + y] = e;
         dp[i + y] = ds;
@@ -330,10 +340,10 @@ struct BwdPlan {
   int64_t q_tiles, q_chunk, k_tiles, k_chunk;
 };
 
-static BwdPlan bwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t D) {
+static BwdPlan bwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t D, int dtype, bool mask) {
   BwdPlan f;
   const int64_t R = H / Hk * Lq;
-  f.qt = D <= 64 && R > 128 ? 2 : 1;
+  f.qt = dtype == FOVI_BF16 && D <= 32 && !mask && R > 128 ? 2 : 1;
   f.q_tiles = (R + 128 * f.qt - 1) / (128 * f.qt);
   f.k_tiles = (Lk + 127) / 128;
   // splits for two workgroups a compute unit, each with at least 256 states or 256 rows to walk
@@ -356,18 +366,22 @@ static BwdPlan bwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk
 static int64_t align16(int64_t n) { return (n + 15) / 16 * 16; }
 
 int64_t attn_bwd_workspace(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t D, int dtype) {
-  (void)dtype;
-  const BwdPlan f = bwd_plan(B, Lq, Lk, H, Hk, D);
-  // delta, then the partial sums of dq, later those of dk and dv in their place
-  const int64_t q = f.q_splits > 1 ? f.q_splits * B * H * Lq * D * 4 : 0, k = f.k_splits > 1 ? f.k_splits * B * Hk * Lk * 2 * D * 4 : 0;
-  return align16(B * H * Lq * 4) + (q > k ? q : k);
+  int64_t most = 0;
+  for (const bool mask : {false, true}) {
+    const BwdPlan f = bwd_plan(B, Lq, Lk, H, Hk, D, dtype, mask);
+    // delta, then the partial sums of dq, later those of dk and dv in their place
+    const int64_t q = f.q_splits > 1 ? f.q_splits * B * H * Lq * D * 4 : 0, k = f.k_splits > 1 ? f.k_splits * B * Hk * Lk * 2 * D * 4 : 0;
+    if (q > most) most = q;
+    if (k > most) most = k;
+  }
+  return align16(B * H * Lq * 4) + most;
 }
 
 template <typename T, int DP, int KIND>
 static void bwd_dq(const AttnParams& p, int qt, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>((p.B * p.Hk * p.tiles + 7) / 8 * 8), static_cast<unsigned>(p.splits));
   if (qt == 1) attn_dq_kernel<T, DP, 1, KIND><<<grid, 256, 0, s>>>(p);
-  else if constexpr (DP <= 64) attn_dq_kernel<T, DP, 2, KIND><<<grid, 256, 0, s>>>(p);
+  else if constexpr (DP == 32 && sizeof(T) == 2 && KIND == 0) attn_dq_kernel<T, DP, 2, KIND><<<grid, 256, 0, s>>>(p);
 }
 
 template <typename T, int DP, int KIND>
@@ -378,7 +392,7 @@ static void bwd_dkv(const AttnParams& p, hipStream_t s) {
 
 template <typename T>
 static int bwd_type(AttnParams& p, hipStream_t s) {
-  const BwdPlan f = bwd_plan(p.B, p.Lq, p.Lk, p.H, p.Hk, p.D);
+  const BwdPlan f = bwd_plan(p.B, p.Lq, p.Lk, p.H, p.Hk, p.D, sizeof(T) == 2 ? FOVI_BF16 : FOVI_F32, p.kind != 0);
   p.delta = p.part;
   p.part = reinterpret_cast<float*>(reinterpret_cast<char*>(p.part) + align16(p.B * p.H * p.Lq * 4));
   const int64_t rows = p.B * p.H * p.Lq;

@@ -55,11 +55,7 @@ __device__ __forceinline__ void softmax_blocks(const AttnParams& p, RowState<T, 
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb) {
     if (KIND) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int64_t at = j + kb * 32 + 8 * (i / 4) + 4 * h + i % 4;
-        s[kb][i] = at < n ? masked_score(p, st.mrow[t], at, s[kb][i]) : kNegInf;
-      }
+      mask_block(p, st.mrow[t], j + kb * 32 + 4 * h, n, s[kb]);
     } else if (j + kb * 32 + 32 > n) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
@@ -71,7 +67,7 @@ __device__ __forceinline__ void softmax_blocks(const AttnParams& p, RowState<T, 
   for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
     for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][i]);
-  top = fmaxf(top, __shfl_xor(top, 32));
+  top = fmaxf(top, other_half(top));
   const float at = top == kNegInf ? 0.0f : top;
   if (__any(top != st.m[t])) {                 // the maxima settle after the first tiles
     const float keep = exp2_fast((st.m[t] - at) * c);
@@ -99,8 +95,17 @@ __device__ __forceinline__ int64_t stat_at(const AttnParams& p, int64_t b, int h
   return (b * p.H + static_cast<int64_t>(hk) * p.G) * p.Lq + r;      // row (b, head, query) of the statistics
 }
 
+// Waves a SIMD shall hold: two (256 registers each) wherever a kernel fits without spilling much; a lone
+// wave waits out every latency (bf16, heads of 64, 1024 x 4096 x 192 heads: 602 us with one, 390 with two).
+template <typename T> constexpr int tile_waves(int DP, int KIND) {
+  return sizeof(T) == 2 ? (KIND && DP == 128 ? 1 : 2) : (DP == 128 || (KIND && DP == 96) ? 1 : 2);
+}
+template <typename T> constexpr int few_waves(int DP, int KIND) {
+  return sizeof(T) == 2 ? (KIND && DP >= 96 ? 1 : 2) : (DP >= 96 || (KIND && DP == 64) ? 1 : 2);
+}
+
 template <typename T, int DP, int QT, int KIND>
-__global__ __launch_bounds__(256) void attn_fwd_tile_kernel(AttnParams p) {
+__global__ __launch_bounds__(256, tile_waves<T>(DP, KIND)) void attn_fwd_tile_kernel(AttnParams p) {
   constexpr int LP = DP == 96 ? 128 : DP, KB = sizeof(T) == 2 ? 2 : 1, KT = 32 * KB, DT = DP / 32;
   constexpr int STEPS = RowState<T, DP, QT>::STEPS;
   __shared__ __attribute__((aligned(16))) char tiles[2][2][KT * LP * sizeof(T)];
@@ -171,7 +176,7 @@ __global__ __launch_bounds__(256) void attn_fwd_tile_kernel(AttnParams p) {
 #pragma unroll
   for (int q = 0; q < QT; ++q) {
     const int64_t r = r0 + 32 * q + (lane & 31);
-    const float sum = st.l[q] + __shfl_xor(st.l[q], 32), m = KIND ? st.m[q] : st.m[q] * p.c;
+    const float sum = st.l[q] + other_half(st.l[q]), m = KIND ? st.m[q] : st.m[q] * p.c;
     if (r >= p.R) continue;
     if (p.splits > 1) {
       float* out = p.part + ((split * p.B * p.Hk + bh) * p.R + r) * (p.D + 2);
@@ -225,7 +230,7 @@ __device__ __forceinline__ void put_row(const AttnParams& p, int64_t b, int hk, 
 }
 
 template <typename T, int DP, int QT, int KIND>
-__global__ __launch_bounds__(256) void attn_fwd_few_kernel(AttnParams p) {
+__global__ __launch_bounds__(256, few_waves<T>(DP, KIND)) void attn_fwd_few_kernel(AttnParams p) {
   constexpr int LP = DP == 96 ? 128 : DP, DT = DP / 32, STEPS = RowState<T, DP, QT>::STEPS;
   constexpr int TILE = 32 * LP * static_cast<int>(sizeof(T)), JOIN = 32 * (DP + 1) * 4;
   __shared__ __attribute__((aligned(16))) char lds[4 * (TILE > JOIN ? TILE : JOIN)];
@@ -278,7 +283,7 @@ __global__ __launch_bounds__(256) void attn_fwd_few_kernel(AttnParams p) {
   for (int q = 0; q < QT; ++q) {
     if (q * 32 >= p.R) break;
     __syncthreads();
-    const float sum = st.l[q] + __shfl_xor(st.l[q], 32);
+    const float sum = st.l[q] + other_half(st.l[q]);
     if (l < 32) { wm[w][l] = KIND ? st.m[q] : st.m[q] * p.c; wl[w][l] = sum; }
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -344,15 +349,16 @@ struct FwdPlan {
   int64_t tiles, chunk;
 };
 
-static FwdPlan fwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t D, int dtype) {
+static FwdPlan fwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t D, int dtype, bool mask) {
   FwdPlan f;
   const int64_t R = H / Hk * Lq;
-  f.few = R <= (dtype == FOVI_BF16 && D <= 64 ? 64 : 32);      // (two blocks of rows need too many registers else)
+  const bool two = dtype == FOVI_BF16 && D <= 64 && !mask;     // two blocks of rows a wave fit its registers
+  f.few = R <= (two ? 64 : 32);
   if (f.few) {
     f.qt = R <= 32 ? 1 : 2;
     f.tiles = 1;
   } else {
-    f.qt = D <= 64 && R > 128 ? 2 : 1;
+    f.qt = two && R > 128 ? 2 : 1;
     f.tiles = (R + 128 * f.qt - 1) / (128 * f.qt);
   }
   // about four workgroups a compute unit (few rows), two (tiles), each with at least 256 states
@@ -368,8 +374,13 @@ static FwdPlan fwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk
 }
 
 int64_t attn_fwd_workspace(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t D, int dtype) {
-  const FwdPlan f = fwd_plan(B, Lq, Lk, H, Hk, D, dtype);
-  return f.splits > 1 ? f.splits * B * H * Lq * (D + 2) * 4 : 0;
+  int64_t most = 0;
+  for (const bool mask : {false, true}) {
+    const FwdPlan f = fwd_plan(B, Lq, Lk, H, Hk, D, dtype, mask);
+    const int64_t need = f.splits > 1 ? f.splits * B * H * Lq * (D + 2) * 4 : 0;
+    if (need > most) most = need;
+  }
+  return most;
 }
 
 template <typename T, int DP, int KIND>
@@ -378,17 +389,17 @@ static void fwd_launch(const AttnParams& p, const FwdPlan& f, hipStream_t s) {
   if (f.few) {
     const dim3 grid(static_cast<unsigned>(all), static_cast<unsigned>(f.splits));
     if (f.qt == 1) attn_fwd_few_kernel<T, DP, 1, KIND><<<grid, 256, 0, s>>>(p);
-    else if constexpr (DP <= 64 && sizeof(T) == 2) attn_fwd_few_kernel<T, DP, 2, KIND><<<grid, 256, 0, s>>>(p);
+    else if constexpr (DP <= 64 && sizeof(T) == 2 && KIND == 0) attn_fwd_few_kernel<T, DP, 2, KIND><<<grid, 256, 0, s>>>(p);
   } else {
     const dim3 grid(static_cast<unsigned>((all + 7) / 8 * 8), static_cast<unsigned>(f.splits));
     if (f.qt == 1) attn_fwd_tile_kernel<T, DP, 1, KIND><<<grid, 256, 0, s>>>(p);
-    else if constexpr (DP <= 64) attn_fwd_tile_kernel<T, DP, 2, KIND><<<grid, 256, 0, s>>>(p);
+    else if constexpr (DP <= 64 && sizeof(T) == 2 && KIND == 0) attn_fwd_tile_kernel<T, DP, 2, KIND><<<grid, 256, 0, s>>>(p);
   }
 }
 
 template <typename T>
 static int fwd_type(AttnParams& p, hipStream_t s) {
-  const FwdPlan f = fwd_plan(p.B, p.Lq, p.Lk, p.H, p.Hk, p.D, sizeof(T) == 2 ? FOVI_BF16 : FOVI_F32);
+  const FwdPlan f = fwd_plan(p.B, p.Lq, p.Lk, p.H, p.Hk, p.D, sizeof(T) == 2 ? FOVI_BF16 : FOVI_F32, p.kind != 0);
   p.splits = f.splits;
   p.chunk = f.chunk;
   p.tiles = f.tiles;
