@@ -231,6 +231,11 @@ __device__ __forceinline__ float other_half(float x) {
   return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
 }
 
+// Waits for every load so far. In front of the loops: without it the compiler does not know that the
+// operands loaded once have arrived, and waits for them inside the loop, and with them for the next
+// tile's loads.
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // The mask over a lane's 16 pairs of a block whose columns are query rows: states j0 + 8 (i / 4) + i % 4

@@ -42,13 +42,8 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(AttnParams p) {
 // into the shift (factor 1). A row that keeps nothing has shift +inf: probabilities 0.
 struct RowStat { float shift, factor, delta; };
 template <int KIND>
-__device__ __forceinline__ RowStat row_stat(const AttnParams& p, int64_t at) {
-  const float m = p.stats[at], sum = p.stats[p.B * p.H * p.Lq + at];
-  RowStat r;
-  r.shift = sum == 0 ? __builtin_inff() : KIND ? m : m + log2f(sum);
-  r.factor = KIND ? (sum == 0 ? 0.0f : 1.0f / sum) : 1.0f;
-  r.delta = p.delta[at];
-  return r;
+__device__ __forceinline__ RowStat row_stat(float m, float sum, float delta) {
+  return {sum == 0 ? __builtin_inff() : KIND ? m : m + log2f(sum), KIND && sum != 0 ? 1.0f / sum : KIND ? 0.0f : 1.0f, delta};
 }
 
 // Probability and score gradient of one pair; KIND 1: t is the masked score, left-out pairs become kLeftOut.
@@ -100,7 +95,8 @@ __global__ __launch_bounds__(256, dq_waves<T>(DP, KIND)) void attn_dq_kernel(Att
       q[t][s] = load_chunk<T>(qr, 2 * s + (l >> 5), r < p.R ? p.D : 0);
       g[t][s] = load_chunk<T>(gg, 2 * s + (l >> 5), r < p.R ? p.D : 0);
     }
-    st[t] = row_stat<KIND>(p, (b * p.H + h) * p.Lq + i);
+    const int64_t at = (b * p.H + h) * p.Lq + i;
+    st[t] = row_stat<KIND>(p.stats[at], p.stats[p.B * p.H * p.Lq + at], p.delta[at]);
     mrow[t] = KIND ? mask_row(p, b, h, i) : nullptr;
   }
   const T* k = static_cast<const T*>(p.k) + b * p.ks[0] + hk * p.ks[2];
@@ -119,6 +115,7 @@ __global__ __launch_bounds__(256, dq_waves<T>(DP, KIND)) void attn_dq_kernel(Att
     vr.load(v + j0 * p.vs[1], p.vs[1], n - j0, p.D, threadIdx.x);
     put(0, 0);
   }
+  wait_loads();
   for (int64_t j = j0; j < n; j += KT, ++at) {
     const int64_t next = j + KT;
     if (next < n) {
@@ -128,6 +125,7 @@ __global__ __launch_bounds__(256, dq_waves<T>(DP, KIND)) void attn_dq_kernel(Att
     __syncthreads();
     const char* kt = tiles[at & 1][0];
     const char* vt = tiles[at & 1][1];
+    const int left = static_cast<int>(n - j < KT ? n - j : KT);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       f32x16 s[QT] = {}, dp[QT] = {};
@@ -143,12 +141,17 @@ __global__ __launch_bounds__(256, dq_waves<T>(DP, KIND)) void attn_dq_kernel(Att
       }
 #pragma unroll
       for (int x = 0; x < QT; ++x) {
-        if (KIND) mask_block(p, mrow[x], j + kb * 32 + 4 * (l >> 5), n, s[x]);
+        if (KIND) {
+          mask_block(p, mrow[x], j + kb * 32 + 4 * (l >> 5), n, s[x]);
+        } else if (left < kb * 32 + 32) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (kb * 32 + 8 * (i / 4) + 4 * (l >> 5) + i % 4 >= left) s[x][i] = kNegInf;
+        }
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          float t = s[x][i], e, ds;
-          if (!KIND && j + kb * 32 + 32 > n) t = j + kb * 32 + 8 * (i / 4) + 4 * (l >> 5) + i % 4 < n ? t : kNegInf;
-          pair_grad<KIND>(t, p.c, st[x].shift, st[x].factor, st[x].delta, dp[x][i], e, ds);
+          float e, ds;
+          pair_grad<KIND>(s[x][i], p.c, st[x].shift, st[x].factor, st[x].delta, dp[x][i], e, ds);
           s[x][i] = ds;
         }
         if (KIND && bad_tile[at & 1] == at) {
@@ -181,11 +184,14 @@ __global__ __launch_bounds__(256, dq_waves<T>(DP, KIND)) void attn_dq_kernel(Att
   }
 }
 
+// Blocks of 32 rows in a tile of the dk, dv kernel.
+template <typename T> constexpr int dkv_blocks(int DP) { return sizeof(T) == 2 && DP <= 64 ? 2 : 1; }
+
 template <typename T, int DP, int KIND>
 __global__ __launch_bounds__(256, dkv_waves<T>(DP, KIND)) void attn_dkv_kernel(AttnParams p) {
-  constexpr int LP = DP == 96 ? 128 : DP, DT = DP / 32, STEPS = DP / (2 * Chunk<T>::N);
-  __shared__ __attribute__((aligned(16))) char tiles[2][2][32 * LP * sizeof(T)];
-  __shared__ __attribute__((aligned(16))) float stats[2][3][32];
+  constexpr int LP = DP == 96 ? 128 : DP, DT = DP / 32, STEPS = DP / (2 * Chunk<T>::N), RB = dkv_blocks<T>(DP), RT = 32 * RB;
+  __shared__ __attribute__((aligned(16))) char tiles[2][2][RT * LP * sizeof(T)];
+  __shared__ __attribute__((aligned(16))) float stats[2][3][RT];
   __shared__ int bad_tile[2][2];
   const int64_t all = p.tiles * p.B * p.Hk, id = xcd_tile(blockIdx.x, gridDim.x);
   if (id >= all) return;
@@ -201,85 +207,94 @@ __global__ __launch_bounds__(256, dkv_waves<T>(DP, KIND)) void attn_dkv_kernel(A
     v[s] = load_chunk<T>(vp, 2 * s + (l >> 5), j < n ? p.D : 0);
   }
   f32x16 dk[DT] = {}, dv[DT] = {};
-  // tiles of 32 rows, head by head: tile x is rows 32 (x % per) .. of head x / per of the group
-  const int64_t per = (p.Lq + 31) / 32, end = per * p.G;
-  int64_t x = split * p.chunk;
-  const int64_t x1 = w0 >= n ? x : end < x + p.chunk ? end : x + p.chunk;
-  Staged<T, DP, LP, 32, 256> qr, gr;
-  RowStat sr;
+  // tiles of RT rows, head by head; split s walks tiles s * chunk .. of the p.G * per there are
+  const int per = static_cast<int>((p.Lq + RT - 1) / RT);
+  const int64_t first = split * p.chunk, end = static_cast<int64_t>(per) * p.G;
+  const int count = w0 >= n ? 0 : static_cast<int>(end < first + p.chunk ? end - first : p.chunk);
+  Staged<T, DP, LP, RT, 256> qr, gr;
+  float m = 0, sum = 0, delta = 0;                 // raw: nothing waits for them before the tile is stored
   if (KIND && threadIdx.x < 4) bad_tile[threadIdx.x >> 1][threadIdx.x & 1] = -1;
   if (KIND) __syncthreads();
-  auto fetch = [&](int64_t tile) {
-    const int64_t h = hk * p.G + tile / per, i = tile % per * 32;
-    qr.load(static_cast<const T*>(p.q) + b * p.qs[0] + i * p.qs[1] + h * p.qs[2], p.qs[1], p.Lq - i, p.D, threadIdx.x);
-    gr.load(static_cast<const T*>(p.dout) + b * p.dos[0] + i * p.dos[1] + h * p.dos[2], p.dos[1], p.Lq - i, p.D, threadIdx.x);
-    if (threadIdx.x < 32) {
-      if (i + threadIdx.x < p.Lq) sr = row_stat<KIND>(p, (b * p.H + h) * p.Lq + i + threadIdx.x);
-      else sr = {__builtin_inff(), 0.0f, 0.0f};
+  int h = hk * p.G + static_cast<int>(first / per), i0 = static_cast<int>(first % per) * RT;      // the next tile to fetch
+  auto fetch = [&]() {
+    qr.load(static_cast<const T*>(p.q) + b * p.qs[0] + i0 * p.qs[1] + h * p.qs[2], p.qs[1], p.Lq - i0, p.D, threadIdx.x);
+    gr.load(static_cast<const T*>(p.dout) + b * p.dos[0] + i0 * p.dos[1] + h * p.dos[2], p.dos[1], p.Lq - i0, p.D, threadIdx.x);
+    if (threadIdx.x < RT) {
+      const bool in = i0 + threadIdx.x < p.Lq;
+      const int64_t at = (b * p.H + h) * p.Lq + (in ? i0 + threadIdx.x : 0);
+      m = p.stats[at];
+      sum = in ? p.stats[p.B * p.H * p.Lq + at] : 0.0f;
+      delta = p.delta[at];
     }
   };
   auto put = [&](int buf, int tile) {
     qr.store(tiles[buf][0], threadIdx.x);
     gr.store(tiles[buf][1], threadIdx.x);
-    if (threadIdx.x < 32) {
+    if (threadIdx.x < RT) {
+      const RowStat sr = row_stat<KIND>(m, sum, sum == 0 ? 0.0f : delta);
       stats[buf][0][threadIdx.x] = sr.shift;
-      stats[buf][1][threadIdx.x] = sr.factor;
+      if (KIND) stats[buf][1][threadIdx.x] = sr.factor;
       stats[buf][2][threadIdx.x] = sr.delta;
     }
     if (KIND && qr.bad()) bad_tile[buf][0] = tile;
     if (KIND && gr.bad()) bad_tile[buf][1] = tile;
   };
-  int at = 0;
-  if (x < x1) {
-    fetch(x);
+  if (count > 0) {
+    fetch();
     put(0, 0);
   }
-  for (; x < x1; ++x, ++at) {
-    if (x + 1 < x1) fetch(x + 1);
+  wait_loads();
+  for (int at = 0; at < count; ++at) {
+    const int h_at = h, i_at = i0;
+    i0 += RT;
+    if (i0 >= p.Lq) { i0 = 0; ++h; }
+    if (at + 1 < count) fetch();
     __syncthreads();
-    const char* qt = tiles[at & 1][0];
-    const char* gt = tiles[at & 1][1];
-    f32x16 s = {}, dp = {};
+#pragma unroll 1                        // (both blocks at once would not fit 256 registers)
+    for (int rb = 0; rb < RB; ++rb) {
+      const char* qt = tiles[at & 1][0] + rb * 32 * LP * sizeof(T);
+      const char* gt = tiles[at & 1][1] + rb * 32 * LP * sizeof(T);
+      f32x16 s = {}, dp = {};
 #pragma unroll
-    for (int t = 0; t < STEPS; ++t) {
-      const int off = tile_at<T, LP>(l & 31, 2 * t + (l >> 5));
-      s = mma_step(T(), *reinterpret_cast<const uint4*>(qt + off), k[t], s);
-      dp = mma_step(T(), *reinterpret_cast<const uint4*>(gt + off), v[t], dp);
-    }
-    if (KIND) {
-      const int64_t h = hk * p.G + x / per, i0 = x % per * 32 + 4 * (l >> 5);
-      const char* col = static_cast<const char*>(mask_row(p, b, h, 0)) + (j < n ? j : 0) * p.ms[3] * (p.kind == FOVI_MASK_KEEP ? 1 : 4);
-      mask_column(p, col, i0, j < n ? p.Lq : 0, s);
-    }
+      for (int t = 0; t < STEPS; ++t) {
+        const int off = tile_at<T, LP>(l & 31, 2 * t + (l >> 5));
+        s = mma_step(T(), *reinterpret_cast<const uint4*>(qt + off), k[t], s);
+        dp = mma_step(T(), *reinterpret_cast<const uint4*>(gt + off), v[t], dp);
+      }
+      if (KIND) {
+        const char* col = static_cast<const char*>(mask_row(p, b, h_at, 0)) + (j < n ? j : 0) * p.ms[3] * (p.kind == FOVI_MASK_KEEP ? 1 : 4);
+        mask_column(p, col, i_at + rb * 32 + 4 * (l >> 5), j < n ? p.Lq : 0, s);
+      }
 #pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      const int r = 2 * i + 4 * (l >> 5);
-      const f32x4 shift = *reinterpret_cast<const f32x4*>(&stats[at & 1][0][r]), delta = *reinterpret_cast<const f32x4*>(&stats[at & 1][2][r]);
-      f32x4 factor;
-      if (KIND) factor = *reinterpret_cast<const f32x4*>(&stats[at & 1][1][r]);
+      for (int i = 0; i < 16; i += 4) {
+        const int r = rb * 32 + 2 * i + 4 * (l >> 5);
+        const f32x4 shift = *reinterpret_cast<const f32x4*>(&stats[at & 1][0][r]), delta = *reinterpret_cast<const f32x4*>(&stats[at & 1][2][r]);
+        f32x4 factor;
+        if (KIND) factor = *reinterpret_cast<const f32x4*>(&stats[at & 1][1][r]);
 #pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        float t = s[i + y], e, ds;
-        pair_grad<KIND>(t, p.c, shift[y], KIND ? factor[y] : 1.0f, delta[y], dp[i + y], e, ds);
-        s[i + y] = e;
-        dp[i + y] = ds;
+        for (int y = 0; y < 4; ++y) {
+          float e, ds;
+          pair_grad<KIND>(s[i + y], p.c, shift[y], KIND ? factor[y] : 1.0f, delta[y], dp[i + y], e, ds);
+          s[i + y] = e;
+          dp[i + y] = ds;
+        }
+      }
+      if (KIND && bad_tile[at & 1][1] == at) {
+        slow_second<T, LP, DT>(gt, 0, s, dv);
+      } else {
+        const Block<T> e(s);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) dv[d] = mma_second<LP>(T(), gt, 0, d, e, dv[d]);
+      }
+      if (KIND && bad_tile[at & 1][0] == at) {
+        slow_second<T, LP, DT>(qt, 0, dp, dk);
+      } else {
+        const Block<T> ds(dp);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) dk[d] = mma_second<LP>(T(), qt, 0, d, ds, dk[d]);
       }
     }
-    if (KIND && bad_tile[at & 1][1] == at) {
-      slow_second<T, LP, DT>(gt, 0, s, dv);
-    } else {
-      const Block<T> e(s);
-#pragma unroll
-      for (int d = 0; d < DT; ++d) dv[d] = mma_second<LP>(T(), gt, 0, d, e, dv[d]);
-    }
-    if (KIND && bad_tile[at & 1][0] == at) {
-      slow_second<T, LP, DT>(qt, 0, dp, dk);
-    } else {
-      const Block<T> ds(dp);
-#pragma unroll
-      for (int d = 0; d < DT; ++d) dk[d] = mma_second<LP>(T(), qt, 0, d, ds, dk[d]);
-    }
-    if (x + 1 < x1) put((at + 1) & 1, at + 1);
+    if (at + 1 < count) put((at + 1) & 1, at + 1);
   }
   if (j >= p.Lk) return;
   T* dko = static_cast<T*>(p.dk) + b * p.dks[0] + j * p.dks[1] + hk * p.dks[2];
@@ -340,6 +355,8 @@ struct BwdPlan {
   int64_t q_tiles, q_chunk, k_tiles, k_chunk;
 };
 
+static int64_t dkv_tile(int64_t D, int dtype) { return 32 * (dtype == FOVI_BF16 && D <= 64 ? 2 : 1); }
+
 static BwdPlan bwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t D, int dtype, bool mask) {
   BwdPlan f;
   const int64_t R = H / Hk * Lq;
@@ -347,7 +364,8 @@ static BwdPlan bwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk
   f.q_tiles = (R + 128 * f.qt - 1) / (128 * f.qt);
   f.k_tiles = (Lk + 127) / 128;
   // splits for two workgroups a compute unit, each with at least 256 states or 256 rows to walk
-  const int64_t gq = B * Hk * f.q_tiles, gk = B * Hk * f.k_tiles, row_tiles = H / Hk * ((Lq + 31) / 32);
+  const int64_t gq = B * Hk * f.q_tiles, gk = B * Hk * f.k_tiles, row_tile = dkv_tile(D, dtype),
+                row_tiles = H / Hk * ((Lq + row_tile - 1) / row_tile);
   int64_t s = gq > 0 ? 512 / gq : 1;
   if (s > Lk / 256) s = Lk / 256;
   if (s < 1) s = 1;
@@ -355,7 +373,7 @@ static BwdPlan bwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk
   if (f.q_chunk < 128) f.q_chunk = 128;
   f.q_splits = static_cast<int>(Lk ? (Lk + f.q_chunk - 1) / f.q_chunk : 1);
   s = gk > 0 ? 512 / gk : 1;
-  if (s > row_tiles / 8) s = row_tiles / 8;
+  if (s > row_tiles * row_tile / 256) s = row_tiles * row_tile / 256;
   if (s < 1) s = 1;
   f.k_chunk = (row_tiles + s - 1) / s;
   if (f.k_chunk < 1) f.k_chunk = 1;

@@ -19,7 +19,7 @@ struct RowState {
   static constexpr int DT = DP / 32, STEPS = DP / (2 * Chunk<T>::N);
   uint4 q[QT][STEPS];
   f32x16 o[QT][DT];
-  float m[QT], l[QT];         // the row's maximum so far; the lane's share of the sum
+  float m[QT], l[QT];         // the row's maximum so far, or a little less; the lane's share of the sum
   const void* mrow[QT];
 };
 
@@ -52,14 +52,15 @@ __device__ __forceinline__ void softmax_blocks(const AttnParams& p, RowState<T, 
                                                int64_t j, int64_t n) {
   const int h = (threadIdx.x & 63) >> 5;
   const float c = KIND ? 1.0f : p.c;
+  const int left = static_cast<int>(n - j < 32 * KB ? n - j : 32 * KB);
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb) {
     if (KIND) {
       mask_block(p, st.mrow[t], j + kb * 32 + 4 * h, n, s[kb]);
-    } else if (j + kb * 32 + 32 > n) {
+    } else if (left < kb * 32 + 32) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        if (j + kb * 32 + 8 * (i / 4) + 4 * h + i % 4 >= n) s[kb][i] = kNegInf;
+        if (kb * 32 + 8 * (i / 4) + 4 * h + i % 4 >= left) s[kb][i] = kNegInf;
     }
   }
   float top = st.m[t];
@@ -68,15 +69,17 @@ __device__ __forceinline__ void softmax_blocks(const AttnParams& p, RowState<T, 
 #pragma unroll
     for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][i]);
   top = fmaxf(top, other_half(top));
-  const float at = top == kNegInf ? 0.0f : top;
-  if (__any(top != st.m[t])) {                 // the maxima settle after the first tiles
-    const float keep = exp2_fast((st.m[t] - at) * c);
+  // m is the maximum of the tile that last moved it. It follows only where a row's maximum has grown by
+  // more than 8 (in log2), which leaves probabilities up to 256 (no loss in floating point) and saves
+  // scaling the outputs after most tiles, where some row's maximum still grows a little.
+  if (__any((top - st.m[t]) * c > 8.0f)) {
+    const float at = top == kNegInf ? 0.0f : top, keep = exp2_fast((st.m[t] - at) * c);
     st.l[t] *= keep;
 #pragma unroll
     for (int d = 0; d < RowState<T, DP, QT>::DT; ++d) st.o[t][d] *= keep;
     st.m[t] = top;
   }
-  const float mc = at * c;
+  const float mc = (st.m[t] == kNegInf ? 0.0f : st.m[t]) * c;
   float sum = 0;
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb) {
@@ -135,6 +138,7 @@ __global__ __launch_bounds__(256, tile_waves<T>(DP, KIND)) void attn_fwd_tile_ke
     vr.load(v + j0 * p.vs[1], p.vs[1], n - j0, p.D, threadIdx.x);
     put(0, 0);
   }
+  wait_loads();
   for (int64_t j = j0; j < n; j += KT, ++at) {
     const int64_t next = j + KT;
     if (next < n) {
@@ -253,6 +257,7 @@ __global__ __launch_bounds__(256, few_waves<T>(DP, KIND)) void attn_fwd_few_kern
       ka[t] = j + (l & 31) < n ? load_chunk<T>(row, 2 * t + (l >> 5), p.D) : make_uint4(0, 0, 0, 0);
     vr.load(v + j * p.vs[1], p.vs[1], n - j, p.D, l);
   };
+  wait_loads();
   if (j0 + 32 * w < n) fetch(j0 + 32 * w);
   for (int64_t j = j0 + 32 * w; j < n; j += 128) {
     f32x16 s[QT][1] = {};
