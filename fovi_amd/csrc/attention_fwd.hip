@@ -94,6 +94,11 @@ __device__ __forceinline__ void softmax_blocks(const AttnParams& p, RowState<T, 
   st.l[t] += sum;
 }
 
+// Partial results: unscaled outputs [split][key head][row][D], then (maximum, sum) of each.
+__device__ __forceinline__ float2* part_stats(const AttnParams& p) {
+  return reinterpret_cast<float2*>(p.part + static_cast<int64_t>(p.splits) * p.B * p.Hk * p.R * p.D);
+}
+
 __device__ __forceinline__ int64_t stat_at(const AttnParams& p, int64_t b, int hk, int64_t r) {
   return (b * p.H + static_cast<int64_t>(hk) * p.G) * p.Lq + r;      // row (b, head, query) of the statistics
 }
@@ -149,30 +154,32 @@ __global__ __launch_bounds__(256, tile_waves<T>(DP, KIND)) void attn_fwd_tile_ke
     const char* kt = tiles[at & 1][0];
     const char* vt = tiles[at & 1][1];
     const int l = threadIdx.x & 63;
-    f32x16 s[QT][KB] = {};
-    Block<T> e[QT][KB];
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-      for (int t = 0; t < STEPS; ++t) {
-        const uint4 a = *reinterpret_cast<const uint4*>(kt + kb * 32 * LP * sizeof(T) + tile_at<T, LP>(l & 31, 2 * t + (l >> 5)));
-#pragma unroll
-        for (int q = 0; q < QT; ++q) s[q][kb] = mma_step(T(), a, st.q[q][t], s[q][kb]);
-      }
-#pragma unroll
-    for (int q = 0; q < QT; ++q) softmax_blocks<T, DP, QT, KIND, KB>(p, st, q, s[q], e[q], j, n);
-    if (KIND && bad_tile[at & 1] == at) {
-#pragma unroll
-      for (int q = 0; q < QT; ++q)
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) slow_second<T, LP, DT>(vt, kb * 32, s[q][kb], st.o[q]);
-    } else {
+    if (r0 < p.R) {                                    // (the last workgroup's waves may have no rows)
+      f32x16 s[QT][KB] = {};
+      Block<T> e[QT][KB];
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
+        for (int t = 0; t < STEPS; ++t) {
+          const uint4 a = *reinterpret_cast<const uint4*>(kt + kb * 32 * LP * sizeof(T) + tile_at<T, LP>(l & 31, 2 * t + (l >> 5)));
+#pragma unroll
+          for (int q = 0; q < QT; ++q) s[q][kb] = mma_step(T(), a, st.q[q][t], s[q][kb]);
+        }
+#pragma unroll
+      for (int q = 0; q < QT; ++q) softmax_blocks<T, DP, QT, KIND, KB>(p, st, q, s[q], e[q], j, n);
+      if (KIND && bad_tile[at & 1] == at) {
+#pragma unroll
         for (int q = 0; q < QT; ++q)
 #pragma unroll
-          for (int d = 0; d < DT; ++d) st.o[q][d] = mma_second<LP>(T(), vt, kb * 32, d, e[q][kb], st.o[q][d]);
+          for (int kb = 0; kb < KB; ++kb) slow_second<T, LP, DT>(vt, kb * 32, s[q][kb], st.o[q]);
+      } else {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int q = 0; q < QT; ++q)
+#pragma unroll
+            for (int d = 0; d < DT; ++d) st.o[q][d] = mma_second<LP>(T(), vt, kb * 32, d, e[q][kb], st.o[q][d]);
+      }
     }
     if (next < n) put((at + 1) & 1, at + 1);
   }
@@ -183,15 +190,14 @@ __global__ __launch_bounds__(256, tile_waves<T>(DP, KIND)) void attn_fwd_tile_ke
     const float sum = st.l[q] + other_half(st.l[q]), m = KIND ? st.m[q] : st.m[q] * p.c;
     if (r >= p.R) continue;
     if (p.splits > 1) {
-      float* out = p.part + ((split * p.B * p.Hk + bh) * p.R + r) * (p.D + 2);
-      if (lane < 32) { out[p.D] = m; out[p.D + 1] = sum; }
+      const int64_t row = (split * p.B * p.Hk + bh) * p.R + r;
+      if (lane < 32) part_stats(p)[row] = make_float2(m, sum);
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int at_d = d * 32 + 8 * (e / 4) + 4 * (lane >> 5) + e % 4;
-          if (at_d < p.D) out[at_d] = st.o[q][d][e];
-        }
+        for (int e = 0; e < 16; e += 4)
+          store_run(p.part + row * p.D, d * 32 + 2 * e + 4 * (lane >> 5), p.D, st.o[q][d][e], st.o[q][d][e + 1], st.o[q][d][e + 2],
+                    st.o[q][d][e + 3]);
       continue;
     }
     const int64_t g = r / p.Lq, i = r - g * p.Lq, off = b * p.os[0] + i * p.os[1] + (hk * p.G + g) * p.os[2];
@@ -308,9 +314,9 @@ __global__ __launch_bounds__(256, few_waves<T>(DP, KIND)) void attn_fwd_few_kern
       }
       const int64_t row = q * 32 + r;
       if (p.splits > 1) {
-        float* out = p.part + ((split * p.B * p.Hk + bh) * p.R + row) * (p.D + 2);
-        out[d] = value;
-        if (d == 0) { out[p.D] = m; out[p.D + 1] = total; }
+        const int64_t at_row = (split * p.B * p.Hk + bh) * p.R + row;
+        p.part[at_row * p.D + d] = value;
+        if (d == 0) part_stats(p)[at_row] = make_float2(m, total);
       } else {
         put_row<T>(p, b, hk, row, d, value, m, total);
       }
@@ -318,33 +324,51 @@ __global__ __launch_bounds__(256, few_waves<T>(DP, KIND)) void attn_fwd_few_kern
   }
 }
 
-// The partial results of a row's splits added up; one wave per row.
-template <typename T>
+// The partial results of a row's splits added up in a fixed order: 32 lanes a row and group, four
+// elements each; GROUPS 8 (one row a workgroup) where there are many splits, whose loads would
+// otherwise follow one another (256 splits of 16 x 4 rows: 191 us by one wave a row).
+template <typename T, int GROUPS>
 __global__ __launch_bounds__(256) void attn_fwd_join_kernel(AttnParams p) {
-  const int64_t rows = p.B * p.Hk * p.R, x = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  __shared__ float sh[GROUPS][32][6];
+  const int64_t rows = p.B * p.Hk * p.R, x = static_cast<int64_t>(blockIdx.x) * (8 / GROUPS) + (GROUPS == 1 ? threadIdx.x >> 5 : 0);
   if (x >= rows) return;
-  const int l = threadIdx.x & 63;
-  const int64_t bh = x / p.R, b = bh / p.Hk, len = attn_len(p, b), step = rows * (p.D + 2);
-  int64_t used = (len + p.chunk - 1) / p.chunk;
+  const int d = (threadIdx.x & 31) * 4, group = GROUPS == 1 ? 0 : threadIdx.x >> 5;
+  const int64_t bh = x / p.R, b = bh / p.Hk, len = attn_len(p, b);
+  int used = static_cast<int>((len + p.chunk - 1) / p.chunk);
   if (used < 1) used = 1;
-  const float* part = p.part + x * (p.D + 2);
-  float m = kNegInf;
-  for (int64_t s = l; s < used; s += 64) m = fmaxf(m, part[s * step + p.D]);
+  const float2* stats = part_stats(p) + x;
+  float m = kNegInf, sum = 0;
+  f32x4 y = {};
+#pragma unroll 4
+  for (int s = group; s < used; s += GROUPS) {
+    const float2 ml = stats[s * rows];
+    const f32x4 v = d < p.D ? *reinterpret_cast<const f32x4*>(p.part + (s * rows + x) * p.D + d) : f32x4{};
+    const float top = fmaxf(m, ml.x), at = top == kNegInf ? 0.0f : top, old = exp2_fast(m - at), f = exp2_fast(ml.x - at);
+    sum = fmaf(sum, old, ml.y * f);
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-  const float at = m == kNegInf ? 0.0f : m;
-  float sum = 0, y[2] = {0, 0};
-  for (int64_t s = 0; s < used; ++s) {
-    const float* row = part + s * step;
-    const float f = exp2_fast(row[p.D] - at);
-    sum = fmaf(row[p.D + 1], f, sum);
+    for (int e = 0; e < 4; ++e) y[e] = fmaf(y[e], old, v[e] * f);
+    m = top;
+  }
+  if (GROUPS > 1) {
+    float* mine = sh[group][threadIdx.x & 31];
+    mine[0] = m; mine[1] = sum;
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
-      if (l + 64 * c < p.D) y[c] = fmaf(row[l + 64 * c], f, y[c]);
+    for (int e = 0; e < 4; ++e) mine[2 + e] = y[e];
+    __syncthreads();
+    if (group) return;
+#pragma unroll
+    for (int g = 1; g < GROUPS; ++g) {
+      const float* o = sh[g][threadIdx.x & 31];
+      const float top = fmaxf(m, o[0]), at = top == kNegInf ? 0.0f : top, old = exp2_fast(m - at), f = exp2_fast(o[0] - at);
+      sum = fmaf(sum, old, o[1] * f);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = fmaf(y[e], old, o[2 + e] * f);
+      m = top;
+    }
   }
 #pragma unroll
-  for (int c = 0; c < 2; ++c)
-    if (l + 64 * c < p.D) put_row<T>(p, b, static_cast<int>(bh - b * p.Hk), x - bh * p.R, l + 64 * c, y[c], m, sum);
+  for (int e = 0; e < 4; ++e)
+    if (d + e < p.D) put_row<T>(p, b, static_cast<int>(bh - b * p.Hk), x - bh * p.R, d + e, y[e], m, sum);
 }
 
 // How a call is laid out. Few rows: every workgroup has them all. Else tiles of 128 or 256 rows.
@@ -353,6 +377,12 @@ struct FwdPlan {
   int qt, splits;
   int64_t tiles, chunk;
 };
+
+// Workgroups of the few-row kernel on a compute unit: its waves a SIMD.
+static int few_waves_at(int dtype, int64_t D, bool mask) {
+  const int dp = D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128;
+  return dtype == FOVI_BF16 ? few_waves<uint16_t>(dp, mask) + (dp <= 64 && !mask) : few_waves<float>(dp, mask);
+}
 
 static FwdPlan fwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t D, int dtype, bool mask) {
   FwdPlan f;
@@ -363,13 +393,18 @@ static FwdPlan fwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk
     f.qt = R <= 32 ? 1 : 2;
     f.tiles = 1;
   } else {
-    f.qt = two && R > 128 ? 2 : 1;
+    // 256 rows a workgroup read each state half as often, unless they leave more rows empty
+    f.qt = two && (R + 255) / 256 * 16 <= (R + 127) / 128 * 9 ? 2 : 1;
     f.tiles = (R + 128 * f.qt - 1) / (128 * f.qt);
   }
-  // about four workgroups a compute unit (few rows), two (tiles), each with at least 256 states
-  const int64_t groups = B * Hk * f.tiles, want = f.few ? 1024 : 512;
+  // The states are split until the card is full (few rows: twice, lengths differ), in parts that are
+  // still worth a workgroup's start and the join: 512 states for few rows (131072 states, 4 groups, heads
+  // of 128: parts of 512 60 + 9 us, of 256 80 + 14), 128 for tiles (515 states, 32 groups, fp32 under a
+  // mask: parts of 128 14 us, of 256 23; the join 5 each).
+  const int waves = f.few ? few_waves_at(dtype, D, mask) : 2;
+  const int64_t groups = B * Hk * f.tiles, want = f.few ? 512 * waves : 512, least = f.few ? 512 : 128;
   int64_t splits = groups > 0 ? want / groups : 1;
-  if (splits > (Lk + 255) / 256) splits = (Lk + 255) / 256;
+  if (splits > (Lk + least - 1) / least) splits = (Lk + least - 1) / least;
   if (splits > 1024) splits = 1024;
   if (splits < 1) splits = 1;
   f.chunk = ((Lk + splits - 1) / splits + 127) / 128 * 128;
@@ -422,7 +457,8 @@ static int fwd_type(AttnParams& p, hipStream_t s) {
   if (check_launch("fovi_attention_fwd")) return 1;
   if (f.splits > 1) {
     const int64_t rows = p.B * p.Hk * p.R;
-    attn_fwd_join_kernel<T><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, s>>>(p);
+    if (f.splits >= 16) attn_fwd_join_kernel<T, 8><<<static_cast<unsigned>(rows), 256, 0, s>>>(p);
+    else attn_fwd_join_kernel<T, 1><<<static_cast<unsigned>((rows + 7) / 8), 256, 0, s>>>(p);
     return check_launch("fovi_attention_fwd");
   }
   return 0;
