@@ -27,10 +27,10 @@ def _strides(t):
 
 def _whole(t):
     """Whether the kernels can read (or write) ``t`` where it is: heads of whole 16-byte pieces at
-    aligned addresses."""
+    aligned addresses, tokens less than 64 MiB apart."""
     rest = (7 if t.dtype == torch.bfloat16 else 3)
     s0, s1, s2 = _strides(t)
-    return t.stride(3) == 1 and (s0 | s1 | s2 | t.shape[3]) & rest == 0 and t.data_ptr() & 15 == 0
+    return t.stride(3) == 1 and (s0 | s1 | s2 | t.shape[3]) & rest == 0 and t.data_ptr() & 15 == 0 and s1 < 1 << 24
 
 
 def _pieces(t):

@@ -40,6 +40,7 @@ __device__ __forceinline__ int64_t attn_len(const AttnParams& p, int64_t b) {
   return n < 0 ? 0 : n < p.Lk ? n : p.Lk;
 }
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));     // (a struct of four would be loaded in parts)
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
@@ -47,20 +48,20 @@ template <typename T> struct Chunk { static constexpr int N = 16 / sizeof(T); };
 
 // 16 bytes of a row from element c * N on; zeros beyond the D elements of a head (a multiple of N).
 template <typename T>
-__device__ __forceinline__ uint4 load_chunk(const T* row, int c, int D) {
-  return c * Chunk<T>::N < D ? *reinterpret_cast<const uint4*>(row + c * Chunk<T>::N) : make_uint4(0, 0, 0, 0);
+__device__ __forceinline__ u32x4 load_chunk(const T* row, int c, int D) {
+  return c * Chunk<T>::N < D ? *reinterpret_cast<const u32x4*>(row + c * Chunk<T>::N) : u32x4{0, 0, 0, 0};
 }
 
 // Whether any of the chunk's values is infinite or NaN.
-template <typename T> __device__ __forceinline__ bool chunk_bad(uint4 u);
-template <> __device__ __forceinline__ bool chunk_bad<float>(uint4 u) {
+template <typename T> __device__ __forceinline__ bool chunk_bad(u32x4 u);
+template <> __device__ __forceinline__ bool chunk_bad<float>(u32x4 u) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
   bool bad = false;
 #pragma unroll
   for (int i = 0; i < 4; ++i) bad |= (w[i] & 0x7f800000u) == 0x7f800000u;
   return bad;
 }
-template <> __device__ __forceinline__ bool chunk_bad<uint16_t>(uint4 u) {
+template <> __device__ __forceinline__ bool chunk_bad<uint16_t>(u32x4 u) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
   bool bad = false;
 #pragma unroll
@@ -87,10 +88,10 @@ template <typename T, int LP> __device__ __forceinline__ int tile_at(int r, int 
 }
 
 // One step of a product over the head elements: both operands hold the chunk 2 t + l / 32 of their row.
-__device__ __forceinline__ f32x16 mma_step(uint16_t, uint4 a, uint4 b, f32x16 c) {
+__device__ __forceinline__ f32x16 mma_step(uint16_t, u32x4 a, u32x4 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
-__device__ __forceinline__ f32x16 mma_step(float, uint4 a, uint4 b, f32x16 c) {
+__device__ __forceinline__ f32x16 mma_step(float, u32x4 a, u32x4 b, f32x16 c) {
   c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.x), __uint_as_float(b.x), c, 0, 0, 0);
   c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.y), __uint_as_float(b.y), c, 0, 0, 0);
   c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.z), __uint_as_float(b.z), c, 0, 0, 0);
@@ -142,30 +143,86 @@ __device__ __forceinline__ s16x4 read_tr(const char* p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p));
 }
 
-// acc[32 head elements dt * 32 .. , columns] += tile[base .. base + 31, those elements]^T * block
-template <int LP>
-__device__ __forceinline__ f32x16 mma_second(uint16_t, const char* tile, int base, int dt, const Block<uint16_t>& s, f32x16 acc) {
-  const int l = threadIdx.x & 63;
-  const int r = 4 * (l >> 5) + ((l & 15) >> 2), c = dt * 4 + 2 * ((l >> 4) & 1) + ((l & 3) >> 1);
+// The A operand of tile[base .. base + 31, 32 head elements dt * 32 ..]^T, in the order of a block, and
+// acc += it * block. Reads and products are apart so that the reads of several operands can be in
+// flight together: left to itself the compiler saves registers and waits for every one.
+template <typename T, int LP> struct Turned;
+template <int LP> struct Turned<uint16_t, LP> {
+  bf16x8 a[2];
+  __device__ __forceinline__ void read(const char* tile, int base, int dt) {
+    const int l = threadIdx.x & 63;
+    const int r = 4 * (l >> 5) + ((l & 15) >> 2), c = dt * 4 + 2 * ((l >> 4) & 1) + ((l & 3) >> 1);
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const char* at = tile + (base + 16 * t) * LP * 2 + (l & 1) * 8;
-    const s16x4 lo = read_tr(at + tile_at<uint16_t, LP>(r, c)), hi = read_tr(at + tile_at<uint16_t, LP>(r + 8, c));
-    const bf16x8 a = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, s.b[t], acc, 0, 0, 0);
+    for (int t = 0; t < 2; ++t) {
+      const char* at = tile + (base + 16 * t) * LP * 2 + (l & 1) * 8;
+      const s16x4 lo = read_tr(at + tile_at<uint16_t, LP>(r, c)), hi = read_tr(at + tile_at<uint16_t, LP>(r + 8, c));
+      a[t] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
   }
-  return acc;
+  __device__ __forceinline__ f32x16 mma(const Block<uint16_t>& s, f32x16 acc) const {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], s.b[0], acc, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[1], s.b[1], acc, 0, 0, 0);
+  }
+};
+template <int LP> struct Turned<float, LP> {
+  float a[16];
+  __device__ __forceinline__ void read(const char* tile, int base, int dt) {
+    const int l = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int r = 8 * (i / 4) + 4 * (l >> 5) + i % 4, d = dt * 32 + (l & 31);
+      a[i] = *reinterpret_cast<const float*>(tile + base * LP * 4 + tile_at<float, LP>(r, d >> 2) + (d & 3) * 4);
+    }
+  }
+  __device__ __forceinline__ f32x16 mma(const Block<float>& s, f32x16 acc) const {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], s.b[i], acc, 0, 0, 0);
+    return acc;
+  }
+};
+
+// Reads stay above, products below.
+__device__ __forceinline__ void reads_done() { __builtin_amdgcn_sched_barrier(0); }
+
+// s (and s2) += the 32 rows of `tile` (`tile2`) times the columns b (b2), over the head elements.
+template <typename T, int LP, int STEPS>
+__device__ __forceinline__ void row_product(const char* tile, const u32x4 (&b)[STEPS], f32x16& s) {
+  constexpr int G = STEPS < 4 ? STEPS : 4;
+  const int l = threadIdx.x & 63;
+#pragma unroll
+  for (int t = 0; t < STEPS; t += G) {
+    u32x4 a[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+      if (t + g < STEPS) a[g] = *reinterpret_cast<const u32x4*>(tile + tile_at<T, LP>(l & 31, 2 * (t + g) + (l >> 5)));
+    reads_done();
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+      if (t + g < STEPS) s = mma_step(T(), a[g], b[t + g], s);
+  }
 }
-template <int LP>
-__device__ __forceinline__ f32x16 mma_second(float, const char* tile, int base, int dt, const Block<float>& s, f32x16 acc) {
+template <typename T, int LP, int G, int STEPS>
+__device__ __forceinline__ void row_products(const char* tile, const char* tile2, const u32x4 (&b)[STEPS], const u32x4 (&b2)[STEPS],
+                                             f32x16& s, f32x16& s2) {
   const int l = threadIdx.x & 63;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int r = 8 * (i / 4) + 4 * (l >> 5) + i % 4, d = dt * 32 + (l & 31);
-    const float a = *reinterpret_cast<const float*>(tile + base * LP * 4 + tile_at<float, LP>(r, d >> 2) + (d & 3) * 4);
-    acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a, s.b[i], acc, 0, 0, 0);
+  for (int t = 0; t < STEPS; t += G) {
+    u32x4 a[G], a2[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+      if (t + g < STEPS) {
+        const int at = tile_at<T, LP>(l & 31, 2 * (t + g) + (l >> 5));
+        a[g] = *reinterpret_cast<const u32x4*>(tile + at);
+        a2[g] = *reinterpret_cast<const u32x4*>(tile2 + at);
+      }
+    reads_done();
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+      if (t + g < STEPS) {
+        s = mma_step(T(), a[g], b[t + g], s);
+        s2 = mma_step(T(), a2[g], b2[t + g], s2);
+      }
   }
-  return acc;
 }
 
 // The same product pair by pair, leaving out the pairs whose block value is kLeftOut: for tiles that
@@ -196,25 +253,50 @@ __device__ __forceinline__ void slow_second(const char* tile, int base, const f3
   }
 }
 
-// A tile of ROWS rows on its way from memory to LDS through the registers of 256 threads.
-template <typename T, int DP, int LP, int ROWS, int THREADS>
+// A tile of ROWS rows on its way from memory to LDS through the registers of THREADS threads. A thread
+// keeps its 16-byte column; its place in the tile is a 32-bit offset from the tile's (uniform) address, so
+// that a full tile's loads take no vector arithmetic: on this machine matrix and vector instructions of
+// a SIMD hardly overlap, and every vector instruction of the loop adds to its time. Loads are never
+// predicated (that would wait for earlier ones): rows behind the last are the last row again, which
+// the products meet with probability 0, and which every row reads that could notice.
+constexpr int64_t kMostPitch = int64_t(1) << 26;       // bytes between rows: 64 of them stay below 2^32
+
+template <typename T, int LP, int ROWS, int THREADS>
 struct Staged {
-  static constexpr int NC = DP / Chunk<T>::N, N = (ROWS * NC + THREADS - 1) / THREADS;
-  uint4 r[N];
-  // rows [0, n) of `base`, zeros beyond
-  __device__ __forceinline__ void load(const T* base, int64_t stride, int64_t n, int D, int thread) {
+  static constexpr int NC = LP / Chunk<T>::N, STEP = THREADS / NC, N = (ROWS + STEP - 1) / STEP;
+  u32x4 r[N];
+  uint32_t off, pitch, col;   // bytes
+  int row, c;
+  __device__ __forceinline__ void init(int64_t stride, int D, int thread) {
+    row = thread / NC < ROWS ? thread / NC : ROWS - 1;
+    c = thread % NC;
+    col = c * Chunk<T>::N < D ? c * 16 : 0;
+    pitch = static_cast<uint32_t>(stride * static_cast<int64_t>(sizeof(T)));
+    off = row * pitch + col;
+  }
+  // rows [0, n) of `base`, n > 0
+  __device__ __forceinline__ void load(const T* base, int64_t n) {
+    const bool full = n >= ROWS;
+    const int last = full ? ROWS - 1 : static_cast<int>(n) - 1;
+    const char* at = reinterpret_cast<const char*>(base);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int at = thread + i * THREADS, row = at / NC, c = at - row * NC;
-      r[i] = row < n && at < ROWS * NC ? load_chunk<T>(base + row * stride, c, D) : make_uint4(0, 0, 0, 0);
+      uint32_t o = off + i * STEP * pitch;
+      if (!full) o = (row + i * STEP < last ? row + i * STEP : last) * pitch + col;
+      r[i] = *reinterpret_cast<const u32x4*>(at + o);
     }
   }
-  __device__ __forceinline__ void store(char* tile, int thread) const {
+  // Columns behind the D head elements are zero in LDS from the start (clear) and stay so.
+  __device__ __forceinline__ bool in(int D) const { return c * Chunk<T>::N < D; }
+  __device__ __forceinline__ void clear(char* tile, int D) const {
+    if (in(D)) return;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int at = thread + i * THREADS, row = at / NC, c = at - row * NC;
-      if (at < ROWS * NC) *reinterpret_cast<uint4*>(tile + tile_at<T, LP>(row, c)) = r[i];
-    }
+    for (int i = 0; i < N; ++i) *reinterpret_cast<u32x4*>(tile + tile_at<T, LP>(row + i * STEP, c)) = u32x4{0, 0, 0, 0};
+  }
+  __device__ __forceinline__ void store(char* tile, int D) const {
+    if (!in(D)) return;
+#pragma unroll
+    for (int i = 0; i < N; ++i) *reinterpret_cast<u32x4*>(tile + tile_at<T, LP>(row + i * STEP, c)) = r[i];
   }
   __device__ __forceinline__ bool bad() const {
     bool b = false;

@@ -25,9 +25,9 @@ static int attn_check(const fovi_attention_args* a, const char* what) {
   return 0;
 }
 
-// Rows of 16-byte pieces: pointers and strides of whole pieces.
+// Rows of 16-byte pieces: pointers and strides of whole pieces, rows less than kMostPitch apart.
 static bool whole(const void* p, const int64_t* stride, int es) {
-  if (reinterpret_cast<uintptr_t>(p) % 16) return false;
+  if (reinterpret_cast<uintptr_t>(p) % 16 || stride[1] < 0 || stride[1] * es >= kMostPitch) return false;
   for (int i = 0; i < 3; ++i)
     if (stride[i] * es % 16) return false;
   return true;
@@ -37,7 +37,7 @@ static int attn_check_rows(const fovi_attention_args* a, const char* what) {
   const int es = a->dtype == FOVI_BF16 ? 2 : 4;
   if (a->head_dim * es % 16 || !whole(a->q, a->q_stride, es) || !whole(a->k, a->k_stride, es) || !whole(a->v, a->v_stride, es) ||
       !whole(a->out, a->out_stride, es) || !whole(a->out_rest, a->out_stride, es)) {
-    set_error("%s: heads must be whole 16-byte pieces, aligned", what);
+    set_error("%s: heads must be whole 16-byte pieces, aligned, and rows less than 64 MiB apart", what);
     return 1;
   }
   return 0;
@@ -102,7 +102,7 @@ extern "C" int fovi_attention_bwd(const fovi_attention_bwd_args* a, void* stream
   if (attn_check_rows(f, "fovi_attention_bwd")) return 1;
   if (!whole(a->dout, a->dout_stride, es) || !whole(a->dq, a->dq_stride, es) || !whole(a->dk, a->dk_stride, es) ||
       !whole(a->dv, a->dv_stride, es)) {
-    set_error("fovi_attention_bwd: heads must be whole 16-byte pieces, aligned");
+    set_error("fovi_attention_bwd: heads must be whole 16-byte pieces, aligned, and rows less than 64 MiB apart");
     return 1;
   }
   AttnParams p = attn_params(f);

@@ -24,8 +24,8 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(AttnParams p) {
     const int64_t off = b * p.os[0] + i * p.os[1] + h * p.os[2];
     for (int c = threadIdx.x & 15; c * N < p.D; c += 16) {
       T a[N], o[N], r[N];
-      const uint4 ga = load_chunk<T>(g, c, p.D), oa = load_chunk<T>(static_cast<const T*>(p.o) + off, c, p.D);
-      const uint4 ra = p.rest ? load_chunk<T>(static_cast<const T*>(p.rest) + off, c, p.D) : make_uint4(0, 0, 0, 0);
+      const u32x4 ga = load_chunk<T>(g, c, p.D), oa = load_chunk<T>(static_cast<const T*>(p.o) + off, c, p.D);
+      const u32x4 ra = p.rest ? load_chunk<T>(static_cast<const T*>(p.rest) + off, c, p.D) : u32x4{0, 0, 0, 0};
       __builtin_memcpy(a, &ga, 16);
       __builtin_memcpy(o, &oa, 16);
       __builtin_memcpy(r, &ra, 16);
@@ -46,26 +46,26 @@ __device__ __forceinline__ RowStat row_stat(float m, float sum, float delta) {
   return {sum == 0 ? __builtin_inff() : KIND ? m : m + log2f(sum), KIND && sum != 0 ? 1.0f / sum : KIND ? 0.0f : 1.0f, delta};
 }
 
-// Probability and score gradient of one pair; KIND 1: t is the masked score, left-out pairs become kLeftOut.
+// Probability and score gradient of one pair, dp = do.v - delta (the product starts from -delta); KIND 1: t is the masked score, left-out pairs become kLeftOut.
 template <int KIND>
-__device__ __forceinline__ void pair_grad(float t, float c, float shift, float factor, float delta, float dp, float& e, float& ds) {
+__device__ __forceinline__ void pair_grad(float t, float c, float shift, float factor, float dp, float& e, float& ds) {
   if (KIND) {
     const bool out = t == kNegInf || shift == __builtin_inff();
     e = exp2_fast(t - shift) * factor;
-    ds = out ? kLeftOut : e * (dp - delta);
+    ds = out ? kLeftOut : e * dp;
     e = out ? kLeftOut : e;
   } else {
     e = exp2_fast(fmaf(t, c, -shift));
-    ds = e * (dp - delta);
+    ds = e * dp;
   }
 }
 
 // Waves a SIMD shall hold: two wherever a kernel fits 256 registers without spilling much.
 template <typename T> constexpr int dq_waves(int DP, int KIND) {
-  return sizeof(T) == 2 ? (KIND && DP == 128 ? 1 : 2) : DP >= 96 ? 1 : 2;
+  return sizeof(T) == 2 ? (DP == 128 ? 1 : DP == 64 && !KIND ? 3 : 2) : DP >= 96 ? 1 : 2;
 }
 template <typename T> constexpr int dkv_waves(int DP, int KIND) {
-  return sizeof(T) == 2 ? (KIND && DP >= 96 ? 1 : 2) : DP >= 96 || (KIND && DP == 64) ? 1 : 2;
+  return sizeof(T) == 2 ? (DP >= 96 ? 1 : 2) : DP >= 64 ? 1 : 2;
 }
 
 template <typename T, int DP, int QT, int KIND>
@@ -80,9 +80,11 @@ __global__ __launch_bounds__(256, dq_waves<T>(DP, KIND)) void attn_dq_kernel(Att
   const int64_t len = attn_len(p, b), j0 = split * p.chunk, n = len < j0 + p.chunk ? len : j0 + p.chunk;
   if (split && n <= j0) return;
   const int64_t r0 = (id - bh * p.tiles) * (128 * QT) + (threadIdx.x >> 6) * (32 * QT);
-  uint4 q[QT][STEPS], g[QT][STEPS];
+  u32x4 q[QT][STEPS], g[QT][STEPS];
   f32x16 dq[QT][DT] = {};
   RowStat st[QT];
+  constexpr bool START = sizeof(T) == 2 && (DP == 32 || DP==128);   // -delta as a block of its own, where registers allow
+  f32x16 start[START ? QT : 1];
   const void* mrow[QT];
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
@@ -97,30 +99,37 @@ __global__ __launch_bounds__(256, dq_waves<T>(DP, KIND)) void attn_dq_kernel(Att
     }
     const int64_t at = (b * p.H + h) * p.Lq + i;
     st[t] = row_stat<KIND>(p.stats[at], p.stats[p.B * p.H * p.Lq + at], p.delta[at]);
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      if (START) start[t][e] = -st[t].delta;
     mrow[t] = KIND ? mask_row(p, b, h, i) : nullptr;
   }
   const T* k = static_cast<const T*>(p.k) + b * p.ks[0] + hk * p.ks[2];
   const T* v = static_cast<const T*>(p.v) + b * p.vs[0] + hk * p.vs[2];
-  Staged<T, DP, LP, KT, 256> kr, vr;
+  Staged<T, LP, KT, 256> kr, vr;
+  kr.init(p.ks[1], p.D, threadIdx.x);
+  vr.init(p.vs[1], p.D, threadIdx.x);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) kr.clear(tiles[i >> 1][i & 1], p.D);
   if (KIND && threadIdx.x < 2) bad_tile[threadIdx.x] = -1;
   if (KIND) __syncthreads();
   int at = 0;
   auto put = [&](int buf, int tile) {
-    kr.store(tiles[buf][0], threadIdx.x);
-    vr.store(tiles[buf][1], threadIdx.x);
+    kr.store(tiles[buf][0], p.D);
+    vr.store(tiles[buf][1], p.D);
     if (KIND && kr.bad()) bad_tile[buf] = tile;
   };
   if (j0 < n) {
-    kr.load(k + j0 * p.ks[1], p.ks[1], n - j0, p.D, threadIdx.x);
-    vr.load(v + j0 * p.vs[1], p.vs[1], n - j0, p.D, threadIdx.x);
+    kr.load(k + j0 * p.ks[1], n - j0);
+    vr.load(v + j0 * p.vs[1], n - j0);
     put(0, 0);
   }
   wait_loads();
   for (int64_t j = j0; j < n; j += KT, ++at) {
     const int64_t next = j + KT;
     if (next < n) {
-      kr.load(k + next * p.ks[1], p.ks[1], n - next, p.D, threadIdx.x);
-      vr.load(v + next * p.vs[1], p.vs[1], n - next, p.D, threadIdx.x);
+      kr.load(k + next * p.ks[1], n - next);
+      vr.load(v + next * p.vs[1], n - next);
     }
     __syncthreads();
     const char* kt = tiles[at & 1][0];
@@ -128,17 +137,19 @@ __global__ __launch_bounds__(256, dq_waves<T>(DP, KIND)) void attn_dq_kernel(Att
     const int left = static_cast<int>(n - j < KT ? n - j : KT);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
-      f32x16 s[QT] = {}, dp[QT] = {};
+      f32x16 s[QT] = {}, dp[QT];
 #pragma unroll
-      for (int t = 0; t < STEPS; ++t) {
-        const int off = kb * 32 * LP * static_cast<int>(sizeof(T)) + tile_at<T, LP>(l & 31, 2 * t + (l >> 5));
-        const uint4 ka = *reinterpret_cast<const uint4*>(kt + off), va = *reinterpret_cast<const uint4*>(vt + off);
-#pragma unroll
-        for (int x = 0; x < QT; ++x) {
-          s[x] = mma_step(T(), ka, q[x][t], s[x]);
-          dp[x] = mma_step(T(), va, g[x][t], dp[x]);
-        }
+      for (int x = 0; x < QT; ++x) {
+        if (START) dp[x] = start[x];
+        else dp[x] = f32x16{};
       }
+#pragma unroll
+      for (int x = 0; x < QT; ++x)
+        row_products<T, LP, (DP == 64 || DP == 96 ? 2 : STEPS < 4 ? STEPS : 4)>(kt + kb * 32 * LP * sizeof(T), vt + kb * 32 * LP * sizeof(T), q[x], g[x], s[x], dp[x]);
+      Turned<T, LP> ka[DT];
+#pragma unroll
+      for (int d = 0; d < DT; ++d) ka[d].read(kt, kb * 32, d);
+      reads_done();
 #pragma unroll
       for (int x = 0; x < QT; ++x) {
         if (KIND) {
@@ -151,7 +162,7 @@ __global__ __launch_bounds__(256, dq_waves<T>(DP, KIND)) void attn_dq_kernel(Att
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           float e, ds;
-          pair_grad<KIND>(s[x][i], p.c, st[x].shift, st[x].factor, st[x].delta, dp[x][i], e, ds);
+          pair_grad<KIND>(s[x][i], p.c, st[x].shift, st[x].factor, START ? dp[x][i] : dp[x][i] - st[x].delta, e, ds);
           s[x][i] = ds;
         }
         if (KIND && bad_tile[at & 1] == at) {
@@ -159,7 +170,7 @@ __global__ __launch_bounds__(256, dq_waves<T>(DP, KIND)) void attn_dq_kernel(Att
         } else {
           const Block<T> ds(s[x]);
 #pragma unroll
-          for (int d = 0; d < DT; ++d) dq[x][d] = mma_second<LP>(T(), kt, kb * 32, d, ds, dq[x][d]);
+          for (int d = 0; d < DT; ++d) dq[x][d] = ka[d].mma(ds, dq[x][d]);
         }
       }
     }
@@ -200,7 +211,7 @@ __global__ __launch_bounds__(256, dkv_waves<T>(DP, KIND)) void attn_dkv_kernel(A
   const int64_t n = attn_len(p, b), w0 = (id - bh * p.tiles) * 128, j = w0 + (threadIdx.x >> 6) * 32 + (l & 31);
   const T* kp = static_cast<const T*>(p.k) + b * p.ks[0] + j * p.ks[1] + hk * p.ks[2];
   const T* vp = static_cast<const T*>(p.v) + b * p.vs[0] + j * p.vs[1] + hk * p.vs[2];
-  uint4 k[STEPS], v[STEPS];
+  u32x4 k[STEPS], v[STEPS];
 #pragma unroll
   for (int s = 0; s < STEPS; ++s) {
     k[s] = load_chunk<T>(kp, 2 * s + (l >> 5), j < n ? p.D : 0);
@@ -211,14 +222,18 @@ __global__ __launch_bounds__(256, dkv_waves<T>(DP, KIND)) void attn_dkv_kernel(A
   const int per = static_cast<int>((p.Lq + RT - 1) / RT);
   const int64_t first = split * p.chunk, end = static_cast<int64_t>(per) * p.G;
   const int count = w0 >= n ? 0 : static_cast<int>(end < first + p.chunk ? end - first : p.chunk);
-  Staged<T, DP, LP, RT, 256> qr, gr;
+  Staged<T, LP, RT, 256> qr, gr;
+  qr.init(p.qs[1], p.D, threadIdx.x);
+  gr.init(p.dos[1], p.D, threadIdx.x);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) qr.clear(tiles[i >> 1][i & 1], p.D);
   float m = 0, sum = 0, delta = 0;                 // raw: nothing waits for them before the tile is stored
   if (KIND && threadIdx.x < 4) bad_tile[threadIdx.x >> 1][threadIdx.x & 1] = -1;
   if (KIND) __syncthreads();
   int h = hk * p.G + static_cast<int>(first / per), i0 = static_cast<int>(first % per) * RT;      // the next tile to fetch
   auto fetch = [&]() {
-    qr.load(static_cast<const T*>(p.q) + b * p.qs[0] + i0 * p.qs[1] + h * p.qs[2], p.qs[1], p.Lq - i0, p.D, threadIdx.x);
-    gr.load(static_cast<const T*>(p.dout) + b * p.dos[0] + i0 * p.dos[1] + h * p.dos[2], p.dos[1], p.Lq - i0, p.D, threadIdx.x);
+    qr.load(static_cast<const T*>(p.q) + b * p.qs[0] + i0 * p.qs[1] + h * p.qs[2], p.Lq - i0);
+    gr.load(static_cast<const T*>(p.dout) + b * p.dos[0] + i0 * p.dos[1] + h * p.dos[2], p.Lq - i0);
     if (threadIdx.x < RT) {
       const bool in = i0 + threadIdx.x < p.Lq;
       const int64_t at = (b * p.H + h) * p.Lq + (in ? i0 + threadIdx.x : 0);
@@ -228,13 +243,13 @@ __global__ __launch_bounds__(256, dkv_waves<T>(DP, KIND)) void attn_dkv_kernel(A
     }
   };
   auto put = [&](int buf, int tile) {
-    qr.store(tiles[buf][0], threadIdx.x);
-    gr.store(tiles[buf][1], threadIdx.x);
+    qr.store(tiles[buf][0], p.D);
+    gr.store(tiles[buf][1], p.D);
     if (threadIdx.x < RT) {
       const RowStat sr = row_stat<KIND>(m, sum, sum == 0 ? 0.0f : delta);
       stats[buf][0][threadIdx.x] = sr.shift;
       if (KIND) stats[buf][1][threadIdx.x] = sr.factor;
-      stats[buf][2][threadIdx.x] = sr.delta;
+      stats[buf][2][threadIdx.x] = -sr.delta;
     }
     if (KIND && qr.bad()) bad_tile[buf][0] = tile;
     if (KIND && gr.bad()) bad_tile[buf][1] = tile;
@@ -254,13 +269,18 @@ __global__ __launch_bounds__(256, dkv_waves<T>(DP, KIND)) void attn_dkv_kernel(A
     for (int rb = 0; rb < RB; ++rb) {
       const char* qt = tiles[at & 1][0] + rb * 32 * LP * sizeof(T);
       const char* gt = tiles[at & 1][1] + rb * 32 * LP * sizeof(T);
-      f32x16 s = {}, dp = {};
+      f32x16 s = {}, dp;
 #pragma unroll
-      for (int t = 0; t < STEPS; ++t) {
-        const int off = tile_at<T, LP>(l & 31, 2 * t + (l >> 5));
-        s = mma_step(T(), *reinterpret_cast<const uint4*>(qt + off), k[t], s);
-        dp = mma_step(T(), *reinterpret_cast<const uint4*>(gt + off), v[t], dp);
+      for (int i = 0; i < 16; i += 4) {
+        const f32x4 start = *reinterpret_cast<const f32x4*>(&stats[at & 1][2][rb * 32 + 2 * i + 4 * (l >> 5)]);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) dp[i + y] = start[y];
       }
+      row_products<T, LP, (STEPS < 4 ? STEPS : 4)>(qt, gt, k, v, s, dp);
+      Turned<T, LP> ga[DT], qa[DT];
+#pragma unroll
+      for (int d = 0; d < DT; ++d) ga[d].read(gt, 0, d);
+      reads_done();
       if (KIND) {
         const char* col = static_cast<const char*>(mask_row(p, b, h_at, 0)) + (j < n ? j : 0) * p.ms[3] * (p.kind == FOVI_MASK_KEEP ? 1 : 4);
         mask_column(p, col, i_at + rb * 32 + 4 * (l >> 5), j < n ? p.Lq : 0, s);
@@ -268,13 +288,13 @@ __global__ __launch_bounds__(256, dkv_waves<T>(DP, KIND)) void attn_dkv_kernel(A
 #pragma unroll
       for (int i = 0; i < 16; i += 4) {
         const int r = rb * 32 + 2 * i + 4 * (l >> 5);
-        const f32x4 shift = *reinterpret_cast<const f32x4*>(&stats[at & 1][0][r]), delta = *reinterpret_cast<const f32x4*>(&stats[at & 1][2][r]);
+        const f32x4 shift = *reinterpret_cast<const f32x4*>(&stats[at & 1][0][r]);
         f32x4 factor;
         if (KIND) factor = *reinterpret_cast<const f32x4*>(&stats[at & 1][1][r]);
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
           float e, ds;
-          pair_grad<KIND>(s[i + y], p.c, shift[y], KIND ? factor[y] : 1.0f, delta[y], dp[i + y], e, ds);
+          pair_grad<KIND>(s[i + y], p.c, shift[y], KIND ? factor[y] : 1.0f, dp[i + y], e, ds);
           s[i + y] = e;
           dp[i + y] = ds;
         }
@@ -284,14 +304,22 @@ __global__ __launch_bounds__(256, dkv_waves<T>(DP, KIND)) void attn_dkv_kernel(A
       } else {
         const Block<T> e(s);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) dv[d] = mma_second<LP>(T(), gt, 0, d, e, dv[d]);
+        for (int d = 0; d < DT; ++d)
+          if (!KIND) qa[d].read(qt, 0, d);
+        reads_done();
+#pragma unroll
+        for (int d = 0; d < DT; ++d) dv[d] = ga[d].mma(e, dv[d]);
       }
       if (KIND && bad_tile[at & 1][0] == at) {
         slow_second<T, LP, DT>(qt, 0, dp, dk);
       } else {
         const Block<T> ds(dp);
+        if (KIND) {
 #pragma unroll
-        for (int d = 0; d < DT; ++d) dk[d] = mma_second<LP>(T(), qt, 0, d, ds, dk[d]);
+          for (int d = 0; d < DT; ++d) qa[d].read(qt, 0, d);
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d) dk[d] = qa[d].mma(ds, dk[d]);
       }
     }
     if (at + 1 < count) put((at + 1) & 1, at + 1);

@@ -17,7 +17,7 @@ namespace fovi {
 template <typename T, int DP, int QT>
 struct RowState {
   static constexpr int DT = DP / 32, STEPS = DP / (2 * Chunk<T>::N);
-  uint4 q[QT][STEPS];
+  u32x4 q[QT][STEPS];
   f32x16 o[QT][DT];
   float m[QT], l[QT];         // the row's maximum so far, or a little less; the lane's share of the sum
   const void* mrow[QT];
@@ -34,7 +34,7 @@ __device__ __forceinline__ void init_rows(const AttnParams& p, RowState<T, DP, Q
     const T* q = static_cast<const T*>(p.q) + b * p.qs[0] + i * p.qs[1] + h * p.qs[2];
 #pragma unroll
     for (int s = 0; s < RowState<T, DP, QT>::STEPS; ++s)
-      st.q[t][s] = r < p.R ? load_chunk<T>(q, 2 * s + (l >> 5), p.D) : make_uint4(0, 0, 0, 0);
+      st.q[t][s] = r < p.R ? load_chunk<T>(q, 2 * s + (l >> 5), p.D) : u32x4{0, 0, 0, 0};
     st.m[t] = kNegInf;
     st.l[t] = 0;
     st.mrow[t] = p.kind ? mask_row(p, b, h, i) : nullptr;
@@ -106,16 +106,16 @@ __device__ __forceinline__ int64_t stat_at(const AttnParams& p, int64_t b, int h
 // Waves a SIMD shall hold: two (256 registers each) wherever a kernel fits without spilling much; a lone
 // wave waits out every latency (bf16, heads of 64, 1024 x 4096 x 192 heads: 602 us with one, 390 with two).
 template <typename T> constexpr int tile_waves(int DP, int KIND) {
-  return sizeof(T) == 2 ? (KIND && DP == 128 ? 1 : 2) : (DP == 128 || (KIND && DP == 96) ? 1 : 2);
+  return sizeof(T) == 2 ? (KIND ? (DP == 128 ? 1 : 2) : DP <= 64 ? 3 : 2) : (DP == 128 || (KIND && DP == 96) ? 1 : 2);
 }
 template <typename T> constexpr int few_waves(int DP, int KIND) {
   return sizeof(T) == 2 ? (KIND && DP >= 96 ? 1 : 2) : (DP >= 96 || (KIND && DP == 64) ? 1 : 2);
 }
 
-template <typename T, int DP, int QT, int KIND>
+template <typename T, int DP, int KIND>
 __global__ __launch_bounds__(256, tile_waves<T>(DP, KIND)) void attn_fwd_tile_kernel(AttnParams p) {
   constexpr int LP = DP == 96 ? 128 : DP, KB = sizeof(T) == 2 ? 2 : 1, KT = 32 * KB, DT = DP / 32;
-  constexpr int STEPS = RowState<T, DP, QT>::STEPS;
+  constexpr int STEPS = RowState<T, DP, 1>::STEPS;
   __shared__ __attribute__((aligned(16))) char tiles[2][2][KT * LP * sizeof(T)];
   __shared__ int bad_tile[2];
   const int64_t all = p.tiles * p.B * p.Hk, id = xcd_tile(blockIdx.x, gridDim.x);
@@ -124,71 +124,73 @@ __global__ __launch_bounds__(256, tile_waves<T>(DP, KIND)) void attn_fwd_tile_ke
   const int hk = static_cast<int>(bh - b * p.Hk), split = blockIdx.y;
   const int64_t len = attn_len(p, b), j0 = split * p.chunk, n = len < j0 + p.chunk ? len : j0 + p.chunk;
   if (split && n <= j0) return;                        // (split 0 writes the rows of images without states)
-  const int64_t r0 = (id - bh * p.tiles) * (128 * QT) + (threadIdx.x >> 6) * (32 * QT);
-  RowState<T, DP, QT> st;
-  init_rows<T, DP, QT>(p, st, b, hk, r0);
+  const int64_t r0 = (id - bh * p.tiles) * 128 + (threadIdx.x >> 6) * 32;
+  RowState<T, DP, 1> st;
+  init_rows<T, DP, 1>(p, st, b, hk, r0);
   const T* k = static_cast<const T*>(p.k) + b * p.ks[0] + hk * p.ks[2];
   const T* v = static_cast<const T*>(p.v) + b * p.vs[0] + hk * p.vs[2];
-  Staged<T, DP, LP, KT, 256> kr, vr;
+  Staged<T, LP, KT, 256> kr, vr;
+  kr.init(p.ks[1], p.D, threadIdx.x);
+  vr.init(p.vs[1], p.D, threadIdx.x);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) kr.clear(tiles[i >> 1][i & 1], p.D);
   if (KIND && threadIdx.x < 2) bad_tile[threadIdx.x] = -1;
   if (KIND) __syncthreads();
   int at = 0;
   auto put = [&](int buf, int tile) {
-    kr.store(tiles[buf][0], threadIdx.x);
-    vr.store(tiles[buf][1], threadIdx.x);
+    kr.store(tiles[buf][0], p.D);
+    vr.store(tiles[buf][1], p.D);
     if (KIND && vr.bad()) bad_tile[buf] = tile;
   };
   if (j0 < n) {
-    kr.load(k + j0 * p.ks[1], p.ks[1], n - j0, p.D, threadIdx.x);
-    vr.load(v + j0 * p.vs[1], p.vs[1], n - j0, p.D, threadIdx.x);
+    kr.load(k + j0 * p.ks[1], n - j0);
+    vr.load(v + j0 * p.vs[1], n - j0);
     put(0, 0);
   }
   wait_loads();
   for (int64_t j = j0; j < n; j += KT, ++at) {
     const int64_t next = j + KT;
     if (next < n) {
-      kr.load(k + next * p.ks[1], p.ks[1], n - next, p.D, threadIdx.x);
-      vr.load(v + next * p.vs[1], p.vs[1], n - next, p.D, threadIdx.x);
+      kr.load(k + next * p.ks[1], n - next);
+      vr.load(v + next * p.vs[1], n - next);
     }
     __syncthreads();                                   // tile `at` is in LDS, tile at - 1 is done with
     const char* kt = tiles[at & 1][0];
     const char* vt = tiles[at & 1][1];
-    const int l = threadIdx.x & 63;
     if (r0 < p.R) {                                    // (the last workgroup's waves may have no rows)
-      f32x16 s[QT][KB] = {};
-      Block<T> e[QT][KB];
+      f32x16 s[KB] = {};
+      Block<T> e[KB];
+      Turned<T, LP> va[2][DT];
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
+      for (int kb = 0; kb < KB; ++kb) row_product<T, LP>(kt + kb * 32 * LP * sizeof(T), st.q[0], s[kb]);
 #pragma unroll
-        for (int t = 0; t < STEPS; ++t) {
-          const uint4 a = *reinterpret_cast<const uint4*>(kt + kb * 32 * LP * sizeof(T) + tile_at<T, LP>(l & 31, 2 * t + (l >> 5)));
-#pragma unroll
-          for (int q = 0; q < QT; ++q) s[q][kb] = mma_step(T(), a, st.q[q][t], s[q][kb]);
-        }
-#pragma unroll
-      for (int q = 0; q < QT; ++q) softmax_blocks<T, DP, QT, KIND, KB>(p, st, q, s[q], e[q], j, n);
+      for (int d = 0; d < DT; ++d) va[0][d].read(vt, 0, d);
+      reads_done();
+      softmax_blocks<T, DP, 1, KIND, KB>(p, st, 0, s, e, j, n);
       if (KIND && bad_tile[at & 1] == at) {
 #pragma unroll
-        for (int q = 0; q < QT; ++q)
-#pragma unroll
-          for (int kb = 0; kb < KB; ++kb) slow_second<T, LP, DT>(vt, kb * 32, s[q][kb], st.o[q]);
+        for (int kb = 0; kb < KB; ++kb) slow_second<T, LP, DT>(vt, kb * 32, s[kb], st.o[0]);
       } else {
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
+        for (int kb = 0; kb < KB; ++kb) {
+          if (kb + 1 < KB) {
 #pragma unroll
-          for (int q = 0; q < QT; ++q)
+            for (int d = 0; d < DT; ++d) va[(kb + 1) & 1][d].read(vt, (kb + 1) * 32, d);
+            reads_done();
+          }
 #pragma unroll
-            for (int d = 0; d < DT; ++d) st.o[q][d] = mma_second<LP>(T(), vt, kb * 32, d, e[q][kb], st.o[q][d]);
+          for (int d = 0; d < DT; ++d) st.o[0][d] = va[kb & 1][d].mma(e[kb], st.o[0][d]);
+        }
       }
     }
     if (next < n) put((at + 1) & 1, at + 1);
   }
   const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int q = 0; q < QT; ++q) {
-    const int64_t r = r0 + 32 * q + (lane & 31);
+  {
+    constexpr int q = 0;
+    const int64_t r = r0 + (lane & 31);
     const float sum = st.l[q] + other_half(st.l[q]), m = KIND ? st.m[q] : st.m[q] * p.c;
-    if (r >= p.R) continue;
+    if (r >= p.R) return;
     if (p.splits > 1) {
       const int64_t row = (split * p.B * p.Hk + bh) * p.R + r;
       if (lane < 32) part_stats(p)[row] = make_float2(m, sum);
@@ -198,7 +200,7 @@ __global__ __launch_bounds__(256, tile_waves<T>(DP, KIND)) void attn_fwd_tile_ke
         for (int e = 0; e < 16; e += 4)
           store_run(p.part + row * p.D, d * 32 + 2 * e + 4 * (lane >> 5), p.D, st.o[q][d][e], st.o[q][d][e + 1], st.o[q][d][e + 2],
                     st.o[q][d][e + 3]);
-      continue;
+      return;
     }
     const int64_t g = r / p.Lq, i = r - g * p.Lq, off = b * p.os[0] + i * p.os[1] + (hk * p.G + g) * p.os[2];
     T* out = static_cast<T*>(p.o) + off;
@@ -246,7 +248,7 @@ __global__ __launch_bounds__(256, few_waves<T>(DP, KIND)) void attn_fwd_few_kern
   __shared__ __attribute__((aligned(16))) char lds[4 * (TILE > JOIN ? TILE : JOIN)];
   __shared__ float wm[4][32], wl[4][32];
   const int64_t bh = blockIdx.x, b = bh / p.Hk;
-  const int hk = static_cast<int>(bh - b * p.Hk), split = blockIdx.y, w = threadIdx.x >> 6, l = threadIdx.x & 63;
+  const int hk = static_cast<int>(bh - b * p.Hk), split = blockIdx.y, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63;
   const int64_t len = attn_len(p, b), j0 = split * p.chunk, n = len < j0 + p.chunk ? len : j0 + p.chunk;
   if (split && n <= j0) return;
   RowState<T, DP, QT> st;
@@ -254,28 +256,34 @@ __global__ __launch_bounds__(256, few_waves<T>(DP, KIND)) void attn_fwd_few_kern
   const T* k = static_cast<const T*>(p.k) + b * p.ks[0] + hk * p.ks[2];
   const T* v = static_cast<const T*>(p.v) + b * p.vs[0] + hk * p.vs[2];
   char* vt = lds + w * TILE;
-  uint4 ka[STEPS];
-  Staged<T, DP, LP, 32, 64> vr;
+  u32x4 ka[STEPS];
+  Staged<T, LP, 32, 64> vr;
+  vr.init(p.vs[1], p.D, l);
+  vr.clear(vt, p.D);
   auto fetch = [&](int64_t j) {
     const T* row = k + (j + (l & 31)) * p.ks[1];
 #pragma unroll
     for (int t = 0; t < STEPS; ++t)
-      ka[t] = j + (l & 31) < n ? load_chunk<T>(row, 2 * t + (l >> 5), p.D) : make_uint4(0, 0, 0, 0);
-    vr.load(v + j * p.vs[1], p.vs[1], n - j, p.D, l);
+      ka[t] = j + (l & 31) < n ? load_chunk<T>(row, 2 * t + (l >> 5), p.D) : u32x4{0, 0, 0, 0};
+    vr.load(v + j * p.vs[1], n - j);
   };
   wait_loads();
   if (j0 + 32 * w < n) fetch(j0 + 32 * w);
   for (int64_t j = j0 + 32 * w; j < n; j += 128) {
     f32x16 s[QT][1] = {};
     Block<T> e[QT][1];
+    Turned<T, LP> va[DT];
 #pragma unroll
     for (int t = 0; t < STEPS; ++t)
 #pragma unroll
       for (int q = 0; q < QT; ++q) s[q][0] = mma_step(T(), ka[t], st.q[q][t], s[q][0]);
-    vr.store(vt, l);                       // the wave's own tile: LDS serves a wave's accesses in order
+    vr.store(vt, p.D);                     // the wave's own tile: LDS serves a wave's accesses in order
     __builtin_amdgcn_wave_barrier();
     const bool bad = KIND && __any(vr.bad());
     if (j + 128 < n) fetch(j + 128);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) va[d].read(vt, 0, d);
+    reads_done();
 #pragma unroll
     for (int q = 0; q < QT; ++q) softmax_blocks<T, DP, QT, KIND, 1>(p, st, q, s[q], e[q], j, n);
 #pragma unroll
@@ -284,7 +292,7 @@ __global__ __launch_bounds__(256, few_waves<T>(DP, KIND)) void attn_fwd_few_kern
         slow_second<T, LP, DT>(vt, 0, s[q][0], st.o[q]);
       } else {
 #pragma unroll
-        for (int d = 0; d < DT; ++d) st.o[q][d] = mma_second<LP>(T(), vt, 0, d, e[q][0], st.o[q][d]);
+        for (int d = 0; d < DT; ++d) st.o[q][d] = va[d].mma(e[q][0], st.o[q][d]);
       }
     }
     __builtin_amdgcn_wave_barrier();
@@ -393,9 +401,8 @@ static FwdPlan fwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk
     f.qt = R <= 32 ? 1 : 2;
     f.tiles = 1;
   } else {
-    // 256 rows a workgroup read each state half as often, unless they leave more rows empty
-    f.qt = two && (R + 255) / 256 * 16 <= (R + 127) / 128 * 9 ? 2 : 1;
-    f.tiles = (R + 128 * f.qt - 1) / (128 * f.qt);
+    f.qt = 1;
+    f.tiles = (R + 127) / 128;
   }
   // The states are split until the card is full (few rows: twice, lengths differ), in parts that are
   // still worth a workgroup's start and the join: 512 states for few rows (131072 states, 4 groups, heads
@@ -432,8 +439,7 @@ static void fwd_launch(const AttnParams& p, const FwdPlan& f, hipStream_t s) {
     else if constexpr (DP <= 64 && sizeof(T) == 2 && KIND == 0) attn_fwd_few_kernel<T, DP, 2, KIND><<<grid, 256, 0, s>>>(p);
   } else {
     const dim3 grid(static_cast<unsigned>((all + 7) / 8 * 8), static_cast<unsigned>(f.splits));
-    if (f.qt == 1) attn_fwd_tile_kernel<T, DP, 1, KIND><<<grid, 256, 0, s>>>(p);
-    else if constexpr (DP <= 64 && sizeof(T) == 2 && KIND == 0) attn_fwd_tile_kernel<T, DP, 2, KIND><<<grid, 256, 0, s>>>(p);
+    attn_fwd_tile_kernel<T, DP, KIND><<<grid, 256, 0, s>>>(p);
   }
 }
 

@@ -830,7 +830,8 @@ int fovi_rotary(const fovi_rotary_args* args, void* stream);
  * scores. mask strides [batch, head, query, state], 0 where it is broadcast. kv_lengths: int32
  * [batch] on the device, NULL for kv_len; taken as within [0, kv_len].
  * dtype F32 or BF16 for q, k, v, out and the gradients; strides [batch, token, head], head elements
- * adjacent, every head of whole 16-byte pieces at a 16-byte aligned address; head_dim up to 128;
+ * adjacent, every head of whole 16-byte pieces at a 16-byte aligned address, tokens less than 64 MiB
+ * apart (the tensors may be of any size); head_dim up to 128;
  * scale > 0. Scores, statistics and sums are fp32.
  * stats [2, batch, heads, q_len]: each row's largest score and its sum of exponentials below it (units
  * of the library's own; apart, because the log of the sum vanishes beside a bias of the type's lowest

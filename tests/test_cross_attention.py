@@ -324,6 +324,27 @@ def test_offsets_beyond_32_bits(lq):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lq", [1, 40])
+def test_long_rows_beyond_32_bits(lq):
+    """150 states almost 32 MiB apart, read where they are: byte offsets to 5 * 10^9, element offsets
+    past 2^31, within one tensor."""
+    from fovi_amd.arch.attention import _whole, cross_attention
+    q, k, v, dout, _ = _inputs(1, lq, 150, 1, 1, 32, torch.bfloat16, seed=15)
+    step = (1 << 24) - 8
+    room = torch.empty(149 * step + 64, dtype=torch.bfloat16, device="cuda")
+    far = torch.as_strided(room, (1, 150, 1, 32), (0, step, 32, 1))
+    far.copy_(k)
+    assert _whole(far) and 149 * step > 2 ** 31
+    leaves = [t.detach().requires_grad_(True) for t in (q, far, v)]
+    out = cross_attention(*leaves)
+    assert torch.equal(out, cross_attention(q, k, v))
+    near = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    want = torch.autograd.grad(cross_attention(*near), near, dout)
+    got = torch.autograd.grad(out, [leaves[0], leaves[2]], dout)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[2])
+
+
+@pytest.mark.gpu
 def test_gradients_against_differences():
     """Central differences in fp32 with step 2e-2: the second-order error is step^2 / 6 times third
     derivatives of order 1 (7e-5), the rounding 2^-24 * 10 / 4e-2 (2e-5) times a few."""
