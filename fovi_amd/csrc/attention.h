@@ -184,7 +184,8 @@ template <int LP> struct Turned<float, LP> {
 // Reads stay above, products below.
 __device__ __forceinline__ void reads_done() { __builtin_amdgcn_sched_barrier(0); }
 
-// s (and s2) += the 32 rows of `tile` (`tile2`) times the columns b (b2), over the head elements.
+// s (and s2) += the 32 rows of `tile` (`tile2`) times the columns b (b2), over the head elements, G pieces
+// of each read ahead.
 template <typename T, int LP, int STEPS>
 __device__ __forceinline__ void row_product(const char* tile, const u32x4 (&b)[STEPS], f32x16& s) {
   constexpr int G = STEPS < 4 ? STEPS : 4;
@@ -201,7 +202,7 @@ __device__ __forceinline__ void row_product(const char* tile, const u32x4 (&b)[S
       if (t + g < STEPS) s = mma_step(T(), a[g], b[t + g], s);
   }
 }
-template <typename T, int LP, int G, int STEPS>
+template <typename T, int LP, int G, bool BATCH, int STEPS>
 __device__ __forceinline__ void row_products(const char* tile, const char* tile2, const u32x4 (&b)[STEPS], const u32x4 (&b2)[STEPS],
                                              f32x16& s, f32x16& s2) {
   const int l = threadIdx.x & 63;
@@ -215,7 +216,7 @@ __device__ __forceinline__ void row_products(const char* tile, const char* tile2
         a[g] = *reinterpret_cast<const u32x4*>(tile + at);
         a2[g] = *reinterpret_cast<const u32x4*>(tile2 + at);
       }
-    reads_done();
+    if (BATCH) reads_done();
 #pragma unroll
     for (int g = 0; g < G; ++g)
       if (t + g < STEPS) {

@@ -62,7 +62,7 @@ __device__ __forceinline__ void pair_grad(float t, float c, float shift, float f
 
 // Waves a SIMD shall hold: two wherever a kernel fits 256 registers without spilling much.
 template <typename T> constexpr int dq_waves(int DP, int KIND) {
-  return sizeof(T) == 2 ? (DP == 128 ? 1 : DP == 64 && !KIND ? 3 : 2) : DP >= 96 ? 1 : 2;
+  return sizeof(T) == 2 ? (KIND && DP == 128 ? 1 : DP == 64 && !KIND ? 3 : 2) : DP >= 96 ? 1 : 2;
 }
 template <typename T> constexpr int dkv_waves(int DP, int KIND) {
   return sizeof(T) == 2 ? (DP >= 96 ? 1 : 2) : DP >= 64 ? 1 : 2;
@@ -83,7 +83,10 @@ __global__ __launch_bounds__(256, dq_waves<T>(DP, KIND)) void attn_dq_kernel(Att
   u32x4 q[QT][STEPS], g[QT][STEPS];
   f32x16 dq[QT][DT] = {};
   RowStat st[QT];
-  constexpr bool START = sizeof(T) == 2 && (DP == 32 || DP==128);   // -delta as a block of its own, where registers allow
+  constexpr bool START = sizeof(T) == 2 && DP == 32;   // -delta as a block of its own, where registers allow
+  // Heads of 96 and 128: operands are read as they are needed. Two waves a SIMD that way (229 us for 8 x 1024 x
+  // 2048 and 16 heads of 128) beat one with its reads in batches (300).
+  constexpr bool LATE = DP > 64;
   f32x16 start[START ? QT : 1];
   const void* mrow[QT];
 #pragma unroll
@@ -145,11 +148,12 @@ __global__ __launch_bounds__(256, dq_waves<T>(DP, KIND)) void attn_dq_kernel(Att
       }
 #pragma unroll
       for (int x = 0; x < QT; ++x)
-        row_products<T, LP, (DP == 64 || DP == 96 ? 2 : STEPS < 4 ? STEPS : 4)>(kt + kb * 32 * LP * sizeof(T), vt + kb * 32 * LP * sizeof(T), q[x], g[x], s[x], dp[x]);
+        row_products<T, LP, (LATE ? 1 : DP == 64 ? 2 : STEPS < 4 ? STEPS : 4), !LATE>(kt + kb * 32 * LP * sizeof(T), vt + kb * 32 * LP * sizeof(T), q[x], g[x], s[x], dp[x]);
       Turned<T, LP> ka[DT];
 #pragma unroll
-      for (int d = 0; d < DT; ++d) ka[d].read(kt, kb * 32, d);
-      reads_done();
+      for (int d = 0; d < DT; ++d)
+        if (!LATE) ka[d].read(kt, kb * 32, d);
+      if (!LATE) reads_done();
 #pragma unroll
       for (int x = 0; x < QT; ++x) {
         if (KIND) {
@@ -170,7 +174,10 @@ __global__ __launch_bounds__(256, dq_waves<T>(DP, KIND)) void attn_dq_kernel(Att
         } else {
           const Block<T> ds(s[x]);
 #pragma unroll
-          for (int d = 0; d < DT; ++d) dq[x][d] = ka[d].mma(ds, dq[x][d]);
+          for (int d = 0; d < DT; ++d) {
+            if (LATE) ka[d].read(kt, kb * 32, d);
+            dq[x][d] = ka[d].mma(ds, dq[x][d]);
+          }
         }
       }
     }
@@ -276,7 +283,7 @@ __global__ __launch_bounds__(256, dkv_waves<T>(DP, KIND)) void attn_dkv_kernel(A
 #pragma unroll
         for (int y = 0; y < 4; ++y) dp[i + y] = start[y];
       }
-      row_products<T, LP, (STEPS < 4 ? STEPS : 4)>(qt, gt, k, v, s, dp);
+      row_products<T, LP, (STEPS < 4 ? STEPS : 4), true>(qt, gt, k, v, s, dp);
       Turned<T, LP> ga[DT], qa[DT];
 #pragma unroll
       for (int d = 0; d < DT; ++d) ga[d].read(gt, 0, d);
