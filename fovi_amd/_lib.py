@@ -38,7 +38,7 @@ EXPORTED = ("fovi_abi_version", "fovi_last_error", "fovi_sampler_fwd", "fovi_knn
             "fovi_knnconv_dw_few_workspace_bytes", "fovi_knnconv_dw_few_us",
             "fovi_layer_norm_fwd", "fovi_layer_norm_workspace_bytes", "fovi_layer_norm_bwd", "fovi_rotary",
             "fovi_attention_fwd_workspace_bytes", "fovi_attention_fwd", "fovi_attention_bwd_workspace_bytes",
-            "fovi_attention_bwd")
+            "fovi_attention_bwd", "fovi_attention_pack_mask")
 
 
 class SamplerArgs(C.Structure):
@@ -344,6 +344,8 @@ def load(path: str = LIB_PATH):
     lib.fovi_attention_fwd.restype = C.c_int
     lib.fovi_attention_bwd.argtypes = [C.POINTER(AttentionBwdArgs), C.c_void_p]
     lib.fovi_attention_bwd.restype = C.c_int
+    lib.fovi_attention_pack_mask.argtypes = [C.c_void_p, C.POINTER(C.c_int64)] + [C.c_int64] * 4 + [C.c_void_p, C.c_void_p]
+    lib.fovi_attention_pack_mask.restype = C.c_int
     got = lib.fovi_abi_version()
     if got != ABI_VERSION:
         raise RuntimeError(f"{path}: ABI version {got}, expected {ABI_VERSION}")

@@ -8,6 +8,7 @@ are fp32; the sums are in a fixed order, so the same inputs give the same bits.
 """
 from __future__ import annotations
 
+import ctypes as C
 import math
 
 import torch
@@ -57,12 +58,24 @@ def _args(a, q, k, v, kv_lengths, mask, scale):
     _, a.kv_len, a.kv_heads, _ = k.shape
     a.q_stride[:], a.k_stride[:], a.v_stride[:] = _strides(q), _strides(k), _strides(v)
     if mask is not None:
-        a.mask_kind = _lib.MASK_KEEP if mask.dtype == torch.bool else _lib.MASK_BIAS
+        a.mask_kind = _lib.MASK_KEEP if mask.dtype == torch.int32 else _lib.MASK_BIAS
         a.mask = mask.data_ptr()
         a.mask_stride[:] = mask.stride()
     if kv_lengths is not None:
         a.kv_lengths = kv_lengths.data_ptr()
     a.scale = scale
+
+
+def _packed(mask, b, h, n, states):
+    """A boolean mask as the kernels read it: 32 states a word, broadcast dimensions packed once."""
+    s = mask.stride()
+    sizes = tuple(1 if step == 0 else m for m, step in zip((b, h, n), s))
+    words = torch.empty(sizes + ((states + 31) // 32,), dtype=torch.int32, device=mask.device)
+    if words.numel():
+        _lib.check(_lib.load().fovi_attention_pack_mask(mask.data_ptr(), (C.c_int64 * 4)(*s), *sizes, states,
+                                                        words.data_ptr(), _lib.stream_of(mask)),
+                   "fovi_attention_pack_mask")
+    return words.expand(b, h, n, words.shape[3])
 
 
 def _workspace(a, size, device):
@@ -192,6 +205,8 @@ def cross_attention(q, k, v, kv_lengths=None, mask=None, scale=None):
             mask = mask.expand(b, hq, lq, lk)
         except RuntimeError:
             raise ValueError(f"cross_attention: mask of shape {tuple(mask.shape)} for {(b, hq, lq, lk)}") from None
+        if mask.dtype == torch.bool:
+            mask = _packed(mask, b, hq, lq, lk)
     q, k, v = _pieces(q), _pieces(k), _pieces(v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out = _CrossAttentionFn.apply(q, k, v, kv_lengths, mask, scale)

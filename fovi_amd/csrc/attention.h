@@ -23,6 +23,7 @@ struct AttnParams {
   void* o; float* stats; void* rest;
   const void* dout; void* dq; void* dk; void* dv;
   float* part;                // partial results of split work
+  float* part_k;              // backward: those of dk and dv (part: dq)
   float* delta;               // backward: dout . out of each row
   int64_t B, Lq, Lk;
   int H, Hk, G, D, kind;
@@ -32,6 +33,7 @@ struct AttnParams {
   int splits;                 // of the summed axis
   int64_t chunk;              // its length per split
   int64_t tiles;              // workgroups along the owned axis
+  int k_splits;               // backward: of dk and dv, for the join
 };
 
 __device__ __forceinline__ int64_t attn_len(const AttnParams& p, int64_t b) {
@@ -321,62 +323,43 @@ __device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// The mask over a lane's 16 pairs of a block whose columns are query rows: states j0 + 8 (i / 4) + i % 4
-// of its row (j0 holds the lane's half; n states in all). Scores in units of log2, -inf where a pair
-// is left out. Where the mask's states are adjacent, bytes come four at a time.
-__device__ __forceinline__ void mask_block(const AttnParams& p, const void* row, int64_t j0, int64_t n, f32x16& s) {
-  const int64_t step = p.ms[3];
-  if (p.kind == FOVI_MASK_KEEP) {
-    const uint8_t* m = static_cast<const uint8_t*>(row) + j0 * step;
+// KIND of a kernel: 0 no mask, 1 bits of states to keep, 2 a bias. A masked score is in units of log2,
+// -inf where a pair is left out.
+//
+// Where a block's columns are query rows, a lane has the word of its row and the block's 32 states; the
+// pairs are its bits 8 (i / 4) + 4 half + i % 4.
+__device__ __forceinline__ void keep_block(const AttnParams& p, uint32_t word, f32x16& s) {
+  const uint32_t w = word >> (4 * ((threadIdx.x & 63) >> 5));
 #pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      uint32_t keep = 0;
-      if (step == 1 && j0 + 2 * i + 4 <= n) {
-        __builtin_memcpy(&keep, m + 2 * i, 4);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (j0 + 2 * i + e < n) keep |= static_cast<uint32_t>(m[(2 * i + e) * step]) << (8 * e);
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[i + e] = (keep >> (8 * e)) & 0xff ? s[i + e] * p.c : kNegInf;
-    }
-  } else {
-    const float* m = static_cast<const float*>(row) + j0 * step;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int at = 8 * (i / 4) + i % 4;
-      const float bias = j0 + at < n ? m[at * step] : kNegInf;
-      // (the type's lowest value times log2(e) is still a number: rows of nothing else read all alike)
-      s[i] = bias == kNegInf ? kNegInf : fmaf(s[i], p.c, fmaxf(bias * kLog2e, -3.402823466e38f));
-    }
-  }
+  for (int i = 0; i < 16; ++i) s[i] = w & (1u << (8 * (i / 4) + i % 4)) ? s[i] * p.c : kNegInf;
 }
 
-// The same where the columns are states: 16 rows i0 + 8 (i / 4) + i % 4 (n in all) of one state, `col` its
-// place in row 0's mask.
-__device__ __forceinline__ void mask_column(const AttnParams& p, const void* col, int64_t i0, int64_t n, f32x16& s) {
-  const int64_t step = p.ms[2];
-  if (p.kind == FOVI_MASK_KEEP) {
-    const uint8_t* m = static_cast<const uint8_t*>(col) + i0 * step;
+__device__ __forceinline__ float biased(const AttnParams& p, float bias, float s) {
+  // (the type's lowest value times log2(e) is still a number: rows of nothing else read all alike)
+  return bias == kNegInf ? kNegInf : fmaf(s, p.c, fmaxf(bias * kLog2e, -3.402823466e38f));
+}
+
+// A bias over a lane's 16 pairs: states j0 + 8 (i / 4) + i % 4 of its row (j0 holds the half; n states in all)...
+__device__ __forceinline__ void bias_block(const AttnParams& p, const float* row, int64_t j0, int64_t n, f32x16& s) {
+  const float* m = row + j0 * p.ms[3];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int at = 8 * (i / 4) + i % 4;
-      const bool keep = i0 + at < n && m[at * step] != 0;
-      s[i] = keep ? s[i] * p.c : kNegInf;
-    }
-  } else {
-    const float* m = static_cast<const float*>(col) + i0 * step;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int at = 8 * (i / 4) + i % 4;
-      const float bias = i0 + at < n ? m[at * step] : kNegInf;
-      s[i] = bias == kNegInf ? kNegInf : fmaf(s[i], p.c, fmaxf(bias * kLog2e, -3.402823466e38f));
-    }
+  for (int i = 0; i < 16; ++i) {
+    const int at = 8 * (i / 4) + i % 4;
+    s[i] = biased(p, j0 + at < n ? m[at * p.ms[3]] : kNegInf, s[i]);
   }
 }
-__device__ __forceinline__ const void* mask_row(const AttnParams& p, int64_t b, int64_t h, int64_t i) {
-  return static_cast<const char*>(p.mask) + (b * p.ms[0] + h * p.ms[1] + i * p.ms[2]) * (p.kind == FOVI_MASK_KEEP ? 1 : 4);
+// ... or rows i0 + 8 (i / 4) + i % 4 (n in all) of one state, `col` its place in row 0.
+__device__ __forceinline__ void bias_column(const AttnParams& p, const float* col, int64_t i0, int64_t n, f32x16& s) {
+  const float* m = col + i0 * p.ms[2];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int at = 8 * (i / 4) + i % 4;
+    s[i] = biased(p, i0 + at < n ? m[at * p.ms[2]] : kNegInf, s[i]);
+  }
+}
+// A row of the mask: its words, or its biases (both of four bytes).
+__device__ __forceinline__ const uint32_t* mask_row(const AttnParams& p, int64_t b, int64_t h, int64_t i) {
+  return static_cast<const uint32_t*>(p.mask) + b * p.ms[0] + h * p.ms[1] + i * p.ms[2];
 }
 
 // Four adjacent head elements from d on, to memory.
@@ -394,6 +377,8 @@ __device__ __forceinline__ void store_run(float* row, int d, int D, float a, flo
 // Host side (attention_fwd.hip, attention_bwd.hip).
 int attn_fwd_launch(AttnParams& p, int dtype, hipStream_t s);
 int64_t attn_fwd_workspace(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t D, int dtype);
+int attn_pack_launch(const void* keep, const int64_t* stride, int64_t n0, int64_t n1, int64_t n2, int64_t states, uint32_t* words,
+                     hipStream_t s);
 int attn_bwd_launch(AttnParams& p, int dtype, hipStream_t s);
 int64_t attn_bwd_workspace(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t D, int dtype);
 

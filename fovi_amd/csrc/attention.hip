@@ -17,7 +17,7 @@ static int attn_check(const fovi_attention_args* a, const char* what) {
   if (a->kv_len && (!a->k || !a->v)) { set_error("%s: null pointer", what); return 1; }
   if (!(a->scale > 0) || a->scale > 2.0e38f) { set_error("%s: scale must be positive and finite", what); return 1; }
   if (a->mask_kind < FOVI_MASK_NONE || a->mask_kind > FOVI_MASK_BIAS) { set_error("%s: unknown mask_kind", what); return 1; }
-  if (a->mask_kind != FOVI_MASK_NONE && !a->mask) { set_error("%s: null mask", what); return 1; }
+  if (a->mask_kind != FOVI_MASK_NONE && a->kv_len && !a->mask) { set_error("%s: null mask", what); return 1; }
   if (a->batch * a->heads * a->q_len > 0x7fffffff || a->batch * a->kv_heads * a->kv_len > 0x7fffffff) {
     set_error("%s: too many rows or states", what);
     return 1;
@@ -58,6 +58,19 @@ static AttnParams attn_params(const fovi_attention_args* a) {
 }  // namespace fovi
 
 using namespace fovi;
+
+extern "C" int fovi_attention_pack_mask(const void* keep, const int64_t* stride, int64_t n0, int64_t n1, int64_t n2, int64_t kv_len,
+                                        uint32_t* words, void* stream) {
+  clear_error();
+  if (!keep || !stride || !words) { set_error("fovi_attention_pack_mask: null pointer"); return 1; }
+  if (n0 < 0 || n1 < 0 || n2 < 0 || kv_len < 0) { set_error("fovi_attention_pack_mask: bad sizes"); return 1; }
+  const int64_t per = (kv_len + 31) / 32, most = int64_t(0x7fffffff) * 256;
+  if (n0 && n1 && n2 && per && (n0 > most / n1 || n0 * n1 > most / n2 || n0 * n1 * n2 > most / per)) {
+    set_error("fovi_attention_pack_mask: mask too large");
+    return 1;
+  }
+  return attn_pack_launch(keep, stride, n0, n1, n2, kv_len, words, static_cast<hipStream_t>(stream));
+}
 
 extern "C" int64_t fovi_attention_fwd_workspace_bytes(int64_t batch, int64_t q_len, int64_t kv_len, int64_t heads, int64_t kv_heads,
                                                       int64_t head_dim, int32_t dtype) {

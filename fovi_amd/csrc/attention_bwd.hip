@@ -3,40 +3,14 @@
 //   p_ij = exp(s_ij - max_i) / sum_i, ds_ij = p_ij (do_i.v_j - delta_i), delta_i = do_i.o_i
 //   dq_i = scale sum_j ds_ij k_j, dk_j = scale sum_i ds_ij q_i, dv_j = sum_i p_ij do_i
 //
-// Three launches: delta; dq, whose workgroups own query rows and walk the states; dk and dv, whose
-// workgroups own states and walk the query rows of all heads that share the key head. The scores
-// are formed twice (7 products instead of 5), and in return every gradient is summed by one
-// workgroup in a fixed order, without atomics and without a score matrix in memory. Where the owned
-// axis is short, the walked one is split over workgroups and the partial sums join in a last launch.
+// Two launches: dq, whose workgroups own query rows and walk the states (and leave delta behind); dk
+// and dv, whose workgroups own states and walk the query rows of all heads that share the key head.
+// The scores are formed twice (7 products instead of 5), and in return every gradient is summed by
+// one workgroup in a fixed order, without atomics and without a score matrix in memory. Where the
+// owned axis is short, the walked one is split over workgroups and the partial sums join in a third.
 #include "attention.h"
 
 namespace fovi {
-
-// delta of four rows per wave: 16 lanes each
-template <typename T>
-__global__ __launch_bounds__(256) void attn_delta_kernel(AttnParams p) {
-  constexpr int N = Chunk<T>::N;
-  const int64_t rows = p.B * p.H * p.Lq, x = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
-  float sum = 0;
-  if (x < rows) {
-    const int64_t bh = x / p.Lq, i = x - bh * p.Lq, b = bh / p.H, h = bh - b * p.H;
-    const T* g = static_cast<const T*>(p.dout) + b * p.dos[0] + i * p.dos[1] + h * p.dos[2];
-    const int64_t off = b * p.os[0] + i * p.os[1] + h * p.os[2];
-    for (int c = threadIdx.x & 15; c * N < p.D; c += 16) {
-      T a[N], o[N], r[N];
-      const u32x4 ga = load_chunk<T>(g, c, p.D), oa = load_chunk<T>(static_cast<const T*>(p.o) + off, c, p.D);
-      const u32x4 ra = p.rest ? load_chunk<T>(static_cast<const T*>(p.rest) + off, c, p.D) : u32x4{0, 0, 0, 0};
-      __builtin_memcpy(a, &ga, 16);
-      __builtin_memcpy(o, &oa, 16);
-      __builtin_memcpy(r, &ra, 16);
-#pragma unroll
-      for (int e = 0; e < N; ++e) sum = fmaf(Elem<T>::load(a + e), Elem<T>::load(o + e) + Elem<T>::load(r + e), sum);
-    }
-  }
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-  if (x < rows && (threadIdx.x & 15) == 0) p.delta[x] = sum;
-}
 
 // What a row's probabilities need: exp2(t - shift) * factor. Without a bias the log of the sum goes
 // into the shift (factor 1). A row that keeps nothing has shift +inf: probabilities 0.
@@ -46,7 +20,8 @@ __device__ __forceinline__ RowStat row_stat(float m, float sum, float delta) {
   return {sum == 0 ? __builtin_inff() : KIND ? m : m + log2f(sum), KIND && sum != 0 ? 1.0f / sum : KIND ? 0.0f : 1.0f, delta};
 }
 
-// Probability and score gradient of one pair, dp = do.v - delta (the product starts from -delta); KIND 1: t is the masked score, left-out pairs become kLeftOut.
+// Probability and score gradient of one pair, dp = do.v - delta (the product starts from -delta). Under a mask t is
+// the masked score, and left-out pairs become kLeftOut.
 template <int KIND>
 __device__ __forceinline__ void pair_grad(float t, float c, float shift, float factor, float dp, float& e, float& ds) {
   if (KIND) {
@@ -88,20 +63,34 @@ __global__ __launch_bounds__(256, dq_waves<T>(DP, KIND)) void attn_dq_kernel(Att
   // 2048 and 16 heads of 128) beat one with its reads in batches (300).
   constexpr bool LATE = DP > 64;
   f32x16 start[START ? QT : 1];
-  const void* mrow[QT];
+  const uint32_t* mrow[QT];
+  uint32_t word[QT][2] = {}, coming[QT][2] = {};       // KIND 1: the blocks' bits, and the next tile's
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     const int64_t r = r0 + 32 * t + (l & 31);
     const int64_t gr = r < p.R ? r / p.Lq : 0, i = r < p.R ? r - gr * p.Lq : 0, h = hk * p.G + gr;
     const T* qr = static_cast<const T*>(p.q) + b * p.qs[0] + i * p.qs[1] + h * p.qs[2];
     const T* gg = static_cast<const T*>(p.dout) + b * p.dos[0] + i * p.dos[1] + h * p.dos[2];
+    // delta = do.o, o before its rounding; half of the elements a lane
+    const int64_t off = b * p.os[0] + i * p.os[1] + h * p.os[2];
+    float delta = 0;
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
       q[t][s] = load_chunk<T>(qr, 2 * s + (l >> 5), r < p.R ? p.D : 0);
       g[t][s] = load_chunk<T>(gg, 2 * s + (l >> 5), r < p.R ? p.D : 0);
+      const u32x4 o = load_chunk<T>(static_cast<const T*>(p.o) + off, 2 * s + (l >> 5), p.D);
+      const u32x4 rest = p.rest ? load_chunk<T>(static_cast<const T*>(p.rest) + off, 2 * s + (l >> 5), p.D) : u32x4{0, 0, 0, 0};
+      T ge[Chunk<T>::N], oe[Chunk<T>::N], re[Chunk<T>::N];
+      __builtin_memcpy(ge, &g[t][s], 16);
+      __builtin_memcpy(oe, &o, 16);
+      __builtin_memcpy(re, &rest, 16);
+#pragma unroll
+      for (int e = 0; e < Chunk<T>::N; ++e) delta = fmaf(Elem<T>::load(ge + e), Elem<T>::load(oe + e) + Elem<T>::load(re + e), delta);
     }
+    delta += other_half(delta);
     const int64_t at = (b * p.H + h) * p.Lq + i;
-    st[t] = row_stat<KIND>(p.stats[at], p.stats[p.B * p.H * p.Lq + at], p.delta[at]);
+    if (split == 0 && l < 32 && r < p.R) p.delta[at] = delta;
+    st[t] = row_stat<KIND>(p.stats[at], p.stats[p.B * p.H * p.Lq + at], delta);
 #pragma unroll
     for (int e = 0; e < 16; ++e)
       if (START) start[t][e] = -st[t].delta;
@@ -117,6 +106,13 @@ __global__ __launch_bounds__(256, dq_waves<T>(DP, KIND)) void attn_dq_kernel(Att
   if (KIND && threadIdx.x < 2) bad_tile[threadIdx.x] = -1;
   if (KIND) __syncthreads();
   int at = 0;
+  auto words = [&](int64_t j) {
+#pragma unroll
+    for (int x = 0; x < QT; ++x)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+        coming[x][kb] = j + 32 * kb < n && r0 + 32 * x + (l & 31) < p.R ? mrow[x][j / 32 + kb] : 0;
+  };
   auto put = [&](int buf, int tile) {
     kr.store(tiles[buf][0], p.D);
     vr.store(tiles[buf][1], p.D);
@@ -125,11 +121,20 @@ __global__ __launch_bounds__(256, dq_waves<T>(DP, KIND)) void attn_dq_kernel(Att
   if (j0 < n) {
     kr.load(k + j0 * p.ks[1], n - j0);
     vr.load(v + j0 * p.vs[1], n - j0);
+    if (KIND == 1) words(j0);
     put(0, 0);
   }
   wait_loads();
   for (int64_t j = j0; j < n; j += KT, ++at) {
     const int64_t next = j + KT;
+    if (KIND == 1) {
+#pragma unroll
+      for (int x = 0; x < QT; ++x) {
+        word[x][0] = coming[x][0];
+        word[x][1] = coming[x][1];
+      }
+      if (next < n) words(next);
+    }
     if (next < n) {
       kr.load(k + next * p.ks[1], n - next);
       vr.load(v + next * p.vs[1], n - next);
@@ -140,6 +145,7 @@ __global__ __launch_bounds__(256, dq_waves<T>(DP, KIND)) void attn_dq_kernel(Att
     const int left = static_cast<int>(n - j < KT ? n - j : KT);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
+      if (KIND == 1 && QT == 1 && !__any(word[0][kb] != 0)) continue;      // no row reads these states
       f32x16 s[QT] = {}, dp[QT];
 #pragma unroll
       for (int x = 0; x < QT; ++x) {
@@ -156,9 +162,9 @@ __global__ __launch_bounds__(256, dq_waves<T>(DP, KIND)) void attn_dq_kernel(Att
       if (!LATE) reads_done();
 #pragma unroll
       for (int x = 0; x < QT; ++x) {
-        if (KIND) {
-          mask_block(p, mrow[x], j + kb * 32 + 4 * (l >> 5), n, s[x]);
-        } else if (left < kb * 32 + 32) {
+        if (KIND == 1) keep_block(p, word[x][kb], s[x]);
+        if (KIND == 2) bias_block(p, reinterpret_cast<const float*>(mrow[x]), j + kb * 32 + 4 * (l >> 5), n, s[x]);
+        if (KIND < 2 && left < kb * 32 + 32) {
 #pragma unroll
           for (int i = 0; i < 16; ++i)
             if (kb * 32 + 8 * (i / 4) + 4 * (l >> 5) + i % 4 >= left) s[x][i] = kNegInf;
@@ -211,6 +217,7 @@ __global__ __launch_bounds__(256, dkv_waves<T>(DP, KIND)) void attn_dkv_kernel(A
   __shared__ __attribute__((aligned(16))) char tiles[2][2][RT * LP * sizeof(T)];
   __shared__ __attribute__((aligned(16))) float stats[2][3][RT];
   __shared__ int bad_tile[2][2];
+  __shared__ __attribute__((aligned(16))) uint32_t bits[2][4][KIND == 1 ? RT : 4];     // [wave][row]: its 32 states
   const int64_t all = p.tiles * p.B * p.Hk, id = xcd_tile(blockIdx.x, gridDim.x);
   if (id >= all) return;
   const int64_t bh = id / p.tiles, b = bh / p.Hk;
@@ -226,7 +233,7 @@ __global__ __launch_bounds__(256, dkv_waves<T>(DP, KIND)) void attn_dkv_kernel(A
   }
   f32x16 dk[DT] = {}, dv[DT] = {};
   // tiles of RT rows, head by head; split s walks tiles s * chunk .. of the p.G * per there are
-  const int per = static_cast<int>((p.Lq + RT - 1) / RT);
+  const int per = p.Lq > 0 ? static_cast<int>((p.Lq + RT - 1) / RT) : 1;
   const int64_t first = split * p.chunk, end = static_cast<int64_t>(per) * p.G;
   const int count = w0 >= n ? 0 : static_cast<int>(end < first + p.chunk ? end - first : p.chunk);
   Staged<T, LP, RT, 256> qr, gr;
@@ -235,6 +242,7 @@ __global__ __launch_bounds__(256, dkv_waves<T>(DP, KIND)) void attn_dkv_kernel(A
 #pragma unroll
   for (int i = 0; i < 4; ++i) qr.clear(tiles[i >> 1][i & 1], p.D);
   float m = 0, sum = 0, delta = 0;                 // raw: nothing waits for them before the tile is stored
+  uint32_t word = 0;
   if (KIND && threadIdx.x < 4) bad_tile[threadIdx.x >> 1][threadIdx.x & 1] = -1;
   if (KIND) __syncthreads();
   int h = hk * p.G + static_cast<int>(first / per), i0 = static_cast<int>(first % per) * RT;      // the next tile to fetch
@@ -248,6 +256,10 @@ __global__ __launch_bounds__(256, dkv_waves<T>(DP, KIND)) void attn_dkv_kernel(A
       sum = in ? p.stats[p.B * p.H * p.Lq + at] : 0.0f;
       delta = p.delta[at];
     }
+    if (KIND == 1) {
+      const int r = threadIdx.x % RT, w = threadIdx.x / RT;
+      word = w < 4 && i0 + r < p.Lq && w0 + 32 * w < p.Lk ? mask_row(p, b, h, i0 + r)[w0 / 32 + w] : 0;
+    }
   };
   auto put = [&](int buf, int tile) {
     qr.store(tiles[buf][0], p.D);
@@ -258,6 +270,7 @@ __global__ __launch_bounds__(256, dkv_waves<T>(DP, KIND)) void attn_dkv_kernel(A
       if (KIND) stats[buf][1][threadIdx.x] = sr.factor;
       stats[buf][2][threadIdx.x] = -sr.delta;
     }
+    if (KIND == 1 && threadIdx.x / RT < 4) bits[buf][threadIdx.x / RT][threadIdx.x % RT] = word;
     if (KIND && qr.bad()) bad_tile[buf][0] = tile;
     if (KIND && gr.bad()) bad_tile[buf][1] = tile;
   };
@@ -276,6 +289,17 @@ __global__ __launch_bounds__(256, dkv_waves<T>(DP, KIND)) void attn_dkv_kernel(A
     for (int rb = 0; rb < RB; ++rb) {
       const char* qt = tiles[at & 1][0] + rb * 32 * LP * sizeof(T);
       const char* gt = tiles[at & 1][1] + rb * 32 * LP * sizeof(T);
+      uint32_t keep = 0;                  // KIND 1: the lane's 16 pairs
+      if (KIND == 1) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          const u32x4 w = *reinterpret_cast<const u32x4*>(&bits[at & 1][threadIdx.x >> 6][rb * 32 + 2 * i + 4 * (l >> 5)]);
+#pragma unroll
+          for (int y = 0; y < 4; ++y) keep |= ((w[y] >> (l & 31)) & 1u) << (i + y);
+        }
+        if (j >= n) keep = 0;
+        if (!__any(keep != 0)) continue;  // no pair of the block
+      }
       f32x16 s = {}, dp;
 #pragma unroll
       for (int i = 0; i < 16; i += 4) {
@@ -288,10 +312,13 @@ __global__ __launch_bounds__(256, dkv_waves<T>(DP, KIND)) void attn_dkv_kernel(A
 #pragma unroll
       for (int d = 0; d < DT; ++d) ga[d].read(gt, 0, d);
       reads_done();
-      if (KIND) {
-        const char* col = static_cast<const char*>(mask_row(p, b, h_at, 0)) + (j < n ? j : 0) * p.ms[3] * (p.kind == FOVI_MASK_KEEP ? 1 : 4);
-        mask_column(p, col, i_at + rb * 32 + 4 * (l >> 5), j < n ? p.Lq : 0, s);
+      if (KIND == 1) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = keep & (1u << i) ? s[i] * p.c : kNegInf;
       }
+      if (KIND == 2)
+        bias_column(p, reinterpret_cast<const float*>(mask_row(p, b, h_at, 0)) + (j < n ? j : 0) * p.ms[3], i_at + rb * 32 + 4 * (l >> 5),
+                    j < n ? p.Lq : 0, s);
 #pragma unroll
       for (int i = 0; i < 16; i += 4) {
         const int r = rb * 32 + 2 * i + 4 * (l >> 5);
@@ -334,7 +361,7 @@ __global__ __launch_bounds__(256, dkv_waves<T>(DP, KIND)) void attn_dkv_kernel(A
   if (j >= p.Lk) return;
   T* dko = static_cast<T*>(p.dk) + b * p.dks[0] + j * p.dks[1] + hk * p.dks[2];
   T* dvo = static_cast<T*>(p.dv) + b * p.dvs[0] + j * p.dvs[1] + hk * p.dvs[2];
-  float* part = p.part + ((split * p.B * p.Hk + bh) * p.Lk + j) * 2 * p.D;
+  float* part = p.part_k + ((split * p.B * p.Hk + bh) * p.Lk + j) * 2 * p.D;
   const float keep = j < n ? 1.0f : 0.0f;          // (columns behind the length never met a value: 0 or NaN)
 #pragma unroll
   for (int d = 0; d < DT; ++d)
@@ -357,29 +384,27 @@ __global__ __launch_bounds__(256, dkv_waves<T>(DP, KIND)) void attn_dkv_kernel(A
     }
 }
 
-// Partial sums added up in the order of the splits, four elements a thread.
+// Partial sums added up in the order of the splits, four elements a thread: dq's (where it was split),
+// then those of dk and dv. p.splits and p.chunk are dq's.
 template <typename T>
-__global__ __launch_bounds__(256) void attn_dq_join_kernel(AttnParams p) {
+__global__ __launch_bounds__(256) void attn_bwd_join_kernel(AttnParams p) {
   const int per = p.D / 4;
-  const int64_t rows = p.B * p.Hk * p.R, x = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (x >= rows * per) return;
-  const int64_t row = x / per, d = (x - row * per) * 4, bh = row / p.R, r = row - bh * p.R, b = bh / p.Hk, g = r / p.Lq;
-  int64_t used = (attn_len(p, b) + p.chunk - 1) / p.chunk;
-  if (used < 1) used = 1;
+  const int64_t q_all = p.splits > 1 ? p.B * p.Hk * p.R * per : 0, k_all = p.k_splits > 1 ? p.B * p.Hk * p.Lk * 2 * per : 0;
+  int64_t x = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   f32x4 sum = {};
-  for (int64_t s = 0; s < used; ++s) sum += *reinterpret_cast<const f32x4*>(p.part + (s * rows + row) * p.D + d);
-  T* out = static_cast<T*>(p.dq) + b * p.dqs[0] + (r - g * p.Lq) * p.dqs[1] + ((bh - b * p.Hk) * p.G + g) * p.dqs[2];
-  store_run(out, static_cast<int>(d), p.D, sum[0], sum[1], sum[2], sum[3]);
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void attn_dkv_join_kernel(AttnParams p) {
-  const int per = p.D / 4;
-  const int64_t rows = p.B * p.Hk * p.Lk, x = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (x >= rows * 2 * per) return;
-  const int64_t row = x / (2 * per), y = x - row * 2 * per, d = y % per * 4, bh = row / p.Lk, j = row - bh * p.Lk, b = bh / p.Hk;
-  f32x4 sum = {};
-  for (int64_t s = 0; s < p.splits; ++s) sum += *reinterpret_cast<const f32x4*>(p.part + (s * rows + row) * 2 * p.D + y * 4);
+  if (x < q_all) {
+    const int64_t rows = p.B * p.Hk * p.R, row = x / per, d = (x - row * per) * 4, bh = row / p.R, r = row - bh * p.R, b = bh / p.Hk, g = r / p.Lq;
+    int64_t used = (attn_len(p, b) + p.chunk - 1) / p.chunk;
+    if (used < 1) used = 1;
+    for (int64_t s = 0; s < used; ++s) sum += *reinterpret_cast<const f32x4*>(p.part + (s * rows + row) * p.D + d);
+    T* out = static_cast<T*>(p.dq) + b * p.dqs[0] + (r - g * p.Lq) * p.dqs[1] + ((bh - b * p.Hk) * p.G + g) * p.dqs[2];
+    store_run(out, static_cast<int>(d), p.D, sum[0], sum[1], sum[2], sum[3]);
+    return;
+  }
+  x -= q_all;
+  if (x >= k_all) return;
+  const int64_t rows = p.B * p.Hk * p.Lk, row = x / (2 * per), y = x - row * 2 * per, d = y % per * 4, bh = row / p.Lk, j = row - bh * p.Lk, b = bh / p.Hk;
+  for (int64_t s = 0; s < p.k_splits; ++s) sum += *reinterpret_cast<const f32x4*>(p.part_k + (s * rows + row) * 2 * p.D + y * 4);
   T* out = y >= per ? static_cast<T*>(p.dv) + b * p.dvs[0] + j * p.dvs[1] + (bh - b * p.Hk) * p.dvs[2]
                     : static_cast<T*>(p.dk) + b * p.dks[0] + j * p.dks[1] + (bh - b * p.Hk) * p.dks[2];
   store_run(out, static_cast<int>(d), p.D, sum[0], sum[1], sum[2], sum[3]);
@@ -423,10 +448,9 @@ int64_t attn_bwd_workspace(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t
   int64_t most = 0;
   for (const bool mask : {false, true}) {
     const BwdPlan f = bwd_plan(B, Lq, Lk, H, Hk, D, dtype, mask);
-    // delta, then the partial sums of dq, later those of dk and dv in their place
-    const int64_t q = f.q_splits > 1 ? f.q_splits * B * H * Lq * D * 4 : 0, k = f.k_splits > 1 ? f.k_splits * B * Hk * Lk * 2 * D * 4 : 0;
-    if (q > most) most = q;
-    if (k > most) most = k;
+    // delta, then the partial sums of dq, then those of dk and dv
+    const int64_t need = (f.q_splits > 1 ? f.q_splits * B * H * Lq * D * 4 : 0) + (f.k_splits > 1 ? f.k_splits * B * Hk * Lk * 2 * D * 4 : 0);
+    if (need > most) most = need;
   }
   return align16(B * H * Lq * 4) + most;
 }
@@ -444,51 +468,47 @@ static void bwd_dkv(const AttnParams& p, hipStream_t s) {
   attn_dkv_kernel<T, DP, KIND><<<grid, 256, 0, s>>>(p);
 }
 
+template <typename T, int KIND, bool DQ>
+static void bwd_heads(const AttnParams& p, int qt, hipStream_t s) {
+  if constexpr (DQ) {
+    if (p.D <= 32) bwd_dq<T, 32, KIND>(p, qt, s);
+    else if (p.D <= 64) bwd_dq<T, 64, KIND>(p, qt, s);
+    else if (p.D <= 96) bwd_dq<T, 96, KIND>(p, qt, s);
+    else bwd_dq<T, 128, KIND>(p, qt, s);
+  } else {
+    if (p.D <= 32) bwd_dkv<T, 32, KIND>(p, s);
+    else if (p.D <= 64) bwd_dkv<T, 64, KIND>(p, s);
+    else if (p.D <= 96) bwd_dkv<T, 96, KIND>(p, s);
+    else bwd_dkv<T, 128, KIND>(p, s);
+  }
+}
+
 template <typename T>
 static int bwd_type(AttnParams& p, hipStream_t s) {
   const BwdPlan f = bwd_plan(p.B, p.Lq, p.Lk, p.H, p.Hk, p.D, sizeof(T) == 2 ? FOVI_BF16 : FOVI_F32, p.kind != 0);
   p.delta = p.part;
   p.part = reinterpret_cast<float*>(reinterpret_cast<char*>(p.part) + align16(p.B * p.H * p.Lq * 4));
   const int64_t rows = p.B * p.H * p.Lq;
+  p.part_k = p.part + (f.q_splits > 1 ? f.q_splits * rows * p.D : 0);
+  p.k_splits = f.k_splits;
   if (rows) {
-    attn_delta_kernel<T><<<static_cast<unsigned>((rows + 15) / 16), 256, 0, s>>>(p);
-    if (check_launch("fovi_attention_bwd")) return 1;
     p.tiles = f.q_tiles; p.splits = f.q_splits; p.chunk = f.q_chunk;
-    const int dp = p.D <= 32 ? 32 : p.D <= 64 ? 64 : p.D <= 96 ? 96 : 128;
-    if (p.kind) {
-      if (dp == 32) bwd_dq<T, 32, 1>(p, f.qt, s);
-      else if (dp == 64) bwd_dq<T, 64, 1>(p, f.qt, s);
-      else if (dp == 96) bwd_dq<T, 96, 1>(p, f.qt, s);
-      else bwd_dq<T, 128, 1>(p, f.qt, s);
-    } else {
-      if (dp == 32) bwd_dq<T, 32, 0>(p, f.qt, s);
-      else if (dp == 64) bwd_dq<T, 64, 0>(p, f.qt, s);
-      else if (dp == 96) bwd_dq<T, 96, 0>(p, f.qt, s);
-      else bwd_dq<T, 128, 0>(p, f.qt, s);
-    }
+    if (p.kind == FOVI_MASK_NONE) bwd_heads<T, 0, true>(p, f.qt, s);
+    else if (p.kind == FOVI_MASK_KEEP) bwd_heads<T, 1, true>(p, f.qt, s);
+    else bwd_heads<T, 2, true>(p, f.qt, s);
     if (check_launch("fovi_attention_bwd")) return 1;
-    if (f.q_splits > 1) {
-      attn_dq_join_kernel<T><<<static_cast<unsigned>((rows * (p.D / 4) + 255) / 256), 256, 0, s>>>(p);
-      if (check_launch("fovi_attention_bwd")) return 1;
-    }
   }
   if (p.Lk == 0 || p.B == 0) return 0;
   p.tiles = f.k_tiles; p.splits = f.k_splits; p.chunk = f.k_chunk;
-  if (p.kind) {
-    if (p.D <= 32) bwd_dkv<T, 32, 1>(p, s);
-    else if (p.D <= 64) bwd_dkv<T, 64, 1>(p, s);
-    else if (p.D <= 96) bwd_dkv<T, 96, 1>(p, s);
-    else bwd_dkv<T, 128, 1>(p, s);
-  } else {
-    if (p.D <= 32) bwd_dkv<T, 32, 0>(p, s);
-    else if (p.D <= 64) bwd_dkv<T, 64, 0>(p, s);
-    else if (p.D <= 96) bwd_dkv<T, 96, 0>(p, s);
-    else bwd_dkv<T, 128, 0>(p, s);
-  }
+  if (p.kind == FOVI_MASK_NONE) bwd_heads<T, 0, false>(p, 1, s);
+  else if (p.kind == FOVI_MASK_KEEP) bwd_heads<T, 1, false>(p, 1, s);
+  else bwd_heads<T, 2, false>(p, 1, s);
   if (check_launch("fovi_attention_bwd")) return 1;
-  if (f.k_splits > 1) {
-    const int64_t n = p.B * p.Hk * p.Lk * 2 * (p.D / 4);
-    attn_dkv_join_kernel<T><<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(p);
+  if (f.q_splits > 1 || f.k_splits > 1) {
+    p.splits = f.q_splits;
+    p.chunk = f.q_chunk;
+    const int64_t n = (f.q_splits > 1 ? rows : 0) * (p.D / 4) + (f.k_splits > 1 ? p.B * p.Hk * p.Lk : 0) * 2 * (p.D / 4);
+    attn_bwd_join_kernel<T><<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(p);
     return check_launch("fovi_attention_bwd");
   }
   return 0;

@@ -20,7 +20,8 @@ struct RowState {
   u32x4 q[QT][STEPS];
   f32x16 o[QT][DT];
   float m[QT], l[QT];         // the row's maximum so far, or a little less; the lane's share of the sum
-  const void* mrow[QT];
+  const uint32_t* mrow[QT];
+  uint32_t word[QT][2];       // KIND 1: the next blocks' bits
 };
 
 // The rows r0 + 32 t + lane of key head (b, hk): queries as B operands, statistics cleared.
@@ -46,18 +47,18 @@ __device__ __forceinline__ void init_rows(const AttnParams& p, RowState<T, DP, Q
 }
 
 // Scores of KB blocks of 32 states (j .. n valid) into probabilities; the running statistics of
-// rows t and the outputs' scale follow. KIND 1: the mask is applied, pairs that are left out become kLeftOut.
+// rows t and the outputs' scale follow. Under a mask, pairs that are left out become kLeftOut.
 template <typename T, int DP, int QT, int KIND, int KB>
 __device__ __forceinline__ void softmax_blocks(const AttnParams& p, RowState<T, DP, QT>& st, int t, f32x16 (&s)[KB], Block<T> (&e)[KB],
-                                               int64_t j, int64_t n) {
+                                               const uint32_t (&word)[2], int64_t j, int64_t n) {
   const int h = (threadIdx.x & 63) >> 5;
   const float c = KIND ? 1.0f : p.c;
   const int left = static_cast<int>(n - j < 32 * KB ? n - j : 32 * KB);
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb) {
-    if (KIND) {
-      mask_block(p, st.mrow[t], j + kb * 32 + 4 * h, n, s[kb]);
-    } else if (left < kb * 32 + 32) {
+    if (KIND == 1) keep_block(p, word[kb], s[kb]);
+    if (KIND == 2) bias_block(p, reinterpret_cast<const float*>(st.mrow[t]), j + kb * 32 + 4 * h, n, s[kb]);
+    if (KIND < 2 && left < kb * 32 + 32) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         if (kb * 32 + 8 * (i / 4) + 4 * h + i % 4 >= left) s[kb][i] = kNegInf;
@@ -106,7 +107,7 @@ __device__ __forceinline__ int64_t stat_at(const AttnParams& p, int64_t b, int h
 // Waves a SIMD shall hold: two (256 registers each) wherever a kernel fits without spilling much; a lone
 // wave waits out every latency (bf16, heads of 64, 1024 x 4096 x 192 heads: 602 us with one, 390 with two).
 template <typename T> constexpr int tile_waves(int DP, int KIND) {
-  return sizeof(T) == 2 ? (KIND ? (DP == 128 ? 1 : 2) : DP <= 64 ? 3 : 2) : (DP == 128 || (KIND && DP == 96) ? 1 : 2);
+  return sizeof(T) == 2 ? (KIND ? (DP >= 96 ? 1 : 2) : DP <= 64 ? 3 : 2) : (DP == 128 || (KIND && DP == 96) ? 1 : 2);
 }
 template <typename T> constexpr int few_waves(int DP, int KIND) {
   return sizeof(T) == 2 ? (KIND && DP >= 96 ? 1 : 2) : (DP >= 96 || (KIND && DP == 64) ? 1 : 2);
@@ -137,6 +138,11 @@ __global__ __launch_bounds__(256, tile_waves<T>(DP, KIND)) void attn_fwd_tile_ke
   if (KIND && threadIdx.x < 2) bad_tile[threadIdx.x] = -1;
   if (KIND) __syncthreads();
   int at = 0;
+  uint32_t word[2] = {0, 0};
+  auto words = [&](int64_t j) {                        // (words of whole blocks: bits behind the states are 0)
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) st.word[0][kb] = j + 32 * kb < n && r0 + (threadIdx.x & 31) < p.R ? st.mrow[0][j / 32 + kb] : 0;
+  };
   auto put = [&](int buf, int tile) {
     kr.store(tiles[buf][0], p.D);
     vr.store(tiles[buf][1], p.D);
@@ -145,11 +151,17 @@ __global__ __launch_bounds__(256, tile_waves<T>(DP, KIND)) void attn_fwd_tile_ke
   if (j0 < n) {
     kr.load(k + j0 * p.ks[1], n - j0);
     vr.load(v + j0 * p.vs[1], n - j0);
+    if (KIND == 1) words(j0);
     put(0, 0);
   }
   wait_loads();
   for (int64_t j = j0; j < n; j += KT, ++at) {
     const int64_t next = j + KT;
+    if (KIND == 1) {
+      word[0] = st.word[0][0];
+      word[1] = st.word[0][1];
+      if (next < n) words(next);
+    }
     if (next < n) {
       kr.load(k + next * p.ks[1], n - next);
       vr.load(v + next * p.vs[1], n - next);
@@ -157,7 +169,8 @@ __global__ __launch_bounds__(256, tile_waves<T>(DP, KIND)) void attn_fwd_tile_ke
     __syncthreads();                                   // tile `at` is in LDS, tile at - 1 is done with
     const char* kt = tiles[at & 1][0];
     const char* vt = tiles[at & 1][1];
-    if (r0 < p.R) {                                    // (the last workgroup's waves may have no rows)
+    // (the last workgroup's waves may have no rows, and no row may read this tile)
+    if (r0 < p.R && (KIND != 1 || __any((word[0] | (KB > 1 ? word[1] : 0)) != 0))) {
       f32x16 s[KB] = {};
       Block<T> e[KB];
       Turned<T, LP> va[2][DT];
@@ -166,7 +179,7 @@ __global__ __launch_bounds__(256, tile_waves<T>(DP, KIND)) void attn_fwd_tile_ke
 #pragma unroll
       for (int d = 0; d < DT; ++d) va[0][d].read(vt, 0, d);
       reads_done();
-      softmax_blocks<T, DP, 1, KIND, KB>(p, st, 0, s, e, j, n);
+      softmax_blocks<T, DP, 1, KIND, KB>(p, st, 0, s, e, word, j, n);
       if (KIND && bad_tile[at & 1] == at) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) slow_second<T, LP, DT>(vt, kb * 32, s[kb], st.o[0]);
@@ -260,7 +273,12 @@ __global__ __launch_bounds__(256, few_waves<T>(DP, KIND)) void attn_fwd_few_kern
   Staged<T, LP, 32, 64> vr;
   vr.init(p.vs[1], p.D, l);
   vr.clear(vt, p.D);
+  uint32_t word[QT][2] = {};
   auto fetch = [&](int64_t j) {
+    if (KIND == 1) {
+#pragma unroll
+      for (int q = 0; q < QT; ++q) st.word[q][0] = 32 * q + (l & 31) < p.R ? st.mrow[q][j / 32] : 0;
+    }
     const T* row = k + (j + (l & 31)) * p.ks[1];
 #pragma unroll
     for (int t = 0; t < STEPS; ++t)
@@ -280,12 +298,16 @@ __global__ __launch_bounds__(256, few_waves<T>(DP, KIND)) void attn_fwd_few_kern
     vr.store(vt, p.D);                     // the wave's own tile: LDS serves a wave's accesses in order
     __builtin_amdgcn_wave_barrier();
     const bool bad = KIND && __any(vr.bad());
+    if (KIND == 1) {
+#pragma unroll
+      for (int q = 0; q < QT; ++q) word[q][0] = st.word[q][0];
+    }
     if (j + 128 < n) fetch(j + 128);
 #pragma unroll
     for (int d = 0; d < DT; ++d) va[d].read(vt, 0, d);
     reads_done();
 #pragma unroll
-    for (int q = 0; q < QT; ++q) softmax_blocks<T, DP, QT, KIND, 1>(p, st, q, s[q], e[q], j, n);
+    for (int q = 0; q < QT; ++q) softmax_blocks<T, DP, QT, KIND, 1>(p, st, q, s[q], e[q], word[q], j, n);
 #pragma unroll
     for (int q = 0; q < QT; ++q) {
       if (bad) {
@@ -379,6 +401,35 @@ __global__ __launch_bounds__(256) void attn_fwd_join_kernel(AttnParams p) {
     if (d + e < p.D) put_row<T>(p, b, static_cast<int>(bh - b * p.Hk), x - bh * p.R, d + e, y[e], m, sum);
 }
 
+// Bytes of a mask into bits, a word a thread.
+__global__ __launch_bounds__(256) void attn_pack_kernel(const uint8_t* keep, int64_t s0, int64_t s1, int64_t s2, int64_t s3, int64_t n1,
+                                                        int64_t n2, int64_t states, int64_t per, int64_t all, uint32_t* words) {
+  const int64_t x = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (x >= all) return;
+  const int64_t row = x / per, w = x - row * per, i2 = row % n2, i1 = row / n2 % n1, i0 = row / n2 / n1;
+  const uint8_t* m = keep + i0 * s0 + i1 * s1 + i2 * s2 + w * 32 * s3;
+  const int n = static_cast<int>(states - w * 32 < 32 ? states - w * 32 : 32);
+  uint32_t bits = 0;
+  if (s3 == 1 && n == 32) {
+    uint32_t b[8];
+    __builtin_memcpy(b, m, 32);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) bits |= ((b[i >> 2] >> (8 * (i & 3))) & 0xff ? 1u : 0u) << i;
+  } else {
+    for (int i = 0; i < n; ++i) bits |= (m[i * s3] ? 1u : 0u) << i;
+  }
+  words[x] = bits;
+}
+
+int attn_pack_launch(const void* keep, const int64_t* stride, int64_t n0, int64_t n1, int64_t n2, int64_t states, uint32_t* words,
+                     hipStream_t s) {
+  const int64_t per = (states + 31) / 32, all = n0 * n1 * n2 * per;
+  if (all == 0) return 0;
+  attn_pack_kernel<<<static_cast<unsigned>((all + 255) / 256), 256, 0, s>>>(static_cast<const uint8_t*>(keep), stride[0], stride[1],
+                                                                           stride[2], stride[3], n1, n2, states, per, all, words);
+  return check_launch("fovi_attention_pack_mask");
+}
+
 // How a call is laid out. Few rows: every workgroup has them all. Else tiles of 128 or 256 rows.
 struct FwdPlan {
   bool few;
@@ -443,23 +494,23 @@ static void fwd_launch(const AttnParams& p, const FwdPlan& f, hipStream_t s) {
   }
 }
 
+template <typename T, int KIND>
+static void fwd_heads(const AttnParams& p, const FwdPlan& f, hipStream_t s) {
+  if (p.D <= 32) fwd_launch<T, 32, KIND>(p, f, s);
+  else if (p.D <= 64) fwd_launch<T, 64, KIND>(p, f, s);
+  else if (p.D <= 96) fwd_launch<T, 96, KIND>(p, f, s);
+  else fwd_launch<T, 128, KIND>(p, f, s);
+}
+
 template <typename T>
 static int fwd_type(AttnParams& p, hipStream_t s) {
   const FwdPlan f = fwd_plan(p.B, p.Lq, p.Lk, p.H, p.Hk, p.D, sizeof(T) == 2 ? FOVI_BF16 : FOVI_F32, p.kind != 0);
   p.splits = f.splits;
   p.chunk = f.chunk;
   p.tiles = f.tiles;
-  if (p.kind) {
-    if (p.D <= 32) fwd_launch<T, 32, 1>(p, f, s);
-    else if (p.D <= 64) fwd_launch<T, 64, 1>(p, f, s);
-    else if (p.D <= 96) fwd_launch<T, 96, 1>(p, f, s);
-    else fwd_launch<T, 128, 1>(p, f, s);
-  } else {
-    if (p.D <= 32) fwd_launch<T, 32, 0>(p, f, s);
-    else if (p.D <= 64) fwd_launch<T, 64, 0>(p, f, s);
-    else if (p.D <= 96) fwd_launch<T, 96, 0>(p, f, s);
-    else fwd_launch<T, 128, 0>(p, f, s);
-  }
+  if (p.kind == FOVI_MASK_NONE) fwd_heads<T, 0>(p, f, s);
+  else if (p.kind == FOVI_MASK_KEEP) fwd_heads<T, 1>(p, f, s);
+  else fwd_heads<T, 2>(p, f, s);
   if (check_launch("fovi_attention_fwd")) return 1;
   if (f.splits > 1) {
     const int64_t rows = p.B * p.Hk * p.R;

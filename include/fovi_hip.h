@@ -826,8 +826,10 @@ int fovi_rotary(const fovi_rotary_args* args, void* stream);
  * A state is left out of a row where j >= kv_lengths[b], where a boolean mask holds 0, or where the
  * score is -inf; a row that keeps nothing gives zeros, and no gradient. Values in places that a mask
  * or a length leaves out have no effect, infinities and NaN included.
- * mask_kind: FOVI_MASK_NONE; FOVI_MASK_KEEP, bytes, 0 = left out; FOVI_MASK_BIAS, fp32 added to the
- * scores. mask strides [batch, head, query, state], 0 where it is broadcast. kv_lengths: int32
+ * mask_kind: FOVI_MASK_NONE; FOVI_MASK_KEEP, uint32 words of fovi_attention_pack_mask, bit j % 32 of word
+ * j / 32 set where state j is read, strides [batch, head, query] in words (the fourth unused);
+ * FOVI_MASK_BIAS, fp32 added to the scores, strides [batch, head, query, state] in elements. Strides
+ * are 0 where the mask is broadcast. kv_lengths: int32
  * [batch] on the device, NULL for kv_len; taken as within [0, kv_len].
  * dtype F32 or BF16 for q, k, v, out and the gradients; strides [batch, token, head], head elements
  * adjacent, every head of whole 16-byte pieces at a 16-byte aligned address, tokens less than 64 MiB
@@ -863,6 +865,11 @@ typedef struct fovi_attention_args {
   void* workspace;
   int64_t workspace_bytes;
 } fovi_attention_args;
+
+/* keep: bytes [n0, n1, n2, kv_len] (0 = left out), element strides; words: [n0, n1, n2, (kv_len + 31) / 32],
+ * bits behind kv_len 0. */
+int fovi_attention_pack_mask(const void* keep, const int64_t* stride, int64_t n0, int64_t n1, int64_t n2, int64_t kv_len,
+                             uint32_t* words, void* stream);
 
 int64_t fovi_attention_fwd_workspace_bytes(int64_t batch, int64_t q_len, int64_t kv_len, int64_t heads,
                                            int64_t kv_heads, int64_t head_dim, int32_t dtype);
