@@ -280,12 +280,12 @@ struct Staged {
   // rows [0, n) of `base`, n > 0
   __device__ __forceinline__ void load(const T* base, int64_t n) {
     const bool full = n >= ROWS;
-    const int last = full ? ROWS - 1 : static_cast<int>(n) - 1;
+    const int last = static_cast<int>(n) - 1;
     const char* at = reinterpret_cast<const char*>(base);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       uint32_t o = off + i * STEP * pitch;
-      if (!full) o = (row + i * STEP < last ? row + i * STEP : last) * pitch + col;
+      if (!full) [[unlikely]] o = (row + i * STEP < last ? row + i * STEP : last) * pitch + col;
       r[i] = *reinterpret_cast<const u32x4*>(at + o);
     }
   }

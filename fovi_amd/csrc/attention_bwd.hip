@@ -246,19 +246,29 @@ __global__ __launch_bounds__(256, dkv_waves<T>(DP, KIND)) void attn_dkv_kernel(A
   if (KIND && threadIdx.x < 4) bad_tile[threadIdx.x >> 1][threadIdx.x & 1] = -1;
   if (KIND) __syncthreads();
   int h = hk * p.G + static_cast<int>(first / per), i0 = static_cast<int>(first % per) * RT;      // the next tile to fetch
+  // the next tile's rows: pointers move along, a new head sets them anew
+  const T *qp, *gp;
+  const float* sp;
+  const int64_t sums = p.B * p.H * p.Lq;
+  auto rewind = [&]() {
+    qp = static_cast<const T*>(p.q) + b * p.qs[0] + i0 * p.qs[1] + h * p.qs[2];
+    gp = static_cast<const T*>(p.dout) + b * p.dos[0] + i0 * p.dos[1] + h * p.dos[2];
+    sp = p.stats + (b * p.H + h) * p.Lq + i0;
+  };
   auto fetch = [&]() {
-    qr.load(static_cast<const T*>(p.q) + b * p.qs[0] + i0 * p.qs[1] + h * p.qs[2], p.Lq - i0);
-    gr.load(static_cast<const T*>(p.dout) + b * p.dos[0] + i0 * p.dos[1] + h * p.dos[2], p.Lq - i0);
+    const int left = static_cast<int>(p.Lq - i0 < RT ? p.Lq - i0 : RT);
+    qr.load(qp, left);
+    gr.load(gp, left);
     if (threadIdx.x < RT) {
-      const bool in = i0 + threadIdx.x < p.Lq;
-      const int64_t at = (b * p.H + h) * p.Lq + (in ? i0 + threadIdx.x : 0);
-      m = p.stats[at];
-      sum = in ? p.stats[p.B * p.H * p.Lq + at] : 0.0f;
-      delta = p.delta[at];
+      const bool in = static_cast<int>(threadIdx.x) < left;
+      const float* at = sp + (in ? threadIdx.x : 0);
+      m = at[0];
+      sum = in ? at[sums] : 0.0f;
+      delta = p.delta[at - p.stats];
     }
     if (KIND == 1) {
       const int r = threadIdx.x % RT, w = threadIdx.x / RT;
-      word = w < 4 && i0 + r < p.Lq && w0 + 32 * w < p.Lk ? mask_row(p, b, h, i0 + r)[w0 / 32 + w] : 0;
+      word = w < 4 && r < left && w0 + 32 * w < p.Lk ? mask_row(p, b, h, i0 + r)[w0 / 32 + w] : 0;
     }
   };
   auto put = [&](int buf, int tile) {
@@ -274,6 +284,7 @@ __global__ __launch_bounds__(256, dkv_waves<T>(DP, KIND)) void attn_dkv_kernel(A
     if (KIND && qr.bad()) bad_tile[buf][0] = tile;
     if (KIND && gr.bad()) bad_tile[buf][1] = tile;
   };
+  rewind();
   if (count > 0) {
     fetch();
     put(0, 0);
@@ -282,10 +293,17 @@ __global__ __launch_bounds__(256, dkv_waves<T>(DP, KIND)) void attn_dkv_kernel(A
   for (int at = 0; at < count; ++at) {
     const int h_at = h, i_at = i0;
     i0 += RT;
-    if (i0 >= p.Lq) { i0 = 0; ++h; }
+    qp += RT * p.qs[1];
+    gp += RT * p.dos[1];
+    sp += RT;
+    if (i0 >= p.Lq) {
+      i0 = 0;
+      ++h;
+      rewind();
+    }
     if (at + 1 < count) fetch();
     __syncthreads();
-#pragma unroll 1                        // (both blocks at once would not fit 256 registers)
+#pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
       const char* qt = tiles[at & 1][0] + rb * 32 * LP * sizeof(T);
       const char* gt = tiles[at & 1][1] + rb * 32 * LP * sizeof(T);

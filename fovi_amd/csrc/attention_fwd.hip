@@ -455,12 +455,13 @@ static FwdPlan fwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk
     f.qt = 1;
     f.tiles = (R + 127) / 128;
   }
-  // The states are split until the card is full (few rows: twice, lengths differ), in parts that are
-  // still worth a workgroup's start and the join: 512 states for few rows (131072 states, 4 groups, heads
-  // of 128: parts of 512 60 + 9 us, of 256 80 + 14), 128 for tiles (515 states, 32 groups, fp32 under a
-  // mask: parts of 128 14 us, of 256 23; the join 5 each).
+  // The states are split until the card is full (few rows of many key heads: twice, since lengths
+  // differ), in parts that are still worth a workgroup's start and the join: 512 states for few rows
+  // (131072 states, 4 key heads of 128: 128 parts 51.6 + 6.7 us, 256 parts 53.5 + 8.9, 64 parts 52.7 + 5.5, but
+  // where a wave a SIMD is all there is, 9000 fp32 states and 32 heads of 80: 8 parts 57, 4 98), 128 for
+  // tiles (515 states, 32 groups, fp32 under a mask: parts of 128 14 us, of 256 23; the join 5 each).
   const int waves = f.few ? few_waves_at(dtype, D, mask) : 2;
-  const int64_t groups = B * Hk * f.tiles, want = f.few ? 512 * waves : 512, least = f.few ? 512 : 128;
+  const int64_t groups = B * Hk * f.tiles, least = f.few ? 512 : 128, want = f.few ? (groups < 64 ? 256 : 512) * waves : 512;
   int64_t splits = groups > 0 ? want / groups : 1;
   if (splits > (Lk + least - 1) / least) splits = (Lk + least - 1) / least;
   if (splits > 1024) splits = 1024;
