@@ -42,7 +42,6 @@ __device__ __forceinline__ int64_t attn_len(const AttnParams& p, int64_t b) {
   return n < 0 ? 0 : n < p.Lk ? n : p.Lk;
 }
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));     // (a struct of four would be loaded in parts)
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 

@@ -18,7 +18,8 @@ static int attn_check(const fovi_attention_args* a, const char* what) {
   if (!(a->scale > 0) || a->scale > 2.0e38f) { set_error("%s: scale must be positive and finite", what); return 1; }
   if (a->mask_kind < FOVI_MASK_NONE || a->mask_kind > FOVI_MASK_BIAS) { set_error("%s: unknown mask_kind", what); return 1; }
   if (a->mask_kind != FOVI_MASK_NONE && a->kv_len && !a->mask) { set_error("%s: null mask", what); return 1; }
-  if (a->batch * a->heads * a->q_len > 0x7fffffff || a->batch * a->kv_heads * a->kv_len > 0x7fffffff) {
+  if (a->q_len > 0x7fffffff / a->heads / (a->batch ? a->batch : 1) ||
+      a->kv_len > 0x7fffffff / a->kv_heads / (a->batch ? a->batch : 1)) {
     set_error("%s: too many rows or states", what);
     return 1;
   }

@@ -29,22 +29,6 @@ __device__ __forceinline__ float norm_param(const void* p, int64_t c, int bf16, 
   return bf16 ? bf16_bits_to_f32(static_cast<const uint16_t*>(p)[c]) : static_cast<const float*>(p)[c];
 }
 
-// VEC parameters from channel c on (wide loads: a workgroup's first work), `none` without any.
-template <int VEC>
-__device__ __forceinline__ void norm_params_at(const void* p, int64_t c, int64_t C, int bf16, float none, float (&v)[VEC]) {
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) v[i] = none;
-  if (!p || c >= C) return;
-  if (bf16) {
-    uint16_t e[VEC];
-    __builtin_memcpy(e, static_cast<const uint16_t*>(p) + c, sizeof(e));
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = bf16_bits_to_f32(e[i]);
-  } else {
-    __builtin_memcpy(v, static_cast<const float*>(p) + c, sizeof(v));
-  }
-}
-
 // Sum over the workgroup of 256; every thread gets the result.
 __device__ __forceinline__ float block_sum(float v, float* sh) {
 #pragma unroll
@@ -55,32 +39,74 @@ __device__ __forceinline__ float block_sum(float v, float* sh) {
   return (sh[0] + sh[1]) + (sh[2] + sh[3]);
 }
 
-// VEC adjacent channels from c on as floats; zeros from C on. VEC > 1: 16 bytes, C a multiple of VEC.
+// VEC adjacent channels (16 bytes) from c on as floats; zeros from C on. The accesses need no alignment, so
+// that rows of any width and offset come in whole pieces. short_piece (a constant): the piece may pass the
+// end of the row; then it is read as the row's last 16 bytes and shifted down (reading it by elements cost
+// rows of 385 bf16 channels 15 %), and written in parts of 8, 4 and 2 bytes.
 template <typename T, int VEC>
-__device__ __forceinline__ void norm_load(const T* row, int64_t c, int64_t C, float (&v)[VEC]) {
-  if (VEC == 1) {
-    v[0] = c < C ? Elem<T>::load(row + c) : 0.0f;
-    return;
+__device__ __forceinline__ void norm_load(const T* row, int64_t c, int64_t C, float (&v)[VEC], bool short_piece) {
+  T e[VEC];
+  if (!short_piece) {
+    u32x4 u = {0, 0, 0, 0};
+    if (c < C) __builtin_memcpy(&u, row + c, 16);
+    __builtin_memcpy(e, &u, sizeof(e));
+  } else if (C >= VEC) {
+    const int64_t at = c + VEC <= C ? c : C - VEC;
+    u32x4 u;
+    __builtin_memcpy(&u, row + at, 16);
+    uint64_t w[2];
+    __builtin_memcpy(w, &u, 16);
+    const int64_t over = (c - at) * 8 * static_cast<int>(sizeof(T));
+    const int bits = static_cast<int>(over) & 63;
+    if (over >= 64) { w[0] = over < 128 ? w[1] : 0; w[1] = 0; }
+    w[0] = (w[0] >> bits) | (w[1] << 1 << (63 - bits));
+    w[1] >>= bits;
+    __builtin_memcpy(e, w, sizeof(e));
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) e[i] = c + i < C ? row[c + i] : T(0);
   }
-  const uint4 u = c < C ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
-  T e[16 / sizeof(T)];
-  __builtin_memcpy(e, &u, 16);
 #pragma unroll
   for (int i = 0; i < VEC; ++i) v[i] = Elem<T>::load(e + i);
 }
 template <typename T, int VEC>
-__device__ __forceinline__ void norm_store(T* row, int64_t c, int64_t C, const float (&v)[VEC]) {
-  if (c >= C) return;
-  if (VEC == 1) {
-    Elem<T>::store(row + c, v[0]);
-    return;
-  }
-  T e[16 / sizeof(T)];
+__device__ __forceinline__ void norm_store(T* row, int64_t c, int64_t C, const float (&v)[VEC], bool short_piece) {
+  T e[VEC];
 #pragma unroll
   for (int i = 0; i < VEC; ++i) Elem<T>::store(e + i, v[i]);
-  uint4 u;
-  __builtin_memcpy(&u, e, 16);
-  *reinterpret_cast<uint4*>(row + c) = u;
+  if (c + (short_piece ? VEC - 1 : 0) < C) {
+    u32x4 u;
+    __builtin_memcpy(&u, e, sizeof(e));
+    __builtin_memcpy(row + c, &u, 16);
+  } else if (short_piece && c < C) {
+    T* at = row + c;
+    const int n = static_cast<int>(C - c);
+    uint64_t w[2];
+    __builtin_memcpy(w, e, sizeof(e));
+    if (n * sizeof(T) & 8) { __builtin_memcpy(at, w, 8); at += 8 / sizeof(T); w[0] = w[1]; }
+    if (n * sizeof(T) & 4) { __builtin_memcpy(at, w, 4); at += 4 / sizeof(T); w[0] >>= 32; }
+    if (n * sizeof(T) & 2) __builtin_memcpy(at, w, 2);
+  }
+}
+
+// VEC parameters from channel c on (wide loads: a workgroup's first work), `none` without any.
+template <int VEC>
+__device__ __forceinline__ void norm_params_at(const void* p, int64_t c, int64_t C, int bf16, float none, float (&v)[VEC]) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) v[i] = none;
+  if (!p || c >= C) return;
+  if (c + VEC > C) {
+#pragma unroll
+    for (int i = 0; i < VEC - 1; ++i)
+      if (c + i < C) v[i] = norm_param(p, c + i, bf16, none);
+  } else if (bf16) {
+    uint16_t e[VEC];
+    __builtin_memcpy(e, static_cast<const uint16_t*>(p) + c, sizeof(e));
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = bf16_bits_to_f32(e[i]);
+  } else {
+    __builtin_memcpy(v, static_cast<const float*>(p) + c, sizeof(v));
+  }
 }
 
 // Sum over a group of LANES; every lane gets the result.
@@ -92,7 +118,7 @@ __device__ __forceinline__ float group_sum(float v, float* sh) {
   return v;
 }
 
-template <typename T, int VEC, int LANES, int NV>
+template <typename T, int VEC, int LANES, int NV, bool TAIL>
 __global__ __launch_bounds__(256) void norm_fwd_rows_kernel(NormParams p) {
   __shared__ float sh[4];
   const int lane = threadIdx.x % LANES;
@@ -110,7 +136,7 @@ __global__ __launch_bounds__(256) void norm_fwd_rows_kernel(NormParams p) {
     T* yr = static_cast<T*>(p.y) + i0 * p.ys[0] + i1 * p.ys[1];
     float x[NV][VEC], s = 0;
 #pragma unroll
-    for (int k = 0; k < NV; ++k) norm_load<T, VEC>(xr, static_cast<int64_t>(lane + k * LANES) * VEC, p.C, x[k]);
+    for (int k = 0; k < NV; ++k) norm_load<T, VEC>(xr, static_cast<int64_t>(lane + k * LANES) * VEC, p.C, x[k], TAIL && k == NV - 1);
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
@@ -119,10 +145,10 @@ __global__ __launch_bounds__(256) void norm_fwd_rows_kernel(NormParams p) {
     s = 0;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const bool in = static_cast<int64_t>(lane + k * LANES) * VEC < p.C;
+      const int64_t c = static_cast<int64_t>(lane + k * LANES) * VEC;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        x[k][i] = in ? x[k][i] - mean : 0.0f;
+        x[k][i] = c + (TAIL ? i : 0) < p.C ? x[k][i] - mean : 0.0f;
         s = fmaf(x[k][i], x[k][i], s);
       }
     }
@@ -133,13 +159,13 @@ __global__ __launch_bounds__(256) void norm_fwd_rows_kernel(NormParams p) {
       float y[VEC];
 #pragma unroll
       for (int i = 0; i < VEC; ++i) y[i] = fmaf(x[k][i] * rstd, w[k][i], b[k][i]);
-      norm_store<T, VEC>(yr, static_cast<int64_t>(lane + k * LANES) * VEC, p.C, y);
+      norm_store<T, VEC>(yr, static_cast<int64_t>(lane + k * LANES) * VEC, p.C, y, TAIL && k == NV - 1);
     }
   }
 }
 
 // dx of the rows and, with `partial`, the workgroup's sums of dy * h and dy: partial[(block * 2 + {0, 1}) * C + c].
-template <typename T, int VEC, int LANES, int NV>
+template <typename T, int VEC, int LANES, int NV, bool TAIL>
 __global__ __launch_bounds__(256) void norm_bwd_rows_kernel(NormParams p, float* partial) {
   __shared__ float sh[4];
   const int lane = threadIdx.x % LANES;
@@ -161,15 +187,15 @@ __global__ __launch_bounds__(256) void norm_bwd_rows_kernel(NormParams p, float*
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int64_t c = static_cast<int64_t>(lane + k * LANES) * VEC;
-      norm_load<T, VEC>(xr, c, p.C, h[k]);
-      norm_load<T, VEC>(gr, c, p.C, g[k]);
+      norm_load<T, VEC>(xr, c, p.C, h[k], TAIL && k == NV - 1);
+      norm_load<T, VEC>(gr, c, p.C, g[k], TAIL && k == NV - 1);
     }
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const bool in = static_cast<int64_t>(lane + k * LANES) * VEC < p.C;
+      const int64_t c = static_cast<int64_t>(lane + k * LANES) * VEC;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        h[k][i] = in ? (h[k][i] - mean) * rstd : 0.0f;
+        h[k][i] = c + (TAIL ? i : 0) < p.C ? (h[k][i] - mean) * rstd : 0.0f;
         dw[k][i] = fmaf(g[k][i], h[k][i], dw[k][i]);
         db[k][i] += g[k][i];
         g[k][i] *= w[k][i];
@@ -186,7 +212,7 @@ __global__ __launch_bounds__(256) void norm_bwd_rows_kernel(NormParams p, float*
       float dx[VEC];
 #pragma unroll
       for (int i = 0; i < VEC; ++i) dx[i] = rstd * (g[k][i] - sg - h[k][i] * sgh);
-      norm_store<T, VEC>(dxr, static_cast<int64_t>(lane + k * LANES) * VEC, p.C, dx);
+      norm_store<T, VEC>(dxr, static_cast<int64_t>(lane + k * LANES) * VEC, p.C, dx, TAIL && k == NV - 1);
     }
   }
   if (!partial) return;
@@ -326,26 +352,19 @@ __global__ __launch_bounds__(256) void norm_dw_join_kernel(const float* partial,
   else static_cast<float*>(out)[c] = t;
 }
 
-// The shape of a call: VEC channels a load (16 bytes, or one where rows or widths are not whole
-// pieces), the lanes of a row and the loads a lane holds; nv 0: too wide for registers. Rows of up to 64
-// pieces take 16 lanes (4 rows a wave: a shorter reduction, no idle lanes at 48 pieces), unless
-// there are too few rows to fill the card that way.
-struct NormPlan { bool vec; int lanes, nv; };
+// The shape of a call: the lanes of a row and the 16-byte pieces a lane holds (nv 0: too wide for registers).
+// Rows of up to 64 pieces take 16 lanes (4 rows a wave: a shorter reduction, no idle lanes at 48 pieces),
+// unless there are too few rows to fill the card that way. Rows that are not whole pieces take pieces too
+// (element by element, 60000 bf16 rows of 385 took 39 and 133 us forward and backward, now 26 and 35; fp32
+// rows of 771 take 13 and 18 us either way within 10 %).
+struct NormPlan { bool tail; int lanes, nv; };
 
-static NormPlan norm_plan(int64_t rows, int64_t C, int es, bool aligned) {
+static NormPlan norm_plan(int64_t rows, int64_t C, int es) {
   NormPlan f;
-  f.vec = aligned && C * es % 16 == 0;
-  const int64_t n = f.vec ? C * es / 16 : C;
-  if (n <= 64) {
-    f.lanes = rows >= 4096 || !f.vec ? 16 : 64;
-    f.nv = static_cast<int>((n + f.lanes - 1) / f.lanes);
-  } else if (f.vec) {
-    f.lanes = n <= 256 ? 64 : 256;
-    f.nv = n <= 1024 ? static_cast<int>((n + f.lanes - 1) / f.lanes) : 0;
-  } else {
-    f.lanes = n <= 1024 ? 64 : 256;
-    f.nv = n <= 128 ? 2 : n <= 256 ? 4 : n <= 512 ? 8 : n <= 1024 ? 16 : n <= 2048 ? 8 : n <= 4096 ? 16 : 0;
-  }
+  f.tail = C * es % 16 != 0;
+  const int64_t n = (C * es + 15) / 16;
+  f.lanes = n <= 64 ? (rows >= 4096 ? 16 : 64) : n <= 256 ? 64 : 256;
+  f.nv = n <= 1024 ? static_cast<int>((n + f.lanes - 1) / f.lanes) : 0;
   return f;
 }
 
@@ -361,35 +380,31 @@ static int64_t norm_chunks(int64_t rows, int64_t C) {
   return chunks < 1 ? 1 : chunks;
 }
 
-// Calls fn<T, VEC, LANES, NV>; false where the plan has no such kernel.
-#define FOVI_NORM_CASES(CALL)                                                                        \
-  if (f.vec) {                                                                                       \
-    constexpr int V = 16 / sizeof(T);                                                                \
-    if (f.lanes == 16) {                                                                             \
-      if (f.nv == 1) CALL(V, 16, 1) else if (f.nv == 2) CALL(V, 16, 2) else if (f.nv == 3) CALL(V, 16, 3) else CALL(V, 16, 4) \
-    } else if (f.lanes == 64) {                                                                      \
-      if (f.nv == 1) CALL(V, 64, 1) else if (f.nv == 2) CALL(V, 64, 2) else if (f.nv == 3) CALL(V, 64, 3) else CALL(V, 64, 4) \
-    } else {                                                                                         \
-      if (f.nv == 2) CALL(V, 256, 2) else if (f.nv == 3) CALL(V, 256, 3) else CALL(V, 256, 4)        \
-    }                                                                                                \
-  } else if (f.lanes == 16) {                                                                        \
-    if (f.nv == 1) CALL(1, 16, 1) else if (f.nv == 2) CALL(1, 16, 2) else if (f.nv == 3) CALL(1, 16, 3) else CALL(1, 16, 4) \
-  } else if (f.lanes == 64) {                                                                        \
-    if (f.nv == 2) CALL(1, 64, 2) else if (f.nv == 4) CALL(1, 64, 4) else if (f.nv == 8) CALL(1, 64, 8) else CALL(1, 64, 16) \
-  } else {                                                                                           \
-    if (f.nv == 8) CALL(1, 256, 8) else CALL(1, 256, 16)                                             \
+// CALL(lanes, pieces, short last piece) of a plan.
+#define FOVI_NORM_TAIL(CALL, L, N) \
+  if (f.tail) CALL(L, N, true) else CALL(L, N, false)
+#define FOVI_NORM_CASES(CALL)                                                                            \
+  if (f.lanes == 16) {                                                                                   \
+    if (f.nv == 1) { FOVI_NORM_TAIL(CALL, 16, 1) } else if (f.nv == 2) { FOVI_NORM_TAIL(CALL, 16, 2) }   \
+    else if (f.nv == 3) { FOVI_NORM_TAIL(CALL, 16, 3) } else { FOVI_NORM_TAIL(CALL, 16, 4) }             \
+  } else if (f.lanes == 64) {                                                                            \
+    if (f.nv == 1) { FOVI_NORM_TAIL(CALL, 64, 1) } else if (f.nv == 2) { FOVI_NORM_TAIL(CALL, 64, 2) }   \
+    else if (f.nv == 3) { FOVI_NORM_TAIL(CALL, 64, 3) } else { FOVI_NORM_TAIL(CALL, 64, 4) }             \
+  } else {                                                                                               \
+    if (f.nv == 2) { FOVI_NORM_TAIL(CALL, 256, 2) } else if (f.nv == 3) { FOVI_NORM_TAIL(CALL, 256, 3) } \
+    else { FOVI_NORM_TAIL(CALL, 256, 4) }                                                                \
   }
 
 template <typename T>
-static void norm_fwd_launch(const NormParams& p, bool aligned, hipStream_t s) {
+static void norm_fwd_launch(const NormParams& p, hipStream_t s) {
   const int64_t rows = p.rows0 * p.rows1;
-  const NormPlan f = norm_plan(rows, p.C, sizeof(T), aligned);
+  const NormPlan f = norm_plan(rows, p.C, sizeof(T));
   if (f.nv == 0) {
     norm_fwd_kernel<T><<<static_cast<unsigned>(rows < (1 << 16) ? rows : (1 << 16)), 256, 0, s>>>(p);
     return;
   }
   const unsigned grid = static_cast<unsigned>(norm_groups(rows, f, 2048));
-#define CALL(V, L, N) norm_fwd_rows_kernel<T, V, L, N><<<grid, 256, 0, s>>>(p);
+#define CALL(L, N, TAIL) norm_fwd_rows_kernel<T, 16 / sizeof(T), L, N, TAIL><<<grid, 256, 0, s>>>(p);
   FOVI_NORM_CASES(CALL)
 #undef CALL
 }
@@ -397,9 +412,9 @@ static void norm_fwd_launch(const NormParams& p, bool aligned, hipStream_t s) {
 constexpr int64_t kNormBlocks = 512;                 // workgroups of the backward: rows of partial sums
 
 template <typename T>
-static int64_t norm_bwd_launch(const NormParams& p, bool aligned, float* partial, hipStream_t s) {
+static int64_t norm_bwd_launch(const NormParams& p, float* partial, hipStream_t s) {
   const int64_t rows = p.rows0 * p.rows1;
-  const NormPlan f = norm_plan(rows, p.C, sizeof(T), aligned);
+  const NormPlan f = norm_plan(rows, p.C, sizeof(T));
   if (f.nv == 0) {
     if (p.dx) norm_dx_kernel<T><<<static_cast<unsigned>(rows < (1 << 16) ? rows : (1 << 16)), 256, 0, s>>>(p);
     if (!partial) return 0;
@@ -409,15 +424,12 @@ static int64_t norm_bwd_launch(const NormParams& p, bool aligned, float* partial
   }
   const int64_t groups = norm_groups(rows, f, kNormBlocks);
   const unsigned grid = static_cast<unsigned>(groups);
-#define CALL(V, L, N) \
-  norm_bwd_rows_kernel<T, V, L, N><<<grid, 256, partial && L < 256 ? 4 * 2 * L * N * V * 4 : 0, s>>>(p, partial);
+#define CALL(L, N, TAIL)                                       \
+  norm_bwd_rows_kernel<T, 16 / sizeof(T), L, N, TAIL>          \
+      <<<grid, 256, partial && L < 256 ? 4 * 2 * L * N * (16 / sizeof(T)) * 4 : 0, s>>>(p, partial);
   FOVI_NORM_CASES(CALL)
 #undef CALL
   return groups;
-}
-
-static bool norm_aligned(const void* p, const int64_t* stride, int es) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride[0] * es % 16 == 0 && stride[1] * es % 16 == 0;
 }
 
 static int norm_check(const fovi_layer_norm_args* a, const char* what) {
@@ -456,11 +468,9 @@ extern "C" int fovi_layer_norm_fwd(const fovi_layer_norm_args* a, void* stream) 
   const int64_t rows = a->rows0 * a->rows1;
   if (rows == 0) return 0;
   const NormParams p = norm_params(a);
-  const int es = a->dtype == FOVI_BF16 ? 2 : 4;
-  const bool aligned = norm_aligned(p.x, p.xs, es) && norm_aligned(p.y, p.ys, es);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (a->dtype == FOVI_BF16) norm_fwd_launch<uint16_t>(p, aligned, s);
-  else norm_fwd_launch<float>(p, aligned, s);
+  if (a->dtype == FOVI_BF16) norm_fwd_launch<uint16_t>(p, s);
+  else norm_fwd_launch<float>(p, s);
   return check_launch("fovi_layer_norm_fwd");
 }
 
@@ -487,9 +497,7 @@ extern "C" int fovi_layer_norm_bwd(const fovi_layer_norm_args* a, void* stream) 
   int64_t chunks = 0;
   float* partial = params ? static_cast<float*>(a->workspace) : nullptr;
   if (rows) {
-    const int es = a->dtype == FOVI_BF16 ? 2 : 4;
-    const bool aligned = norm_aligned(p.x, p.xs, es) && norm_aligned(p.dy, p.dys, es) && (!p.dx || norm_aligned(p.dx, p.dxs, es));
-    chunks = a->dtype == FOVI_BF16 ? norm_bwd_launch<uint16_t>(p, aligned, partial, s) : norm_bwd_launch<float>(p, aligned, partial, s);
+    chunks = a->dtype == FOVI_BF16 ? norm_bwd_launch<uint16_t>(p, partial, s) : norm_bwd_launch<float>(p, partial, s);
     if (check_launch("fovi_layer_norm_bwd")) return 1;
   }
   if (!params) return 0;

@@ -33,21 +33,47 @@ __device__ __forceinline__ float2 rotary_angle(const RotaryParams& p, int64_t to
   return make_float2(c, p.inverse ? -s : s);
 }
 
-// N adjacent elements in one access (N * sizeof(T) is 2 to 16 bytes, aligned).
-template <typename T, int N> struct alignas(N * sizeof(T)) Run { T e[N]; };
+// Runs of 16 bytes (N elements, any alignment): whole, or with SHORT the first n elements.
+template <typename T, int N, bool SHORT>
+__device__ __forceinline__ void load_run(const T* p, int n, T (&e)[N]) {
+  u32x4 u = {0, 0, 0, 0};
+  if (!SHORT || n >= N) __builtin_memcpy(&u, p, 16);
+  __builtin_memcpy(e, &u, 16);
+  if (SHORT && n < N) {
+#pragma unroll
+    for (int i = 0; i < N - 1; ++i)
+      if (i < n) e[i] = p[i];
+  }
+}
+template <typename T, int N, bool SHORT>
+__device__ __forceinline__ void save_run(T* p, int n, const T (&e)[N]) {
+  if (!SHORT || n >= N) {
+    u32x4 u;
+    __builtin_memcpy(&u, e, 16);
+    __builtin_memcpy(p, &u, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N - 1; ++i)
+      if (i < n) p[i] = e[i];
+  }
+}
 
-// VEC: elements of an access. Half pairing: a unit is VEC pairs (j .. j + VEC, and n_pairs further on),
-// then come units of VEC copied elements; VEC divides n_pairs and head_dim. Adjacent pairing: a unit
-// is VEC elements, VEC / 2 pairs, turned or copied; VEC divides head_dim. A thread keeps its unit of a
-// token's row and goes from token to token.
-template <typename T, int VEC, bool ADJACENT>
+// Half pairing: a unit is VEC pairs (j .. j + VEC, and n_pairs further on), then come units of VEC copied
+// elements. Adjacent pairing: a unit is VEC elements, VEC / 2 pairs, turned or copied. A thread keeps its
+// unit of a token's row and goes from token to token. ODD: the units do not divide those runs; the last one
+// of a run starts VEC before its end, beside elements that the unit before writes as well (the same values),
+// or is short where the run is, or where an odd head would split its pairs.
+template <typename T, bool ADJACENT, bool ODD>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p) {
+  constexpr int VEC = 16 / sizeof(T);
   __shared__ __attribute__((aligned(16))) float2 table[kRotaryTable];
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.tokens, all = p.B * p.L;
   const int n = static_cast<int>(all - t0 < p.tokens ? all - t0 : p.tokens);
   for (int i = threadIdx.x; i < n * p.P; i += 256) table[i] = rotary_angle(p, t0 + i / p.P, i % p.P);
   __syncthreads();
-  const int per = ADJACENT ? p.D / VEC : (p.D - p.P) / VEC, units = p.H * per, at_once = units < 256 ? 256 / units : 1;
+  const int turned = (p.P + VEC - 1) / VEC, rest = p.D - 2 * p.P;
+  const int per = ADJACENT ? (p.D + VEC - 1) / VEC : turned + (rest + VEC - 1) / VEC, units = p.H * per;
+  const int at_once = units < 256 ? 256 / units : 1;
   const int64_t b0 = t0 / p.L, l0 = t0 - b0 * p.L;
   for (int t = threadIdx.x / units; t < n; t += at_once) {
     if (units < 256 && threadIdx.x >= static_cast<unsigned>(units * at_once)) break;
@@ -57,91 +83,67 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p) {
     T* yt = static_cast<T*>(p.y) + b * p.ys[0] + l * p.ys[1];
     const float2* turn = table + t * p.P;
     for (int u = units < 256 ? threadIdx.x % units : threadIdx.x; u < units; u += 256) {
-      const int h = u / per, j = (u - h * per) * VEC;
-      const T* x = xt + h * p.xs[2] + j;
-      T* y = yt + h * p.ys[2] + j;
+      const int h = u / per, r = u - h * per;
+      int j = r * VEC;
       if (ADJACENT) {
-        const Run<T, VEC> a = *reinterpret_cast<const Run<T, VEC>*>(x);
-        Run<T, VEC> o = a;
+        if (ODD && j + VEC > p.D && p.D >= VEC && p.D % 2 == 0) j = p.D - VEC;
+        const T* x = xt + h * p.xs[2] + j;
+        T* y = yt + h * p.ys[2] + j;
+        T a[VEC], o[VEC];
+        load_run<T, VEC, ODD>(x, p.D - j, a);
 #pragma unroll
-        for (int i = 0; i + 1 < VEC; i += 2)
+        for (int i = 0; i < VEC; i += 2) {
+          o[i] = a[i];
+          o[i + 1] = a[i + 1];
           if (j + i < 2 * p.P) {
             const float2 cs = turn[(j + i) / 2];
-            const float u0 = Elem<T>::load(&a.e[i]), v0 = Elem<T>::load(&a.e[i + 1]);
-            Elem<T>::store(&o.e[i], u0 * cs.x - v0 * cs.y);
-            Elem<T>::store(&o.e[i + 1], v0 * cs.x + u0 * cs.y);
+            const float u0 = Elem<T>::load(&a[i]), v0 = Elem<T>::load(&a[i + 1]);
+            Elem<T>::store(&o[i], u0 * cs.x - v0 * cs.y);
+            Elem<T>::store(&o[i + 1], v0 * cs.x + u0 * cs.y);
           }
-        *reinterpret_cast<Run<T, VEC>*>(y) = o;
-      } else if (j >= p.P) {
-        *reinterpret_cast<Run<T, VEC>*>(y + p.P) = *reinterpret_cast<const Run<T, VEC>*>(x + p.P);
+        }
+        save_run<T, VEC, ODD>(y, p.D - j, o);
+        continue;
+      }
+      const bool copied = r >= turned;
+      if (ODD) {
+        if (copied) j -= turned * VEC - p.P;
+        const int run = copied ? rest : p.P, end = copied ? p.D - p.P : p.P;
+        if (j + VEC > end && run >= VEC) j = end - VEC;
+      }
+      const T* x = xt + h * p.xs[2] + j;
+      T* y = yt + h * p.ys[2] + j;
+      if (copied) {
+        T c[VEC];
+        load_run<T, VEC, ODD>(x + p.P, p.D - p.P - j, c);
+        save_run<T, VEC, ODD>(y + p.P, p.D - p.P - j, c);
       } else {
-        const Run<T, VEC> a = *reinterpret_cast<const Run<T, VEC>*>(x), c = *reinterpret_cast<const Run<T, VEC>*>(x + p.P);
-        Run<T, VEC> ao, co;
+        T a[VEC], c[VEC], ao[VEC], co[VEC];
+        load_run<T, VEC, ODD>(x, p.P - j, a);
+        load_run<T, VEC, ODD>(x + p.P, p.P - j, c);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-          const float2 cs = turn[j + i];
-          const float u0 = Elem<T>::load(&a.e[i]), v0 = Elem<T>::load(&c.e[i]);
-          Elem<T>::store(&ao.e[i], u0 * cs.x - v0 * cs.y);
-          Elem<T>::store(&co.e[i], v0 * cs.x + u0 * cs.y);
+          const float2 cs = turn[!ODD || j + i < p.P ? j + i : p.P - 1];
+          const float u0 = Elem<T>::load(&a[i]), v0 = Elem<T>::load(&c[i]);
+          Elem<T>::store(&ao[i], u0 * cs.x - v0 * cs.y);
+          Elem<T>::store(&co[i], v0 * cs.x + u0 * cs.y);
         }
-        *reinterpret_cast<Run<T, VEC>*>(y) = ao;
-        *reinterpret_cast<Run<T, VEC>*>(y + p.P) = co;
+        save_run<T, VEC, ODD>(y, p.P - j, ao);
+        save_run<T, VEC, ODD>(y + p.P, p.P - j, co);
       }
     }
   }
 }
 
-// Adjacent pairs of heads of an odd size, or at odd addresses: element by element.
-template <typename T>
-__global__ __launch_bounds__(256) void rotary_pairs_kernel(RotaryParams p) {
-  __shared__ float2 table[kRotaryTable];
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.tokens, all = p.B * p.L;
-  const int n = static_cast<int>(all - t0 < p.tokens ? all - t0 : p.tokens);
-  for (int i = threadIdx.x; i < n * p.P; i += 256) table[i] = rotary_angle(p, t0 + i / p.P, i % p.P);
-  __syncthreads();
-  const int per = p.D - p.P;                            // a head's pairs, then its copied elements
-  for (int i = threadIdx.x; i < n * p.H * per; i += 256) {
-    const int t = i / (p.H * per), r = i - t * p.H * per, h = r / per, j = r - h * per;
-    const int64_t b = (t0 + t) / p.L, l = t0 + t - b * p.L;
-    const T* x = static_cast<const T*>(p.x) + b * p.xs[0] + l * p.xs[1] + h * p.xs[2];
-    T* y = static_cast<T*>(p.y) + b * p.ys[0] + l * p.ys[1] + h * p.ys[2];
-    if (j >= p.P) {
-      y[p.P + j] = x[p.P + j];
-      continue;
-    }
-    const float2 cs = table[t * p.P + j];
-    const float u = Elem<T>::load(x + 2 * j), v = Elem<T>::load(x + 2 * j + 1);
-    Elem<T>::store(y + 2 * j, u * cs.x - v * cs.y);
-    Elem<T>::store(y + 2 * j + 1, v * cs.x + u * cs.y);
-  }
-}
-
-// Largest access of 2^k elements, up to 16 bytes, that sizes, strides and addresses allow.
-static int rotary_vec(const RotaryParams& p, int es) {
-  int64_t all = p.D * es;
-  if (!p.adjacent) all |= p.P * es;
-  for (int i = 0; i < 3; ++i) all |= p.xs[i] * es | p.ys[i] * es;
-  all |= static_cast<int64_t>(reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.y));
-  int bytes = 16;
-  while (all % bytes) bytes /= 2;
-  return bytes / es;
-}
-
 template <typename T>
 static void rotary_launch(const RotaryParams& p, unsigned grid, hipStream_t s) {
-  const int vec = rotary_vec(p, sizeof(T));
+  constexpr int VEC = 16 / sizeof(T);
   if (p.adjacent) {
-    if constexpr (sizeof(T) == 2)
-      if (vec == 8) { rotary_kernel<T, 8, true><<<grid, 256, 0, s>>>(p); return; }
-    if (vec >= 4) rotary_kernel<T, 4, true><<<grid, 256, 0, s>>>(p);
-    else if (vec == 2) rotary_kernel<T, 2, true><<<grid, 256, 0, s>>>(p);
-    else rotary_pairs_kernel<T><<<grid, 256, 0, s>>>(p);
+    if (p.D % VEC) rotary_kernel<T, true, true><<<grid, 256, 0, s>>>(p);
+    else rotary_kernel<T, true, false><<<grid, 256, 0, s>>>(p);
   } else {
-    if constexpr (sizeof(T) == 2)
-      if (vec == 8) { rotary_kernel<T, 8, false><<<grid, 256, 0, s>>>(p); return; }
-    if (vec >= 4) rotary_kernel<T, 4, false><<<grid, 256, 0, s>>>(p);
-    else if (vec == 2) rotary_kernel<T, 2, false><<<grid, 256, 0, s>>>(p);
-    else rotary_kernel<T, 1, false><<<grid, 256, 0, s>>>(p);
+    if (p.P % VEC || p.D % VEC) rotary_kernel<T, false, true><<<grid, 256, 0, s>>>(p);
+    else rotary_kernel<T, false, false><<<grid, 256, 0, s>>>(p);
   }
 }
 

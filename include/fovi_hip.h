@@ -796,7 +796,7 @@ int fovi_layer_norm_bwd(const fovi_layer_norm_args* args, void* stream);
  * from 2 * n_pairs on are copied. inverse != 0 turns by the negative angle (the gradient). The
  * angle is reduced in fp64, so that it keeps fp32 accuracy at any position.
  * x and y: F32 or BF16, strides [batch, token, head], head elements adjacent. positions: fp32,
- * strides [batch, token], axes adjacent.
+ * strides [batch, token], axes adjacent. y does not overlap x.
  */
 enum fovi_pairing { FOVI_PAIR_HALF = 0, FOVI_PAIR_ADJACENT = 1 };
 #define FOVI_ROTARY_MAX_AXES 4

@@ -9,6 +9,7 @@ ratio of sum p|v| to |sum p v| over these random inputs: 6e-3. A score gradient 
 p (do.v - do.o), which may cancel (one state, equal values): its terms' roundings, 2^-21 of
 p (|do.v| + |do.o|) in fp32 and 2^-16 in bf16 (o is kept to 2^-18 there), come on top in dq and dk.
 """
+import ctypes as C
 import math
 
 import pytest
@@ -465,3 +466,82 @@ def test_c_arguments_are_refused():
     assert lib.fovi_attention_fwd(a, None) != 0 and b"null mask" in lib.fovi_last_error()
     b = _lib.AttentionBwdArgs()
     assert lib.fovi_attention_bwd(b, None) != 0 and b"null pointer" in lib.fovi_last_error()
+
+
+def _pattern(kind, lq, lk):
+    i, j = torch.arange(lq)[:, None], torch.arange(lk)[None]
+    at = i * lk // lq                                    # the state beside row i
+    if kind == "causal":
+        return j <= at
+    if kind == "band":
+        return (j - at).abs() <= 9
+    if kind == "blocks":                                 # three groups that see only themselves, 34 rows that see nothing
+        return (i * 3 // lq == j * 3 // lk) & ((i < lq // 3) | (i >= lq // 3 + 34))
+    return (j >= lk - 5) & (i % 2 == 0)                  # "end": the last states, for every other row
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kind", ["causal", "band", "blocks", "end"])
+@pytest.mark.parametrize("lq,lk,d", [(150, 333, 64), (301, 140, 32), (131, 260, 128), (2, 1500, 64), (9, 700, 40)])
+@pytest.mark.parametrize("as_bias", [False, True])
+def test_masks_that_leave_whole_tiles_empty(lq, lk, d, kind, dtype, as_bias):
+    b, hq, hk = 1, 4, 2
+    q, k, v, dout, g = _inputs(b, lq, lk, hq, hk, d, dtype, seed=11)
+    mask = _pattern(kind, lq, lk)
+    if as_bias:
+        mask = torch.randn(lq, lk, generator=g).masked_fill(~mask, -INF)
+    out, (dq, dk, dv) = _check(q, k, v, dout, mask=mask.cuda(), kv_lengths=torch.tensor([lk - 3], device="cuda"))
+    keep = _pattern(kind, lq, lk) & (torch.arange(lk) < lk - 3)
+    rows, states = ~keep.any(1), ~keep.any(0)
+    assert not out[:, rows].any() and not dq[:, rows].any() and not dk[:, states].any() and not dv[:, states].any()
+
+
+@pytest.mark.gpu
+def test_mask_per_head_and_image_of_many_tiles():
+    """Patterns that differ by head and image, shared key heads (rows of two heads in one tile)."""
+    b, lq, lk, hq, hk, d = 2, 70, 200, 4, 2, 64
+    q, k, v, dout, _ = _inputs(b, lq, lk, hq, hk, d, torch.bfloat16, seed=12)
+    kinds = ["causal", "band", "end", "blocks", "band", "causal", "causal", "end"]
+    mask = torch.stack([_pattern(kind, lq, lk) for kind in kinds]).view(b, hq, lq, lk).cuda()
+    _check(q, k, v, dout, mask=mask)
+    _check(q[:, :3], k, v, dout[:, :3], mask=mask[:, :, :3])
+
+
+def test_c_layouts_workspaces_and_masks_are_refused():
+    lib = _lib.load()
+    a = _lib.AttentionArgs()
+    a.q = a.k = a.v = a.out = 4096
+    a.dtype, a.scale = _lib.BF16, 0.125
+    a.batch, a.q_len, a.kv_len, a.heads, a.kv_heads, a.head_dim = 1, 4, 100000, 2, 2, 64
+    for f in (a.q_stride, a.k_stride, a.v_stride, a.out_stride):
+        f[:] = (1 << 30, 128, 64)
+
+    def refused(match, **kw):
+        keep = {name: getattr(a, name) for name in kw}
+        for name, value in kw.items():
+            setattr(a, name, value)
+        assert lib.fovi_attention_fwd(a, None) != 0 and match in lib.fovi_last_error(), lib.fovi_last_error()
+        for name, value in keep.items():
+            setattr(a, name, value)
+
+    refused(b"16-byte", q=4098)
+    refused(b"16-byte", head_dim=63)
+    a.k_stride[1] = 129
+    refused(b"16-byte")
+    a.k_stride[1] = 1 << 25                              # 64 MiB of bf16
+    refused(b"64 MiB")
+    a.k_stride[1] = 128
+    refused(b"workspace")
+    refused(b"too many", q_len=1 << 40)
+    refused(b"too many", batch=1 << 62)
+    refused(b"scale", scale=float("nan"))
+    need = lib.fovi_attention_fwd_workspace_bytes(1, 4, 100000, 2, 2, 64, _lib.BF16)
+    assert need > 0
+    refused(b"workspace", workspace=4096, workspace_bytes=need - 1)
+    refused(b"workspace", workspace=4104, workspace_bytes=need)
+    stride = (C.c_int64 * 4)(0, 0, 0, 1)
+    assert lib.fovi_attention_pack_mask(None, stride, 1, 1, 1, 8, 4096, None) != 0 and b"null pointer" in lib.fovi_last_error()
+    assert lib.fovi_attention_pack_mask(4096, stride, 1, -1, 1, 8, 4096, None) != 0 and b"bad sizes" in lib.fovi_last_error()
+    assert lib.fovi_attention_pack_mask(4096, stride, 1 << 30, 1 << 30, 1, 8, 4096, None) != 0
+    assert b"too large" in lib.fovi_last_error()

@@ -269,3 +269,38 @@ def test_struct_layout_matches_header(py, c, tmp_path):
     assert C.sizeof(py) == size
     for f, off in zip(fields, offs):
         assert getattr(py, f).offset == off, f
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,c", [(4100, 3), (4097, 7), (4100, 9), (4099, 61), (4100, 131), (4100, 255), (4097, 385),
+                                    (40, 255), (70, 513), (33, 1023), (20, 1537), (20, 2046), (5, 4095), (3, 8191)])
+def test_odd_widths(rows, c, dtype):
+    """Rows that end inside a 16-byte piece, in each shape of the kernels (16, 64 and 256 lanes a row)."""
+    test_values_and_gradients(rows, c, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,c", [(5, 3), (4099, 13), (9, 385), (2, 1030), (2, 20001)])
+def test_writes_its_rows_only(rows, c, dtype):
+    """y and dx are slices of wider rows, at odd offsets: what lies around them keeps its value."""
+    x, dy, _ = _data((rows, c), dtype)
+    lib = _lib.load()
+    outs = [torch.full((rows + 2, c + 11), 7.0, dtype=dtype, device="cuda") for _ in range(2)]
+    y, dx = (t[1:-1, 5:5 + c] for t in outs)
+    stats = torch.empty(2, rows, device="cuda")
+    a = _lib.LayerNormArgs()
+    a.x, a.dtype, a.rows0, a.rows1, a.channels, a.eps = x.data_ptr(), _lib.dtype_code(dtype), 1, rows, c, 1e-5
+    a.x_stride[:] = a.dy_stride[:] = (0, c)
+    a.y_stride[:] = a.dx_stride[:] = (0, c + 11)
+    a.y, a.dy, a.dx, a.mean, a.rstd = y.data_ptr(), dy.data_ptr(), dx.data_ptr(), stats[0].data_ptr(), stats[1].data_ptr()
+    _lib.check(lib.fovi_layer_norm_fwd(a, _lib.stream_of(x)), "forward")
+    _lib.check(lib.fovi_layer_norm_bwd(a, _lib.stream_of(x)), "backward")
+    ry, rdx, _, _ = _reference(x, None, None, 1e-5, dy)
+    tol = F32_TOL if dtype == torch.float32 else BF16_TOL
+    _close(y, ry, tol, "y")
+    _close(dx, rdx, tol, "dx")
+    for t, inner in zip(outs, (y, dx)):
+        inner.fill_(7.0)
+        assert (t == 7.0).all()

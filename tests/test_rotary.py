@@ -228,3 +228,38 @@ def test_c_arguments_are_refused():
     assert lib.fovi_rotary(a, None) != 0 and b"section_end" in lib.fovi_last_error()
     a.section_end[:] = [3, 5, 0, 0]
     assert lib.fovi_rotary(a, None) != 0 and b"bad sizes" in lib.fovi_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("pairing", ["half", "adjacent"])
+@pytest.mark.parametrize("d,sections", [(3, (1,)), (6, (3,)), (10, (5,)), (17, (8,)), (18, (9,)), (22, (4, 4)), (30, (15,)),
+                                        (34, (8, 9)), (41, (3, 9, 4)), (64, (13, 8, 8)), (66, (16, 16)), (90, (1, 30)),
+                                        (128, (3,)), (129, (60, 4))])
+def test_odd_runs(d, sections, pairing, dtype):
+    """Turned and copied runs that are not whole 16-byte pieces, shorter than one, and odd heads."""
+    test_values_and_gradient(3, 21, 3, d, sections, pairing, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("pairing", [0, 1])
+@pytest.mark.parametrize("d,pairs", [(7, 3), (24, 8), (30, 15), (37, 9), (64, 29)])
+def test_writes_its_heads_only(d, pairs, pairing, dtype):
+    """Heads inside wider rows, at odd offsets: what lies around them keeps its value."""
+    b, l, h = 2, 9, 3
+    x, pos, g = _inputs(b, l, h, d, 1, dtype, seed=9)
+    freqs = torch.rand(pairs, generator=g).cuda()
+    wide = torch.full((b, l, h, d + 11), 7.0, dtype=dtype, device="cuda")
+    y = wide[..., 5:5 + d]
+    a = _lib.RotaryArgs()
+    a.x, a.dtype, a.pairing = x.data_ptr(), _lib.dtype_code(dtype), pairing
+    a.batch, a.length, a.heads, a.head_dim = b, l, h, d
+    a.x_stride[:], a.y_stride[:] = x.stride()[:3], y.stride()[:3]
+    a.positions, a.freqs, a.y = pos.data_ptr(), freqs.data_ptr(), y.data_ptr()
+    a.pos_stride[:] = pos.stride()[:2]
+    a.n_axes, a.section_end[0] = 1, pairs
+    _lib.check(_lib.load().fovi_rotary(a, _lib.stream_of(x)), "fovi_rotary")
+    _close(y, _reference(x, pos, freqs, (pairs,), ("half", "adjacent")[pairing]), dtype)
+    y.fill_(7.0)
+    assert (wide == 7.0).all()
