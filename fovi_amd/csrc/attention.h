@@ -185,7 +185,7 @@ template <int LP> struct Turned<float, LP> {
 // Reads stay above, products below.
 __device__ __forceinline__ void reads_done() { __builtin_amdgcn_sched_barrier(0); }
 
-// s (and s2) += the 32 rows of `tile` (and `tile2`) times the columns b (b2), over the head elements, G pieces
+// s (and s2) += the 32 rows of `tile` (`tile2`) times the columns b (b2), over the head elements, G pieces
 // of each read ahead.
 template <typename T, int LP, int STEPS>
 __device__ __forceinline__ void row_product(const char* tile, const u32x4 (&b)[STEPS], f32x16& s) {
@@ -201,25 +201,6 @@ __device__ __forceinline__ void row_product(const char* tile, const u32x4 (&b)[S
 #pragma unroll
     for (int g = 0; g < G; ++g)
       if (t + g < STEPS) s = mma_step(T(), a[g], b[t + g], s);
-  }
-}
-template <typename T, int LP, int STEPS>
-__device__ __forceinline__ void row_product2(const char* tile, const u32x4 (&b)[STEPS], const u32x4 (&b2)[STEPS], f32x16& s, f32x16& s2) {
-  constexpr int G = STEPS < 4 ? STEPS : 4;
-  const int l = threadIdx.x & 63;
-#pragma unroll
-  for (int t = 0; t < STEPS; t += G) {
-    u32x4 a[G];
-#pragma unroll
-    for (int g = 0; g < G; ++g)
-      if (t + g < STEPS) a[g] = *reinterpret_cast<const u32x4*>(tile + tile_at<T, LP>(l & 31, 2 * (t + g) + (l >> 5)));
-    reads_done();
-#pragma unroll
-    for (int g = 0; g < G; ++g)
-      if (t + g < STEPS) {
-        s = mma_step(T(), a[g], b[t + g], s);
-        s2 = mma_step(T(), a[g], b2[t + g], s2);
-      }
   }
 }
 template <typename T, int LP, int G, bool BATCH, int STEPS>

@@ -1,7 +1,7 @@
 // Attention forward: out = softmax(scale q k^T + mask) v, one pass over the states with the running
 // maximum and sum of every row (see attention.h for the block layout).
 //
-//  * tile kernel: a workgroup owns 128 * QT query rows of one key head (the rows of the query heads
+//  * tile kernel: a workgroup owns 4 * 32 * QT query rows of one key head (the rows of the query heads
 //    that share it, in one sequence) and walks the states in tiles that all four waves read from
 //    LDS; the next tile is on its way in registers meanwhile.
 //  * few-row kernel: up to 32 * QT rows in all. Every wave of the workgroup has all the rows and its own
@@ -113,10 +113,10 @@ template <typename T> constexpr int few_waves(int DP, int KIND) {
   return sizeof(T) == 2 ? (KIND && DP >= 96 ? 1 : 2) : (DP >= 96 || (KIND && DP == 64) ? 1 : 2);
 }
 
-template <typename T, int DP, int QT, int KIND>
-__global__ __launch_bounds__(256, QT == 2 ? 2 : tile_waves<T>(DP, KIND)) void attn_fwd_tile_kernel(AttnParams p) {
+template <typename T, int DP, int KIND>
+__global__ __launch_bounds__(256, tile_waves<T>(DP, KIND)) void attn_fwd_tile_kernel(AttnParams p) {
   constexpr int LP = DP == 96 ? 128 : DP, KB = sizeof(T) == 2 ? 2 : 1, KT = 32 * KB, DT = DP / 32;
-  constexpr int STEPS = RowState<T, DP, QT>::STEPS;
+  constexpr int STEPS = RowState<T, DP, 1>::STEPS;
   __shared__ __attribute__((aligned(16))) char tiles[2][2][KT * LP * sizeof(T)];
   __shared__ int bad_tile[2];
   const int64_t all = p.tiles * p.B * p.Hk, id = xcd_tile(blockIdx.x, gridDim.x);
@@ -125,9 +125,9 @@ __global__ __launch_bounds__(256, QT == 2 ? 2 : tile_waves<T>(DP, KIND)) void at
   const int hk = static_cast<int>(bh - b * p.Hk), split = blockIdx.y;
   const int64_t len = attn_len(p, b), j0 = split * p.chunk, n = len < j0 + p.chunk ? len : j0 + p.chunk;
   if (split && n <= j0) return;                        // (split 0 writes the rows of images without states)
-  const int64_t r0 = (id - bh * p.tiles) * (128 * QT) + (threadIdx.x >> 6) * (32 * QT);
-  RowState<T, DP, QT> st;
-  init_rows<T, DP, QT>(p, st, b, hk, r0);
+  const int64_t r0 = (id - bh * p.tiles) * 128 + (threadIdx.x >> 6) * 32;
+  RowState<T, DP, 1> st;
+  init_rows<T, DP, 1>(p, st, b, hk, r0);
   const T* k = static_cast<const T*>(p.k) + b * p.ks[0] + hk * p.ks[2];
   const T* v = static_cast<const T*>(p.v) + b * p.vs[0] + hk * p.vs[2];
   Staged<T, LP, KT, 256> kr, vr;
@@ -171,26 +171,18 @@ __global__ __launch_bounds__(256, QT == 2 ? 2 : tile_waves<T>(DP, KIND)) void at
     const char* vt = tiles[at & 1][1];
     // (the last workgroup's waves may have no rows, and no row may read this tile)
     if (r0 < p.R && (KIND != 1 || __any((word[0] | (KB > 1 ? word[1] : 0)) != 0))) {
-      f32x16 s[QT][KB] = {};
-      Block<T> e[QT][KB];
+      f32x16 s[KB] = {};
+      Block<T> e[KB];
       Turned<T, LP> va[2][DT];
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        if constexpr (QT == 1) row_product<T, LP>(kt + kb * 32 * LP * sizeof(T), st.q[0], s[0][kb]);
-        else row_product2<T, LP>(kt + kb * 32 * LP * sizeof(T), st.q[0], st.q[QT - 1], s[0][kb], s[QT - 1][kb]);
-      }
+      for (int kb = 0; kb < KB; ++kb) row_product<T, LP>(kt + kb * 32 * LP * sizeof(T), st.q[0], s[kb]);
 #pragma unroll
-      for (int q = 0; q < QT; ++q) {
-        if (q == QT - 1) {
-#pragma unroll
-          for (int d = 0; d < DT; ++d) va[0][d].read(vt, 0, d);
-          reads_done();
-        }
-        softmax_blocks<T, DP, QT, KIND, KB>(p, st, q, s[q], e[q], word, j, n);
-      }
+      for (int d = 0; d < DT; ++d) va[0][d].read(vt, 0, d);
+      reads_done();
+      softmax_blocks<T, DP, 1, KIND, KB>(p, st, 0, s, e, word, j, n);
       if (KIND && bad_tile[at & 1] == at) {
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) slow_second<T, LP, DT>(vt, kb * 32, s[0][kb], st.o[0]);
+        for (int kb = 0; kb < KB; ++kb) slow_second<T, LP, DT>(vt, kb * 32, s[kb], st.o[0]);
       } else {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
@@ -200,18 +192,16 @@ __global__ __launch_bounds__(256, QT == 2 ? 2 : tile_waves<T>(DP, KIND)) void at
             reads_done();
           }
 #pragma unroll
-          for (int q = 0; q < QT; ++q)
-#pragma unroll
-            for (int d = 0; d < DT; ++d) st.o[q][d] = va[kb & 1][d].mma(e[q][kb], st.o[q][d]);
+          for (int d = 0; d < DT; ++d) st.o[0][d] = va[kb & 1][d].mma(e[kb], st.o[0][d]);
         }
       }
     }
     if (next < n) put((at + 1) & 1, at + 1);
   }
   const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int q = 0; q < QT; ++q) {
-    const int64_t r = r0 + 32 * q + (lane & 31);
+  {
+    constexpr int q = 0;
+    const int64_t r = r0 + (lane & 31);
     const float sum = st.l[q] + other_half(st.l[q]), m = KIND ? st.m[q] : st.m[q] * p.c;
     if (r >= p.R) return;
     if (p.splits > 1) {
@@ -223,7 +213,7 @@ __global__ __launch_bounds__(256, QT == 2 ? 2 : tile_waves<T>(DP, KIND)) void at
         for (int e = 0; e < 16; e += 4)
           store_run(p.part + row * p.D, d * 32 + 2 * e + 4 * (lane >> 5), p.D, st.o[q][d][e], st.o[q][d][e + 1], st.o[q][d][e + 2],
                     st.o[q][d][e + 3]);
-      continue;
+      return;
     }
     const int64_t g = r / p.Lq, i = r - g * p.Lq, off = b * p.os[0] + i * p.os[1] + (hk * p.G + g) * p.os[2];
     T* out = static_cast<T*>(p.o) + off;
@@ -462,13 +452,8 @@ static FwdPlan fwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk
     f.qt = R <= 32 ? 1 : 2;
     f.tiles = 1;
   } else {
-    // Two row blocks a wave read and stage the states half as often for the same products, but start later,
-    // are two waves a SIMD, not three, and rows fill tiles of 256 worse (heads of 64: 1024 x 4096 x 192 heads
-    // 337 us with one block, 302 with two, 4096 x 4096 x 32: 200 and 194; but 256 x 512 x 768: 47 and 50,
-    // 384 x 768 x 384: 52 and 63; heads of 32 gain nothing).
-    const int64_t wide = (R + 255) / 256;
-    f.qt = two && D > 32 && Lk >= 2048 && B * Hk * wide >= 512 && 8 * R >= 7 * 256 * wide ? 2 : 1;
-    f.tiles = (R + 128 * f.qt - 1) / (128 * f.qt);
+    f.qt = 1;
+    f.tiles = (R + 127) / 128;
   }
   // The states are split until the card is full (few rows of many key heads: twice, since lengths
   // differ), in parts that are still worth a workgroup's start and the join: 512 states for few rows
@@ -506,10 +491,7 @@ static void fwd_launch(const AttnParams& p, const FwdPlan& f, hipStream_t s) {
     else if constexpr (DP <= 64 && sizeof(T) == 2 && KIND == 0) attn_fwd_few_kernel<T, DP, 2, KIND><<<grid, 256, 0, s>>>(p);
   } else {
     const dim3 grid(static_cast<unsigned>((all + 7) / 8 * 8), static_cast<unsigned>(f.splits));
-    if constexpr (sizeof(T) == 2 && DP == 64 && KIND == 0) {
-      if (f.qt == 2) { attn_fwd_tile_kernel<T, DP, 2, KIND><<<grid, 256, 0, s>>>(p); return; }
-    }
-    attn_fwd_tile_kernel<T, DP, 1, KIND><<<grid, 256, 0, s>>>(p);
+    attn_fwd_tile_kernel<T, DP, KIND><<<grid, 256, 0, s>>>(p);
   }
 }
 

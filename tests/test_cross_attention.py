@@ -545,23 +545,3 @@ def test_c_layouts_workspaces_and_masks_are_refused():
     assert lib.fovi_attention_pack_mask(4096, stride, 1, -1, 1, 8, 4096, None) != 0 and b"bad sizes" in lib.fovi_last_error()
     assert lib.fovi_attention_pack_mask(4096, stride, 1 << 30, 1 << 30, 1, 8, 4096, None) != 0
     assert b"too large" in lib.fovi_last_error()
-
-
-@pytest.mark.gpu
-def test_many_long_images_and_each_alone():
-    """Enough rows and states for two row blocks a wave: against calls of one image each, and one image of the
-    batch against the reference. The last rows of an image do not fill a block."""
-    from fovi_amd.arch.attention import cross_attention
-    b, lq, lk, h, d = 260, 227, 2051, 2, 64
-    g = torch.Generator().manual_seed(13)
-    q = (1.3 * torch.randn(b, lq, h, d, generator=g)).bfloat16().cuda()
-    k, v = (torch.randn(b, lk, h, d, generator=g).bfloat16().cuda() for _ in range(2))
-    lengths = torch.randint(0, lk + 1, (b,), generator=g).int().cuda()
-    lengths[3], lengths[5] = lk, 0
-    out = cross_attention(q, k, v, kv_lengths=lengths)
-    for i in range(0, b, 37):
-        one = cross_attention(q[i:i + 1], k[i:i + 1], v[i:i + 1], kv_lengths=lengths[i:i + 1])
-        _close(out[i:i + 1], one.double().cpu(), TOL[torch.bfloat16], f"image {i}")
-    assert not out[5].any()
-    want = _reference(q[3:4], k[3:4], v[3:4])[0]
-    _close(out[3:4], want, TOL[torch.bfloat16], "the longest image")
