@@ -43,7 +43,9 @@ template <typename T> constexpr int dkv_waves(int DP, int KIND) {
   return sizeof(T) == 2 ? (DP >= 96 ? 1 : 2) : DP >= 64 ? 1 : 2;
 }
 
-template <typename T, int DP, int QT, int KIND>
+// As the forward's tile kernel, with three products a pair: 1024 rows x 4096 states x 192 bf16 heads of 64 in
+// 375 us (825 TFLOP/s), matrix unit busy 48 % of the cycles, vector unit 61 %.
+template <typename T, int DP, int KIND>
 __global__ __launch_bounds__(256, dq_waves<T>(DP, KIND)) void attn_dq_kernel(AttnParams p) {
   constexpr int LP = DP == 96 ? 128 : DP, KB = sizeof(T) == 2 ? 2 : 1, KT = 32 * KB, DT = DP / 32, STEPS = DP / (2 * Chunk<T>::N);
   __shared__ __attribute__((aligned(16))) char tiles[2][2][KT * LP * sizeof(T)];
@@ -54,48 +56,43 @@ __global__ __launch_bounds__(256, dq_waves<T>(DP, KIND)) void attn_dq_kernel(Att
   const int hk = static_cast<int>(bh - b * p.Hk), split = blockIdx.y, l = threadIdx.x & 63;
   const int64_t len = attn_len(p, b), j0 = split * p.chunk, n = len < j0 + p.chunk ? len : j0 + p.chunk;
   if (split && n <= j0) return;
-  const int64_t r0 = (id - bh * p.tiles) * (128 * QT) + (threadIdx.x >> 6) * (32 * QT);
-  u32x4 q[QT][STEPS], g[QT][STEPS];
-  f32x16 dq[QT][DT] = {};
-  RowStat st[QT];
+  const int64_t r0 = (id - bh * p.tiles) * 128 + (threadIdx.x >> 6) * 32;
+  u32x4 q[STEPS], g[STEPS];
+  f32x16 dq[DT] = {};
   constexpr bool START = sizeof(T) == 2 && DP == 32;   // -delta as a block of its own, where registers allow
   // Heads of 96 and 128: operands are read as they are needed. Two waves a SIMD that way (229 us for 8 x 1024 x
   // 2048 and 16 heads of 128) beat one with its reads in batches (300).
   constexpr bool LATE = DP > 64;
-  f32x16 start[START ? QT : 1];
-  const uint32_t* mrow[QT];
-  uint32_t word[QT][2] = {}, coming[QT][2] = {};       // KIND 1: the blocks' bits, and the next tile's
+  f32x16 start;
+  uint32_t word[2] = {}, coming[2] = {};       // KIND 1: the blocks' bits, and the next tile's
+  const int64_t r = r0 + (l & 31);
+  const int64_t gr = r < p.R ? r / p.Lq : 0, i = r < p.R ? r - gr * p.Lq : 0, h = hk * p.G + gr;
+  const T* qr = static_cast<const T*>(p.q) + b * p.qs[0] + i * p.qs[1] + h * p.qs[2];
+  const T* gg = static_cast<const T*>(p.dout) + b * p.dos[0] + i * p.dos[1] + h * p.dos[2];
+  // delta = do.o, o before its rounding; half of the elements a lane
+  const int64_t off = b * p.os[0] + i * p.os[1] + h * p.os[2];
+  float delta = 0;
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const int64_t r = r0 + 32 * t + (l & 31);
-    const int64_t gr = r < p.R ? r / p.Lq : 0, i = r < p.R ? r - gr * p.Lq : 0, h = hk * p.G + gr;
-    const T* qr = static_cast<const T*>(p.q) + b * p.qs[0] + i * p.qs[1] + h * p.qs[2];
-    const T* gg = static_cast<const T*>(p.dout) + b * p.dos[0] + i * p.dos[1] + h * p.dos[2];
-    // delta = do.o, o before its rounding; half of the elements a lane
-    const int64_t off = b * p.os[0] + i * p.os[1] + h * p.os[2];
-    float delta = 0;
+  for (int s = 0; s < STEPS; ++s) {
+    q[s] = load_chunk<T>(qr, 2 * s + (l >> 5), r < p.R ? p.D : 0);
+    g[s] = load_chunk<T>(gg, 2 * s + (l >> 5), r < p.R ? p.D : 0);
+    const u32x4 o = load_chunk<T>(static_cast<const T*>(p.o) + off, 2 * s + (l >> 5), p.D);
+    const u32x4 rest = p.rest ? load_chunk<T>(static_cast<const T*>(p.rest) + off, 2 * s + (l >> 5), p.D) : u32x4{0, 0, 0, 0};
+    T ge[Chunk<T>::N], oe[Chunk<T>::N], re[Chunk<T>::N];
+    __builtin_memcpy(ge, &g[s], 16);
+    __builtin_memcpy(oe, &o, 16);
+    __builtin_memcpy(re, &rest, 16);
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      q[t][s] = load_chunk<T>(qr, 2 * s + (l >> 5), r < p.R ? p.D : 0);
-      g[t][s] = load_chunk<T>(gg, 2 * s + (l >> 5), r < p.R ? p.D : 0);
-      const u32x4 o = load_chunk<T>(static_cast<const T*>(p.o) + off, 2 * s + (l >> 5), p.D);
-      const u32x4 rest = p.rest ? load_chunk<T>(static_cast<const T*>(p.rest) + off, 2 * s + (l >> 5), p.D) : u32x4{0, 0, 0, 0};
-      T ge[Chunk<T>::N], oe[Chunk<T>::N], re[Chunk<T>::N];
-      __builtin_memcpy(ge, &g[t][s], 16);
-      __builtin_memcpy(oe, &o, 16);
-      __builtin_memcpy(re, &rest, 16);
-#pragma unroll
-      for (int e = 0; e < Chunk<T>::N; ++e) delta = fmaf(Elem<T>::load(ge + e), Elem<T>::load(oe + e) + Elem<T>::load(re + e), delta);
-    }
-    delta += other_half(delta);
-    const int64_t at = (b * p.H + h) * p.Lq + i;
-    if (split == 0 && l < 32 && r < p.R) p.delta[at] = delta;
-    st[t] = row_stat<KIND>(p.stats[at], p.stats[p.B * p.H * p.Lq + at], delta);
-#pragma unroll
-    for (int e = 0; e < 16; ++e)
-      if (START) start[t][e] = -st[t].delta;
-    mrow[t] = KIND ? mask_row(p, b, h, i) : nullptr;
+    for (int e = 0; e < Chunk<T>::N; ++e) delta = fmaf(Elem<T>::load(ge + e), Elem<T>::load(oe + e) + Elem<T>::load(re + e), delta);
   }
+  delta += other_half(delta);
+  const int64_t at_row = (b * p.H + h) * p.Lq + i;
+  if (split == 0 && l < 32 && r < p.R) p.delta[at_row] = delta;
+  const RowStat st = row_stat<KIND>(p.stats[at_row], p.stats[p.B * p.H * p.Lq + at_row], delta);
+#pragma unroll
+  for (int e = 0; e < 16; ++e)
+    if (START) start[e] = -st.delta;
+  const uint32_t* mrow = KIND ? mask_row(p, b, h, i) : nullptr;
   const T* k = static_cast<const T*>(p.k) + b * p.ks[0] + hk * p.ks[2];
   const T* v = static_cast<const T*>(p.v) + b * p.vs[0] + hk * p.vs[2];
   Staged<T, LP, KT, 256> kr, vr;
@@ -108,10 +105,7 @@ __global__ __launch_bounds__(256, dq_waves<T>(DP, KIND)) void attn_dq_kernel(Att
   int at = 0;
   auto words = [&](int64_t j) {
 #pragma unroll
-    for (int x = 0; x < QT; ++x)
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-        coming[x][kb] = j + 32 * kb < n && r0 + 32 * x + (l & 31) < p.R ? mrow[x][j / 32 + kb] : 0;
+    for (int kb = 0; kb < KB; ++kb) coming[kb] = j + 32 * kb < n && r < p.R ? mrow[j / 32 + kb] : 0;
   };
   auto put = [&](int buf, int tile) {
     kr.store(tiles[buf][0], p.D);
@@ -128,11 +122,8 @@ __global__ __launch_bounds__(256, dq_waves<T>(DP, KIND)) void attn_dq_kernel(Att
   for (int64_t j = j0; j < n; j += KT, ++at) {
     const int64_t next = j + KT;
     if (KIND == 1) {
-#pragma unroll
-      for (int x = 0; x < QT; ++x) {
-        word[x][0] = coming[x][0];
-        word[x][1] = coming[x][1];
-      }
+      word[0] = coming[0];
+      word[1] = coming[1];
       if (next < n) words(next);
     }
     if (next < n) {
@@ -145,72 +136,62 @@ __global__ __launch_bounds__(256, dq_waves<T>(DP, KIND)) void attn_dq_kernel(Att
     const int left = static_cast<int>(n - j < KT ? n - j : KT);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
-      if (KIND == 1 && QT == 1 && !__any(word[0][kb] != 0)) continue;      // no row reads these states
-      f32x16 s[QT] = {}, dp[QT];
-#pragma unroll
-      for (int x = 0; x < QT; ++x) {
-        if (START) dp[x] = start[x];
-        else dp[x] = f32x16{};
-      }
-#pragma unroll
-      for (int x = 0; x < QT; ++x)
-        row_products<T, LP, (LATE ? 1 : DP == 64 ? 2 : STEPS < 4 ? STEPS : 4), !LATE>(kt + kb * 32 * LP * sizeof(T), vt + kb * 32 * LP * sizeof(T), q[x], g[x], s[x], dp[x]);
+      if (KIND == 1 && !__any(word[kb] != 0)) continue;      // no row reads these states
+      f32x16 s = {}, dp = {};
+      if (START) dp = start;
+      row_products<T, LP, (LATE ? 1 : DP == 64 ? 2 : STEPS < 4 ? STEPS : 4), !LATE>(
+          kt + kb * 32 * LP * sizeof(T), vt + kb * 32 * LP * sizeof(T), q, g, s, dp);
       Turned<T, LP> ka[DT];
 #pragma unroll
       for (int d = 0; d < DT; ++d)
         if (!LATE) ka[d].read(kt, kb * 32, d);
       if (!LATE) reads_done();
+      if (KIND == 1) keep_block(p, word[kb], s);
+      if (KIND == 2) bias_block(p, reinterpret_cast<const float*>(mrow), j + kb * 32 + 4 * (l >> 5), n, s);
+      if (KIND < 2 && left < kb * 32 + 32) {
 #pragma unroll
-      for (int x = 0; x < QT; ++x) {
-        if (KIND == 1) keep_block(p, word[x][kb], s[x]);
-        if (KIND == 2) bias_block(p, reinterpret_cast<const float*>(mrow[x]), j + kb * 32 + 4 * (l >> 5), n, s[x]);
-        if (KIND < 2 && left < kb * 32 + 32) {
+        for (int i = 0; i < 16; ++i)
+          if (kb * 32 + 8 * (i / 4) + 4 * (l >> 5) + i % 4 >= left) s[i] = kNegInf;
+      }
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (kb * 32 + 8 * (i / 4) + 4 * (l >> 5) + i % 4 >= left) s[x][i] = kNegInf;
-        }
+      for (int i = 0; i < 16; ++i) {
+        float e, ds;
+        pair_grad<KIND>(s[i], p.c, st.shift, st.factor, START ? dp[i] : dp[i] - st.delta, e, ds);
+        s[i] = ds;
+      }
+      if (KIND && bad_tile[at & 1] == at) {
+        slow_second<T, LP, DT>(kt, kb * 32, s, dq);
+      } else {
+        const Block<T> ds(s);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float e, ds;
-          pair_grad<KIND>(s[x][i], p.c, st[x].shift, st[x].factor, START ? dp[x][i] : dp[x][i] - st[x].delta, e, ds);
-          s[x][i] = ds;
-        }
-        if (KIND && bad_tile[at & 1] == at) {
-          slow_second<T, LP, DT>(kt, kb * 32, s[x], dq[x]);
-        } else {
-          const Block<T> ds(s[x]);
-#pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            if (LATE) ka[d].read(kt, kb * 32, d);
-            dq[x][d] = ka[d].mma(ds, dq[x][d]);
-          }
+        for (int d = 0; d < DT; ++d) {
+          if (LATE) ka[d].read(kt, kb * 32, d);
+          dq[d] = ka[d].mma(ds, dq[d]);
         }
       }
     }
     if (next < n) put((at + 1) & 1, at + 1);
   }
+  if (r >= p.R) return;
+  T* out = static_cast<T*>(p.dq) + b * p.dqs[0] + i * p.dqs[1] + (hk * p.G + gr) * p.dqs[2];
+  float* part = p.part + ((split * p.B * p.Hk + bh) * p.R + r) * p.D;
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const int64_t r = r0 + 32 * t + (l & 31);
-    if (r >= p.R) continue;
-    const int64_t gr = r / p.Lq, i = r - gr * p.Lq;
-    T* out = static_cast<T*>(p.dq) + b * p.dqs[0] + i * p.dqs[1] + (hk * p.G + gr) * p.dqs[2];
-    float* part = p.part + ((split * p.B * p.Hk + bh) * p.R + r) * p.D;
+  for (int d = 0; d < DT; ++d)
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const int at_d = d * 32 + 2 * e + 4 * (l >> 5);
-        const float a = dq[t][d][e] * p.scale, bb = dq[t][d][e + 1] * p.scale, c = dq[t][d][e + 2] * p.scale, f = dq[t][d][e + 3] * p.scale;
-        if (p.splits > 1) store_run(part, at_d, p.D, a, bb, c, f);
-        else store_run(out, at_d, p.D, a, bb, c, f);
-      }
-  }
+    for (int e = 0; e < 16; e += 4) {
+      const int at_d = d * 32 + 2 * e + 4 * (l >> 5);
+      const float a = dq[d][e] * p.scale, bb = dq[d][e + 1] * p.scale, c = dq[d][e + 2] * p.scale, f = dq[d][e + 3] * p.scale;
+      if (p.splits > 1) store_run(part, at_d, p.D, a, bb, c, f);
+      else store_run(out, at_d, p.D, a, bb, c, f);
+    }
 }
 
 // Blocks of 32 rows in a tile of the dk, dv kernel.
 template <typename T> constexpr int dkv_blocks(int DP) { return sizeof(T) == 2 && DP <= 64 ? 2 : 1; }
 
+// Four products a pair: the same sizes in 555 us (742 TFLOP/s), matrix unit busy 40 % of the cycles and vector
+// unit 40 %. Keys, values and both gradients of 32 states hold 160 registers a lane for heads of 64, so that only
+// two waves share a SIMD and not every latency is hidden (lone waves, for wider heads, hide less).
 template <typename T, int DP, int KIND>
 __global__ __launch_bounds__(256, dkv_waves<T>(DP, KIND)) void attn_dkv_kernel(AttnParams p) {
   constexpr int LP = DP == 96 ? 128 : DP, DT = DP / 32, STEPS = DP / (2 * Chunk<T>::N), RB = dkv_blocks<T>(DP), RT = 32 * RB;
@@ -429,17 +410,16 @@ __global__ __launch_bounds__(256) void attn_bwd_join_kernel(AttnParams p) {
 }
 
 struct BwdPlan {
-  int qt, q_splits, k_splits;
+  int q_splits, k_splits;
   int64_t q_tiles, q_chunk, k_tiles, k_chunk;
 };
 
 static int64_t dkv_tile(int64_t D, int dtype) { return 32 * (dtype == FOVI_BF16 && D <= 64 ? 2 : 1); }
 
-static BwdPlan bwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t D, int dtype, bool mask) {
+static BwdPlan bwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t D, int dtype) {
   BwdPlan f;
   const int64_t R = H / Hk * Lq;
-  f.qt = dtype == FOVI_BF16 && D <= 32 && !mask && R > 128 ? 2 : 1;
-  f.q_tiles = (R + 128 * f.qt - 1) / (128 * f.qt);
+  f.q_tiles = (R + 127) / 128;
   f.k_tiles = (Lk + 127) / 128;
   // splits for two workgroups a compute unit, each with at least 128 states or 64 rows to walk (fp32 under a
   // mask, 8 x 77 x 4 rows over 515 states: dq 38 -> 17 us, dk and dv 62 -> 22, the joins 5 each)
@@ -463,21 +443,16 @@ static BwdPlan bwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk
 static int64_t align16(int64_t n) { return (n + 15) / 16 * 16; }
 
 int64_t attn_bwd_workspace(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t D, int dtype) {
-  int64_t most = 0;
-  for (const bool mask : {false, true}) {
-    const BwdPlan f = bwd_plan(B, Lq, Lk, H, Hk, D, dtype, mask);
-    // delta, then the partial sums of dq, then those of dk and dv
-    const int64_t need = (f.q_splits > 1 ? f.q_splits * B * H * Lq * D * 4 : 0) + (f.k_splits > 1 ? f.k_splits * B * Hk * Lk * 2 * D * 4 : 0);
-    if (need > most) most = need;
-  }
-  return align16(B * H * Lq * 4) + most;
+  const BwdPlan f = bwd_plan(B, Lq, Lk, H, Hk, D, dtype);
+  // delta, then the partial sums of dq, then those of dk and dv
+  return align16(B * H * Lq * 4) + (f.q_splits > 1 ? f.q_splits * B * H * Lq * D * 4 : 0) +
+         (f.k_splits > 1 ? f.k_splits * B * Hk * Lk * 2 * D * 4 : 0);
 }
 
 template <typename T, int DP, int KIND>
-static void bwd_dq(const AttnParams& p, int qt, hipStream_t s) {
+static void bwd_dq(const AttnParams& p, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>((p.B * p.Hk * p.tiles + 7) / 8 * 8), static_cast<unsigned>(p.splits));
-  if (qt == 1) attn_dq_kernel<T, DP, 1, KIND><<<grid, 256, 0, s>>>(p);
-  else if constexpr (DP == 32 && sizeof(T) == 2 && KIND == 0) attn_dq_kernel<T, DP, 2, KIND><<<grid, 256, 0, s>>>(p);
+  attn_dq_kernel<T, DP, KIND><<<grid, 256, 0, s>>>(p);
 }
 
 template <typename T, int DP, int KIND>
@@ -487,12 +462,12 @@ static void bwd_dkv(const AttnParams& p, hipStream_t s) {
 }
 
 template <typename T, int KIND, bool DQ>
-static void bwd_heads(const AttnParams& p, int qt, hipStream_t s) {
+static void bwd_heads(const AttnParams& p, hipStream_t s) {
   if constexpr (DQ) {
-    if (p.D <= 32) bwd_dq<T, 32, KIND>(p, qt, s);
-    else if (p.D <= 64) bwd_dq<T, 64, KIND>(p, qt, s);
-    else if (p.D <= 96) bwd_dq<T, 96, KIND>(p, qt, s);
-    else bwd_dq<T, 128, KIND>(p, qt, s);
+    if (p.D <= 32) bwd_dq<T, 32, KIND>(p, s);
+    else if (p.D <= 64) bwd_dq<T, 64, KIND>(p, s);
+    else if (p.D <= 96) bwd_dq<T, 96, KIND>(p, s);
+    else bwd_dq<T, 128, KIND>(p, s);
   } else {
     if (p.D <= 32) bwd_dkv<T, 32, KIND>(p, s);
     else if (p.D <= 64) bwd_dkv<T, 64, KIND>(p, s);
@@ -503,7 +478,7 @@ static void bwd_heads(const AttnParams& p, int qt, hipStream_t s) {
 
 template <typename T>
 static int bwd_type(AttnParams& p, hipStream_t s) {
-  const BwdPlan f = bwd_plan(p.B, p.Lq, p.Lk, p.H, p.Hk, p.D, sizeof(T) == 2 ? FOVI_BF16 : FOVI_F32, p.kind != 0);
+  const BwdPlan f = bwd_plan(p.B, p.Lq, p.Lk, p.H, p.Hk, p.D, sizeof(T) == 2 ? FOVI_BF16 : FOVI_F32);
   p.delta = p.part;
   p.part = reinterpret_cast<float*>(reinterpret_cast<char*>(p.part) + align16(p.B * p.H * p.Lq * 4));
   const int64_t rows = p.B * p.H * p.Lq;
@@ -511,16 +486,16 @@ static int bwd_type(AttnParams& p, hipStream_t s) {
   p.k_splits = f.k_splits;
   if (rows) {
     p.tiles = f.q_tiles; p.splits = f.q_splits; p.chunk = f.q_chunk;
-    if (p.kind == FOVI_MASK_NONE) bwd_heads<T, 0, true>(p, f.qt, s);
-    else if (p.kind == FOVI_MASK_KEEP) bwd_heads<T, 1, true>(p, f.qt, s);
-    else bwd_heads<T, 2, true>(p, f.qt, s);
+    if (p.kind == FOVI_MASK_NONE) bwd_heads<T, 0, true>(p, s);
+    else if (p.kind == FOVI_MASK_KEEP) bwd_heads<T, 1, true>(p, s);
+    else bwd_heads<T, 2, true>(p, s);
     if (check_launch("fovi_attention_bwd")) return 1;
   }
   if (p.Lk == 0 || p.B == 0) return 0;
   p.tiles = f.k_tiles; p.splits = f.k_splits; p.chunk = f.k_chunk;
-  if (p.kind == FOVI_MASK_NONE) bwd_heads<T, 0, false>(p, 1, s);
-  else if (p.kind == FOVI_MASK_KEEP) bwd_heads<T, 1, false>(p, 1, s);
-  else bwd_heads<T, 2, false>(p, 1, s);
+  if (p.kind == FOVI_MASK_NONE) bwd_heads<T, 0, false>(p, s);
+  else if (p.kind == FOVI_MASK_KEEP) bwd_heads<T, 1, false>(p, s);
+  else bwd_heads<T, 2, false>(p, s);
   if (check_launch("fovi_attention_bwd")) return 1;
   if (f.q_splits > 1 || f.k_splits > 1) {
     p.splits = f.q_splits;

@@ -1,10 +1,10 @@
 // Attention forward: out = softmax(scale q k^T + mask) v, one pass over the states with the running
 // maximum and sum of every row (see attention.h for the block layout).
 //
-//  * tile kernel: a workgroup owns 4 * 32 * QT query rows of one key head (the rows of the query heads
-//    that share it, in one sequence) and walks the states in tiles that all four waves read from
-//    LDS; the next tile is on its way in registers meanwhile.
-//  * few-row kernel: up to 32 * QT rows in all. Every wave of the workgroup has all the rows and its own
+//  * tile kernel: a workgroup owns 128 query rows of one key head (the rows of the query heads that share
+//    it, in one sequence) and walks the states in tiles that all four waves read from LDS; the next tile is
+//    on its way in registers meanwhile.
+//  * few-row kernel: up to 32 rows in all. Every wave of the workgroup has all the rows and its own
 //    states: keys straight from memory as matrix operands, values through an LDS tile of the
 //    wave's own (only the transposing read needs it), no barrier until the four waves' results join.
 //
@@ -14,42 +14,37 @@
 
 namespace fovi {
 
-template <typename T, int DP, int QT>
+template <typename T, int DP>
 struct RowState {
   static constexpr int DT = DP / 32, STEPS = DP / (2 * Chunk<T>::N);
-  u32x4 q[QT][STEPS];
-  f32x16 o[QT][DT];
-  float m[QT], l[QT];         // the row's maximum so far, or a little less; the lane's share of the sum
-  const uint32_t* mrow[QT];
-  uint32_t word[QT][2];       // KIND 1: the next blocks' bits
+  u32x4 q[STEPS];
+  f32x16 o[DT];
+  float m, l;                 // the row's maximum so far, or a little less; the lane's share of the sum
+  const uint32_t* mrow;
+  uint32_t word[2];           // KIND 1: the next blocks' bits
 };
 
-// The rows r0 + 32 t + lane of key head (b, hk): queries as B operands, statistics cleared.
-template <typename T, int DP, int QT>
-__device__ __forceinline__ void init_rows(const AttnParams& p, RowState<T, DP, QT>& st, int64_t b, int hk, int64_t r0) {
+// The rows r0 + lane of key head (b, hk): queries as B operands, statistics cleared.
+template <typename T, int DP>
+__device__ __forceinline__ void init_rows(const AttnParams& p, RowState<T, DP>& st, int64_t b, int hk, int64_t r0) {
   const int l = threadIdx.x & 63;
+  const int64_t r = r0 + (l & 31), g = r < p.R ? r / p.Lq : 0, i = r < p.R ? r - g * p.Lq : 0, h = hk * p.G + g;
+  const T* q = static_cast<const T*>(p.q) + b * p.qs[0] + i * p.qs[1] + h * p.qs[2];
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const int64_t r = r0 + 32 * t + (l & 31);
-    const int64_t g = r < p.R ? r / p.Lq : 0, i = r < p.R ? r - g * p.Lq : 0, h = hk * p.G + g;
-    const T* q = static_cast<const T*>(p.q) + b * p.qs[0] + i * p.qs[1] + h * p.qs[2];
+  for (int s = 0; s < RowState<T, DP>::STEPS; ++s) st.q[s] = r < p.R ? load_chunk<T>(q, 2 * s + (l >> 5), p.D) : u32x4{0, 0, 0, 0};
+  st.m = kNegInf;
+  st.l = 0;
+  st.mrow = p.kind ? mask_row(p, b, h, i) : nullptr;
 #pragma unroll
-    for (int s = 0; s < RowState<T, DP, QT>::STEPS; ++s)
-      st.q[t][s] = r < p.R ? load_chunk<T>(q, 2 * s + (l >> 5), p.D) : u32x4{0, 0, 0, 0};
-    st.m[t] = kNegInf;
-    st.l[t] = 0;
-    st.mrow[t] = p.kind ? mask_row(p, b, h, i) : nullptr;
+  for (int d = 0; d < RowState<T, DP>::DT; ++d)
 #pragma unroll
-    for (int d = 0; d < RowState<T, DP, QT>::DT; ++d)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) st.o[t][d][e] = 0;
-  }
+    for (int e = 0; e < 16; ++e) st.o[d][e] = 0;
 }
 
 // Scores of KB blocks of 32 states (j .. n valid) into probabilities; the running statistics of
-// rows t and the outputs' scale follow. Under a mask, pairs that are left out become kLeftOut.
-template <typename T, int DP, int QT, int KIND, int KB>
-__device__ __forceinline__ void softmax_blocks(const AttnParams& p, RowState<T, DP, QT>& st, int t, f32x16 (&s)[KB], Block<T> (&e)[KB],
+// the rows and the outputs' scale follow. Under a mask, pairs that are left out become kLeftOut.
+template <typename T, int DP, int KIND, int KB>
+__device__ __forceinline__ void softmax_blocks(const AttnParams& p, RowState<T, DP>& st, f32x16 (&s)[KB], Block<T> (&e)[KB],
                                                const uint32_t (&word)[2], int64_t j, int64_t n) {
   const int h = (threadIdx.x & 63) >> 5;
   const float c = KIND ? 1.0f : p.c;
@@ -57,14 +52,14 @@ __device__ __forceinline__ void softmax_blocks(const AttnParams& p, RowState<T, 
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb) {
     if (KIND == 1) keep_block(p, word[kb], s[kb]);
-    if (KIND == 2) bias_block(p, reinterpret_cast<const float*>(st.mrow[t]), j + kb * 32 + 4 * h, n, s[kb]);
+    if (KIND == 2) bias_block(p, reinterpret_cast<const float*>(st.mrow), j + kb * 32 + 4 * h, n, s[kb]);
     if (KIND < 2 && left < kb * 32 + 32) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         if (kb * 32 + 8 * (i / 4) + 4 * h + i % 4 >= left) s[kb][i] = kNegInf;
     }
   }
-  float top = st.m[t];
+  float top = st.m;
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -73,14 +68,14 @@ __device__ __forceinline__ void softmax_blocks(const AttnParams& p, RowState<T, 
   // m is the maximum of the tile that last moved it. It follows only where a row's maximum has grown by
   // more than 8 (in log2), which leaves probabilities up to 256 (no loss in floating point) and saves
   // scaling the outputs after most tiles, where some row's maximum still grows a little.
-  if (__any((top - st.m[t]) * c > 8.0f)) {
-    const float at = top == kNegInf ? 0.0f : top, keep = exp2_fast((st.m[t] - at) * c);
-    st.l[t] *= keep;
+  if (__any((top - st.m) * c > 8.0f)) {
+    const float at = top == kNegInf ? 0.0f : top, keep = exp2_fast((st.m - at) * c);
+    st.l *= keep;
 #pragma unroll
-    for (int d = 0; d < RowState<T, DP, QT>::DT; ++d) st.o[t][d] *= keep;
-    st.m[t] = top;
+    for (int d = 0; d < RowState<T, DP>::DT; ++d) st.o[d] *= keep;
+    st.m = top;
   }
-  const float mc = (st.m[t] == kNegInf ? 0.0f : st.m[t]) * c;
+  const float mc = (st.m == kNegInf ? 0.0f : st.m) * c;
   float sum = 0;
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb) {
@@ -92,7 +87,7 @@ __device__ __forceinline__ void softmax_blocks(const AttnParams& p, RowState<T, 
     e[kb] = Block<T>(s[kb]);
     sum = e[kb].sum(sum);
   }
-  st.l[t] += sum;
+  st.l += sum;
 }
 
 // Partial results: unscaled outputs [split][key head][row][D], then (maximum, sum) of each.
@@ -113,10 +108,17 @@ template <typename T> constexpr int few_waves(int DP, int KIND) {
   return sizeof(T) == 2 ? (KIND && DP >= 96 ? 1 : 2) : (DP >= 96 || (KIND && DP == 64) ? 1 : 2);
 }
 
+// Bound by the matrix and the vector instructions of a SIMD, which hardly overlap on this machine: of 1024
+// rows x 4096 states x 192 bf16 heads of 64 (325 us, 634 TFLOP/s) the matrix unit is busy 35 % of the cycles
+// and the vector unit 58 % (an exponential takes as long as two or three other instructions). A loop of the same
+// instructions on registers alone takes 250 us; staging the tiles costs most of the rest. Two row blocks a
+// wave would stage and read half as much, but leave two waves a SIMD instead of three: 359 us where one
+// block takes 347 (52 and 63 us for 384 x 768 x 384). Asynchronous loads into LDS were no way out either: every
+// LDS read then waits for all of them.
 template <typename T, int DP, int KIND>
 __global__ __launch_bounds__(256, tile_waves<T>(DP, KIND)) void attn_fwd_tile_kernel(AttnParams p) {
   constexpr int LP = DP == 96 ? 128 : DP, KB = sizeof(T) == 2 ? 2 : 1, KT = 32 * KB, DT = DP / 32;
-  constexpr int STEPS = RowState<T, DP, 1>::STEPS;
+  constexpr int STEPS = RowState<T, DP>::STEPS;
   __shared__ __attribute__((aligned(16))) char tiles[2][2][KT * LP * sizeof(T)];
   __shared__ int bad_tile[2];
   const int64_t all = p.tiles * p.B * p.Hk, id = xcd_tile(blockIdx.x, gridDim.x);
@@ -126,8 +128,8 @@ __global__ __launch_bounds__(256, tile_waves<T>(DP, KIND)) void attn_fwd_tile_ke
   const int64_t len = attn_len(p, b), j0 = split * p.chunk, n = len < j0 + p.chunk ? len : j0 + p.chunk;
   if (split && n <= j0) return;                        // (split 0 writes the rows of images without states)
   const int64_t r0 = (id - bh * p.tiles) * 128 + (threadIdx.x >> 6) * 32;
-  RowState<T, DP, 1> st;
-  init_rows<T, DP, 1>(p, st, b, hk, r0);
+  RowState<T, DP> st;
+  init_rows<T, DP>(p, st, b, hk, r0);
   const T* k = static_cast<const T*>(p.k) + b * p.ks[0] + hk * p.ks[2];
   const T* v = static_cast<const T*>(p.v) + b * p.vs[0] + hk * p.vs[2];
   Staged<T, LP, KT, 256> kr, vr;
@@ -141,7 +143,7 @@ __global__ __launch_bounds__(256, tile_waves<T>(DP, KIND)) void attn_fwd_tile_ke
   uint32_t word[2] = {0, 0};
   auto words = [&](int64_t j) {                        // (words of whole blocks: bits behind the states are 0)
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) st.word[0][kb] = j + 32 * kb < n && r0 + (threadIdx.x & 31) < p.R ? st.mrow[0][j / 32 + kb] : 0;
+    for (int kb = 0; kb < KB; ++kb) st.word[kb] = j + 32 * kb < n && r0 + (threadIdx.x & 31) < p.R ? st.mrow[j / 32 + kb] : 0;
   };
   auto put = [&](int buf, int tile) {
     kr.store(tiles[buf][0], p.D);
@@ -158,8 +160,8 @@ __global__ __launch_bounds__(256, tile_waves<T>(DP, KIND)) void attn_fwd_tile_ke
   for (int64_t j = j0; j < n; j += KT, ++at) {
     const int64_t next = j + KT;
     if (KIND == 1) {
-      word[0] = st.word[0][0];
-      word[1] = st.word[0][1];
+      word[0] = st.word[0];
+      word[1] = st.word[1];
       if (next < n) words(next);
     }
     if (next < n) {
@@ -175,14 +177,14 @@ __global__ __launch_bounds__(256, tile_waves<T>(DP, KIND)) void attn_fwd_tile_ke
       Block<T> e[KB];
       Turned<T, LP> va[2][DT];
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) row_product<T, LP>(kt + kb * 32 * LP * sizeof(T), st.q[0], s[kb]);
+      for (int kb = 0; kb < KB; ++kb) row_product<T, LP>(kt + kb * 32 * LP * sizeof(T), st.q, s[kb]);
 #pragma unroll
       for (int d = 0; d < DT; ++d) va[0][d].read(vt, 0, d);
       reads_done();
-      softmax_blocks<T, DP, 1, KIND, KB>(p, st, 0, s, e, word, j, n);
+      softmax_blocks<T, DP, KIND, KB>(p, st, s, e, word, j, n);
       if (KIND && bad_tile[at & 1] == at) {
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) slow_second<T, LP, DT>(vt, kb * 32, s[kb], st.o[0]);
+        for (int kb = 0; kb < KB; ++kb) slow_second<T, LP, DT>(vt, kb * 32, s[kb], st.o);
       } else {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
@@ -192,51 +194,48 @@ __global__ __launch_bounds__(256, tile_waves<T>(DP, KIND)) void attn_fwd_tile_ke
             reads_done();
           }
 #pragma unroll
-          for (int d = 0; d < DT; ++d) st.o[0][d] = va[kb & 1][d].mma(e[kb], st.o[0][d]);
+          for (int d = 0; d < DT; ++d) st.o[d] = va[kb & 1][d].mma(e[kb], st.o[d]);
         }
       }
     }
     if (next < n) put((at + 1) & 1, at + 1);
   }
   const int lane = threadIdx.x & 63;
-  {
-    constexpr int q = 0;
-    const int64_t r = r0 + (lane & 31);
-    const float sum = st.l[q] + other_half(st.l[q]), m = KIND ? st.m[q] : st.m[q] * p.c;
-    if (r >= p.R) return;
-    if (p.splits > 1) {
-      const int64_t row = (split * p.B * p.Hk + bh) * p.R + r;
-      if (lane < 32) part_stats(p)[row] = make_float2(m, sum);
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; e += 4)
-          store_run(p.part + row * p.D, d * 32 + 2 * e + 4 * (lane >> 5), p.D, st.o[q][d][e], st.o[q][d][e + 1], st.o[q][d][e + 2],
-                    st.o[q][d][e + 3]);
-      return;
-    }
-    const int64_t g = r / p.Lq, i = r - g * p.Lq, off = b * p.os[0] + i * p.os[1] + (hk * p.G + g) * p.os[2];
-    T* out = static_cast<T*>(p.o) + off;
-    const float inv = sum == 0 ? 0.0f : 1.0f / sum;
+  const int64_t r = r0 + (lane & 31);
+  const float sum = st.l + other_half(st.l), m = KIND ? st.m : st.m * p.c;
+  if (r >= p.R) return;
+  if (p.splits > 1) {
+    const int64_t row = (split * p.B * p.Hk + bh) * p.R + r;
+    if (lane < 32) part_stats(p)[row] = make_float2(m, sum);
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const int at_d = d * 32 + 2 * e + 4 * (lane >> 5);
-        float y[4], rest[4];
+      for (int e = 0; e < 16; e += 4)
+        store_run(p.part + row * p.D, d * 32 + 2 * e + 4 * (lane >> 5), p.D, st.o[d][e], st.o[d][e + 1], st.o[d][e + 2],
+                  st.o[d][e + 3]);
+    return;
+  }
+  const int64_t g = r / p.Lq, i = r - g * p.Lq, off = b * p.os[0] + i * p.os[1] + (hk * p.G + g) * p.os[2];
+  T* out = static_cast<T*>(p.o) + off;
+  const float inv = sum == 0 ? 0.0f : 1.0f / sum;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          y[x] = st.o[q][d][e + x] * inv;
-          rest[x] = y[x] - bf16_bits_to_f32(f32_to_bf16_bits(y[x]));
-        }
-        store_run(out, at_d, p.D, y[0], y[1], y[2], y[3]);
-        if (p.rest) store_run(static_cast<T*>(p.rest) + off, at_d, p.D, rest[0], rest[1], rest[2], rest[3]);
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const int at_d = d * 32 + 2 * e + 4 * (lane >> 5);
+      float y[4], rest[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        y[x] = st.o[d][e + x] * inv;
+        rest[x] = y[x] - bf16_bits_to_f32(f32_to_bf16_bits(y[x]));
       }
-    if (p.stats && lane < 32) {
-      const int64_t w = stat_at(p, b, hk, r);
-      p.stats[w] = m;
-      p.stats[p.B * p.H * p.Lq + w] = sum;
+      store_run(out, at_d, p.D, y[0], y[1], y[2], y[3]);
+      if (p.rest) store_run(static_cast<T*>(p.rest) + off, at_d, p.D, rest[0], rest[1], rest[2], rest[3]);
     }
+  if (p.stats && lane < 32) {
+    const int64_t w = stat_at(p, b, hk, r);
+    p.stats[w] = m;
+    p.stats[p.B * p.H * p.Lq + w] = sum;
   }
 }
 
@@ -254,9 +253,12 @@ __device__ __forceinline__ void put_row(const AttnParams& p, int64_t b, int hk, 
   }
 }
 
-template <typename T, int DP, int QT, int KIND>
+// Bound by memory: every key and value is read once, for all rows of its key head. 4 rows of 16 heads over
+// 131072 bf16 states of 4 key heads of 128: 268 MB in 52 us, 5.2 TB/s; one row of 128 images over 256 to 5120
+// states, 6 heads of 64: 528 MB in 120 us, 4.4 TB/s (a copy of this size reaches 4.9).
+template <typename T, int DP, int KIND>
 __global__ __launch_bounds__(256, few_waves<T>(DP, KIND)) void attn_fwd_few_kernel(AttnParams p) {
-  constexpr int LP = DP == 96 ? 128 : DP, DT = DP / 32, STEPS = RowState<T, DP, QT>::STEPS;
+  constexpr int LP = DP == 96 ? 128 : DP, DT = DP / 32, STEPS = RowState<T, DP>::STEPS;
   constexpr int TILE = 32 * LP * static_cast<int>(sizeof(T)), JOIN = 32 * (DP + 1) * 4;
   __shared__ __attribute__((aligned(16))) char lds[4 * (TILE > JOIN ? TILE : JOIN)];
   __shared__ float wm[4][32], wl[4][32];
@@ -264,8 +266,8 @@ __global__ __launch_bounds__(256, few_waves<T>(DP, KIND)) void attn_fwd_few_kern
   const int hk = static_cast<int>(bh - b * p.Hk), split = blockIdx.y, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63;
   const int64_t len = attn_len(p, b), j0 = split * p.chunk, n = len < j0 + p.chunk ? len : j0 + p.chunk;
   if (split && n <= j0) return;
-  RowState<T, DP, QT> st;
-  init_rows<T, DP, QT>(p, st, b, hk, 0);
+  RowState<T, DP> st;
+  init_rows<T, DP>(p, st, b, hk, 0);
   const T* k = static_cast<const T*>(p.k) + b * p.ks[0] + hk * p.ks[2];
   const T* v = static_cast<const T*>(p.v) + b * p.vs[0] + hk * p.vs[2];
   char* vt = lds + w * TILE;
@@ -273,12 +275,9 @@ __global__ __launch_bounds__(256, few_waves<T>(DP, KIND)) void attn_fwd_few_kern
   Staged<T, LP, 32, 64> vr;
   vr.init(p.vs[1], p.D, l);
   vr.clear(vt, p.D);
-  uint32_t word[QT][2] = {};
+  uint32_t word[2] = {};
   auto fetch = [&](int64_t j) {
-    if (KIND == 1) {
-#pragma unroll
-      for (int q = 0; q < QT; ++q) st.word[q][0] = 32 * q + (l & 31) < p.R ? st.mrow[q][j / 32] : 0;
-    }
+    if (KIND == 1) st.word[0] = (l & 31) < p.R ? st.mrow[j / 32] : 0;
     const T* row = k + (j + (l & 31)) * p.ks[1];
 #pragma unroll
     for (int t = 0; t < STEPS; ++t)
@@ -288,68 +287,55 @@ __global__ __launch_bounds__(256, few_waves<T>(DP, KIND)) void attn_fwd_few_kern
   wait_loads();
   if (j0 + 32 * w < n) fetch(j0 + 32 * w);
   for (int64_t j = j0 + 32 * w; j < n; j += 128) {
-    f32x16 s[QT][1] = {};
-    Block<T> e[QT][1];
+    f32x16 s[1] = {};
+    Block<T> e[1];
     Turned<T, LP> va[DT];
 #pragma unroll
-    for (int t = 0; t < STEPS; ++t)
-#pragma unroll
-      for (int q = 0; q < QT; ++q) s[q][0] = mma_step(T(), ka[t], st.q[q][t], s[q][0]);
+    for (int t = 0; t < STEPS; ++t) s[0] = mma_step(T(), ka[t], st.q[t], s[0]);
     vr.store(vt, p.D);                     // the wave's own tile: LDS serves a wave's accesses in order
     __builtin_amdgcn_wave_barrier();
     const bool bad = KIND && __any(vr.bad());
-    if (KIND == 1) {
-#pragma unroll
-      for (int q = 0; q < QT; ++q) word[q][0] = st.word[q][0];
-    }
+    if (KIND == 1) word[0] = st.word[0];
     if (j + 128 < n) fetch(j + 128);
 #pragma unroll
     for (int d = 0; d < DT; ++d) va[d].read(vt, 0, d);
     reads_done();
+    softmax_blocks<T, DP, KIND, 1>(p, st, s, e, word, j, n);
+    if (bad) {
+      slow_second<T, LP, DT>(vt, 0, s[0], st.o);
+    } else {
 #pragma unroll
-    for (int q = 0; q < QT; ++q) softmax_blocks<T, DP, QT, KIND, 1>(p, st, q, s[q], e[q], word[q], j, n);
-#pragma unroll
-    for (int q = 0; q < QT; ++q) {
-      if (bad) {
-        slow_second<T, LP, DT>(vt, 0, s[q][0], st.o[q]);
-      } else {
-#pragma unroll
-        for (int d = 0; d < DT; ++d) st.o[q][d] = va[d].mma(e[q][0], st.o[q][d]);
-      }
+      for (int d = 0; d < DT; ++d) st.o[d] = va[d].mma(e[0], st.o[d]);
     }
     __builtin_amdgcn_wave_barrier();
   }
   float* join = reinterpret_cast<float*>(lds) + w * (JOIN / 4);
+  __syncthreads();
+  const float sum = st.l + other_half(st.l);
+  if (l < 32) { wm[w][l] = KIND ? st.m : st.m * p.c; wl[w][l] = sum; }
 #pragma unroll
-  for (int q = 0; q < QT; ++q) {
-    if (q * 32 >= p.R) break;
-    __syncthreads();
-    const float sum = st.l[q] + other_half(st.l[q]);
-    if (l < 32) { wm[w][l] = KIND ? st.m[q] : st.m[q] * p.c; wl[w][l] = sum; }
+  for (int d = 0; d < DT; ++d)
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
+    for (int e = 0; e < 16; ++e) join[(l & 31) * (DP + 1) + d * 32 + 8 * (e / 4) + 4 * (l >> 5) + e % 4] = st.o[d][e];
+  __syncthreads();
+  const int rows = static_cast<int>(p.R);
+  for (int x = threadIdx.x; x < rows * p.D; x += 256) {
+    const int r = x / p.D, d = x - r * p.D;
+    const float m = fmaxf(fmaxf(wm[0][r], wm[1][r]), fmaxf(wm[2][r], wm[3][r])), at = m == kNegInf ? 0.0f : m;
+    float value = 0, total = 0;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) join[(l & 31) * (DP + 1) + d * 32 + 8 * (e / 4) + 4 * (l >> 5) + e % 4] = st.o[q][d][e];
-    __syncthreads();
-    const int rows = static_cast<int>(p.R - q * 32 < 32 ? p.R - q * 32 : 32);
-    for (int x = threadIdx.x; x < rows * p.D; x += 256) {
-      const int r = x / p.D, d = x - r * p.D;
-      const float m = fmaxf(fmaxf(wm[0][r], wm[1][r]), fmaxf(wm[2][r], wm[3][r])), at = m == kNegInf ? 0.0f : m;
-      float value = 0, total = 0;
-#pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        const float f = exp2_fast(wm[y][r] - at);
-        total = fmaf(wl[y][r], f, total);
-        value = fmaf(reinterpret_cast<const float*>(lds)[y * (JOIN / 4) + r * (DP + 1) + d], f, value);
-      }
-      const int64_t row = q * 32 + r;
-      if (p.splits > 1) {
-        const int64_t at_row = (split * p.B * p.Hk + bh) * p.R + row;
-        p.part[at_row * p.D + d] = value;
-        if (d == 0) part_stats(p)[at_row] = make_float2(m, total);
-      } else {
-        put_row<T>(p, b, hk, row, d, value, m, total);
-      }
+    for (int y = 0; y < 4; ++y) {
+      const float f = exp2_fast(wm[y][r] - at);
+      total = fmaf(wl[y][r], f, total);
+      value = fmaf(reinterpret_cast<const float*>(lds)[y * (JOIN / 4) + r * (DP + 1) + d], f, value);
+    }
+    const int64_t row = r;
+    if (p.splits > 1) {
+      const int64_t at_row = (split * p.B * p.Hk + bh) * p.R + row;
+      p.part[at_row * p.D + d] = value;
+      if (d == 0) part_stats(p)[at_row] = make_float2(m, total);
+    } else {
+      put_row<T>(p, b, hk, row, d, value, m, total);
     }
   }
 }
@@ -433,7 +419,7 @@ int attn_pack_launch(const void* keep, const int64_t* stride, int64_t n0, int64_
 // How a call is laid out. Few rows: every workgroup has them all. Else tiles of 128 or 256 rows.
 struct FwdPlan {
   bool few;
-  int qt, splits;
+  int splits;
   int64_t tiles, chunk;
 };
 
@@ -446,15 +432,10 @@ static int few_waves_at(int dtype, int64_t D, bool mask) {
 static FwdPlan fwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t D, int dtype, bool mask) {
   FwdPlan f;
   const int64_t R = H / Hk * Lq;
-  const bool two = dtype == FOVI_BF16 && D <= 64 && !mask;     // two blocks of rows a wave fit its registers
-  f.few = R <= (two ? 64 : 32);
-  if (f.few) {
-    f.qt = R <= 32 ? 1 : 2;
-    f.tiles = 1;
-  } else {
-    f.qt = 1;
-    f.tiles = (R + 127) / 128;
-  }
+  // Up to a block of rows (48 rows, 64 x 6 heads of 64 over 600 states: 20 us by tiles; the few-row kernel with two
+  // blocks of rows a wave took 28 and a join of 8)
+  f.few = R <= 32;
+  f.tiles = f.few ? 1 : (R + 127) / 128;
   // The states are split until the card is full (few rows of many key heads: twice, since lengths
   // differ), in parts that are still worth a workgroup's start and the join: 512 states for few rows
   // (131072 states, 4 key heads of 128: 128 parts 51.6 + 6.7 us, 256 parts 53.5 + 8.9, 64 parts 52.7 + 5.5, but
@@ -487,8 +468,7 @@ static void fwd_launch(const AttnParams& p, const FwdPlan& f, hipStream_t s) {
   const int64_t all = p.B * p.Hk * f.tiles;
   if (f.few) {
     const dim3 grid(static_cast<unsigned>(all), static_cast<unsigned>(f.splits));
-    if (f.qt == 1) attn_fwd_few_kernel<T, DP, 1, KIND><<<grid, 256, 0, s>>>(p);
-    else if constexpr (DP <= 64 && sizeof(T) == 2 && KIND == 0) attn_fwd_few_kernel<T, DP, 2, KIND><<<grid, 256, 0, s>>>(p);
+    attn_fwd_few_kernel<T, DP, KIND><<<grid, 256, 0, s>>>(p);
   } else {
     const dim3 grid(static_cast<unsigned>((all + 7) / 8 * 8), static_cast<unsigned>(f.splits));
     attn_fwd_tile_kernel<T, DP, KIND><<<grid, 256, 0, s>>>(p);

@@ -4,7 +4,7 @@
 // head, so a workgroup computes the cosines and sines of its tokens once into LDS and turns all
 // heads from there. The product of two floats is exact in fp64; reduced to [-pi, pi] there, the
 // angle reaches the sine with fp32 accuracy at any position (an fp32 product at position 10000 is
-// already wrong by 5e-4).
+// already wrong by 5e-4). 131072 tokens of 6 bf16 heads of 64: 46 us (201 MB, 4.4 TB/s).
 #include "common.h"
 
 namespace fovi {
