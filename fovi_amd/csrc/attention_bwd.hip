@@ -50,13 +50,13 @@ __global__ __launch_bounds__(256, dq_waves<T>(DP, KIND)) void attn_dq_kernel(Att
   constexpr int LP = DP == 96 ? 128 : DP, KB = sizeof(T) == 2 ? 2 : 1, KT = 32 * KB, DT = DP / 32, STEPS = DP / (2 * Chunk<T>::N);
   __shared__ __attribute__((aligned(16))) char tiles[2][2][KT * LP * sizeof(T)];
   __shared__ int bad_tile[2];
-  const int64_t all = p.tiles * p.B * p.Hk, id = xcd_tile(blockIdx.x, gridDim.x);
+  const int64_t all = p.tiles * p.splits * p.B * p.Hk, id = xcd_tile(blockIdx.x, gridDim.x);
   if (id >= all) return;
-  const int64_t bh = id / p.tiles, b = bh / p.Hk;
-  const int hk = static_cast<int>(bh - b * p.Hk), split = blockIdx.y, l = threadIdx.x & 63;
+  const int64_t group = id / p.tiles, bh = group / p.splits, b = bh / p.Hk;
+  const int hk = static_cast<int>(bh - b * p.Hk), split = static_cast<int>(group - bh * p.splits), l = threadIdx.x & 63;
   const int64_t len = attn_len(p, b), j0 = split * p.chunk, n = len < j0 + p.chunk ? len : j0 + p.chunk;
   if (split && n <= j0) return;
-  const int64_t r0 = (id - bh * p.tiles) * 128 + (threadIdx.x >> 6) * 32;
+  const int64_t r0 = (id - group * p.tiles) * 128 + (threadIdx.x >> 6) * 32;
   u32x4 q[STEPS], g[STEPS];
   f32x16 dq[DT] = {};
   constexpr bool START = sizeof(T) == 2 && DP == 32;   // -delta as a block of its own, where registers allow
@@ -199,11 +199,11 @@ __global__ __launch_bounds__(256, dkv_waves<T>(DP, KIND)) void attn_dkv_kernel(A
   __shared__ __attribute__((aligned(16))) float stats[2][3][RT];
   __shared__ int bad_tile[2][2];
   __shared__ __attribute__((aligned(16))) uint32_t bits[2][4][KIND == 1 ? RT : 4];     // [wave][row]: its 32 states
-  const int64_t all = p.tiles * p.B * p.Hk, id = xcd_tile(blockIdx.x, gridDim.x);
+  const int64_t all = p.tiles * p.splits * p.B * p.Hk, id = xcd_tile(blockIdx.x, gridDim.x);
   if (id >= all) return;
-  const int64_t bh = id / p.tiles, b = bh / p.Hk;
-  const int hk = static_cast<int>(bh - b * p.Hk), split = blockIdx.y, l = threadIdx.x & 63;
-  const int64_t n = attn_len(p, b), w0 = (id - bh * p.tiles) * 128, j = w0 + (threadIdx.x >> 6) * 32 + (l & 31);
+  const int64_t group = id / p.tiles, bh = group / p.splits, b = bh / p.Hk;
+  const int hk = static_cast<int>(bh - b * p.Hk), split = static_cast<int>(group - bh * p.splits), l = threadIdx.x & 63;
+  const int64_t n = attn_len(p, b), w0 = (id - group * p.tiles) * 128, j = w0 + (threadIdx.x >> 6) * 32 + (l & 31);
   const T* kp = static_cast<const T*>(p.k) + b * p.ks[0] + j * p.ks[1] + hk * p.ks[2];
   const T* vp = static_cast<const T*>(p.v) + b * p.vs[0] + j * p.vs[1] + hk * p.vs[2];
   u32x4 k[STEPS], v[STEPS];
@@ -451,13 +451,13 @@ int64_t attn_bwd_workspace(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t
 
 template <typename T, int DP, int KIND>
 static void bwd_dq(const AttnParams& p, hipStream_t s) {
-  const dim3 grid(static_cast<unsigned>((p.B * p.Hk * p.tiles + 7) / 8 * 8), static_cast<unsigned>(p.splits));
+  const unsigned grid = static_cast<unsigned>((p.B * p.Hk * p.tiles * p.splits + 7) / 8 * 8);
   attn_dq_kernel<T, DP, KIND><<<grid, 256, 0, s>>>(p);
 }
 
 template <typename T, int DP, int KIND>
 static void bwd_dkv(const AttnParams& p, hipStream_t s) {
-  const dim3 grid(static_cast<unsigned>((p.B * p.Hk * p.tiles + 7) / 8 * 8), static_cast<unsigned>(p.splits));
+  const unsigned grid = static_cast<unsigned>((p.B * p.Hk * p.tiles * p.splits + 7) / 8 * 8);
   attn_dkv_kernel<T, DP, KIND><<<grid, 256, 0, s>>>(p);
 }
 

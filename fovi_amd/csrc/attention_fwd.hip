@@ -4,7 +4,7 @@
 //  * tile kernel: a workgroup owns 128 query rows of one key head (the rows of the query heads that share
 //    it, in one sequence) and walks the states in tiles that all four waves read from LDS; the next tile is
 //    on its way in registers meanwhile.
-//  * few-row kernel: up to 32 rows in all. Every wave of the workgroup has all the rows and its own
+//  * few-row kernel (fp32, or under a mask): up to 32 rows in all. Every wave of the workgroup has all the rows and its own
 //    states: keys straight from memory as matrix operands, values through an LDS tile of the
 //    wave's own (only the transposing read needs it), no barrier until the four waves' results join.
 //
@@ -105,7 +105,7 @@ template <typename T> constexpr int tile_waves(int DP, int KIND) {
   return sizeof(T) == 2 ? (KIND ? (DP >= 96 ? 1 : 2) : DP <= 64 ? 3 : 2) : (DP == 128 || (KIND && DP == 96) ? 1 : 2);
 }
 template <typename T> constexpr int few_waves(int DP, int KIND) {
-  return sizeof(T) == 2 ? (KIND && DP >= 96 ? 1 : 2) : (DP >= 96 || (KIND && DP == 64) ? 1 : 2);
+  return sizeof(T) == 2 ? (DP >= 96 ? 1 : 2) : (DP >= 96 || (KIND && DP == 64) ? 1 : 2);
 }
 
 // Bound by the matrix and the vector instructions of a SIMD, which hardly overlap on this machine: of 1024
@@ -114,20 +114,22 @@ template <typename T> constexpr int few_waves(int DP, int KIND) {
 // instructions on registers alone takes 250 us; staging the tiles costs most of the rest. Two row blocks a
 // wave would stage and read half as much, but leave two waves a SIMD instead of three: 359 us where one
 // block takes 347 (52 and 63 us for 384 x 768 x 384). Asynchronous loads into LDS were no way out either: every
-// LDS read then waits for all of them.
+// LDS read then waits for all of them. Few rows are bound by memory: 4 rows of 16 heads over 131072 states of 4
+// key heads of 128 take 44 us (268 MB, 6.1 TB/s), one row of 128 images over 256 to 5120 states, 6 heads of 64,
+// 117 us (528 MB, 4.5 TB/s; a copy of this size reaches 4.9).
 template <typename T, int DP, int KIND>
 __global__ __launch_bounds__(256, tile_waves<T>(DP, KIND)) void attn_fwd_tile_kernel(AttnParams p) {
   constexpr int LP = DP == 96 ? 128 : DP, KB = sizeof(T) == 2 ? 2 : 1, KT = 32 * KB, DT = DP / 32;
   constexpr int STEPS = RowState<T, DP>::STEPS;
   __shared__ __attribute__((aligned(16))) char tiles[2][2][KT * LP * sizeof(T)];
   __shared__ int bad_tile[2];
-  const int64_t all = p.tiles * p.B * p.Hk, id = xcd_tile(blockIdx.x, gridDim.x);
+  const int64_t all = p.tiles * p.splits * p.B * p.Hk, id = xcd_tile(blockIdx.x, gridDim.x);
   if (id >= all) return;
-  const int64_t bh = id / p.tiles, b = bh / p.Hk;
-  const int hk = static_cast<int>(bh - b * p.Hk), split = blockIdx.y;
+  const int64_t group = id / p.tiles, bh = group / p.splits, b = bh / p.Hk;
+  const int hk = static_cast<int>(bh - b * p.Hk), split = static_cast<int>(group - bh * p.splits);
   const int64_t len = attn_len(p, b), j0 = split * p.chunk, n = len < j0 + p.chunk ? len : j0 + p.chunk;
   if (split && n <= j0) return;                        // (split 0 writes the rows of images without states)
-  const int64_t r0 = (id - bh * p.tiles) * 128 + (threadIdx.x >> 6) * 32;
+  const int64_t r0 = (id - group * p.tiles) * 128 + (threadIdx.x >> 6) * 32;
   RowState<T, DP> st;
   init_rows<T, DP>(p, st, b, hk, r0);
   const T* k = static_cast<const T*>(p.k) + b * p.ks[0] + hk * p.ks[2];
@@ -253,9 +255,8 @@ __device__ __forceinline__ void put_row(const AttnParams& p, int64_t b, int hk, 
   }
 }
 
-// Bound by memory: every key and value is read once, for all rows of its key head. 4 rows of 16 heads over
-// 131072 bf16 states of 4 key heads of 128: 268 MB in 52 us, 5.2 TB/s; one row of 128 images over 256 to 5120
-// states, 6 heads of 64: 528 MB in 120 us, 4.4 TB/s (a copy of this size reaches 4.9).
+// Every key and value is read once, for all rows of its key head. 64 images, 2048 states, 6 heads of 64: 403 MB
+// of fp32 in 106 us, 3.8 TB/s, with the products of a whole block of rows however few there are.
 template <typename T, int DP, int KIND>
 __global__ __launch_bounds__(256, few_waves<T>(DP, KIND)) void attn_fwd_few_kernel(AttnParams p) {
   constexpr int LP = DP == 96 ? 128 : DP, DT = DP / 32, STEPS = RowState<T, DP>::STEPS;
@@ -426,21 +427,22 @@ struct FwdPlan {
 // Workgroups of the few-row kernel on a compute unit: its waves a SIMD.
 static int few_waves_at(int dtype, int64_t D, bool mask) {
   const int dp = D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128;
-  return dtype == FOVI_BF16 ? few_waves<uint16_t>(dp, mask) + (dp <= 64 && !mask) : few_waves<float>(dp, mask);
+  return dtype == FOVI_BF16 ? few_waves<uint16_t>(dp, mask) : few_waves<float>(dp, mask);
 }
 
 static FwdPlan fwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t D, int dtype, bool mask) {
   FwdPlan f;
   const int64_t R = H / Hk * Lq;
-  // Up to a block of rows (48 rows, 64 x 6 heads of 64 over 600 states: 20 us by tiles; the few-row kernel with two
-  // blocks of rows a wave took 28 and a join of 8)
-  f.few = R <= 32;
+  // Few rows of fp32, whose products are slow (four waves share them: 64 x 6 heads of 64, one row over 2048
+  // states: 106 us and a join of 6, by tiles 168), or under a mask (bf16, the same sizes: 40 + 5, by tiles 61).
+  // Plain bf16 rows go by tiles, whose one wave keeps up with memory (128 images, 256 to 5120 states: 117 us, 125 +
+  // 5 here; 131072 states, 4 key heads of 128: 44, 51 here).
+  f.few = R <= 32 && (dtype == FOVI_F32 || mask);
   f.tiles = f.few ? 1 : (R + 127) / 128;
   // The states are split until the card is full (few rows of many key heads: twice, since lengths
-  // differ), in parts that are still worth a workgroup's start and the join: 512 states for few rows
-  // (131072 states, 4 key heads of 128: 128 parts 51.6 + 6.7 us, 256 parts 53.5 + 8.9, 64 parts 52.7 + 5.5, but
-  // where a wave a SIMD is all there is, 9000 fp32 states and 32 heads of 80: 8 parts 57, 4 98), 128 for
-  // tiles (515 states, 32 groups, fp32 under a mask: parts of 128 14 us, of 256 23; the join 5 each).
+  // differ), in parts that are still worth a workgroup's start and the join: 512 states for few rows (where a
+  // wave a SIMD is all there is, 9000 fp32 states and 32 heads of 80: 8 parts 57 us, 4 98), 128 for tiles (515
+  // states, 32 groups, fp32 under a mask: parts of 128 14 us, of 256 23; the join 5 each).
   const int waves = f.few ? few_waves_at(dtype, D, mask) : 2;
   const int64_t groups = B * Hk * f.tiles, least = f.few ? 512 : 128, want = f.few ? (groups < 64 ? 256 : 512) * waves : 512;
   int64_t splits = groups > 0 ? want / groups : 1;
@@ -468,9 +470,9 @@ static void fwd_launch(const AttnParams& p, const FwdPlan& f, hipStream_t s) {
   const int64_t all = p.B * p.Hk * f.tiles;
   if (f.few) {
     const dim3 grid(static_cast<unsigned>(all), static_cast<unsigned>(f.splits));
-    attn_fwd_few_kernel<T, DP, KIND><<<grid, 256, 0, s>>>(p);
+    if constexpr (sizeof(T) == 4 || KIND != 0) attn_fwd_few_kernel<T, DP, KIND><<<grid, 256, 0, s>>>(p);
   } else {
-    const dim3 grid(static_cast<unsigned>((all + 7) / 8 * 8), static_cast<unsigned>(f.splits));
+    const unsigned grid = static_cast<unsigned>((all * f.splits + 7) / 8 * 8);
     attn_fwd_tile_kernel<T, DP, KIND><<<grid, 256, 0, s>>>(p);
   }
 }
