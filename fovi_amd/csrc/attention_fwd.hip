@@ -264,7 +264,8 @@ __global__ __launch_bounds__(256, few_waves<T>(DP, KIND)) void attn_fwd_few_kern
   __shared__ __attribute__((aligned(16))) char lds[4 * (TILE > JOIN ? TILE : JOIN)];
   __shared__ float wm[4][32], wl[4][32];
   const int64_t bh = blockIdx.x, b = bh / p.Hk;
-  const int hk = static_cast<int>(bh - b * p.Hk), split = blockIdx.y, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63;
+  const int hk = static_cast<int>(bh - b * p.Hk), split = blockIdx.y, l = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t len = attn_len(p, b), j0 = split * p.chunk, n = len < j0 + p.chunk ? len : j0 + p.chunk;
   if (split && n <= j0) return;
   RowState<T, DP> st;
