@@ -213,10 +213,11 @@ __global__ __launch_bounds__(256, dkv_waves<T>(DP, KIND)) void attn_dkv_kernel(A
     v[s] = load_chunk<T>(vp, 2 * s + (l >> 5), j < n ? p.D : 0);
   }
   f32x16 dk[DT] = {}, dv[DT] = {};
-  // tiles of RT rows, head by head; split s walks tiles s * chunk .. of the p.G * per there are
+  // tiles of RT rows, head by head; split s walks tiles s * chunk .. of the p.G * per there are (none without
+  // queries: then no row, statistic or mask has an element, and the gradients below are zeros)
   const int per = p.Lq > 0 ? static_cast<int>((p.Lq + RT - 1) / RT) : 1;
   const int64_t first = split * p.chunk, end = static_cast<int64_t>(per) * p.G;
-  const int count = w0 >= n ? 0 : static_cast<int>(end < first + p.chunk ? end - first : p.chunk);
+  const int count = w0 >= n || p.Lq == 0 ? 0 : static_cast<int>(end < first + p.chunk ? end - first : p.chunk);
   Staged<T, LP, RT, 256> qr, gr;
   qr.init(p.qs[1], p.D, threadIdx.x);
   gr.init(p.dos[1], p.D, threadIdx.x);

@@ -545,3 +545,33 @@ def test_c_layouts_workspaces_and_masks_are_refused():
     assert lib.fovi_attention_pack_mask(4096, stride, 1, -1, 1, 8, 4096, None) != 0 and b"bad sizes" in lib.fovi_last_error()
     assert lib.fovi_attention_pack_mask(4096, stride, 1 << 30, 1 << 30, 1, 8, 4096, None) != 0
     assert b"too large" in lib.fovi_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kind", [_lib.MASK_NONE, _lib.MASK_KEEP, _lib.MASK_BIAS])
+@pytest.mark.parametrize("lk,hq,hk,d", [(1, 1, 1, 8), (70, 4, 2, 64), (300, 3, 1, 128)])
+def test_no_queries_in_the_c_backward(lk, hq, hk, d, kind, dtype):
+    """States without a query: dk and dv are written whole, as zeros, without a workspace. Queries,
+    statistics and masks have no element; their pointers have a place of their own all the same."""
+    b, lib = 2, _lib.load()
+    k = torch.randn(b, lk, hk, d, device="cuda").to(dtype)
+    dk, dv = torch.full_like(k, 7.0), torch.full_like(k, 7.0)
+    place = torch.zeros(1024, device="cuda")
+    a = _lib.AttentionBwdArgs()
+    f = a.fwd
+    f.q = f.out = f.stats = f.mask = a.dout = a.dq = place.data_ptr()
+    if dtype == torch.bfloat16:
+        f.out_rest = place.data_ptr()
+    f.k = f.v = k.data_ptr()
+    f.dtype, f.mask_kind, f.scale = _lib.dtype_code(dtype), kind, 0.125
+    f.batch, f.q_len, f.kv_len, f.heads, f.kv_heads, f.head_dim = b, 0, lk, hq, hk, d
+    for s in (f.k_stride, f.v_stride, a.dk_stride, a.dv_stride):
+        s[:] = k.stride()[:3]
+    for s in (f.q_stride, f.out_stride, a.dout_stride, a.dq_stride):
+        s[:] = (0, hq * d, d)
+    a.dk, a.dv = dk.data_ptr(), dv.data_ptr()
+    assert lib.fovi_attention_bwd_workspace_bytes(b, 0, lk, hq, hk, d, f.dtype) == 0
+    _lib.check(lib.fovi_attention_bwd(a, _lib.stream_of(k)), "fovi_attention_bwd")
+    torch.cuda.synchronize()
+    assert not dk.any() and not dv.any() and not place.any()
