@@ -403,12 +403,23 @@ def require_device(*tensors):
                                "there is no CPU fallback")
 
 
-@torch.autograd.function.once_differentiable
-def _once(ctx, backward, *grads):
-    return backward(ctx, *grads)
+class _Once(torch.autograd.Function):
+    """The gradients ``backward(of, *grads)`` of an autograd function, as a function of ``grads`` and of the
+    differentiable inputs that ``of`` kept, with no derivative of its own."""
+
+    @staticmethod
+    def forward(ctx, backward, of, n, *args):
+        return backward(of, *args[:n])
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("the gradients of fovi_amd's operators can be differentiated once only")
 
 
 def differentiated_once(backward, ctx, *grads):
-    """``backward(ctx, *grads)`` of an autograd function whose gradients have none: a second
-    differentiation raises. The guard that does it is left out where no graph is being made."""
-    return _once(ctx, backward, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    """``backward(ctx, *grads)`` of an autograd function whose gradients have none: whatever leads through
+    them a second time raises, also where the incoming gradients are constants (the inputs that
+    the function kept are enough). The guard that does it is left out where no graph is being made."""
+    if not torch.is_grad_enabled():
+        return backward(ctx, *grads)
+    return _Once.apply(backward, ctx, len(grads), *grads, *[t for t in ctx.saved_tensors if t is not None and t.requires_grad])

@@ -48,23 +48,20 @@ def _launch(x, positions, freqs, ends, pairing, inverse):
     return y
 
 
-def _backward(ctx, dy):
-    positions, freqs = ctx.saved_tensors
-    return _launch(dy, positions, freqs, ctx.ends, ctx.pairing, 1), None, None, None, None
-
-
 class _RotaryFn(torch.autograd.Function):
-    """``fovi_rotary``; its gradient is the rotation by the negative angles."""
+    """``fovi_rotary``; its gradient is the rotation by the negative angles, itself differentiable."""
 
     @staticmethod
-    def forward(ctx, x, positions, freqs, ends, pairing):
+    def forward(ctx, x, positions, freqs, ends, pairing, inverse):
         ctx.save_for_backward(positions, freqs)
-        ctx.ends, ctx.pairing = ends, pairing
-        return _launch(x, positions, freqs, ends, pairing, 0)
+        ctx.ends, ctx.pairing, ctx.inverse = ends, pairing, inverse
+        return _launch(x, positions, freqs, ends, pairing, inverse)
 
     @staticmethod
     def backward(ctx, dy):
-        return _lib.differentiated_once(_backward, ctx, dy)
+        positions, freqs = ctx.saved_tensors
+        call = _RotaryFn.apply if torch.is_grad_enabled() else _launch
+        return call(dy, positions, freqs, ctx.ends, ctx.pairing, 1 - ctx.inverse), None, None, None, None, None
 
 
 def rotary(x, positions, freqs, sections, pairing="half"):
@@ -74,7 +71,7 @@ def rotary(x, positions, freqs, sections, pairing="half"):
     number of pairs of each of the A axes, in order (their sum is P, 2 P <= D; 1 to 4 axes).
     ``pairing``: 'half' pairs elements (j, j + P), 'adjacent' (2 j, 2 j + 1); elements from 2 P on
     stay as they are, and so does a token at position 0 (a class token, say). Differentiable in
-    ``x``; the layout of ``x`` is kept where it is dense.
+    ``x``, any number of times; the layout of ``x`` is kept where it is dense.
     """
     _lib.require_device(x, positions, freqs)
     if x.dim() != 4 or x.shape[3] < 2:
@@ -110,7 +107,7 @@ def rotary(x, positions, freqs, sections, pairing="half"):
     if freqs.dtype != torch.float32 or not freqs.is_contiguous():
         freqs = freqs.float().contiguous()
     if torch.is_grad_enabled() and x.requires_grad:
-        return _RotaryFn.apply(x, positions, freqs, ends, _PAIRINGS[pairing])
+        return _RotaryFn.apply(x, positions, freqs, ends, _PAIRINGS[pairing], 0)
     return _launch(x, positions, freqs, ends, _PAIRINGS[pairing], 0)
 
 

@@ -575,3 +575,22 @@ def test_no_queries_in_the_c_backward(lk, hq, hk, d, kind, dtype):
     _lib.check(lib.fovi_attention_bwd(a, _lib.stream_of(k)), "fovi_attention_bwd")
     torch.cuda.synchronize()
     assert not dk.any() and not dv.any() and not place.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("constant", [True, False])
+def test_differentiating_twice_raises(constant):
+    """With a constant incoming gradient and with one that has a gradient itself, in every input; a
+    gradient that is only recorded, and not differentiated, is the gradient."""
+    from fovi_amd.arch.attention import cross_attention
+    q, k, v, dout, _ = _inputs(2, 5, 9, 2, 1, 16, torch.float32, seed=20)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    dout.requires_grad_(not constant)
+    out = cross_attention(*leaves)
+    grads = torch.autograd.grad(out, leaves, dout, create_graph=True)
+    want = torch.autograd.grad(cross_attention(*leaves), leaves, dout.detach())
+    assert all(torch.equal(a, b) for a, b in zip(grads, want))
+    for g in grads:
+        for leaf in leaves + ([] if constant else [dout]):
+            with pytest.raises(RuntimeError, match="differentiated once"):
+                torch.autograd.grad(cross_attention(*leaves).sum() + dout.sum() + g.square().sum(), leaf, retain_graph=True)

@@ -304,3 +304,21 @@ def test_writes_its_rows_only(rows, c, dtype):
     for t, inner in zip(outs, (y, dx)):
         inner.fill_(7.0)
         assert (t == 7.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("constant", [True, False])
+def test_differentiating_twice_raises(constant):
+    """With a constant incoming gradient and with one that has a gradient itself, in every input; a
+    gradient that is only recorded, and not differentiated, is the gradient."""
+    from fovi_amd.arch.norm import layer_norm
+    g = torch.Generator().manual_seed(20)
+    leaves = [torch.randn(s, generator=g).cuda().requires_grad_(True) for s in ((7, 40), (40,), (40,))]
+    dy = torch.randn(7, 40, generator=g).cuda().requires_grad_(not constant)
+    grads = torch.autograd.grad(layer_norm(*leaves), leaves, dy, create_graph=True)
+    want = torch.autograd.grad(layer_norm(*leaves), leaves, dy.detach())
+    assert all(torch.equal(a, b) for a, b in zip(grads, want))
+    for got in grads:
+        for leaf in leaves + ([] if constant else [dy]):
+            with pytest.raises(RuntimeError, match="differentiated once"):
+                torch.autograd.grad(layer_norm(*leaves).sum() + dy.sum() + got.square().sum(), leaf, retain_graph=True)

@@ -263,3 +263,35 @@ def test_writes_its_heads_only(d, pairs, pairing, dtype):
     _close(y, _reference(x, pos, freqs, (pairs,), ("half", "adjacent")[pairing]), dtype)
     y.fill_(7.0)
     assert (wide == 7.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("constant", [True, False])
+def test_second_gradients(constant):
+    """A penalty on a gradient. The rotation is linear, so that its gradient is differentiable as it is. Six
+    turns of 5e-7 follow one another at most (y enters squared), with ten roundings of 6e-8: 4e-6."""
+    from fovi_amd.arch.rotary import rotary
+    x, pos, g = _inputs(2, 9, 3, 24, 2, torch.float32, seed=20)
+    freqs = torch.rand(11, generator=g).cuda() * 6
+    dy = torch.randn(x.shape, generator=g).cuda()
+
+    def penalty(x, dy, turn):
+        if constant:
+            (dx,) = torch.autograd.grad((turn(x) * dy).sum(), x, create_graph=True)
+            return (turn(x) ** 3).sum() + dx.square().sum()
+        (dx,) = torch.autograd.grad((turn(x) ** 3 * dy).sum(), x, create_graph=True)
+        return dx.square().sum()
+
+    def plain(x):
+        p = pos.double().cpu()
+        angle = torch.cat([p[..., :1] * freqs[:5].double().cpu(), p[..., 1:] * freqs[5:].double().cpu()], -1)[:, :, None]
+        u, v, rest = x[..., :11], x[..., 11:22], x[..., 22:]
+        return torch.cat([u * angle.cos() - v * angle.sin(), v * angle.cos() + u * angle.sin(), rest], -1)
+
+    x.requires_grad_(True)
+    dy.requires_grad_(not constant)
+    got = torch.autograd.grad(penalty(x, dy, lambda t: rotary(t, pos, freqs, (5, 6))), [x] if constant else [x, dy])
+    rx, ry = x.detach().double().cpu().requires_grad_(True), dy.detach().double().cpu().requires_grad_(True)
+    want = torch.autograd.grad(penalty(rx, ry, plain), [rx] if constant else [rx, ry])
+    for a, b in zip(got, want):
+        assert ((a.double().cpu() - b).norm() / b.norm()).item() < 4e-6
