@@ -10,6 +10,7 @@ import ctypes as C
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libfovi_hip.so")
@@ -403,6 +404,12 @@ def require_device(*tensors):
                                "there is no CPU fallback")
 
 
+def forward_mode():
+    """Whether forward-mode differentiation is on. The kernels would drop a tangent; an autograd function
+    refuses it."""
+    return forward_ad._current_level >= 0
+
+
 class _Once(torch.autograd.Function):
     """The gradients ``backward(of, *grads)`` of an autograd function, as a function of ``grads`` and of the
     differentiable inputs that ``of`` kept, with no derivative of its own."""
@@ -420,6 +427,6 @@ def differentiated_once(backward, ctx, *grads):
     """``backward(ctx, *grads)`` of an autograd function whose gradients have none: whatever leads through
     them a second time raises, also where the incoming gradients are constants (the inputs that
     the function kept are enough). The guard that does it is left out where no graph is being made."""
-    if not torch.is_grad_enabled():
+    if not (torch.is_grad_enabled() or forward_mode()):
         return backward(ctx, *grads)
     return _Once.apply(backward, ctx, len(grads), *grads, *[t for t in ctx.saved_tensors if t is not None and t.requires_grad])

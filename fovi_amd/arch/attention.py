@@ -208,7 +208,7 @@ def cross_attention(q, k, v, kv_lengths=None, mask=None, scale=None):
         if mask.dtype == torch.bool:
             mask = _packed(mask, b, hq, lq, lk)
     q, k, v = _pieces(q), _pieces(k), _pieces(v)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)) or _lib.forward_mode():
         out = _CrossAttentionFn.apply(q, k, v, kv_lengths, mask, scale)
     else:
         out = _forward(q, k, v, kv_lengths, mask, scale, False)[0]

@@ -147,8 +147,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
         return y
     weight = weight if weight is None else weight.contiguous()
     bias = bias if bias is None else bias.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
+    if (torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                     or (bias is not None and bias.requires_grad))) or _lib.forward_mode():
         return _LayerNormFn.apply(x, weight, bias, float(eps))
     return _forward(x, weight, bias, eps, None)
 

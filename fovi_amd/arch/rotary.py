@@ -60,7 +60,7 @@ class _RotaryFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         positions, freqs = ctx.saved_tensors
-        call = _RotaryFn.apply if torch.is_grad_enabled() else _launch
+        call = _RotaryFn.apply if torch.is_grad_enabled() or _lib.forward_mode() else _launch
         return call(dy, positions, freqs, ctx.ends, ctx.pairing, 1 - ctx.inverse), None, None, None, None, None
 
 
@@ -106,7 +106,7 @@ def rotary(x, positions, freqs, sections, pairing="half"):
         positions = positions.contiguous()
     if freqs.dtype != torch.float32 or not freqs.is_contiguous():
         freqs = freqs.float().contiguous()
-    if torch.is_grad_enabled() and x.requires_grad:
+    if (torch.is_grad_enabled() and x.requires_grad) or _lib.forward_mode():
         return _RotaryFn.apply(x, positions, freqs, ends, _PAIRINGS[pairing], 0)
     return _launch(x, positions, freqs, ends, _PAIRINGS[pairing], 0)
 

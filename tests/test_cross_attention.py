@@ -594,3 +594,28 @@ def test_differentiating_twice_raises(constant):
         for leaf in leaves + ([] if constant else [dout]):
             with pytest.raises(RuntimeError, match="differentiated once"):
                 torch.autograd.grad(cross_attention(*leaves).sum() + dout.sum() + g.square().sum(), leaf, retain_graph=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", range(4))
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_raises(which, grad):
+    """A tangent of any input, the bias among them, is refused, not dropped; with a level open and no tangent the call
+    is the ordinary one."""
+    from torch.autograd import forward_ad
+    from fovi_amd.arch.attention import cross_attention
+    q, k, v, _, g = _inputs(1, 3, 5, 2, 2, 16, torch.float32, seed=21)
+    args = [q, k, v, torch.randn(3, 5, generator=g).cuda()]
+    want = cross_attention(*args[:3], mask=args[3])
+    if grad and which < 3:
+        args[which].requires_grad_(True)
+    leaf = args[0].detach().requires_grad_(True)
+    y = cross_attention(leaf, *args[1:3], mask=args[3])
+    with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward mode"):
+        torch.autograd.grad(y, leaf, forward_ad.make_dual(torch.ones_like(want), torch.ones_like(want)))
+    with forward_ad.dual_level():
+        assert torch.equal(cross_attention(*args[:3], mask=args[3]), want)
+        args[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+        for off in (False, True):
+            with torch.set_grad_enabled(not off), pytest.raises(NotImplementedError, match="forward mode"):
+                cross_attention(*args[:3], mask=args[3])

@@ -322,3 +322,26 @@ def test_differentiating_twice_raises(constant):
         for leaf in leaves + ([] if constant else [dy]):
             with pytest.raises(RuntimeError, match="differentiated once"):
                 torch.autograd.grad(layer_norm(*leaves).sum() + dy.sum() + got.square().sum(), leaf, retain_graph=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", range(3))
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_raises(which, grad):
+    """A tangent of any input is refused, not dropped; with a level open and no tangent the call is the
+    ordinary one."""
+    from torch.autograd import forward_ad
+    from fovi_amd.arch.norm import layer_norm
+    args = [torch.randn(s, device="cuda") for s in ((4, 24), (24,), (24,))]
+    want = layer_norm(*args)
+    args[which].requires_grad_(grad)
+    leaf = args[0].detach().requires_grad_(True)
+    y = layer_norm(leaf, *args[1:])
+    with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward mode"):
+        torch.autograd.grad(y, leaf, forward_ad.make_dual(torch.ones_like(want), torch.ones_like(want)))
+    with forward_ad.dual_level():
+        assert torch.equal(layer_norm(*args), want)
+        args[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+        for off in (False, True):
+            with torch.set_grad_enabled(not off), pytest.raises(NotImplementedError, match="forward mode"):
+                layer_norm(*args)

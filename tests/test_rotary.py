@@ -295,3 +295,28 @@ def test_second_gradients(constant):
     want = torch.autograd.grad(penalty(rx, ry, plain), [rx] if constant else [rx, ry])
     for a, b in zip(got, want):
         assert ((a.double().cpu() - b).norm() / b.norm()).item() < 4e-6
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", range(3))
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_raises(which, grad):
+    """A tangent of any input, positions and frequencies among them, is refused, not dropped; with a level open and
+    no tangent the call is the ordinary one."""
+    from torch.autograd import forward_ad
+    from fovi_amd.arch.rotary import rotary
+    x, pos, g = _inputs(1, 4, 2, 16, 2, torch.float32, seed=21)
+    args = [x, pos, torch.rand(8, generator=g).cuda()]
+    want = rotary(*args, (4, 4))
+    if grad and which == 0:
+        x.requires_grad_(True)
+    leaf = args[0].detach().requires_grad_(True)
+    y = rotary(leaf, *args[1:], (4, 4))
+    with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward mode"):
+        torch.autograd.grad(y, leaf, forward_ad.make_dual(torch.ones_like(want), torch.ones_like(want)))
+    with forward_ad.dual_level():
+        assert torch.equal(rotary(*args, (4, 4)), want)
+        args[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+        for off in (False, True):
+            with torch.set_grad_enabled(not off), pytest.raises(NotImplementedError, match="forward mode"):
+                rotary(*args, (4, 4))
