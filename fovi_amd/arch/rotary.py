@@ -115,7 +115,7 @@ class AxialRotary(nn.Module):
     """``rotary`` with its frequencies: axis a of n pairs has ``scale / base ** (j / n)``, j = 0 .. n-1.
 
     ``sections`` defaults to two axes over the whole head; ``base`` and ``scale`` are one value or
-    one per axis.
+    one per axis. The frequencies stay in fp32 when the module is converted to another type.
     """
 
     def __init__(self, head_dim, sections=None, base=100.0, scale=2 * math.pi, pairing="half", device="cuda"):
@@ -135,6 +135,13 @@ class AxialRotary(nn.Module):
         freqs = [scale[a] * float(base[a]) ** (-j / n) for a, n in enumerate(self.sections) for j in range(n)]
         self.register_buffer("freqs", torch.tensor(freqs, dtype=torch.float64, device="cpu").float().to(device),
                              persistent=False)
+
+    def _apply(self, fn, recurse=True):
+        freqs = self.freqs
+        super()._apply(fn, recurse)
+        if self.freqs.dtype != torch.float32:           # .bfloat16() and the like convert parameters; rounded
+            self.freqs = freqs.to(self.freqs.device)    # frequencies would turn by other angles
+        return self
 
     def forward(self, x, positions):
         if x.shape[-1] != self.head_dim:

@@ -320,3 +320,23 @@ def test_forward_mode_raises(which, grad):
         for off in (False, True):
             with torch.set_grad_enabled(not off), pytest.raises(NotImplementedError, match="forward mode"):
                 rotary(*args, (4, 4))
+
+
+@pytest.mark.parametrize("convert", [lambda m: m.bfloat16(), lambda m: m.half(), lambda m: m.to(torch.bfloat16), lambda m: m.double(),
+                                     lambda m: torch.nn.Sequential(m).bfloat16()[0]])
+def test_converted_modules_keep_their_frequencies(convert):
+    """A reader in bf16 turns its heads as it did in fp32: frequencies are not parameters to be rounded."""
+    from fovi_amd.arch.rotary import AxialRotary
+    want = AxialRotary(64, (8, 12, 12), device="cpu").freqs
+    got = convert(AxialRotary(64, (8, 12, 12), device="cpu")).freqs
+    assert got.dtype == torch.float32 and torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_converted_modules_turn_alike():
+    from fovi_amd.arch.rotary import AxialRotary
+    x, pos, _ = _inputs(2, 30, 3, 64, 3, torch.bfloat16, seed=22, spread=20.0)
+    rope = AxialRotary(64, (8, 12, 12), device="cpu")
+    want = rope.cuda()(x, pos)
+    assert rope.freqs.is_cuda and torch.equal(rope.bfloat16()(x, pos), want)
+    assert list(rope.state_dict()) == []
