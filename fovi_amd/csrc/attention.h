@@ -322,9 +322,18 @@ __device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// KIND of a kernel: 0 no mask, 1 bits of states to keep, 2 a bias. A masked score is in units of log2,
-// -inf where a pair is left out.
-//
+// KIND of a kernel: 0 no mask, 1 bits of states to keep, 2 a bias. A masked score is -inf where a pair is left
+// out; else it is in units of log2 under KIND 1, so that exponentials take it as it is, and in those of the bias
+// under KIND 2: biases up to the type's limits are numbers there, and differences among them count (times
+// log2(e) they would overflow). unit<KIND>(p) is what a difference of such scores (KIND 0: of products q.k) is
+// multiplied with for exp2.
+template <int KIND> __device__ __forceinline__ float unit(const AttnParams& p) { return KIND == 0 ? p.c : KIND == 1 ? 1.0f : kLog2e; }
+
+// exp2((s - top) unit), top finite. Under a bias the difference comes first: top * unit may pass the type's limits.
+template <int KIND> __device__ __forceinline__ float exp2_below(float s, float top, float c) {
+  return exp2_fast(KIND == 2 ? (s - top) * c : fmaf(s, c, -top * c));
+}
+
 // Where a block's columns are query rows, a lane has the word of its row and the block's 32 states; the
 // pairs are its bits 8 (i / 4) + 4 half + i % 4.
 __device__ __forceinline__ void keep_block(const AttnParams& p, uint32_t word, f32x16& s) {
@@ -334,8 +343,7 @@ __device__ __forceinline__ void keep_block(const AttnParams& p, uint32_t word, f
 }
 
 __device__ __forceinline__ float biased(const AttnParams& p, float bias, float s) {
-  // (the type's lowest value times log2(e) is still a number: rows of nothing else read all alike)
-  return bias == kNegInf ? kNegInf : fmaf(s, p.c, fmaxf(bias * kLog2e, -3.402823466e38f));
+  return bias == kNegInf ? kNegInf : fmaf(s, p.scale, bias);
 }
 
 // A bias over a lane's 16 pairs: states j0 + 8 (i / 4) + i % 4 of its row (j0 holds the half; n states in all)...

@@ -12,7 +12,7 @@
 
 namespace fovi {
 
-// What a row's probabilities need: exp2(t - shift) * factor. Without a bias the log of the sum goes
+// What a row's probabilities need: exp2((t - shift) unit) * factor. Without a mask the log of the sum goes
 // into the shift (factor 1). A row that keeps nothing has shift +inf: probabilities 0.
 struct RowStat { float shift, factor, delta; };
 template <int KIND>
@@ -26,7 +26,7 @@ template <int KIND>
 __device__ __forceinline__ void pair_grad(float t, float c, float shift, float factor, float dp, float& e, float& ds) {
   if (KIND) {
     const bool out = t == kNegInf || shift == __builtin_inff();
-    e = exp2_fast(t - shift) * factor;
+    e = exp2_fast(KIND == 2 ? (t - shift) * kLog2e : t - shift) * factor;
     ds = out ? kLeftOut : e * dp;
     e = out ? kLeftOut : e;
   } else {

@@ -47,7 +47,7 @@ template <typename T, int DP, int KIND, int KB>
 __device__ __forceinline__ void softmax_blocks(const AttnParams& p, RowState<T, DP>& st, f32x16 (&s)[KB], Block<T> (&e)[KB],
                                                const uint32_t (&word)[2], int64_t j, int64_t n) {
   const int h = (threadIdx.x & 63) >> 5;
-  const float c = KIND ? 1.0f : p.c;
+  const float c = unit<KIND>(p);
   const int left = static_cast<int>(n - j < 32 * KB ? n - j : 32 * KB);
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb) {
@@ -75,13 +75,13 @@ __device__ __forceinline__ void softmax_blocks(const AttnParams& p, RowState<T, 
     for (int d = 0; d < RowState<T, DP>::DT; ++d) st.o[d] *= keep;
     st.m = top;
   }
-  const float mc = (st.m == kNegInf ? 0.0f : st.m) * c;
+  const float m = st.m == kNegInf ? 0.0f : st.m;
   float sum = 0;
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float x = exp2_fast(fmaf(s[kb][i], c, -mc));
+      const float x = exp2_below<KIND>(s[kb][i], m, c);
       s[kb][i] = KIND && s[kb][i] == kNegInf ? kLeftOut : x;
     }
     e[kb] = Block<T>(s[kb]);
@@ -327,7 +327,7 @@ __global__ __launch_bounds__(256, few_waves<T>(DP, KIND)) void attn_fwd_few_kern
     float value = 0, total = 0;
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
-      const float f = exp2_fast(wm[y][r] - at);
+      const float f = exp2_fast((wm[y][r] - at) * (KIND == 2 ? kLog2e : 1.0f));
       total = fmaf(wl[y][r], f, total);
       value = fmaf(reinterpret_cast<const float*>(lds)[y * (JOIN / 4) + r * (DP + 1) + d], f, value);
     }
@@ -355,13 +355,14 @@ __global__ __launch_bounds__(256) void attn_fwd_join_kernel(AttnParams p) {
   int used = static_cast<int>((len + p.chunk - 1) / p.chunk);
   if (used < 1) used = 1;
   const float2* stats = part_stats(p) + x;
+  const float c = p.kind == FOVI_MASK_BIAS ? kLog2e : 1.0f;      // the maxima's unit
   float m = kNegInf, sum = 0;
   f32x4 y = {};
 #pragma unroll 4
   for (int s = group; s < used; s += GROUPS) {
     const float2 ml = stats[s * rows];
     const f32x4 v = d < p.D ? *reinterpret_cast<const f32x4*>(p.part + (s * rows + x) * p.D + d) : f32x4{};
-    const float top = fmaxf(m, ml.x), at = top == kNegInf ? 0.0f : top, old = exp2_fast(m - at), f = exp2_fast(ml.x - at);
+    const float top = fmaxf(m, ml.x), at = top == kNegInf ? 0.0f : top, old = exp2_fast((m - at) * c), f = exp2_fast((ml.x - at) * c);
     sum = fmaf(sum, old, ml.y * f);
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[e] = fmaf(y[e], old, v[e] * f);
@@ -377,7 +378,7 @@ __global__ __launch_bounds__(256) void attn_fwd_join_kernel(AttnParams p) {
 #pragma unroll
     for (int g = 1; g < GROUPS; ++g) {
       const float* o = sh[g][threadIdx.x & 31];
-      const float top = fmaxf(m, o[0]), at = top == kNegInf ? 0.0f : top, old = exp2_fast(m - at), f = exp2_fast(o[0] - at);
+      const float top = fmaxf(m, o[0]), at = top == kNegInf ? 0.0f : top, old = exp2_fast((m - at) * c), f = exp2_fast((o[0] - at) * c);
       sum = fmaf(sum, old, o[1] * f);
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[e] = fmaf(y[e], old, o[2 + e] * f);

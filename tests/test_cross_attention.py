@@ -619,3 +619,42 @@ def test_forward_mode_raises(which, grad):
         for off in (False, True):
             with torch.set_grad_enabled(not off), pytest.raises(NotImplementedError, match="forward mode"):
                 cross_attention(*args[:3], mask=args[3])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lq,lk", [(1, 40), (7, 70), (45, 130), (3, 9000), (45, 3000)])
+def test_extreme_biases(lq, lk, dtype):
+    """Biases of the size of the type's limits: differences among them count as any others do, and so does one
+    state with the largest value; long rows of the lowest value alone, in parts that are joined, read all alike."""
+    b, hq, hk, d = 2, 2, 1, 32
+    q, k, v, dout, g = _inputs(b, lq, lk, hq, hk, d, dtype, seed=23)
+    top = torch.finfo(torch.float32).max
+    bias = torch.full((b, hq, lq, lk), -top)
+    bias[0, 0] = -2.5e38 - 0.8e38 * torch.rand(lq, lk, generator=g)          # one state of each row is read
+    bias[0, 1] = torch.randn(lq, lk, generator=g)
+    bias[0, 1, :, lk // 2] = top
+    bias[1, 0, :, ::3] = torch.finfo(torch.bfloat16).min                     # a third of the states, alike
+    out, _ = _check(q, k, v, dout, mask=bias.cuda())
+    want = v[0, :, 0].double().cpu()[bias[0, 0].argmax(-1)]
+    assert ((out[0, :, 0].double().cpu() - want).norm() / want.norm()) < TOL[dtype]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lq,lk", [(2, 40), (45, 130), (2, 9000)])
+def test_nan_bias_is_seen(lq, lk, dtype):
+    """A bias that is not a number makes its row so, and the gradients that the row enters; other rows stay."""
+    from fovi_amd.arch.attention import cross_attention
+    q, k, v, dout, g = _inputs(1, lq, lk, 2, 2, 32, dtype, seed=24)
+    bias = torch.randn(1, 1, lq, lk, generator=g).cuda()
+    bad = bias.clone()
+    bad[..., 1, lk // 2] = float("nan")
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    out, clean = cross_attention(*leaves, mask=bad), cross_attention(*leaves, mask=bias)
+    rows = [i for i in range(lq) if i != 1]
+    assert out[:, 1].isnan().all() and torch.equal(out[:, rows], clean[:, rows])
+    dq, dk, dv = torch.autograd.grad(out, leaves, dout)
+    want = torch.autograd.grad(clean, leaves, dout)[0]
+    assert dq[:, 1].isnan().all() and torch.equal(dq[:, rows], want[:, rows])
+    assert dk.isnan().all() and dv.isnan().all()
