@@ -13,11 +13,13 @@
 namespace fovi {
 
 // What a row's probabilities need: exp2((t - shift) unit) * factor. Without a mask the log of the sum goes
-// into the shift (factor 1). A row that keeps nothing has shift +inf: probabilities 0.
+// into the shift (factor 1). A row that keeps nothing has shift +inf: probabilities 0. A row whose sum is NaN (it
+// keeps a NaN, or a score of +inf, which is its maximum then) has shift NaN, so that its gradients are NaN as well.
 struct RowStat { float shift, factor, delta; };
 template <int KIND>
 __device__ __forceinline__ RowStat row_stat(float m, float sum, float delta) {
-  return {sum == 0 ? __builtin_inff() : KIND ? m : m + log2f(sum), KIND && sum != 0 ? 1.0f / sum : KIND ? 0.0f : 1.0f, delta};
+  const float shift = KIND ? m + 0.0f * sum : m + log2f(sum);       // (0 * sum: 0, or NaN)
+  return {sum == 0 ? __builtin_inff() : shift, KIND && sum != 0 ? 1.0f / sum : KIND ? 0.0f : 1.0f, delta};
 }
 
 // Probability and score gradient of one pair, dp = do.v - delta (the product starts from -delta). Under a mask t is

@@ -658,3 +658,35 @@ def test_nan_bias_is_seen(lq, lk, dtype):
     want = torch.autograd.grad(clean, leaves, dout)[0]
     assert dq[:, 1].isnan().all() and torch.equal(dq[:, rows], want[:, rows])
     assert dk.isnan().all() and dv.isnan().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kind", ["key", "bias"])
+@pytest.mark.parametrize("lq,lk", [(2, 40), (45, 130)])
+def test_infinite_scores_have_no_gradient_of_zero(lq, lk, kind, dtype):
+    """A score of +inf that a row keeps (from a key under a boolean mask, or from a bias) leaves its output NaN, and so its
+    gradients, not zeros; rows and states that do not meet it stay as they are."""
+    from fovi_amd.arch.attention import cross_attention
+    q, k, v, dout, g = _inputs(1, lq, lk, 1, 1, 32, dtype, seed=29)
+    keep = torch.rand(lq, lk, generator=g) < 0.7
+    keep[1, :lk // 2], keep[1, lk // 2:] = True, False    # row 1 reads the first half, others all but state 3
+    keep[:, 3] = False
+    keep[1, 3] = True
+    mask = keep if kind == "key" else torch.zeros(lq, lk).masked_fill(~keep, -INF)
+    mask = mask.cuda()
+    bad, far = mask.clone(), k.clone()
+    if kind == "key":
+        far[0, 3] = INF * q[0, 1, 0].sign()
+    else:
+        bad[1, 3] = INF
+    leaves = [t.requires_grad_(True) for t in (q, far, v)]
+    out = cross_attention(*leaves, mask=bad)
+    rows = [i for i in range(lq) if i != 1]
+    mask[:, 3] = False if kind == "key" else -INF
+    assert out[:, 1].isnan().all() and torch.equal(out[:, rows], cross_attention(q, k, v, mask=mask)[:, rows])
+    dq, dk, dv = torch.autograd.grad(out, leaves, dout)
+    want = torch.autograd.grad(cross_attention(q, leaves[1], v, mask=mask), [q, v], dout)
+    assert dq[:, 1].isnan().all() and torch.equal(dq[:, rows], want[0][:, rows])
+    assert dk[:, :lk // 2].isnan().all() and dv[:, :lk // 2].isnan().all()
+    assert torch.equal(dv[:, lk // 2:], want[1][:, lk // 2:])
