@@ -259,8 +259,10 @@ __device__ __forceinline__ void slow_second(const char* tile, int base, const f3
 // keeps its 16-byte column; its place in the tile is a 32-bit offset from the tile's (uniform) address, so
 // that a full tile's loads take no vector arithmetic: on this machine matrix and vector instructions of
 // a SIMD hardly overlap, and every vector instruction of the loop adds to its time. Loads are never
-// predicated (that would wait for earlier ones): rows behind the last are the last row again, which
-// the products meet with probability 0, and which every row reads that could notice.
+// predicated (that would wait for earlier ones): rows behind the last are the last row again, which the products
+// meet with probability 0. Where an infinity in it would turn that into NaN, clear_tail() makes them zeros: without
+// a mask, for what probabilities are multiplied with (under a mask a tile with infinities leaves pairs out one by
+// one; of keys and queries an infinity is in the scores already).
 constexpr int64_t kMostPitch = int64_t(1) << 26;       // bytes between rows: 64 of them stay below 2^32
 
 template <typename T, int LP, int ROWS, int THREADS>
@@ -268,7 +270,7 @@ struct Staged {
   static constexpr int NC = LP / Chunk<T>::N, STEP = THREADS / NC, N = (ROWS + STEP - 1) / STEP;
   u32x4 r[N];
   uint32_t off, pitch, col;   // bytes
-  int row, c;
+  int row, c, last;           // last: of the rows that the tile has
   __device__ __forceinline__ void init(int64_t stride, int D, int thread) {
     row = thread / NC < ROWS ? thread / NC : ROWS - 1;
     c = thread % NC;
@@ -279,7 +281,7 @@ struct Staged {
   // rows [0, n) of `base`, n > 0
   __device__ __forceinline__ void load(const T* base, int64_t n) {
     const bool full = n >= ROWS;
-    const int last = static_cast<int>(n) - 1;
+    last = full ? ROWS - 1 : static_cast<int>(n) - 1;
     const char* at = reinterpret_cast<const char*>(base);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -294,6 +296,13 @@ struct Staged {
     if (in(D)) return;
 #pragma unroll
     for (int i = 0; i < N; ++i) *reinterpret_cast<u32x4*>(tile + tile_at<T, LP>(row + i * STEP, c)) = u32x4{0, 0, 0, 0};
+  }
+  __device__ __forceinline__ void clear_tail() {
+    if (last < ROWS - 1) [[unlikely]] {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (row + i * STEP > last) r[i] = u32x4{0, 0, 0, 0};
+    }
   }
   __device__ __forceinline__ void store(char* tile, int D) const {
     if (!in(D)) return;

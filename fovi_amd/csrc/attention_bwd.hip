@@ -257,6 +257,7 @@ __global__ __launch_bounds__(256, dkv_waves<T>(DP, KIND)) void attn_dkv_kernel(A
   };
   auto put = [&](int buf, int tile) {
     qr.store(tiles[buf][0], p.D);
+    if (!KIND) gr.clear_tail();
     gr.store(tiles[buf][1], p.D);
     if (threadIdx.x < RT) {
       const RowStat sr = row_stat<KIND>(m, sum, sum == 0 ? 0.0f : delta);

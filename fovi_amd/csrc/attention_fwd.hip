@@ -149,6 +149,7 @@ __global__ __launch_bounds__(256, tile_waves<T>(DP, KIND)) void attn_fwd_tile_ke
   };
   auto put = [&](int buf, int tile) {
     kr.store(tiles[buf][0], p.D);
+    if (!KIND) vr.clear_tail();
     vr.store(tiles[buf][1], p.D);
     if (KIND && vr.bad()) bad_tile[buf] = tile;
   };
@@ -294,6 +295,7 @@ __global__ __launch_bounds__(256, few_waves<T>(DP, KIND)) void attn_fwd_few_kern
     Turned<T, LP> va[DT];
 #pragma unroll
     for (int t = 0; t < STEPS; ++t) s[0] = mma_step(T(), ka[t], st.q[t], s[0]);
+    if (!KIND) vr.clear_tail();
     vr.store(vt, p.D);                     // the wave's own tile: LDS serves a wave's accesses in order
     __builtin_amdgcn_wave_barrier();
     const bool bad = KIND && __any(vr.bad());

@@ -690,3 +690,29 @@ def test_infinite_scores_have_no_gradient_of_zero(lq, lk, kind, dtype):
     assert dq[:, 1].isnan().all() and torch.equal(dq[:, rows], want[0][:, rows])
     assert dk[:, :lk // 2].isnan().all() and dv[:, :lk // 2].isnan().all()
     assert torch.equal(dv[:, lk // 2:], want[1][:, lk // 2:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+@pytest.mark.parametrize("lq,lk", [(1, 1), (1, 65), (45, 33), (150, 127), (3, 1000)])
+def test_infinities_at_the_last_place(lq, lk, d, dtype):
+    """No mask, and an infinite value in the last state (behind which a tile has nothing more): outputs of that
+    element are infinite, not NaN, all others as without it. The same of the last query's incoming gradient and dv."""
+    from fovi_amd.arch.attention import cross_attention
+    q, k, v, dout, _ = _inputs(2, lq, lk, 2, 2, d, dtype, seed=25)
+    lengths = torch.tensor([lk, max(1, lk - 30)], device="cuda")
+    other = [0] + list(range(2, d))
+    want = cross_attention(q, k, v, kv_lengths=lengths)
+    far = v.clone()
+    for i, n in enumerate(lengths.tolist()):
+        far[i, n - 1, :, 1] = INF
+    out = cross_attention(q, k, far, kv_lengths=lengths)
+    assert (out[..., 1] == INF).all() and torch.equal(out[..., other], want[..., other])
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    want = torch.autograd.grad(cross_attention(*leaves, kv_lengths=lengths), leaves, dout)[2]
+    dout[:, -1, :, 1] = -INF
+    dv = torch.autograd.grad(cross_attention(*leaves, kv_lengths=lengths), leaves, dout)[2]
+    for i, n in enumerate(lengths.tolist()):
+        assert (dv[i, :n, :, 1] == -INF).all() and not dv[i, n:].any()
+    assert torch.equal(dv[..., other], want[..., other])
