@@ -193,7 +193,7 @@ def cross_attention(q, k, v, kv_lengths=None, mask=None, scale=None):
         if kv_lengths.stride(0) != 1:
             kv_lengths = kv_lengths.contiguous()
     if mask is not None:
-        if mask.requires_grad:
+        if mask.requires_grad and torch.is_grad_enabled():
             raise ValueError("cross_attention: no gradient for the mask")
         if mask.device != q.device:
             raise ValueError("cross_attention: mask must be on the device of q")

@@ -96,7 +96,7 @@ def rotary(x, positions, freqs, sections, pairing="half"):
     want = (x.shape[1], axes)
     if tuple(positions.shape) not in (want, (x.shape[0],) + want):
         raise ValueError(f"rotary: positions of shape {tuple(positions.shape)} for tokens {tuple(x.shape[:2])} and {axes} axes")
-    if positions.requires_grad or freqs.requires_grad:
+    if (positions.requires_grad or freqs.requires_grad) and torch.is_grad_enabled():
         raise ValueError("rotary: no gradient for positions or frequencies")
     if positions.device != x.device or freqs.device != x.device:
         raise ValueError("rotary: positions and freqs must be on the device of x")

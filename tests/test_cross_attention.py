@@ -716,3 +716,18 @@ def test_infinities_at_the_last_place(lq, lk, d, dtype):
     for i, n in enumerate(lengths.tolist()):
         assert (dv[i, :n, :, 1] == -INF).all() and not dv[i, n:].any()
     assert torch.equal(dv[..., other], want[..., other])
+
+
+@pytest.mark.gpu
+def test_learned_bias_without_gradients():
+    """A bias that is a parameter (learned elsewhere) is taken where no gradient is asked for."""
+    from fovi_amd.arch.attention import cross_attention
+    q, k, v, _, g = _inputs(1, 5, 9, 2, 2, 16, torch.float32, seed=26)
+    bias = torch.nn.Parameter(torch.randn(2, 5, 9, generator=g).cuda())
+    want = cross_attention(q, k, v, mask=bias.detach())
+    with torch.no_grad():
+        assert torch.equal(cross_attention(q, k, v, mask=bias), want)
+    with torch.inference_mode():
+        assert torch.equal(cross_attention(q, k, v, mask=bias), want)
+    with pytest.raises(ValueError, match="no gradient"):
+        cross_attention(q, k, v, mask=bias)

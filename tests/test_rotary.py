@@ -340,3 +340,18 @@ def test_converted_modules_turn_alike():
     want = rope.cuda()(x, pos)
     assert rope.freqs.is_cuda and torch.equal(rope.bfloat16()(x, pos), want)
     assert list(rope.state_dict()) == []
+
+
+@pytest.mark.gpu
+def test_learned_positions_without_gradients():
+    """Positions and frequencies that are parameters are taken where no gradient is asked for."""
+    from fovi_amd.arch.rotary import rotary
+    x, pos, g = _inputs(2, 5, 3, 32, 2, torch.float32, seed=23)
+    freqs = torch.rand(16, generator=g).cuda()
+    want = rotary(x, pos, freqs, (8, 8))
+    pos, freqs = torch.nn.Parameter(pos), torch.nn.Parameter(freqs)
+    for args in ((x, pos, freqs.detach(), (8, 8)), (x, pos.detach(), freqs, (8, 8))):
+        with torch.no_grad():
+            assert torch.equal(rotary(*args), want)
+        with pytest.raises(ValueError, match="no gradient"):
+            rotary(*args)
