@@ -8,6 +8,8 @@ the block with them and the number of states that each image has so far.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 import torch.nn as nn
 
@@ -32,10 +34,13 @@ class FixationReader(nn.Module):
     queries that have one).
 
     ``sections``: pairs per axis of a head (fixation number, row, column), by default a quarter of
-    the pairs and the rest in two halves. ``kv_heads`` < ``heads`` shares key heads.
+    the pairs and the rest in two halves. ``base`` and ``scale`` as in ``AxialRotary``; by default row and
+    column, in [-1, 1], turn by 2 pi at most, and fixations, counted in whole numbers, by one radian each (whole
+    turns would tell none apart). ``kv_heads`` < ``heads`` shares key heads.
     """
 
-    def __init__(self, dim, state_dim, heads, head_dim=64, kv_heads=None, sections=None, base=100.0, device="cuda"):
+    def __init__(self, dim, state_dim, heads, head_dim=64, kv_heads=None, sections=None, base=100.0, device="cuda",
+                 scale=None):
         super().__init__()
         kv_heads = heads if kv_heads is None else kv_heads
         if heads % kv_heads:
@@ -43,12 +48,14 @@ class FixationReader(nn.Module):
         if sections is None:
             row = (head_dim // 2 - head_dim // 8) // 2
             sections = (head_dim // 2 - 2 * row, row, row)
+        if scale is None:
+            scale = (1.0, 2 * math.pi, 2 * math.pi) if len(sections) == 3 else 2 * math.pi
         self.dim, self.state_dim, self.heads, self.kv_heads, self.head_dim = dim, state_dim, heads, kv_heads, head_dim
         self.norm, self.state_norm = LayerNorm(dim, device=device), LayerNorm(state_dim, device=device)
         self.to_q = nn.Linear(dim, heads * head_dim, bias=False, device=device)
         self.to_kv = nn.Linear(state_dim, 2 * kv_heads * head_dim, bias=False, device=device)
         self.to_out = nn.Linear(heads * head_dim, dim, device=device)
-        self.rotary = AxialRotary(head_dim, sections, base=base, device=device)
+        self.rotary = AxialRotary(head_dim, sections, base=base, scale=scale, device=device)
 
     def project(self, states, positions):
         """Keys and values ``[B, S, kv_heads, head_dim]`` of ``states [B, S, state_dim]`` at ``positions

@@ -1,4 +1,6 @@
 """FixationReader: the three operators together, from sampled fixations to gradients and to serving steps."""
+import math
+
 import pytest
 import torch
 
@@ -111,3 +113,20 @@ def test_refusals():
             reader(x, **kw)
     with pytest.raises(ValueError):
         FixationReader(16, 16, heads=3, kv_heads=2)
+
+
+def test_every_pair_tells_fixations_apart():
+    """Fixations are numbered 0, 1, 2, ...: no pair of that axis turns by whole turns between two of the first 20
+    (in fp64; the nearest pair of angles is more than 1e-3 of a turn from one another)."""
+    from fovi_amd.arch.reader import FixationReader
+    for head_dim in (32, 64, 128):
+        rope = FixationReader(16, 16, heads=2, head_dim=head_dim, device="cpu").rotary
+        turns = torch.arange(20).double()[:, None] * rope.freqs[:rope.sections[0]].double() / (2 * math.pi)
+        apart = (turns[:, None] - turns[None] + 0.5) % 1 - 0.5
+        assert (apart.abs() + torch.eye(20)[..., None]).min() > 1e-3
+    # row and column stay in [-1, 1]: two pi, as the default of the two-axis positions
+    assert rope.freqs[rope.sections[0]] == torch.tensor(2 * math.pi)
+    same = FixationReader(16, 16, heads=2, scale=2 * math.pi, device="cpu").rotary.freqs
+    assert same[0] == torch.tensor(2 * math.pi)
+    two = FixationReader(16, 16, heads=2, head_dim=32, sections=(8, 8), device="cpu").rotary
+    assert two.freqs[0] == two.freqs[8] == torch.tensor(2 * math.pi)
