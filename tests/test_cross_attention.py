@@ -731,3 +731,48 @@ def test_learned_bias_without_gradients():
         assert torch.equal(cross_attention(q, k, v, mask=bias), want)
     with pytest.raises(ValueError, match="no gradient"):
         cross_attention(q, k, v, mask=bias)
+
+
+def _poison():
+    """Leaves NaN in the allocator's free memory, where the next workspaces come from."""
+    torch.cuda.synchronize()
+    held = [torch.full((1 << 26,), float("nan"), device="cuda")]
+    held += [torch.full((1 << n,), float("nan"), device="cuda") for n in range(8, 19) for _ in range(4)]
+    torch.cuda.synchronize()
+    del held
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kind", ["none", "bool", "bias"])
+@pytest.mark.parametrize("lq,lk,hq,hk", [(1, 3000, 1, 1), (45, 3000, 2, 1), (45, 3000, 6, 6), (3, 3000, 6, 6), (2, 9000, 2, 1),
+                                         (200, 3000, 2, 2)])
+def test_lengths_that_end_before_later_parts(lq, lk, hq, hk, kind, dtype):
+    """States split over workgroups (joins of fewer than 16 parts and of more) and images that have none, one, one
+    part, whole parts and a state, half or all of them: parts that an image does not have are not read."""
+    from fovi_amd.arch.attention import cross_attention
+    lengths = torch.tensor([0, 1, 128, 513, lk // 2, lk])
+    q, k, v, dout, g = _inputs(6, lq, lk, hq, hk, 32, dtype, seed=27)
+    mask = None
+    if kind != "none":
+        mask = torch.rand(lq, lk, generator=g) < 0.8
+        mask[lq // 2] = False
+        if kind == "bias":
+            mask = torch.randn(lq, lk, generator=g).masked_fill(~mask, -INF)
+        mask = mask.cuda()
+    kw = dict(kv_lengths=lengths.cuda(), mask=mask)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    _poison()
+    plain = cross_attention(q, k, v, **kw)
+    _poison()
+    out = cross_attention(*leaves, **kw)
+    _poison()
+    grads = torch.autograd.grad(out, leaves, dout)
+    want = _reference(q, k, v, lengths, mask, None, dout)
+    _close(plain, want[0], TOL[dtype], "out without gradients")
+    _close(out, want[0], TOL[dtype], "out")
+    for name, got, ref, terms in zip(("dq", "dk", "dv"), grads, want[1:4], (want[4], want[5], 0.0)):
+        _close(got, ref, TOL[dtype], name, TERMS[dtype] * terms)
+    assert not out[0].any() and not grads[0][0].any()
+    for i, n in enumerate(lengths.tolist()):
+        assert not grads[1][i, n:].any() and not grads[2][i, n:].any()
