@@ -776,3 +776,40 @@ def test_lengths_that_end_before_later_parts(lq, lk, hq, hk, kind, dtype):
     assert not out[0].any() and not grads[0][0].any()
     for i, n in enumerate(lengths.tolist()):
         assert not grads[1][i, n:].any() and not grads[2][i, n:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lq", [2, 50])
+def test_capture_with_gradients(lq, dtype):
+    """Forward under a mask and backward, captured; replayed with new inputs and with work of its own between."""
+    from fovi_amd.arch.attention import cross_attention
+    q, k, v, dout, g = _inputs(2, lq, 700, 4, 2, 64, dtype, seed=28)
+    mask = (torch.rand(lq, 700, generator=g) < 0.7).cuda()
+    lengths = torch.tensor([700, 130], device="cuda", dtype=torch.int32)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+
+    def step():
+        out = cross_attention(*leaves, kv_lengths=lengths, mask=mask)
+        return (out.detach(),) + torch.autograd.grad(out, leaves, dout)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(4):
+        with torch.no_grad():
+            for t in leaves + [dout]:
+                t.copy_(torch.randn(t.shape, generator=g))
+            lengths.copy_(torch.tensor([700 - 100 * i, 33 * i]))
+            mask.copy_(torch.rand(mask.shape, generator=g) < 0.7)
+        want = step()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), i

@@ -345,3 +345,38 @@ def test_forward_mode_raises(which, grad):
         for off in (False, True):
             with torch.set_grad_enabled(not off), pytest.raises(NotImplementedError, match="forward mode"):
                 layer_norm(*args)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,c", [(5, 48), (5000, 385), (9, 20000)])
+def test_capture(rows, c, dtype):
+    """Forward and backward captured; replayed with new inputs and with work of its own between."""
+    from fovi_amd.arch.norm import layer_norm
+    g = torch.Generator().manual_seed(21)
+    leaves = [torch.randn(rows, c, generator=g).to(dtype).cuda().requires_grad_(True)]
+    leaves += [torch.randn(c, generator=g).cuda().requires_grad_(True) for _ in range(2)]
+    dy = torch.randn(rows, c, generator=g).to(dtype).cuda()
+
+    def step():
+        y = layer_norm(*leaves)
+        return (y.detach(),) + torch.autograd.grad(y, leaves, dy)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(4):
+        with torch.no_grad():
+            for t in leaves + [dy]:
+                t.copy_(torch.randn(t.shape, generator=g))
+        want = step()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), i

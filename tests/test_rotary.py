@@ -355,3 +355,38 @@ def test_learned_positions_without_gradients():
             assert torch.equal(rotary(*args), want)
         with pytest.raises(ValueError, match="no gradient"):
             rotary(*args)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("pairing", ["half", "adjacent"])
+def test_capture(pairing, dtype):
+    """Both directions captured; replayed with new inputs and positions and with work of its own between."""
+    from fovi_amd.arch.rotary import rotary
+    x, pos, g = _inputs(3, 70, 4, 64, 3, dtype, seed=24)
+    freqs = torch.rand(32, generator=g).cuda() * 6
+    dy = torch.randn(x.shape, generator=g).to(dtype).cuda()
+    x.requires_grad_(True)
+
+    def step():
+        y = rotary(x, pos, freqs, (8, 12, 12), pairing)
+        return (y.detach(),) + torch.autograd.grad(y, x, dy)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(4):
+        with torch.no_grad():
+            for t in (x, dy, pos):
+                t.copy_(torch.randn(t.shape, generator=g))
+        want = step()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), i
