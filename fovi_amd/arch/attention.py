@@ -5,6 +5,12 @@ fixations, or tokens over themselves. Several query heads may share a key head. 
 matrix that keeps no state gives zeros and passes no gradient; what lies in places that a length or
 a mask leaves out has no effect, infinities and NaN included. Scores, softmax statistics and sums
 are fp32; the sums are in a fixed order, so the same inputs give the same bits.
+
+With bf16 inputs the matrix products take bf16 on both sides: probabilities are rounded to it before the
+products with ``v`` and with the incoming gradient, score gradients before those with ``k`` and ``q`` (2^-9
+of each value at most), and the part of the output that its rounding takes away is kept for the backward in
+bf16. Outputs of normal inputs were 0.0019 to 0.0024 off the exact ones (norm of the difference over the
+norm), where fp32 probabilities give 0.0017, most of it the rounding of the output itself.
 """
 from __future__ import annotations
 
@@ -161,7 +167,8 @@ def cross_attention(q, k, v, kv_lengths=None, mask=None, scale=None):
     ``kv_lengths [B]`` (integers on the device): image b has only its first ``kv_lengths[b]`` states.
     ``mask``, broadcastable to ``[B, Hq, Lq, Lk]``: boolean, True where a row may read a state, or a
     float bias added to the scores (-inf leaves a state out). ``scale`` defaults to D ** -0.5.
-    Differentiable once in ``q``, ``k`` and ``v``.
+    Differentiable once in ``q``, ``k`` and ``v``. bf16 inputs: probabilities and score gradients are rounded to
+    bf16 before their products.
     """
     _lib.require_device(q, k, v, kv_lengths, mask)
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:

@@ -46,7 +46,7 @@ template <typename T> constexpr int dkv_waves(int DP, int KIND) {
 }
 
 // As the forward's tile kernel, with three products a pair: 1024 rows x 4096 states x 192 bf16 heads of 64 in
-// 375 us (825 TFLOP/s), matrix unit busy 48 % of the cycles, vector unit 61 %.
+// 366 us (845 TFLOP/s), matrix unit busy 48 % of the cycles, vector unit 61 % (some of both at once).
 template <typename T, int DP, int KIND>
 __global__ __launch_bounds__(256, dq_waves<T>(DP, KIND)) void attn_dq_kernel(AttnParams p) {
   constexpr int LP = DP == 96 ? 128 : DP, KB = sizeof(T) == 2 ? 2 : 1, KT = 32 * KB, DT = DP / 32, STEPS = DP / (2 * Chunk<T>::N);
@@ -191,8 +191,8 @@ __global__ __launch_bounds__(256, dq_waves<T>(DP, KIND)) void attn_dq_kernel(Att
 // Blocks of 32 rows in a tile of the dk, dv kernel.
 template <typename T> constexpr int dkv_blocks(int DP) { return sizeof(T) == 2 && DP <= 64 ? 2 : 1; }
 
-// Four products a pair: the same sizes in 555 us (742 TFLOP/s), matrix unit busy 40 % of the cycles and vector
-// unit 40 %. Keys, values and both gradients of 32 states hold 160 registers a lane for heads of 64, so that only
+// Four products a pair: the same sizes in 560 us (736 TFLOP/s), matrix unit busy 40 % of the cycles and vector
+// unit 40 %, a fifth of them neither. Keys, values and both gradients of 32 states hold 160 registers a lane for heads of 64, so that only
 // two waves share a SIMD and not every latency is hidden (lone waves, for wider heads, hide less).
 template <typename T, int DP, int KIND>
 __global__ __launch_bounds__(256, dkv_waves<T>(DP, KIND)) void attn_dkv_kernel(AttnParams p) {

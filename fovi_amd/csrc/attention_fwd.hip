@@ -108,15 +108,15 @@ template <typename T> constexpr int few_waves(int DP, int KIND) {
   return sizeof(T) == 2 ? (DP >= 96 ? 1 : 2) : (DP >= 96 || (KIND && DP == 64) ? 1 : 2);
 }
 
-// Bound by the matrix and the vector instructions of a SIMD, which hardly overlap on this machine: of 1024
-// rows x 4096 states x 192 bf16 heads of 64 (325 us, 634 TFLOP/s) the matrix unit is busy 35 % of the cycles
+// Bound by the matrix and the vector instructions of a SIMD, which hardly overlap here: of 1024
+// rows x 4096 states x 192 bf16 heads of 64 (319 us, 646 TFLOP/s) the matrix unit is busy 35 % of the cycles
 // and the vector unit 58 % (an exponential takes as long as two or three other instructions). A loop of the same
 // instructions on registers alone takes 250 us; staging the tiles costs most of the rest. Two row blocks a
 // wave would stage and read half as much, but leave two waves a SIMD instead of three: 359 us where one
 // block takes 347 (52 and 63 us for 384 x 768 x 384). Asynchronous loads into LDS were no way out either: every
 // LDS read then waits for all of them. Few rows are bound by memory: 4 rows of 16 heads over 131072 states of 4
-// key heads of 128 take 44 us (268 MB, 6.1 TB/s), one row of 128 images over 256 to 5120 states, 6 heads of 64,
-// 117 us (528 MB, 4.5 TB/s; a copy of this size reaches 4.9).
+// key heads of 128 take 43 us (268 MB, 6.2 TB/s), one row of 128 images over 256 to 5120 states, 6 heads of 64,
+// 116 us (528 MB, 4.6 TB/s; a copy of this size reaches 4.9).
 template <typename T, int DP, int KIND>
 __global__ __launch_bounds__(256, tile_waves<T>(DP, KIND)) void attn_fwd_tile_kernel(AttnParams p) {
   constexpr int LP = DP == 96 ? 128 : DP, KB = sizeof(T) == 2 ? 2 : 1, KT = 32 * KB, DT = DP / 32;
@@ -257,7 +257,7 @@ __device__ __forceinline__ void put_row(const AttnParams& p, int64_t b, int hk, 
 }
 
 // Every key and value is read once, for all rows of its key head. 64 images, 2048 states, 6 heads of 64: 403 MB
-// of fp32 in 106 us, 3.8 TB/s, with the products of a whole block of rows however few there are.
+// of fp32 in 104 us, 3.9 TB/s, with the products of a whole block of rows however few there are.
 template <typename T, int DP, int KIND>
 __global__ __launch_bounds__(256, few_waves<T>(DP, KIND)) void attn_fwd_few_kernel(AttnParams p) {
   constexpr int LP = DP == 96 ? 128 : DP, DT = DP / 32, STEPS = RowState<T, DP>::STEPS;
@@ -421,7 +421,7 @@ int attn_pack_launch(const void* keep, const int64_t* stride, int64_t n0, int64_
   return check_launch("fovi_attention_pack_mask");
 }
 
-// How a call is laid out. Few rows: every workgroup has them all. Else tiles of 128 or 256 rows.
+// How a call is laid out. Few rows: every workgroup has them all. Else tiles of 128 rows.
 struct FwdPlan {
   bool few;
   int splits;
@@ -438,13 +438,16 @@ static FwdPlan fwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk
   FwdPlan f;
   const int64_t R = H / Hk * Lq;
   // Few rows of fp32, whose products are slow (four waves share them: 64 x 6 heads of 64, one row over 2048
-  // states: 106 us and a join of 6, by tiles 168), or under a mask (bf16, the same sizes: 40 + 5, by tiles 61).
+  // states: 104 us and a join of 5, by tiles 168), or under a mask (bf16, the same sizes: 40 + 5, by tiles 61).
   // Plain bf16 rows go by tiles, whose one wave keeps up with memory (128 images, 256 to 5120 states: 117 us, 125 +
   // 5 here; 131072 states, 4 key heads of 128: 44, 51 here).
   f.few = R <= 32 && (dtype == FOVI_F32 || mask);
   f.tiles = f.few ? 1 : (R + 127) / 128;
-  // The states are split until the card is full (few rows of many key heads: twice, since lengths
-  // differ), in parts that are still worth a workgroup's start and the join: 512 states for few rows (where a
+  // The states are split until the card is full, few rows of 64 key heads and images or more twice, since lengths
+  // differ then and a last round of workgroups costs less (32 images of 256 to 5120 states, 6 heads of 64, fp32: 85 us,
+  // filled once 122; all of 5120: 115 and 139; but 8 images of 9000 states and 8 heads: 77 and 72). Below that once
+  // (4 images of 9000 states, 8 heads of 64, fp32: 44 us, twice 47; 131072 states, 4 heads of 128: 126 and 142). Parts
+  // are still worth a workgroup's start and the join: 512 states for few rows (where a
   // wave a SIMD is all there is, 9000 fp32 states and 32 heads of 80: 8 parts 57 us, 4 98), 128 for tiles (515
   // states, 32 groups, fp32 under a mask: parts of 128 14 us, of 256 23; the join 5 each).
   const int waves = f.few ? few_waves_at(dtype, D, mask) : 2;

@@ -828,13 +828,15 @@ int fovi_rotary(const fovi_rotary_args* args, void* stream);
  * or a length leaves out have no effect, infinities and NaN included.
  * mask_kind: FOVI_MASK_NONE; FOVI_MASK_KEEP, uint32 words of fovi_attention_pack_mask, bit j % 32 of word
  * j / 32 set where state j is read, strides [batch, head, query] in words (the fourth unused);
- * FOVI_MASK_BIAS, fp32 added to the scores, strides [batch, head, query, state] in elements. Strides
+ * FOVI_MASK_BIAS, fp32 added to the scores (any value: NaN makes its row NaN), strides [batch, head, query, state] in elements. Strides
  * are 0 where the mask is broadcast. kv_lengths: int32
  * [batch] on the device, NULL for kv_len; taken as within [0, kv_len].
  * dtype F32 or BF16 for q, k, v, out and the gradients; strides [batch, token, head], head elements
  * adjacent, every head of whole 16-byte pieces at a 16-byte aligned address, tokens less than 64 MiB
  * apart (the tensors may be of any size); head_dim up to 128;
- * scale > 0. Scores, statistics and sums are fp32.
+ * scale > 0. Scores, statistics and sums are fp32. With BF16 the matrix products take bf16 on both sides:
+ * probabilities are rounded to it (to nearest even) before the products with v and dout, score gradients
+ * before those with k and q.
  * stats [2, batch, heads, q_len]: each row's largest score and its sum of exponentials below it (units
  * of the library's own; apart, because the log of the sum vanishes beside a bias of the type's lowest
  * value); NULL if no backward follows. out_rest (BF16; NULL if no backward follows): what the rounding of out took
