@@ -411,12 +411,12 @@ def forward_mode():
 
 
 class _Once(torch.autograd.Function):
-    """The gradients ``backward(of, *grads)`` of an autograd function, as a function of ``grads`` and of the
-    differentiable inputs that ``of`` kept, with no derivative of its own."""
+    """The gradients ``backward(of, saved, *grads)`` of an autograd function, as a function of ``grads`` and of the
+    differentiable tensors among ``saved``, with no derivative of its own."""
 
     @staticmethod
-    def forward(ctx, backward, of, n, *args):
-        return backward(of, *args[:n])
+    def forward(ctx, backward, of, saved, n, *args):
+        return backward(of, saved, *args[:n])
 
     @staticmethod
     def backward(ctx, *grads):
@@ -424,9 +424,11 @@ class _Once(torch.autograd.Function):
 
 
 def differentiated_once(backward, ctx, *grads):
-    """``backward(ctx, *grads)`` of an autograd function whose gradients have none: whatever leads through
-    them a second time raises, also where the incoming gradients are constants (the inputs that
-    the function kept are enough). The guard that does it is left out where no graph is being made."""
+    """``backward(ctx, saved, *grads)``, with the tensors that ``ctx`` kept, of an autograd function whose gradients
+    have none: whatever leads through them a second time raises, also where the incoming gradients are constants
+    (the inputs that the function kept are enough). The guard that does it is left out where no graph is
+    being made. The kept tensors are asked for once: a checkpointed block recomputes them for one reading."""
+    saved = ctx.saved_tensors
     if not (torch.is_grad_enabled() or forward_mode()):
-        return backward(ctx, *grads)
-    return _Once.apply(backward, ctx, len(grads), *grads, *[t for t in ctx.saved_tensors if t is not None and t.requires_grad])
+        return backward(ctx, saved, *grads)
+    return _Once.apply(backward, ctx, saved, len(grads), *grads, *[t for t in saved if t is not None and t.requires_grad])

@@ -120,8 +120,8 @@ def _forward(q, k, v, kv_lengths, mask, scale, keep):
     return out, stats, rest
 
 
-def _backward(ctx, dout):
-    q, k, v, kv_lengths, mask, out, stats, rest = ctx.saved_tensors
+def _backward(ctx, saved, dout):
+    q, k, v, kv_lengths, mask, out, stats, rest = saved
     dq, dk, dv = _like(q), _like(k), _like(v)
     if q.numel() == 0:
         return dq, dk.zero_(), dv.zero_(), None, None, None

@@ -57,8 +57,8 @@ def _forward(x, weight, bias, eps, stats):
     return y
 
 
-def _backward(ctx, dy):
-    x, weight, bias, stats = ctx.saved_tensors
+def _backward(ctx, saved, dy):
+    x, weight, bias, stats = saved
     need_x, need_w, need_b = ctx.needs_input_grad[:3]
     c = x.shape[-1]
     xr, n0, n1, s0, s1 = _rows(x)

@@ -130,3 +130,25 @@ def test_every_pair_tells_fixations_apart():
     assert same[0] == torch.tensor(2 * math.pi)
     two = FixationReader(16, 16, heads=2, head_dim=32, sections=(8, 8), device="cpu").rotary
     assert two.freqs[0] == two.freqs[8] == torch.tensor(2 * math.pi)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("create_graph", [False, True])
+def test_checkpointed_block(create_graph):
+    """Recomputed in the backward, also where the gradients are recorded: each kept tensor is asked for once."""
+    from torch.utils.checkpoint import checkpoint
+    from fovi_amd.arch.reader import FixationReader
+    torch.manual_seed(4)
+    reader = FixationReader(32, 24, heads=2, head_dim=16)
+    x, states = torch.randn(2, 5, 32, device="cuda"), torch.randn(2, 40, 24, device="cuda")
+    pos, xpos = torch.rand(40, 3, device="cuda"), torch.rand(5, 3, device="cuda")
+    x.requires_grad_(True)
+
+    def block(x):
+        return reader(x, states, pos, x_positions=xpos)
+
+    want = torch.autograd.grad(block(x).square().sum(), [x] + list(reader.parameters()))
+    y = checkpoint(block, x, use_reentrant=False)
+    got = torch.autograd.grad(y.square().sum(), [x] + list(reader.parameters()), create_graph=create_graph)
+    for a, b in zip(got, want):
+        assert ((a - b).norm() / b.norm()).item() < 1e-6
