@@ -15,7 +15,7 @@ from torch.autograd import forward_ad
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libfovi_hip.so")
 
-ABI_VERSION = 37
+ABI_VERSION = 38
 F32, BF16, F8E4M3 = 0, 1, 2
 NEAREST, BILINEAR = 0, 1
 PAD_ZEROS, PAD_BORDER = 0, 1
@@ -25,6 +25,7 @@ POOL_MAX, POOL_AVG, POOL_SUM, POOL_GAUSSIAN = 0, 1, 2, 3
 PAIR_HALF, PAIR_ADJACENT = 0, 1
 ROTARY_MAX_AXES = 4
 MASK_NONE, MASK_KEEP, MASK_BIAS = 0, 1, 2
+GATE_SILU, GATE_GELU = 0, 1
 
 _DTYPE_CODE = {torch.float32: F32, torch.bfloat16: BF16, torch.float8_e4m3fn: F8E4M3}
 
@@ -39,7 +40,10 @@ EXPORTED = ("fovi_abi_version", "fovi_last_error", "fovi_sampler_fwd", "fovi_knn
             "fovi_knnconv_dw_few_workspace_bytes", "fovi_knnconv_dw_few_us",
             "fovi_layer_norm_fwd", "fovi_layer_norm_workspace_bytes", "fovi_layer_norm_bwd", "fovi_rotary",
             "fovi_attention_fwd_workspace_bytes", "fovi_attention_fwd", "fovi_attention_bwd_workspace_bytes",
-            "fovi_attention_bwd", "fovi_attention_pack_mask")
+            "fovi_attention_bwd", "fovi_attention_pack_mask",
+            "fovi_rms_norm_fwd", "fovi_rms_norm_workspace_bytes", "fovi_rms_norm_bwd", "fovi_quantize_rows",
+            "fovi_dequantize_rows", "fovi_linear_int8_workspace_bytes", "fovi_linear_int8", "fovi_gated_mlp_saved_bytes", "fovi_gated_mlp_fwd_workspace_bytes",
+            "fovi_gated_mlp_fwd", "fovi_gated_mlp_bwd_workspace_bytes", "fovi_gated_mlp_bwd")
 
 
 class SamplerArgs(C.Structure):
@@ -264,6 +268,48 @@ class AttentionBwdArgs(C.Structure):
     ]
 
 
+class RmsNormArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("dtype", C.c_int32), ("p_dtype", C.c_int32),
+        ("rows0", C.c_int64), ("rows1", C.c_int64), ("channels", C.c_int64),
+        ("x_stride", C.c_int64 * 2),
+        ("residual", C.c_void_p), ("residual_stride", C.c_int64 * 2),
+        ("weight", C.c_void_p), ("eps", C.c_float), ("reserved0", C.c_int32),
+        ("total", C.c_void_p), ("y", C.c_void_p), ("q", C.c_void_p), ("scale", C.c_void_p), ("rstd", C.c_void_p),
+        ("dy", C.c_void_p), ("dy_stride", C.c_int64 * 2),
+        ("dtotal", C.c_void_p), ("dtotal_stride", C.c_int64 * 2),
+        ("dx", C.c_void_p), ("dweight", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+    ]
+
+
+class LinearInt8Args(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("x_scale", C.c_void_p),
+        ("rows", C.c_int64), ("inputs", C.c_int64), ("outputs", C.c_int64), ("x_stride", C.c_int64),
+        ("weight", C.c_void_p), ("weight_scale", C.c_void_p), ("weight_stride", C.c_int64),
+        ("weight2", C.c_void_p), ("weight2_scale", C.c_void_p), ("weight2_stride", C.c_int64),
+        ("activation", C.c_int32), ("out_dtype", C.c_int32),
+        ("bias", C.c_void_p), ("residual", C.c_void_p), ("residual_stride", C.c_int64),
+        ("out", C.c_void_p), ("out_stride", C.c_int64),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+    ]
+
+
+class GatedMlpArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("w_gate", C.c_void_p), ("w_up", C.c_void_p), ("w_down", C.c_void_p),
+        ("dtype", C.c_int32), ("activation", C.c_int32),
+        ("rows", C.c_int64), ("dim", C.c_int64), ("hidden", C.c_int64),
+        ("x_stride", C.c_int64), ("w_gate_stride", C.c_int64), ("w_up_stride", C.c_int64), ("w_down_stride", C.c_int64),
+        ("residual", C.c_void_p), ("residual_stride", C.c_int64),
+        ("y", C.c_void_p), ("y_stride", C.c_int64), ("saved", C.c_void_p),
+        ("dy", C.c_void_p), ("dy_stride", C.c_int64),
+        ("dx", C.c_void_p), ("dw_gate", C.c_void_p), ("dw_up", C.c_void_p), ("dw_down", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+    ]
+
+
 _lib = None
 
 
@@ -347,6 +393,27 @@ def load(path: str = LIB_PATH):
     lib.fovi_attention_bwd.restype = C.c_int
     lib.fovi_attention_pack_mask.argtypes = [C.c_void_p, C.POINTER(C.c_int64)] + [C.c_int64] * 4 + [C.c_void_p, C.c_void_p]
     lib.fovi_attention_pack_mask.restype = C.c_int
+    for name in ("fovi_rms_norm_fwd", "fovi_rms_norm_bwd"):
+        getattr(lib, name).argtypes = [C.POINTER(RmsNormArgs), C.c_void_p]
+        getattr(lib, name).restype = C.c_int
+    lib.fovi_rms_norm_workspace_bytes.argtypes = [C.c_int64, C.c_int64]
+    lib.fovi_rms_norm_workspace_bytes.restype = C.c_int64
+    lib.fovi_quantize_rows.argtypes = [C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_int64, C.POINTER(C.c_int64),
+                                       C.c_void_p, C.c_void_p, C.c_void_p]
+    lib.fovi_quantize_rows.restype = C.c_int
+    lib.fovi_dequantize_rows.argtypes = [C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_int32,
+                                         C.c_void_p]
+    lib.fovi_dequantize_rows.restype = C.c_int
+    lib.fovi_linear_int8.argtypes = [C.POINTER(LinearInt8Args), C.c_void_p]
+    lib.fovi_linear_int8.restype = C.c_int
+    lib.fovi_linear_int8_workspace_bytes.argtypes = [C.c_int64] * 3 + [C.c_int32]
+    lib.fovi_linear_int8_workspace_bytes.restype = C.c_int64
+    for name in ("fovi_gated_mlp_saved_bytes", "fovi_gated_mlp_fwd_workspace_bytes", "fovi_gated_mlp_bwd_workspace_bytes"):
+        getattr(lib, name).argtypes = [C.c_int64] * 3 + [C.c_int32]
+        getattr(lib, name).restype = C.c_int64
+    for name in ("fovi_gated_mlp_fwd", "fovi_gated_mlp_bwd"):
+        getattr(lib, name).argtypes = [C.POINTER(GatedMlpArgs), C.c_void_p]
+        getattr(lib, name).restype = C.c_int
     got = lib.fovi_abi_version()
     if got != ABI_VERSION:
         raise RuntimeError(f"{path}: ABI version {got}, expected {ABI_VERSION}")

@@ -14,6 +14,7 @@ import torch
 import torch.nn as nn
 
 from .attention import cross_attention
+from .feed_forward import GatedFeedForward
 from .norm import LayerNorm
 from .rotary import AxialRotary
 
@@ -37,10 +38,13 @@ class FixationReader(nn.Module):
     the pairs and the rest in two halves. ``base`` and ``scale`` as in ``AxialRotary``; by default row and
     column, in [-1, 1], turn by 2 pi at most, and fixations, counted in whole numbers, by one radian each (whole
     turns would tell none apart). ``kv_heads`` < ``heads`` shares key heads.
+
+    ``hidden``: the width of a gated feed-forward block behind the attention (``GatedFeedForward``; none by default). A
+    serving program replaces it by its 8-bit form: ``reader.feed_forward = reader.feed_forward.int8()``.
     """
 
     def __init__(self, dim, state_dim, heads, head_dim=64, kv_heads=None, sections=None, base=100.0, device="cuda",
-                 scale=None):
+                 scale=None, hidden=None, activation="silu"):
         super().__init__()
         kv_heads = heads if kv_heads is None else kv_heads
         if heads % kv_heads:
@@ -56,6 +60,7 @@ class FixationReader(nn.Module):
         self.to_kv = nn.Linear(state_dim, 2 * kv_heads * head_dim, bias=False, device=device)
         self.to_out = nn.Linear(heads * head_dim, dim, device=device)
         self.rotary = AxialRotary(head_dim, sections, base=base, scale=scale, device=device)
+        self.feed_forward = None if hidden is None else GatedFeedForward(dim, hidden, activation, device=device)
 
     def project(self, states, positions):
         """Keys and values ``[B, S, kv_heads, head_dim]`` of ``states [B, S, state_dim]`` at ``positions
@@ -80,4 +85,5 @@ class FixationReader(nn.Module):
         if x_positions is not None:
             q = self.rotary(q, x_positions)
         read = cross_attention(q, keys, values, kv_lengths=kv_lengths, mask=mask)
-        return x + self.to_out(read.reshape(b, n, self.heads * self.head_dim))
+        read = self.to_out(read.reshape(b, n, self.heads * self.head_dim))
+        return x + read if self.feed_forward is None else self.feed_forward(read.to(x.dtype), residual=x)

@@ -23,7 +23,7 @@
 extern "C" {
 #endif
 
-#define FOVI_ABI_VERSION 37
+#define FOVI_ABI_VERSION 38
 
 enum fovi_dtype { FOVI_F32 = 0, FOVI_BF16 = 1, FOVI_F8E4M3 = 2 };
 enum fovi_interp { FOVI_NEAREST = 0, FOVI_BILINEAR = 1 };
@@ -895,6 +895,134 @@ typedef struct fovi_attention_bwd_args {
 int64_t fovi_attention_bwd_workspace_bytes(int64_t batch, int64_t q_len, int64_t kv_len, int64_t heads,
                                            int64_t kv_heads, int64_t head_dim, int32_t dtype);
 int fovi_attention_bwd(const fovi_attention_bwd_args* args, void* stream);
+
+/*
+ * RMS norm over the last dimension of token rows, with the residual's addition in front (no counterpart among the
+ * replaced ATen sites):
+ *   total = x + residual (in dtype), rstd = 1 / sqrt(mean(total^2) + eps), y = total * rstd * weight
+ * Rows are indexed (i0, i1); strides are [i0, i1] with the channels adjacent. dtype F32 or BF16 for x, residual,
+ * total, y and their gradients; the weight and its gradient have p_dtype. Statistics and sums are fp32. residual and weight
+ * may be NULL (no addition, total not written; 1). total, y, q and dx are [rows0 * rows1, channels], whole.
+ * forward: total, rstd [rows0 * rows1] unless NULL, and either y, or 8-bit rows: scale [rows0 * rows1] = max|y| / 127 of each
+ * row's unrounded y, q = y / scale rounded to nearest even. A row whose largest value is infinite or NaN has such
+ * a scale and q of 0: the values it stands for are NaN.
+ * backward: from x (the forward's total), dy, rstd and dtotal (the gradient that arrives at total; may be NULL): dx
+ * (the gradient of x and of residual; unless NULL), dweight (unless NULL), which needs a workspace of
+ * fovi_rms_norm_workspace_bytes, 16-byte aligned.
+ */
+typedef struct fovi_rms_norm_args {
+  const void* x;
+  int32_t dtype;
+  int32_t p_dtype;
+  int64_t rows0, rows1, channels;
+  int64_t x_stride[2];
+  const void* residual;
+  int64_t residual_stride[2];
+  const void* weight;
+  float eps;
+  int32_t reserved0;
+  void* total;
+  void* y;
+  int8_t* q;
+  float* scale;
+  float* rstd;
+  const void* dy;             /* backward only, from here on */
+  int64_t dy_stride[2];
+  const void* dtotal;
+  int64_t dtotal_stride[2];
+  void* dx;
+  void* dweight;
+  void* workspace;
+  int64_t workspace_bytes;
+} fovi_rms_norm_args;
+
+int fovi_rms_norm_fwd(const fovi_rms_norm_args* args, void* stream);
+int64_t fovi_rms_norm_workspace_bytes(int64_t rows, int64_t channels);
+int fovi_rms_norm_bwd(const fovi_rms_norm_args* args, void* stream);
+
+/* Rows (F32 or BF16, strides as above) in 8 bits with a scale each, as fovi_rms_norm_fwd does it: q [rows0 * rows1,
+ * channels] whole, scale [rows0 * rows1]. And back: y [rows, channels] whole, from rows `stride` apart. */
+int fovi_quantize_rows(const void* x, int32_t dtype, int64_t rows0, int64_t rows1, int64_t channels, const int64_t* stride,
+                       int8_t* q, float* scale, void* stream);
+int fovi_dequantize_rows(const int8_t* q, const float* scale, int64_t rows, int64_t channels, int64_t stride, void* y,
+                         int32_t dtype, void* stream);
+
+/*
+ * Product of 8-bit rows with 8-bit weights, a scale for each row and for each output:
+ *   out[m, n] = (sum_k x[m, k] weight[n, k]) * x_scale[m] * weight_scale[n] + bias[n] + residual[m, n]
+ * and with weight2 (then without bias and residual) act(that) * the same product with weight2 and weight2_scale.
+ * Strides are in elements between rows, elements adjacent, at any alignment. Sums are exact in int32 (up to 131072 inputs).
+ * out and residual: out_dtype, F32 or BF16; bias fp32 (may be NULL, as may residual). The workspace
+ * (fovi_linear_int8_workspace_bytes, may be 0; 16-byte aligned) holds partial sums where the inputs are split over workgroups.
+ */
+enum fovi_gate_act { FOVI_GATE_SILU = 0, FOVI_GATE_GELU = 1 };
+
+typedef struct fovi_linear_int8_args {
+  const int8_t* x;
+  const float* x_scale;
+  int64_t rows, inputs, outputs;
+  int64_t x_stride;
+  const int8_t* weight;
+  const float* weight_scale;
+  int64_t weight_stride;
+  const int8_t* weight2;
+  const float* weight2_scale;
+  int64_t weight2_stride;
+  int32_t activation;
+  int32_t out_dtype;
+  const float* bias;
+  const void* residual;
+  int64_t residual_stride;
+  void* out;
+  int64_t out_stride;
+  void* workspace;
+  int64_t workspace_bytes;
+} fovi_linear_int8_args;
+
+int64_t fovi_linear_int8_workspace_bytes(int64_t rows, int64_t inputs, int64_t outputs, int32_t gated);
+int fovi_linear_int8(const fovi_linear_int8_args* args, void* stream);
+
+/*
+ * The gated feed-forward block of rows x [rows, dim]:
+ *   gate = x w_gate^T, up = x w_up^T, y = (act(gate) * up) w_down^T + residual
+ * w_gate, w_up [hidden, dim], w_down [dim, hidden]; act(z) is z / (1 + exp(-z)) (FOVI_GATE_SILU) or z Phi(z)
+ * (FOVI_GATE_GELU). dtype F32 or BF16 for everything; strides are in elements between rows, elements adjacent.
+ * Sums are fp32. With BF16 act(gate) * up, and in the backward its gradient's two products, are rounded to it before the
+ * products they enter (the matrix unit takes one type).
+ * saved: gate and up for the backward, of fovi_gated_mlp_saved_bytes (0: the backward forms them again and takes NULL;
+ * NULL if no backward follows).
+ * backward: dx, dw_down and the pair dw_gate, dw_up, each unless NULL, whole; the residual's gradient is dy.
+ * The workspaces are 16-byte aligned.
+ */
+typedef struct fovi_gated_mlp_args {
+  const void* x;
+  const void* w_gate;
+  const void* w_up;
+  const void* w_down;
+  int32_t dtype;
+  int32_t activation;
+  int64_t rows, dim, hidden;
+  int64_t x_stride, w_gate_stride, w_up_stride, w_down_stride;
+  const void* residual;
+  int64_t residual_stride;
+  void* y;
+  int64_t y_stride;
+  void* saved;
+  const void* dy;             /* backward only, from here on */
+  int64_t dy_stride;
+  void* dx;
+  void* dw_gate;
+  void* dw_up;
+  void* dw_down;
+  void* workspace;            /* both directions */
+  int64_t workspace_bytes;
+} fovi_gated_mlp_args;
+
+int64_t fovi_gated_mlp_saved_bytes(int64_t rows, int64_t dim, int64_t hidden, int32_t dtype);
+int64_t fovi_gated_mlp_fwd_workspace_bytes(int64_t rows, int64_t dim, int64_t hidden, int32_t dtype);
+int fovi_gated_mlp_fwd(const fovi_gated_mlp_args* args, void* stream);
+int64_t fovi_gated_mlp_bwd_workspace_bytes(int64_t rows, int64_t dim, int64_t hidden, int32_t dtype);
+int fovi_gated_mlp_bwd(const fovi_gated_mlp_args* args, void* stream);
 
 #ifdef __cplusplus
 }
