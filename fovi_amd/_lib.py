@@ -406,10 +406,12 @@ def load(path: str = LIB_PATH):
     lib.fovi_dequantize_rows.restype = C.c_int
     lib.fovi_linear_int8.argtypes = [C.POINTER(LinearInt8Args), C.c_void_p]
     lib.fovi_linear_int8.restype = C.c_int
-    lib.fovi_linear_int8_workspace_bytes.argtypes = [C.c_int64] * 3 + [C.c_int32]
+    lib.fovi_linear_int8_workspace_bytes.argtypes = [C.POINTER(LinearInt8Args)]
     lib.fovi_linear_int8_workspace_bytes.restype = C.c_int64
-    for name in ("fovi_gated_mlp_saved_bytes", "fovi_gated_mlp_fwd_workspace_bytes", "fovi_gated_mlp_bwd_workspace_bytes"):
-        getattr(lib, name).argtypes = [C.c_int64] * 3 + [C.c_int32]
+    lib.fovi_gated_mlp_saved_bytes.argtypes = [C.c_int64] * 3 + [C.c_int32]
+    lib.fovi_gated_mlp_saved_bytes.restype = C.c_int64
+    for name in ("fovi_gated_mlp_fwd_workspace_bytes", "fovi_gated_mlp_bwd_workspace_bytes"):
+        getattr(lib, name).argtypes = [C.POINTER(GatedMlpArgs)]
         getattr(lib, name).restype = C.c_int64
     for name in ("fovi_gated_mlp_fwd", "fovi_gated_mlp_bwd"):
         getattr(lib, name).argtypes = [C.POINTER(GatedMlpArgs), C.c_void_p]

@@ -47,10 +47,9 @@ def _workspace(a, nbytes, device):
 def _forward(x, w_gate, w_up, w_down, activation, residual, keep_for_backward):
     a, keep = _args(x, w_gate, w_up, w_down, activation)
     lib = _lib.load()
-    sizes = a.rows, a.dim, a.hidden, a.dtype
     saved = None
     if keep_for_backward:
-        n = lib.fovi_gated_mlp_saved_bytes(*sizes)
+        n = lib.fovi_gated_mlp_saved_bytes(a.rows, a.dim, a.hidden, a.dtype)
         if n:
             saved = torch.empty(n, dtype=torch.uint8, device=x.device)
             a.saved = saved.data_ptr()
@@ -59,7 +58,7 @@ def _forward(x, w_gate, w_up, w_down, activation, residual, keep_for_backward):
         a.residual = residual.data_ptr()
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     a.y, a.y_stride = y.data_ptr(), a.dim
-    work = _workspace(a, lib.fovi_gated_mlp_fwd_workspace_bytes(*sizes), x.device)
+    work = _workspace(a, lib.fovi_gated_mlp_fwd_workspace_bytes(a), x.device)
     _lib.check(lib.fovi_gated_mlp_fwd(a, _lib.stream_of(x)), "fovi_gated_mlp_fwd")
     del work, keep
     return y, saved
@@ -92,7 +91,7 @@ def _backward(ctx, saved, dy):
         ddown = like(w_down)
         a.dw_down = ddown.data_ptr()
     if need_x or need_gate or need_up or need_down:
-        work = _workspace(a, lib.fovi_gated_mlp_bwd_workspace_bytes(a.rows, a.dim, a.hidden, a.dtype), x.device)
+        work = _workspace(a, lib.fovi_gated_mlp_bwd_workspace_bytes(a), x.device)
         _lib.check(lib.fovi_gated_mlp_bwd(a, _lib.stream_of(x)), "fovi_gated_mlp_bwd")
         del work
     del keep

@@ -154,7 +154,7 @@ def _product(what, x, weight, weight2, activation, bias, residual, dtype):
     a.weight, a.weight_scale, a.weight_stride = w.data_ptr(), ws.data_ptr(), w.stride(0)
     a.out, a.out_dtype, a.out_stride = out.data_ptr(), _lib.dtype_code(dtype), n
     lib = _lib.load()
-    nbytes = lib.fovi_linear_int8_workspace_bytes(rows, k, n, weight2 is not None)
+    nbytes = lib.fovi_linear_int8_workspace_bytes(a)
     if nbytes:
         work = torch.empty(nbytes, dtype=torch.uint8, device=device)
         keep.append(work)

@@ -18,7 +18,7 @@ SOURCES = ["abi.hip", "sampler.hip", "knnconv.hip", "knnconv_v5.hip", "knnconv_f
            "knnpool.hip", "knnconv_bwd.hip", "knn_tables.hip", "knnconv_dw.hip", "knnconv_fewc.hip",
            "knnconv_fewc_vm.hip", "knnconv_img.hip",
            "knnconv_dw_few.hip", "layer_norm.hip", "rotary.hip", "attention.hip", "attention_fwd.hip",
-           "attention_bwd.hip", "rms_norm.hip", "linear_int8.hip", "gated_mlp.hip"]
+           "attention_bwd.hip", "rms_norm.hip", "matmul.hip", "linear_int8.hip", "gated_mlp.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

@@ -18,156 +18,298 @@ struct MatSegments {
   int n;
 };
 
+// Runs of h, dgate and dup are written whole, with zeros behind the last column: the products that read them go by 16 bytes.
+__device__ __forceinline__ void clear_behind(int count, float (&v)[8]) {
+#pragma unroll
+  for (int i = 1; i < 8; ++i) v[i] = i < count ? v[i] : 0.0f;
+}
+
 template <typename T> struct MlpLinear {               // out = sums (+ residual)
+  static constexpr int STORES = sizeof(T) / 2;         // of 16 bytes for a run of eight
   T* out; int64_t stride;
   const T* residual; int64_t residual_stride;
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const float (&v)[1][4]) const {
-    float y[4] = {v[0][0], v[0][1], v[0][2], v[0][3]};
-    if (residual) {
-      float r[4];
-      load_four(residual + m * residual_stride + n, count, r);
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const float (&v)[1][8]) const {
+    float y[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] += r[i];
+    for (int i = 0; i < 8; ++i) y[i] = v[0][i];
+    if (residual) {
+      float r[8];
+      load_run(residual + m * residual_stride + n, count, r);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] += r[i];
     }
-    store_four(out + m * stride + n, count, y);
+    store_run(out + m * stride + n, count, y);
   }
 };
 
-template <typename T> struct MlpTwoRows {              // rows below `rows` to one output, the others to the next
-  T* out[2]; int64_t rows, stride;
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const float (&v)[1][4]) const {
-    store_four(m < rows ? out[0] + m * stride + n : out[1] + (m - rows) * stride + n, count, v[0]);
+template <typename T> struct MlpTwoRows {              // `rows` rows to one output, those from `next` on to the other
+  static constexpr int STORES = 0;                     // rows between the two are not stored
+  T* out[2]; int64_t rows, next, stride;
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const float (&v)[1][8]) const {
+    if (m < rows) store_run(out[0] + m * stride + n, count, v[0]);
+    else if (m >= next) store_run(out[1] + (m - next) * stride + n, count, v[0]);
   }
 };
 
 struct MlpPartial {                                    // the sums of a share of the reduction
+  static constexpr int STORES = 2;
   float* part; int64_t M, N;
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const float (&v)[1][4]) const {
-    store_four(part + (blockIdx.y * M + m) * N + n, count, v[0]);
+  __device__ __forceinline__ void operator()(int64_t share, int64_t m, int64_t n, int count, const float (&v)[1][8]) const {
+    store_run(part + (share * M + m) * N + n, count, v[0]);
   }
 };
 
 template <typename T> struct MlpGated {                // h, and gate and up where a backward will read them
+  static constexpr int STORES = sizeof(T) / 2;
   T* h; int64_t stride; int act;
   T* gate; T* up; int64_t saved_stride;
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const float (&v)[2][4]) const {
-    float y[4];
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const float (&v)[2][8]) const {
+    float y[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = mat_act<sizeof(T) == 4>(v[0][i], act) * v[1][i];
-    store_four(h + m * stride + n, count, y);
+    for (int i = 0; i < 8; ++i) y[i] = mat_act<sizeof(T) == 4>(v[0][i], act) * v[1][i];
+    clear_behind(count, y);
+    store_run(h + m * stride + n, 8, y);
     if (gate) {
-      store_four(gate + m * saved_stride + n, count, v[0]);
-      store_four(up + m * saved_stride + n, count, v[1]);
+      store_run(gate + m * saved_stride + n, count, v[0]);
+      store_run(up + m * saved_stride + n, count, v[1]);
     }
   }
 };
 
 template <typename T> struct MlpGatedGrad {            // dgate, dup and h from gate, up and dh
+  static constexpr int STORES = 3 * sizeof(T) / 2;
   T* dgate; T* dup; T* h; int64_t stride, h_stride; int act;
   const T* gate; const T* up; int64_t saved_stride;
-  __device__ __forceinline__ void write(int64_t m, int64_t n, int count, const float (&g)[4], const float (&u)[4],
-                                        const float (&dh)[4]) const {
-    float a[4], b[4], c[4];
+  __device__ __forceinline__ void write(int64_t m, int64_t n, int count, const float (&g)[8], const float (&u)[8],
+                                        const float (&dh)[8]) const {
+    float a[8], b[8], c[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
       float value, slope;
       mat_act_grad<sizeof(T) == 4>(g[i], act, value, slope);
       a[i] = dh[i] * u[i] * slope;
       b[i] = dh[i] * value;
       c[i] = value * u[i];
     }
-    store_four(dgate + m * stride + n, count, a);
-    store_four(dup + m * stride + n, count, b);
-    store_four(h + m * h_stride + n, count, c);
+    clear_behind(count, a);
+    clear_behind(count, b);
+    clear_behind(count, c);
+    store_run(dgate + m * stride + n, 8, a);
+    store_run(dup + m * stride + n, 8, b);
+    store_run(h + m * h_stride + n, 8, c);
   }
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const float (&v)[3][4]) const {
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const float (&v)[3][8]) const {
     write(m, n, count, v[0], v[1], v[2]);
   }
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const float (&v)[1][4]) const {
-    float g[4], u[4];
-    load_four(gate + m * saved_stride + n, count, g);
-    load_four(up + m * saved_stride + n, count, u);
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const float (&v)[1][8]) const {
+    float g[8], u[8];
+    load_run(gate + m * saved_stride + n, count, g);
+    load_run(up + m * saved_stride + n, count, u);
     write(m, n, count, g, u, v[0]);
   }
 };
 
+// One product, k in up to two segments (of other operands each), or split in shares of `share`.
+template <typename T, int BM, int BN, bool CX, bool CW, typename Epilogue> struct MlpLinearTile {
+  typedef MatPhase<T, BM, BN, 1, CX, CW> Phase;
+  typedef MatRing<Phase::BYTES, 2 * Phase::MB * Phase::NN * Epilogue::STORES> Ring;
+};
 template <typename T, int BM, int BN, bool CX, bool CW, typename Epilogue>
-__global__ __launch_bounds__(256) void mlp_linear_kernel(MatSegments s, int64_t M, int64_t N, int64_t share, Epilogue epilogue) {
-  typedef MatCore<T, BM, BN, 1, CX, CW> Core;
-  __shared__ __attribute__((aligned(16))) char lds[Core::LDS];
-  int64_t tm, tn;
-  if (!mat_tile((M + BM - 1) / BM, (N + BN - 1) / BN, tm, tn)) return;
-  typename Core::Acc acc[1][Core::MB][Core::NN];
-  mat_clear(acc);
-  for (int i = 0; i < s.n; ++i) {
-    const int64_t from = blockIdx.y * share, to = from + share < s.k[i] ? from + share : s.k[i];
-    if (from < to) Core::run(s.x[i], &s.w[i], tm * BM, tn * BN, from, to, lds, acc);
+__global__ __launch_bounds__((MatUsual<BM, BN>::THREADS), 2) void mlp_linear_kernel(MatSegments s, int64_t M, int64_t N, MatWork work, int64_t share,
+                                                            Epilogue epilogue) {
+  typedef typename MlpLinearTile<T, BM, BN, CX, CW, Epilogue>::Phase Phase;
+  typedef typename MlpLinearTile<T, BM, BN, CX, CW, Epilogue>::Ring Ring;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  MatItem item(work), ahead(work);
+  if (!item.live()) return;
+  auto part = [&](const MatItem& at, int i, int64_t& from) __attribute__((always_inline)) {
+    const int64_t k = i ? s.k[1] : s.k[0];
+    from = at.share(work) * share;
+    return (from + share < k ? from + share : k) - from;
+  };
+  Phase phase;
+  int segment = -1;
+  int64_t left = 0;
+  auto produce = [&](uint32_t to) __attribute__((always_inline)) {
+    while (left <= 0) {
+      if (++segment == s.n) { segment = 0; ahead.next(); }
+      if (!ahead.live()) return false;
+      int64_t from;
+      left = part(ahead, segment, from);
+      const MatOperand w[1] = {segment ? s.w[1] : s.w[0]};
+      int64_t tm, tn;
+      ahead.place(work, tm, tn);
+      phase.open(segment ? s.x[1] : s.x[0], w, tm * BM, tn * BN, from);
+    }
+    phase.start(to, left);
+    left -= Phase::BK;
+    return true;
+  };
+  Ring ring(lds, produce);
+  typename Phase::Step step[2];
+  auto first_step = [&](const char* now) __attribute__((always_inline)) { step[0].read(now, 0); };
+  first_step(ring.now());
+  for (; item.live(); item.next()) {
+    typename Phase::Acc acc[1][Phase::MB][Phase::NN];
+    mat_clear(acc);
+    int64_t stages = 0, from;
+    for (int i = 0; i < s.n; ++i) {
+      const int64_t n = part(item, i, from);
+      stages += n > 0 ? (n + Phase::BK - 1) / Phase::BK : 0;
+    }
+    Phase::run(ring, stages, step, acc, 0, produce, first_step);
+    int64_t tm, tn;
+    item.place(work, tm, tn);
+    if constexpr (__is_same(Epilogue, MlpPartial)) {
+      const int64_t z = item.share(work);
+      ring.stored = mat_finish<typename Phase::Waves, BM, BN, float>(acc, tm * BM, tn * BN, M, N,
+                                [&](int64_t m, int64_t n, int count, const float (&v)[1][8]) { epilogue(z, m, n, count, v); });
+    } else {
+      ring.stored = mat_finish<typename Phase::Waves, BM, BN, float>(acc, tm * BM, tn * BN, M, N, epilogue);
+    }
   }
-  mat_finish<BM, BN, float>(acc, tm * BM, tn * BN, M, N, epilogue);
 }
 
 // out = the shares' sums added up, through the epilogue.
 template <typename Epilogue>
 __global__ __launch_bounds__(256) void mlp_join_kernel(const float* part, int64_t shares, int64_t M, int64_t N, Epilogue epilogue) {
-  const int64_t per = (N + 3) / 4, i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t per = (N + 7) / 8, i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (i >= M * per) return;
-  const int64_t m = i / per, n = (i - m * per) * 4;
-  const int count = static_cast<int>(N - n < 4 ? N - n : 4);
-  float v[1][4] = {{0, 0, 0, 0}};
+  const int64_t m = i / per, n = (i - m * per) * 8;
+  const int count = static_cast<int>(N - n < 8 ? N - n : 8);
+  float v[1][8] = {};
   for (int64_t z = 0; z < shares; ++z) {
-    float t[4];
-    load_four(part + (z * M + m) * N + n, count, t);
+    float t[8];
+    load_run(part + (z * M + m) * N + n, count, t);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[0][e] += t[e];
+    for (int e = 0; e < 8; ++e) v[0][e] += t[e];
   }
   epilogue(m, n, count, v);
 }
 
+template <typename T, int BM, int BN> struct MlpGatedTile {
+  typedef MatPhase<T, BM, BN, 2, false, false> Both;
+  typedef MatRing<Both::BYTES, 2 * Both::MB * Both::NN * MlpGated<T>::STORES> Ring;
+};
+template <typename T, int BM, int BN, typename W> struct MlpGradTile {
+  typedef MatPhase<T, BM, BN, 2, false, false, W> Both;
+  typedef MatPhase<T, BM, BN, 1, false, true, W> Down;
+  typedef MatRing<Both::BYTES, 2 * Both::MB * Both::NN * MlpGatedGrad<T>::STORES> Ring;
+};
+
 template <typename T, int BM, int BN>
-__global__ __launch_bounds__(256) void mlp_gated_kernel(MatOperand x, MatOperand wg, MatOperand wu, int64_t K, int64_t M, int64_t N,
-                                                        MlpGated<T> epilogue) {
-  typedef MatCore<T, BM, BN, 2, false, false> Core;
-  __shared__ __attribute__((aligned(16))) char lds[Core::LDS];
-  int64_t tm, tn;
-  if (!mat_tile((M + BM - 1) / BM, (N + BN - 1) / BN, tm, tn)) return;
-  typename Core::Acc acc[2][Core::MB][Core::NN];
-  mat_clear(acc);
+__global__ __launch_bounds__((MatUsual<BM, BN>::THREADS), 2) void mlp_gated_kernel(MatOperand x, MatOperand wg, MatOperand wu, int64_t K, int64_t M, int64_t N,
+                                                           MatWork work, MlpGated<T> epilogue) {
+  typedef typename MlpGatedTile<T, BM, BN>::Both Phase;
+  typedef typename MlpGatedTile<T, BM, BN>::Ring Ring;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  MatItem item(work), ahead(work);
+  if (!item.live()) return;
   const MatOperand w[2] = {wg, wu};
-  Core::run(x, w, tm * BM, tn * BN, 0, K, lds, acc);
-  mat_finish<BM, BN, float>(acc, tm * BM, tn * BN, M, N, epilogue);
+  Phase phase;
+  int64_t left = -1;                                   // of the tile `ahead`; -1: not begun
+  auto produce = [&](uint32_t to) __attribute__((always_inline)) {
+    if (left <= 0) {
+      if (left == 0) ahead.next();
+      if (!ahead.live()) return false;
+      left = K;
+      int64_t tm, tn;
+      ahead.place(work, tm, tn);
+      phase.open(x, w, tm * BM, tn * BN, 0);
+    }
+    phase.start(to, left);
+    left = left > Phase::BK ? left - Phase::BK : 0;
+    return true;
+  };
+  Ring ring(lds, produce);
+  typename Phase::Step step[2];
+  auto first_step = [&](const char* now) __attribute__((always_inline)) { step[0].read(now, 0); };
+  first_step(ring.now());
+  const int64_t stages = (K + Phase::BK - 1) / Phase::BK;
+  for (; item.live(); item.next()) {
+    typename Phase::Acc acc[2][Phase::MB][Phase::NN];
+    mat_clear(acc);
+    Phase::run(ring, stages, step, acc, 0, produce, first_step);
+    int64_t tm, tn;
+    item.place(work, tm, tn);
+    ring.stored = mat_finish<typename Phase::Waves, BM, BN, float>(acc, tm * BM, tn * BN, M, N, epilogue);
+  }
 }
 
 // gate, up and dh of a tile, one after the other, and what the epilogue makes of them.
-template <typename T, int BM, int BN>
-__global__ __launch_bounds__(256) void mlp_gated_grad_kernel(MatOperand x, MatOperand wg, MatOperand wu, MatOperand dy, MatOperand wd,
-                                                             int64_t K, int64_t M, int64_t N, MlpGatedGrad<T> epilogue) {
-  typedef MatCore<T, BM, BN, 2, false, false> Both;
-  typedef MatCore<T, BM, BN, 1, false, true> Down;
-  __shared__ __attribute__((aligned(16))) char lds[Both::LDS];
-  int64_t tm, tn;
-  if (!mat_tile((M + BM - 1) / BM, (N + BN - 1) / BN, tm, tn)) return;
-  typename Both::Acc acc[3][Both::MB][Both::NN];
-  mat_clear(acc);
-  const MatOperand w[2] = {wg, wu};
-  Both::run(x, w, tm * BM, tn * BN, 0, K, lds, acc);
-  Down::run(dy, &wd, tm * BM, tn * BN, 0, K, lds, acc, 2);
-  mat_finish<BM, BN, float>(acc, tm * BM, tn * BN, M, N, epilogue);
+template <typename T, int BM, int BN, typename W>
+__global__ __launch_bounds__(W::THREADS, 2) void mlp_gated_grad_kernel(MatOperand x, MatOperand wg, MatOperand wu, MatOperand dy, MatOperand wd,
+                                                                int64_t K, int64_t M, int64_t N, MatWork work, MlpGatedGrad<T> epilogue) {
+  typedef typename MlpGradTile<T, BM, BN, W>::Both Both;
+  typedef typename MlpGradTile<T, BM, BN, W>::Down Down;
+  typedef typename MlpGradTile<T, BM, BN, W>::Ring Ring;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  MatItem item(work), ahead(work);
+  if (!item.live()) return;
+  const MatOperand w[2] = {wg, wu}, d[1] = {wd};
+  Both both;
+  Down down;
+  int64_t left = -1;
+  bool second = true;                                  // which of the two runs of stages `left` belongs to
+  auto produce = [&](uint32_t to) __attribute__((always_inline)) {
+    if (left <= 0) {
+      if (left == 0 && second) ahead.next();
+      if (!ahead.live()) return false;
+      left = K;
+      second = !second;
+      int64_t tm, tn;
+      ahead.place(work, tm, tn);
+      if (second) down.open(dy, d, tm * BM, tn * BN, 0);
+      else both.open(x, w, tm * BM, tn * BN, 0);
+    }
+    if (second) down.start(to, left);
+    else both.start(to, left);
+    left = left > Both::BK ? left - Both::BK : 0;
+    return true;
+  };
+  Ring ring(lds, produce);
+  const int64_t stages = (K + Both::BK - 1) / Both::BK;
+  for (; item.live(); item.next()) {
+    typename Both::Acc acc[3][Both::MB][Both::NN];
+    mat_clear(acc);
+    Both::run_lean(ring, stages, acc, 0, produce);
+    Down::run_lean(ring, stages, acc, 2, produce);
+    int64_t tm, tn;
+    item.place(work, tm, tn);
+    ring.stored = mat_finish<W, BM, BN, float>(acc, tm * BM, tn * BN, M, N, epilogue);
+  }
 }
 
-static int64_t tiles_of(int64_t n, int64_t b) { return (n + b - 1) / b; }
-
+template <typename T, int BM, int BN, bool CX, bool CW, typename Epilogue>
+static void mlp_linear_tiles(const MatSegments& s, int64_t M, int64_t N, int64_t share, int64_t shares, const Epilogue& epilogue,
+                             hipStream_t stream) {
+  const MatWork work = mat_work(M, N, BM, BN, shares);
+  mat_launch(mlp_linear_kernel<T, BM, BN, CX, CW, Epilogue>, mat_grid(work, 256 / BM), (MatUsual<BM, BN>::THREADS), MlpLinearTile<T, BM, BN, CX, CW, Epilogue>::Ring::LDS,
+             stream, s, M, N, work, share, epilogue);
+}
 template <typename T, bool CX, bool CW, typename Epilogue>
-static void mlp_linear(const MatSegments& s, int64_t M, int64_t N, const Epilogue& epilogue, hipStream_t stream) {
-  const int64_t tiles = tiles_of(M, 128) * tiles_of(N, 128);
-  mlp_linear_kernel<T, 128, 128, CX, CW, Epilogue><<<mat_grid(tiles), 256, 0, stream>>>(s, M, N, s.k[0] > s.k[1] ? s.k[0] : s.k[1], epilogue);
+static void mlp_linear(const MatSegments& s, int64_t M, int64_t N, int64_t share, int64_t shares, const Epilogue& epilogue,
+                       hipStream_t stream) {
+  const int size = mat_tile_size(M, N, shares, sizeof(T) == 4, mat_columns(N));
+  if constexpr (sizeof(T) == 2) {
+    if (size == 256) {
+      if (mat_columns(N) == 192) mlp_linear_tiles<T, 256, 192, CX, CW>(s, M, N, share, shares, epilogue, stream);
+      else mlp_linear_tiles<T, 256, 256, CX, CW>(s, M, N, share, shares, epilogue, stream);
+      return;
+    }
+  }
+  if (size >= 128) mlp_linear_tiles<T, 128, 128, CX, CW>(s, M, N, share, shares, epilogue, stream);
+  else mlp_linear_tiles<T, 64, 64, CX, CW>(s, M, N, share, shares, epilogue, stream);
 }
 
-// Shares of a reduction over the tokens: workgroups for the whole card twice over, at least 512 tokens each.
+// Shares of a reduction over the tokens: workgroups for the whole card, at least 512 tokens each.
 static int64_t token_shares(int64_t tokens, int64_t M, int64_t N) {
-  const int64_t tiles = tiles_of(M, 128) * tiles_of(N, 128);
-  int64_t shares = (512 + tiles - 1) / tiles;
-  const int64_t most = (tokens + 511) / 512;
-  if (shares > most) shares = most;
+  const int64_t most = (tokens + 511) / 512, big = mat_tiles(M, N, 256, 256), small = mat_tiles(M, N, 64, 64);
+  int64_t shares = (256 + big - 1) / big;
+  if (shares > most) {                                 // small tiles, then
+    shares = (1024 + small - 1) / small;
+    if (shares > most) shares = most;
+  }
   return shares < 1 ? 1 : shares;
 }
 
@@ -176,77 +318,112 @@ template <typename T, typename Epilogue>
 static void token_product(const MatOperand& x, const MatOperand& w, int64_t tokens, int64_t M, int64_t N, float* part,
                           const Epilogue& epilogue, hipStream_t stream) {
   const int64_t shares = token_shares(tokens, M, N);
-  MatSegments s = {{x}, {w}, {tokens, 0}, 1};
+  const MatSegments s = {{x}, {w}, {tokens, 0}, 1};
   if (shares == 1) {
-    mlp_linear<T, true, true>(s, M, N, epilogue, stream);
+    mlp_linear<T, true, true>(s, M, N, tokens, 1, epilogue, stream);
     return;
   }
-  const int64_t bk = Mat<T>::BK, share = ((tokens + shares - 1) / shares + bk - 1) / bk * bk;
+  const int64_t bk = mat_bk<T>(), share = ((tokens + shares - 1) / shares + bk - 1) / bk * bk;
   const int64_t used = (tokens + share - 1) / share;
-  const dim3 grid(mat_grid(tiles_of(M, 128) * tiles_of(N, 128)), static_cast<unsigned>(used));
-  mlp_linear_kernel<T, 128, 128, true, true, MlpPartial><<<grid, 256, 0, stream>>>(s, M, N, share, MlpPartial{part, M, N});
-  mlp_join_kernel<Epilogue><<<static_cast<unsigned>((M * ((N + 3) / 4) + 255) / 256), 256, 0, stream>>>(part, used, M, N, epilogue);
+  mlp_linear<T, true, true>(s, M, N, share, used, MlpPartial{part, M, N}, stream);
+  mlp_join_kernel<Epilogue><<<static_cast<unsigned>((M * ((N + 7) / 8) + 255) / 256), 256, 0, stream>>>(part, used, M, N, epilogue);
 }
 
 static int mlp_check(const fovi_gated_mlp_args* a, const char* what) {
   if (!a || !a->x || !a->w_gate || !a->w_up || !a->w_down) { set_error("%s: null pointer", what); return 1; }
   if (a->dtype != FOVI_F32 && a->dtype != FOVI_BF16) { set_error("%s: dtype must be F32 or BF16", what); return 1; }
   if (a->activation != FOVI_GATE_SILU && a->activation != FOVI_GATE_GELU) { set_error("%s: unknown activation", what); return 1; }
-  if (a->rows < 0 || a->dim < 1 || a->hidden < 1 || a->dim > (1 << 24) || a->hidden > (1 << 24) || a->rows > (1ll << 31)) {
-    set_error("%s: bad sizes (rows to 2^31, dim and hidden to 2^24)", what);
+  if (a->rows < 0 || a->dim < 1 || a->hidden < 1 || a->dim > (1 << 19) || a->hidden > (1 << 19) || a->rows > (1ll << 31)) {
+    set_error("%s: bad sizes (rows to 2^31, dim and hidden to 2^19)", what);
     return 1;
   }
-  const int64_t tiles = (a->rows + 127) / 128 * ((a->hidden > a->dim ? a->hidden : a->dim) / 64 + 1);
-  if (tiles > 0x7ffffff0ll || a->dim * a->hidden > (1ll << 39)) { set_error("%s: too large", what); return 1; }
+  const int64_t widest = a->hidden > a->dim ? a->hidden : a->dim;
+  if (((a->rows > widest ? a->rows : widest) + 63) / 64 > (1ll << 30) / ((widest + 63) / 64)) { set_error("%s: too large", what); return 1; }
   return 0;
 }
 
-template <typename T>
-static MatOperand operand(const void* p, int64_t stride, int64_t extent) {
-  return MatOperand{static_cast<const char*>(p), stride * static_cast<int64_t>(sizeof(T)), extent};
+static int64_t mlp_element(const fovi_gated_mlp_args* a) { return a->dtype == FOVI_F32 ? 4 : 2; }
+static int64_t aligned(int64_t n) { return (n + 255) & ~static_cast<int64_t>(255); }
+static int64_t wide(int64_t n) { return (n + 7) & ~static_cast<int64_t>(7); }
+
+struct MlpInputs {
+  MatInputs in;
+  MatOperand x, wg, wu, wd, dy;
+  MlpInputs(const fovi_gated_mlp_args* a, void* workspace, bool backward) : in(workspace) {
+    const int64_t es = mlp_element(a);
+    x = in.take(a->x, a->x_stride, a->rows, a->dim, es);
+    wg = in.take(a->w_gate, a->w_gate_stride, a->hidden, a->dim, es);
+    wu = in.take(a->w_up, a->w_up_stride, a->hidden, a->dim, es);
+    wd = in.take(a->w_down, a->w_down_stride, a->dim, a->hidden, es);
+    if (backward) dy = in.take(a->dy, a->dy_stride, a->rows, a->dim, es);
+  }
+};
+
+// The operand's columns as rows of an operand by columns.
+static MatOperand columns(const MatOperand& o, int64_t n, int64_t es) { return MatOperand{o.p, o.stride, (n * es + 15) / 16 * 16 / es}; }
+
+template <typename T, int BM, int BN>
+static void mlp_gated_tiles(const MlpInputs& in, int64_t C, int64_t M, int64_t F, const MlpGated<T>& epilogue, hipStream_t s) {
+  const MatWork work = mat_work(M, F, BM, BN, 1);
+  mat_launch(mlp_gated_kernel<T, BM, BN>, mat_grid(work, 256 / BM), (MatUsual<BM, BN>::THREADS), MlpGatedTile<T, BM, BN>::Ring::LDS, s, in.x, in.wg, in.wu, C, M, F, work,
+             epilogue);
+}
+template <typename T, int BM, int BN, typename W>
+static void mlp_gated_grad_tiles(const MlpInputs& in, const MatOperand& wd, int64_t C, int64_t M, int64_t F, const MlpGatedGrad<T>& epilogue,
+                                 hipStream_t s) {
+  const MatWork work = mat_work(M, F, BM, BN, 1);
+  mat_launch(mlp_gated_grad_kernel<T, BM, BN, W>, mat_grid(work, BM == 64 ? 3 : 2), W::THREADS, MlpGradTile<T, BM, BN, W>::Ring::LDS, s, in.x, in.wg, in.wu, in.dy, wd, C,
+             M, F, work, epilogue);
 }
 
 template <typename T> static void mlp_fwd(const fovi_gated_mlp_args* a, hipStream_t s) {
-  const int64_t M = a->rows, C = a->dim, F = a->hidden;
-  T* h = static_cast<T*>(a->workspace);
+  const int64_t M = a->rows, C = a->dim, F = a->hidden, Fp = wide(F);
+  const MlpInputs in(a, a->workspace, false);
+  in.in.copy(s);
+  T* h = reinterpret_cast<T*>(in.in.rest());
   T* gate = static_cast<T*>(a->saved);
-  const MlpGated<T> gated = {h, F, a->activation, gate, gate + F, 2 * F};
-  mlp_gated_kernel<T, 128, 64><<<mat_grid(tiles_of(M, 128) * tiles_of(F, 64)), 256, 0, s>>>(
-      operand<T>(a->x, a->x_stride, M), operand<T>(a->w_gate, a->w_gate_stride, F), operand<T>(a->w_up, a->w_up_stride, F), C, M, F, gated);
-  const MatSegments down = {{operand<T>(h, F, M)}, {operand<T>(a->w_down, a->w_down_stride, C)}, {F, 0}, 1};
+  const MlpGated<T> gated = {h, Fp, a->activation, gate, gate + F, 2 * F};
+  const int size = mat_tile_size(M, 2 * F, 1, sizeof(T) == 4, 256);
+  if constexpr (sizeof(T) == 2) {
+    if (size == 256) mlp_gated_tiles<T, 256, 128>(in, C, M, F, gated, s);
+  }
+  if (size == 256 && sizeof(T) == 2) {
+  } else if (size >= 128) mlp_gated_tiles<T, 128, 64>(in, C, M, F, gated, s);
+  else mlp_gated_tiles<T, 64, 64>(in, C, M, F, gated, s);
+  const MatSegments down = {{MatOperand{reinterpret_cast<char*>(h), Fp * static_cast<int64_t>(sizeof(T)), M}}, {in.wd}, {F, 0}, 1};
   const MlpLinear<T> linear = {static_cast<T*>(a->y), a->y_stride, static_cast<const T*>(a->residual), a->residual_stride};
-  mlp_linear<T, false, false>(down, M, C, linear, s);
+  mlp_linear<T, false, false>(down, M, C, F, 1, linear, s);
 }
 
-static int64_t aligned(int64_t n) { return (n + 255) & ~static_cast<int64_t>(255); }
-
 template <typename T> static void mlp_bwd(const fovi_gated_mlp_args* a, hipStream_t s) {
-  const int64_t M = a->rows, C = a->dim, F = a->hidden;
-  char* work = static_cast<char*>(a->workspace);
-  T* grad = reinterpret_cast<T*>(work);                             // [M, 2 F]: dgate, dup
-  T* h = reinterpret_cast<T*>(work + aligned(M * 2 * F * sizeof(T)));
-  float* part = reinterpret_cast<float*>(reinterpret_cast<char*>(h) + aligned(M * F * sizeof(T)));
-  const MatOperand x = operand<T>(a->x, a->x_stride, M), dy = operand<T>(a->dy, a->dy_stride, M);
-  const MatOperand wg = operand<T>(a->w_gate, a->w_gate_stride, F), wu = operand<T>(a->w_up, a->w_up_stride, F);
-  const MatOperand wd = operand<T>(a->w_down, a->w_down_stride, F); // by columns: k runs over its rows
+  const int64_t M = a->rows, C = a->dim, F = a->hidden, Fp = wide(F), es = sizeof(T);
+  const MlpInputs in(a, a->workspace, true);
+  in.in.copy(s);
+  T* grad = reinterpret_cast<T*>(in.in.rest());                     // [M, 2 Fp]: dgate, dup
+  T* h = reinterpret_cast<T*>(in.in.rest() + aligned(M * 2 * Fp * es));
+  float* part = reinterpret_cast<float*>(reinterpret_cast<char*>(h) + aligned(M * Fp * es));
+  const MatOperand wd = columns(in.wd, F, es);
   const T* gate = static_cast<const T*>(a->saved);
-  const MlpGatedGrad<T> gated = {grad, grad + F, h, 2 * F, F, a->activation, gate, gate + F, 2 * F};
-  if (gate) {
-    const MatSegments down = {{dy}, {wd}, {C, 0}, 1};
-    mlp_linear<T, false, true>(down, M, F, gated, s);
+  const MlpGatedGrad<T> gated = {grad, grad + Fp, h, 2 * Fp, Fp, a->activation, gate, gate + F, 2 * F};
+  if constexpr (sizeof(T) == 4) {
+    const MatSegments down = {{in.dy}, {wd}, {C, 0}, 1};
+    mlp_linear<T, false, true>(down, M, F, C, 1, gated, s);
   } else {
-    mlp_gated_grad_kernel<T, 128, 64><<<mat_grid(tiles_of(M, 128) * tiles_of(F, 64)), 256, 0, s>>>(x, wg, wu, dy, wd, C, M, F, gated);
+    const int size = mat_tile_size(M, 2 * F, 1, false, 256);
+    if (size >= 128) mlp_gated_grad_tiles<T, 128, 64, MatWaves<2, 2>>(in, wd, C, M, F, gated, s);
+    else mlp_gated_grad_tiles<T, 64, 64, MatWaves<2, 2>>(in, wd, C, M, F, gated, s);
   }
+  const char* dgate = reinterpret_cast<const char*>(grad);
   if (a->dx) {
-    const MatSegments both = {{operand<T>(grad, 2 * F, M), operand<T>(grad + F, 2 * F, M)},
-                              {operand<T>(a->w_gate, a->w_gate_stride, C), operand<T>(a->w_up, a->w_up_stride, C)}, {F, F}, 2};
-    mlp_linear<T, false, true>(both, M, C, MlpLinear<T>{static_cast<T*>(a->dx), C, nullptr, 0}, s);
+    const MatSegments both = {{MatOperand{dgate, 2 * Fp * es, M}, MatOperand{dgate + Fp * es, 2 * Fp * es, M}},
+                              {columns(in.wg, C, es), columns(in.wu, C, es)}, {F, F}, 2};
+    mlp_linear<T, false, true>(both, M, C, F, 1, MlpLinear<T>{static_cast<T*>(a->dx), C, nullptr, 0}, s);
   }
   if (a->dw_gate)
-    token_product<T>(operand<T>(grad, 2 * F, 2 * F), operand<T>(a->x, a->x_stride, C), M, 2 * F, C, part,
-                     MlpTwoRows<T>{{static_cast<T*>(a->dw_gate), static_cast<T*>(a->dw_up)}, F, C}, s);
+    token_product<T>(MatOperand{dgate, 2 * Fp * es, 2 * Fp}, columns(in.x, C, es), M, Fp + F, C, part,
+                     MlpTwoRows<T>{{static_cast<T*>(a->dw_gate), static_cast<T*>(a->dw_up)}, F, Fp, C}, s);
   if (a->dw_down)
-    token_product<T>(operand<T>(a->dy, a->dy_stride, C), operand<T>(h, F, F), M, C, F, part,
+    token_product<T>(columns(in.dy, C, es), MatOperand{reinterpret_cast<char*>(h), Fp * es, Fp}, M, C, F, part,
                      MlpLinear<T>{static_cast<T*>(a->dw_down), F, nullptr, 0}, s);
 }
 
@@ -259,23 +436,23 @@ extern "C" int64_t fovi_gated_mlp_saved_bytes(int64_t rows, int64_t dim, int64_t
   return dtype == FOVI_F32 && rows > 0 && hidden > 0 ? rows * 2 * hidden * 4 : 0;
 }
 
-extern "C" int64_t fovi_gated_mlp_fwd_workspace_bytes(int64_t rows, int64_t dim, int64_t hidden, int32_t dtype) {
-  (void)dim;
-  return rows > 0 && hidden > 0 ? rows * hidden * (dtype == FOVI_F32 ? 4 : 2) : 0;
+extern "C" int64_t fovi_gated_mlp_fwd_workspace_bytes(const fovi_gated_mlp_args* a) {
+  if (!a || a->rows < 1 || a->dim < 1 || a->hidden < 1) return 0;
+  return MlpInputs(a, nullptr, false).in.used() + a->rows * wide(a->hidden) * mlp_element(a);
 }
 
-extern "C" int64_t fovi_gated_mlp_bwd_workspace_bytes(int64_t rows, int64_t dim, int64_t hidden, int32_t dtype) {
-  if (rows < 1 || dim < 1 || hidden < 1) return 0;
-  const int64_t es = dtype == FOVI_F32 ? 4 : 2;
-  const int64_t a = token_shares(rows, 2 * hidden, dim) * 2 * hidden * dim, b = token_shares(rows, dim, hidden) * dim * hidden;
-  return aligned(rows * 2 * hidden * es) + aligned(rows * hidden * es) + (a > b ? a : b) * 4;
+extern "C" int64_t fovi_gated_mlp_bwd_workspace_bytes(const fovi_gated_mlp_args* a) {
+  if (!a || a->rows < 1 || a->dim < 1 || a->hidden < 1) return 0;
+  const int64_t es = mlp_element(a), rows = a->rows, C = a->dim, F = a->hidden, Fp = wide(F);
+  const int64_t up = token_shares(rows, Fp + F, C) * (Fp + F) * C, down = token_shares(rows, C, F) * C * F;
+  return MlpInputs(a, nullptr, true).in.used() + aligned(rows * 2 * Fp * es) + aligned(rows * Fp * es) + (up > down ? up : down) * 4;
 }
 
 extern "C" int fovi_gated_mlp_fwd(const fovi_gated_mlp_args* a, void* stream) {
   clear_error();
   if (mlp_check(a, "fovi_gated_mlp_fwd")) return 1;
   if (a->rows == 0) return 0;
-  const int64_t need = fovi_gated_mlp_fwd_workspace_bytes(a->rows, a->dim, a->hidden, a->dtype);
+  const int64_t need = fovi_gated_mlp_fwd_workspace_bytes(a);
   if (!a->y || !a->workspace || a->workspace_bytes < need) {
     set_error("fovi_gated_mlp_fwd: y and a workspace of %lld bytes needed", static_cast<long long>(need));
     return 1;
@@ -295,7 +472,7 @@ extern "C" int fovi_gated_mlp_bwd(const fovi_gated_mlp_args* a, void* stream) {
     set_error("fovi_gated_mlp_bwd: the forward's gate and up are needed");
     return 1;
   }
-  const int64_t need = fovi_gated_mlp_bwd_workspace_bytes(a->rows, a->dim, a->hidden, a->dtype);
+  const int64_t need = fovi_gated_mlp_bwd_workspace_bytes(a);
   if (!a->workspace || a->workspace_bytes < need) {
     set_error("fovi_gated_mlp_bwd: workspace of %lld bytes needed", static_cast<long long>(need));
     return 1;

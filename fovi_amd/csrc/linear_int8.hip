@@ -13,72 +13,131 @@ struct Int8Scales {
 };
 
 template <typename TO> struct Int8Linear {
+  static constexpr int STORES = sizeof(TO) / 2;        // of 16 bytes for a run of eight
   Int8Scales s;
   const float* bias; const TO* residual; int64_t residual_stride;
   TO* out; int64_t stride;
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const int32_t (&v)[1][4]) const {
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const int32_t (&v)[1][8]) const {
     const float sx = s.x[m];
-    float y[4], w[4], t[4];
-    load_four(s.w + n, count, w);
+    float y[8], w[8], t[8];
+    load_run(s.w + n, count, w);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = static_cast<float>(v[0][i]) * sx * w[i];
+    for (int i = 0; i < 8; ++i) y[i] = static_cast<float>(v[0][i]) * sx * w[i];
     if (bias) {
-      load_four(bias + n, count, t);
+      load_run(bias + n, count, t);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] += t[i];
+      for (int i = 0; i < 8; ++i) y[i] += t[i];
     }
     if (residual) {
-      load_four(residual + m * residual_stride + n, count, t);
+      load_run(residual + m * residual_stride + n, count, t);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] += t[i];
+      for (int i = 0; i < 8; ++i) y[i] += t[i];
     }
-    store_four(out + m * stride + n, count, y);
+    store_run(out + m * stride + n, count, y);
   }
 };
 
 template <typename TO> struct Int8Gated {
+  static constexpr int STORES = sizeof(TO) / 2;
   Int8Scales s;
   int act;
   TO* out; int64_t stride;
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const int32_t (&v)[2][4]) const {
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const int32_t (&v)[2][8]) const {
     const float sx = s.x[m];
-    float y[4], g[4], u[4];
-    load_four(s.w + n, count, g);
-    load_four(s.w2 + n, count, u);
+    float y[8], g[8], u[8];
+    load_run(s.w + n, count, g);
+    load_run(s.w2 + n, count, u);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 8; ++i)
       y[i] = mat_act<false>(static_cast<float>(v[0][i]) * sx * g[i], act) * (static_cast<float>(v[1][i]) * sx * u[i]);
-    store_four(out + m * stride + n, count, y);
+    store_run(out + m * stride + n, count, y);
   }
 };
 
+template <int BM, int BN, int NB, typename Epilogue> struct Int8Tile {
+  typedef MatPhase<int8_t, BM, BN, NB, false, false> Phase;
+  typedef MatRing<Phase::BYTES, 2 * Phase::MB * Phase::NN * Epilogue::STORES> Ring;
+};
+
 template <int BM, int BN, int NB, typename Epilogue>
-__global__ __launch_bounds__(256) void int8_kernel(MatOperand x, MatOperand w0, MatOperand w1, int64_t K, int64_t M, int64_t N,
-                                                   Epilogue epilogue) {
-  typedef MatCore<int8_t, BM, BN, NB, false, false> Core;
-  __shared__ __attribute__((aligned(16))) char lds[Core::LDS];
-  int64_t tm, tn;
-  if (!mat_tile((M + BM - 1) / BM, (N + BN - 1) / BN, tm, tn)) return;
-  typename Core::Acc acc[NB][Core::MB][Core::NN];
-  mat_clear(acc);
-  const MatOperand w[2] = {w0, w1};
-  Core::run(x, w, tm * BM, tn * BN, 0, K, lds, acc);
-  mat_finish<BM, BN, int32_t>(acc, tm * BM, tn * BN, M, N, epilogue);
+__global__ __launch_bounds__((MatUsual<BM, BN>::THREADS), 2) void int8_kernel(MatOperand x, MatOperand w0, MatOperand w1, int64_t K, int64_t M, int64_t N, MatWork work,
+                                                      Epilogue epilogue) {
+  typedef typename Int8Tile<BM, BN, NB, Epilogue>::Phase Phase;
+  typedef typename Int8Tile<BM, BN, NB, Epilogue>::Ring Ring;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  MatItem item(work), ahead(work);
+  if (!item.live()) return;
+  MatOperand w[NB];
+  w[0] = w0;
+  if (NB == 2) w[NB - 1] = w1;
+  Phase phase;
+  int64_t left = -1;                                   // of the tile `ahead`; -1: not begun
+  auto produce = [&](uint32_t to) __attribute__((always_inline)) {
+    if (left <= 0) {
+      if (left == 0) ahead.next();
+      if (!ahead.live()) return false;
+      left = K;
+      int64_t tm, tn;
+      ahead.place(work, tm, tn);
+      phase.open(x, w, tm * BM, tn * BN, 0);
+    }
+    phase.start(to, left);
+    left = left > Phase::BK ? left - Phase::BK : 0;
+    return true;
+  };
+  Ring ring(lds, produce);
+  typename Phase::Step step[2];
+  auto first_step = [&](const char* now) __attribute__((always_inline)) { step[0].read(now, 0); };
+  first_step(ring.now());
+  const int64_t stages = (K + Phase::BK - 1) / Phase::BK;
+  for (; item.live(); item.next()) {
+    typename Phase::Acc acc[NB][Phase::MB][Phase::NN];
+    mat_clear(acc);
+    Phase::run(ring, stages, step, acc, 0, produce, first_step);
+    int64_t tm, tn;
+    item.place(work, tm, tn);
+    ring.stored = mat_finish<typename Phase::Waves, BM, BN, int32_t>(acc, tm * BM, tn * BN, M, N, epilogue);
+  }
 }
+
+template <int BM, int BN, int NB, typename Epilogue>
+static void int8_tiles(const MatOperand& x, const MatOperand& w0, const MatOperand& w1, int64_t K, int64_t M, int64_t N,
+                       const Epilogue& epilogue, hipStream_t s) {
+  const MatWork work = mat_work(M, N, BM, BN, 1);
+  mat_launch(int8_kernel<BM, BN, NB, Epilogue>, mat_grid(work, 256 / BM), (MatUsual<BM, BN>::THREADS), Int8Tile<BM, BN, NB, Epilogue>::Ring::LDS, s, x, w0, w1, K, M, N, work,
+             epilogue);
+}
+
+template <int NB, typename Epilogue>
+static void int8_product(const MatOperand& x, const MatOperand& w0, const MatOperand& w1, int64_t K, int64_t M, int64_t N,
+                         const Epilogue& epilogue, hipStream_t s) {
+  const int size = mat_tile_size(M, N * NB, 1, false, 256);
+  if (size == 256) int8_tiles<256, 256 / NB, NB>(x, w0, w1, K, M, N, epilogue, s);
+  else if (size == 128) int8_tiles<128, 128 / NB, NB>(x, w0, w1, K, M, N, epilogue, s);
+  else int8_tiles<64, 64, NB>(x, w0, w1, K, M, N, epilogue, s);
+}
+
+struct Int8Inputs {
+  MatInputs in;
+  MatOperand x, w, w2;
+  Int8Inputs(const fovi_linear_int8_args* a, void* workspace) : in(workspace) {
+    x = in.take(a->x, a->x_stride, a->rows, a->inputs, 1);
+    w = in.take(a->weight, a->weight_stride, a->outputs, a->inputs, 1);
+    w2 = a->weight2 ? in.take(a->weight2, a->weight2_stride, a->outputs, a->inputs, 1) : w;
+  }
+};
 
 template <typename TO> static void int8_launch(const fovi_linear_int8_args* a, hipStream_t stream) {
   const int64_t M = a->rows, N = a->outputs, K = a->inputs;
-  const MatOperand x = {reinterpret_cast<const char*>(a->x), a->x_stride, M}, w = {reinterpret_cast<const char*>(a->weight), a->weight_stride, N},
-                   w2 = {reinterpret_cast<const char*>(a->weight2), a->weight2_stride, N};
+  const Int8Inputs in(a, a->workspace);
+  in.in.copy(stream);
   const Int8Scales scales = {a->x_scale, a->weight_scale, a->weight2_scale};
   TO* out = static_cast<TO*>(a->out);
-  const int64_t tm = (M + 127) / 128;
   if (a->weight2) {
-    const Int8Gated<TO> gated = {scales, a->activation, out, a->out_stride};
-    int8_kernel<128, 64, 2, Int8Gated<TO>><<<mat_grid(tm * ((N + 63) / 64)), 256, 0, stream>>>(x, w, w2, K, M, N, gated);
+    int8_product<2>(in.x, in.w, in.w2, K, M, N, Int8Gated<TO>{scales, a->activation, out, a->out_stride}, stream);
   } else {
     const Int8Linear<TO> linear = {scales, a->bias, static_cast<const TO*>(a->residual), a->residual_stride, out, a->out_stride};
-    int8_kernel<128, 128, 1, Int8Linear<TO>><<<mat_grid(tm * ((N + 127) / 128)), 256, 0, stream>>>(x, w, w, K, M, N, linear);
+    int8_product<1>(in.x, in.w, in.w, K, M, N, linear, stream);
   }
 }
 
@@ -86,9 +145,9 @@ template <typename TO> static void int8_launch(const fovi_linear_int8_args* a, h
 
 using namespace fovi;
 
-extern "C" int64_t fovi_linear_int8_workspace_bytes(int64_t rows, int64_t inputs, int64_t outputs, int32_t gated) {
-  (void)rows; (void)inputs; (void)outputs; (void)gated;
-  return 0;
+extern "C" int64_t fovi_linear_int8_workspace_bytes(const fovi_linear_int8_args* a) {
+  if (!a || a->rows < 1 || a->inputs < 1 || a->outputs < 1) return 0;
+  return Int8Inputs(a, nullptr).in.used();
 }
 
 extern "C" int fovi_linear_int8(const fovi_linear_int8_args* a, void* stream) {
@@ -108,7 +167,12 @@ extern "C" int fovi_linear_int8(const fovi_linear_int8_args* a, void* stream) {
     return 1;
   }
   if (a->rows == 0 || a->outputs == 0) return 0;
-  if ((a->rows + 127) / 128 > 0x7fffff00ll / ((a->outputs + 63) / 64)) { set_error("fovi_linear_int8: too large"); return 1; }
+  if (a->rows > (1ll << 31) || (a->rows + 63) / 64 > (1ll << 30) / ((a->outputs + 63) / 64)) { set_error("fovi_linear_int8: too large"); return 1; }
+  const int64_t need = fovi_linear_int8_workspace_bytes(a);
+  if (need && (!a->workspace || a->workspace_bytes < need)) {
+    set_error("fovi_linear_int8: workspace of %lld bytes needed", static_cast<long long>(need));
+    return 1;
+  }
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (a->out_dtype == FOVI_BF16) int8_launch<uint16_t>(a, s);
   else int8_launch<float>(a, s);

@@ -2,10 +2,15 @@
 // reduction axis contiguous ("rows") or strided ("columns"), several products of the same left operand at once, and
 // the caller's own work on the sums (an epilogue) before they are written.
 //
-// out[m, n] = sum_k x[m, k] w[n, k]. A workgroup of four waves owns a tile of BM x BN and walks k in steps of 128 bytes a row
-// (64 bf16, 128 int8, 32 fp32 elements). Tiles lie in LDS in 16-byte pieces that are swapped within a row
-// (XOR) so that the lanes of a read spread over the banks. The matrix instruction takes w as its first operand:
-// a lane then holds one row m and runs of four adjacent n of its sums, which are written as they are.
+// out[m, n] = sum_k x[m, k] w[n, k]. A workgroup of four waves takes tiles of BM x BN one after another and walks k in
+// stages of 128 bytes a row (64 bf16, 128 int8, 32 fp32 elements): whole cache lines, since parts of one cost as much
+// (loads from L2 into LDS reach 34 TB/s by 128 bytes and 17 by 64). Loads go straight into LDS, a stage ahead of the
+// products and past the end of a tile into the next one, so that a tile's first loads run beside the epilogue of the one
+// before. The matrix instructions of a step run on registers that were read during the step before. There is one
+// barrier a stage, in front of its last step: by then the stage has been read whole (its place is free for the
+// loads of the stage after the next) and the next stage has landed, whose first step is read beside the last products.
+// Within a row of LDS 16-byte pieces are swapped (XOR) so that the lanes of a read spread over the banks. The
+// matrix instruction takes w as its first operand: a lane then holds one row m of the sums and runs of adjacent n.
 #pragma once
 
 #include "common.h"
@@ -18,16 +23,17 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 // One operand: element (r, k) at p + r * stride + k * size where k is contiguous, else p + k * stride + r * size.
-// stride in bytes; `extent` rows r.
+// stride in bytes; `extent` rows r. Starts, strides and contiguous runs are multiples of 16 bytes.
 struct MatOperand {
   const char* p;
   int64_t stride, extent;
 };
 
 template <typename T> struct Mat;
-template <> struct Mat<uint16_t> { typedef f32x16 Acc; typedef float Sum; static constexpr int BK = 64; };
-template <> struct Mat<float> { typedef f32x16 Acc; typedef float Sum; static constexpr int BK = 32; };
-template <> struct Mat<int8_t> { typedef i32x16 Acc; typedef int32_t Sum; static constexpr int BK = 128; };
+template <> struct Mat<uint16_t> { typedef f32x16 Acc; typedef float Sum; };
+template <> struct Mat<float> { typedef f32x16 Acc; typedef float Sum; };
+template <> struct Mat<int8_t> { typedef i32x16 Acc; typedef int32_t Sum; };
+template <typename T> constexpr int mat_bk() { return 128 / sizeof(T); }
 
 // One step of a product: 16 bytes of 32 rows of either operand; lanes 0 .. 31 hold one piece of k, 32 .. 63 the next.
 __device__ __forceinline__ f32x16 mat_step(uint16_t, u32x4 w, u32x4 x, f32x16 c) {
@@ -43,63 +49,19 @@ __device__ __forceinline__ i32x16 mat_step(int8_t, u32x4 w, u32x4 x, i32x16 c) {
   return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, w), __builtin_bit_cast(i32x4, x), c, 0, 0, 0);
 }
 
-// 16 bytes of a run of `len` bytes from `at` on, at any alignment, zeros from its end on.
-__device__ __forceinline__ u32x4 mat_piece(const char* run, int64_t at, int64_t len) {
-  u32x4 u = {0, 0, 0, 0};
-  if (at + 16 <= len) {
-    __builtin_memcpy(&u, run + at, 16);
-  } else if (at < len && len >= 16) {                  // the run's last 16 bytes, shifted down
-    uint64_t w[2];
-    __builtin_memcpy(w, run + len - 16, 16);
-    const int over = static_cast<int>(at + 16 - len) * 8, bits = over & 63;
-    if (over >= 64) { w[0] = w[1]; w[1] = 0; }
-    w[0] = (w[0] >> bits) | (w[1] << 1 << (63 - bits));
-    w[1] >>= bits;
-    __builtin_memcpy(&u, w, 16);
-  } else if (at < len) {                               // a run of fewer than 16 bytes: at is 0
-    uint64_t w[2] = {0, 0};
-    for (int64_t i = 0; i < len; ++i) w[i >> 3] |= static_cast<uint64_t>(static_cast<uint8_t>(run[i])) << ((i & 7) * 8);
-    __builtin_memcpy(&u, w, 16);
-  }
-  return u;
-}
-
-// The tile of an operand in LDS: NR rows of 128 bytes of k, or (COL) BK rows of NR elements.
-template <typename T, int NR, bool COL> struct MatTile {
-  static constexpr int ES = sizeof(T);
+// A stage of an operand in LDS: NR rows of 128 bytes of k, or (COL) k rows of NR elements.
+template <typename T, int NR, bool COL, int WAVES> struct MatTile {
+  static constexpr int ES = sizeof(T), BK = mat_bk<T>();
   static constexpr int BYTES = NR * 128;
   static constexpr int PIECES = COL ? NR * ES / 16 : 8;          // 16-byte pieces of an LDS row
-  static constexpr int PER = NR * 8 / 256;                       // pieces a thread loads
+  static constexpr int LOADS = BYTES / 1024 / WAVES;             // loads a wave makes for a stage
 
   static __device__ __forceinline__ int at(int r, int piece) {
     int s;
     if (!COL) s = (r >> 1) & 7;
-    else s = (ES == 2 ? (r & 3) << 2 : ((r >> 2) & 1) << 3) & (PIECES - 1);
+    else if (ES == 4) s = ((r >> 2) & 1) << 3;
+    else s = PIECES == 24 ? ((r >> 1) & 1) << 2 : ((r & 3) << 2) & (PIECES - 1);
     return r * PIECES * 16 + ((piece ^ s) << 4);
-  }
-
-  u32x4 v[PER];
-  // The tile of rows r0 .., elements k0 .. of k; rows behind the last are the last row again (their sums are not
-  // written), elements behind k_end zeros.
-  __device__ __forceinline__ void load(const MatOperand& o, int64_t r0, int64_t k0, int64_t k_end) {
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int id = threadIdx.x + 256 * i, a = id / PIECES, b = id % PIECES;
-      if (!COL) {
-        const int64_t r = r0 + a < o.extent ? r0 + a : o.extent - 1;
-        v[i] = mat_piece(o.p + r * o.stride, k0 * ES + b * 16, k_end * ES);
-      } else {
-        const int64_t k = k0 + a;
-        v[i] = k < k_end ? mat_piece(o.p + k * o.stride, r0 * ES + b * 16, o.extent * ES) : u32x4{0, 0, 0, 0};
-      }
-    }
-  }
-  __device__ __forceinline__ void put(char* lds) const {
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int id = threadIdx.x + 256 * i;
-      *reinterpret_cast<u32x4*>(lds + at(id / PIECES, id % PIECES)) = v[i];
-    }
   }
   // Step s (of 4) of the 32 rows from r on.
   static __device__ __forceinline__ u32x4 read(const char* lds, int r, int s) {
@@ -123,52 +85,184 @@ template <typename T, int NR, bool COL> struct MatTile {
   }
 };
 
-// acc[b] += the products over k_begin .. k_end of the tile's rows of x and of w[b], b < NB. Every wave holds BM / 64 x
-// BN / 64 blocks of 32 x 32 of each.
-template <typename T, int BM, int BN, int NB, bool CX, bool CW>
-struct MatCore {
-  typedef typename Mat<T>::Acc Acc;
-  typedef MatTile<T, BM, CX> TX;
-  typedef MatTile<T, BN, CW> TW;
-  static constexpr int MB = BM / 64, NN = BN / 64, BK = Mat<T>::BK;
-  static constexpr int LDS = TX::BYTES + NB * TW::BYTES;
+// The loads of an operand's stages. A wave's load writes 64 consecutive pieces of LDS, so the swap of pieces within a row
+// is in the address that each lane reads. Rows behind the last are the last row again (their sums are not written). Pieces
+// behind the last element of k, or behind the rows of an operand by columns, are read behind the buffer's end, where
+// loads give zeros.
+template <typename T, int NR, bool COL, int WAVES> struct MatLoader {
+  typedef MatTile<T, NR, COL, WAVES> Tile;
+  static constexpr int ES = sizeof(T), BK = mat_bk<T>(), LOADS = Tile::LOADS;
+  static constexpr uint32_t END = 0x7fffff00u, OUTSIDE = 0x7fffff80u;
+  uint32_t off[LOADS];
+  uint64_t base;
+  int64_t step;
 
-  template <int NA>
-  static __device__ __forceinline__ void run(const MatOperand& x, const MatOperand* w, int64_t m0, int64_t n0, int64_t k_begin,
-                                             int64_t k_end, char* lds, Acc (&acc)[NA][MB][NN], int first = 0) {
-    const int wave = threadIdx.x >> 6, wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
-    TX tx;
-    TW tw[NB];
-    auto load = [&](int64_t k) {
-      tx.load(x, m0, k, k_end);
+  static __device__ __forceinline__ int piece(int i) { return ((threadIdx.x >> 6) * LOADS + i) * 64 + (threadIdx.x & 63); }
+  // The place of a lane's piece in k: its first byte, or (COL) its k row.
+  static __device__ __forceinline__ int place(int i) {
+    const int id = piece(i), r = id / Tile::PIECES;
+    return COL ? r : Tile::at(r, id % Tile::PIECES) - r * 128;
+  }
+  __device__ __forceinline__ void open(const MatOperand& o, int64_t r0, int64_t k0) {
 #pragma unroll
-      for (int b = 0; b < NB; ++b) tw[b].load(w[b], n0, k, k_end);
-    };
-    load(k_begin);
-    for (int64_t k = k_begin; k < k_end; k += BK) {
-      __syncthreads();
-      tx.put(lds);
-#pragma unroll
-      for (int b = 0; b < NB; ++b) tw[b].put(lds + TX::BYTES + b * TW::BYTES);
-      __syncthreads();
-      if (k + BK < k_end) load(k + BK);
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        u32x4 fx[MB], fw[NB][NN];
-#pragma unroll
-        for (int i = 0; i < MB; ++i) fx[i] = TX::read(lds, wm + 32 * i, s);
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-          for (int j = 0; j < NN; ++j) fw[b][j] = TW::read(lds + TX::BYTES + b * TW::BYTES, wn + 32 * j, s);
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-          for (int i = 0; i < MB; ++i)
-#pragma unroll
-            for (int j = 0; j < NN; ++j) acc[first + b][i][j] = mat_step(T(), fw[b][j], fx[i], acc[first + b][i][j]);
+    for (int i = 0; i < LOADS; ++i) {
+      const int id = piece(i), r = id / Tile::PIECES;
+      const int b = Tile::at(r, id % Tile::PIECES) - r * Tile::PIECES * 16;    // the swap is its own inverse
+      const int stride = static_cast<int>(o.stride);
+      if (!COL) {
+        const int last = static_cast<int>(o.extent - 1 - r0 < NR ? o.extent - 1 - r0 : NR);
+        off[i] = static_cast<uint32_t>((r < last ? r : last) * stride + b);
+      } else {
+        off[i] = r0 * ES + b < o.extent * ES ? static_cast<uint32_t>(r * stride + b) : OUTSIDE;
       }
     }
+    base = reinterpret_cast<uint64_t>(o.p) + (COL ? k0 * o.stride + r0 * ES : r0 * o.stride + k0 * ES);
+    step = COL ? BK * o.stride : 128;
+  }
+  // Starts the loads of the stage whose k has `left` elements, and goes on to the next stage.
+  __device__ __forceinline__ void start(uint32_t lds, int64_t left) {
+    const i32x4 rsrc = {__builtin_amdgcn_readfirstlane(static_cast<int>(base)), __builtin_amdgcn_readfirstlane(static_cast<int>(base >> 32)),
+                        static_cast<int>(END), 0x20000};
+    const bool whole = left >= BK;
+    const int limit = static_cast<int>(COL ? left : left * ES);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const uint32_t to = lds + ((threadIdx.x >> 6) * LOADS + i) * 1024;
+      const uint32_t from = whole || place(i) < limit ? off[i] : OUTSIDE;
+      // m0, the place in LDS, is read by the load: one wait state behind its writing
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                   :: "s"(__builtin_amdgcn_readfirstlane(to)), "v"(from), "s"(rsrc) : "memory");
+    }
+    base += step;
+  }
+};
+
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)p));
+}
+
+// The waves of a workgroup, WM by WN over its tile.
+template <int WM, int WN> struct MatWaves {
+  static constexpr int M = WM, N = WN, ALL = M * N, THREADS = 64 * ALL;
+  static __device__ __forceinline__ int m() { return (threadIdx.x >> 6) / N; }
+  static __device__ __forceinline__ int n() { return (threadIdx.x >> 6) % N; }
+};
+
+// Two by two; two by four for tiles of 256 rows, or four by two with 192 columns.
+template <int BM, int BN> using MatUsual = MatWaves<(BM == 256 && BN == 192 ? 4 : 2), (BM == 256 && BN != 192 ? 4 : 2)>;
+
+// A run of stages: NB products of the tile's rows of x.
+template <typename T, int BM, int BN, int NB, bool CX, bool CW, typename W = MatUsual<BM, BN>>
+struct MatPhase {
+  typedef typename Mat<T>::Acc Acc;
+  typedef W Waves;
+  typedef MatTile<T, BM, CX, Waves::ALL> TX;
+  typedef MatTile<T, BN, CW, Waves::ALL> TW;
+  static constexpr int MB = BM / 32 / Waves::M, NN = BN / 32 / Waves::N, BK = mat_bk<T>();
+  static constexpr int BYTES = TX::BYTES + NB * TW::BYTES, LOADS = TX::LOADS + NB * TW::LOADS;
+
+  MatLoader<T, BM, CX, Waves::ALL> lx;
+  MatLoader<T, BN, CW, Waves::ALL> lw[NB];
+
+  __device__ __forceinline__ void open(const MatOperand& x, const MatOperand (&w)[NB], int64_t m0, int64_t n0, int64_t k0) {
+    lx.open(x, m0, k0);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) lw[b].open(w[b], n0, k0);
+  }
+  __device__ __forceinline__ void start(uint32_t lds, int64_t left) {
+    lx.start(lds, left);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) lw[b].start(lds + TX::BYTES + b * TW::BYTES, left);
+  }
+  // The operands of a step in registers. Every wave holds MB x NN blocks of 32 x 32 of each product.
+  struct Step {
+    u32x4 x[MB], w[NB][NN];
+    __device__ __forceinline__ void read(const char* lds, int s) {
+      const int wm = Waves::m() * (BM / Waves::M), wn = Waves::n() * (BN / Waves::N);
+#pragma unroll
+      for (int i = 0; i < MB; ++i) x[i] = TX::read(lds, wm + 32 * i, s);
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int j = 0; j < NN; ++j) w[b][j] = TW::read(lds + TX::BYTES + b * TW::BYTES, wn + 32 * j, s);
+    }
+    // acc[first + b] += the products.
+    template <int NA>
+    __device__ __forceinline__ void multiply(Acc (&acc)[NA][MB][NN], int first) const {
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+          for (int j = 0; j < NN; ++j) acc[first + b][i][j] = mat_step(T(), w[b][j], x[i], acc[first + b][i][j]);
+    }
+  };
+  // The products of `stages` stages. step[0] holds the first step of the first one; first_step(lds) reads that of the
+  // stage behind the last one, if there is one.
+  template <int NA, typename Ring, typename Produce, typename FirstStep>
+  static __device__ __forceinline__ void run(Ring& ring, int64_t stages, Step (&step)[2], Acc (&acc)[NA][MB][NN], int first,
+                                             const Produce& produce, const FirstStep& first_step) {
+    for (int64_t t = stages; t > 0; --t) {
+      const char* now = ring.now();
+#pragma unroll
+      for (int s = 0; s < 3; ++s) {
+        step[(s + 1) & 1].read(now, s + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        step[s & 1].multiply(acc, first);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (ring.advance(produce)) {
+        if (t > 1) step[0].read(ring.now(), 0);
+        else first_step(ring.now());
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      step[1].multiply(acc, first);
+    }
+  }
+  // The same where the sums leave registers for one step only: its reads are waited for, beside another wave's products.
+  template <int NA, typename Ring, typename Produce>
+  static __device__ __forceinline__ void run_lean(Ring& ring, int64_t stages, Acc (&acc)[NA][MB][NN], int first, const Produce& produce) {
+    Step step;
+    for (int64_t t = stages; t > 0; --t) {
+      const char* now = ring.now();
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        step.read(now, s);
+        if (s == 3) ring.advance(produce);
+        __builtin_amdgcn_sched_barrier(0);
+        step.multiply(acc, first);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+};
+
+// The stages of a workgroup, two in LDS. produce(lds) starts the loads of the next stage; false: there is none left.
+// Loads and stores of a wave end in the order of their issue, so that a stage has landed when no more is outstanding than was
+// issued behind it: the STORES of an epilogue that was run since (at least so many).
+template <int BYTES, int STORES> struct MatRing {
+  static constexpr int LDS = 2 * BYTES;
+  static_assert(STORES < 64, "more than the counter holds");
+  const char* lds;
+  int at;                                              // the stage being multiplied is in this half
+  bool more;                                           // whether the next one was started
+  bool stored;                                         // whether an epilogue has run since then
+  template <typename Produce> __device__ __forceinline__ MatRing(const char* memory, const Produce& produce)
+      : lds(memory), at(0), stored(false) {
+    produce(lds_address(lds));
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    more = produce(lds_address(lds) + BYTES);
+  }
+  __device__ __forceinline__ const char* now() const { return lds + at * BYTES; }
+  // On to the next stage (false: none), when every wave has read this one and everybody's loads of the next have landed.
+  template <typename Produce> __device__ __forceinline__ bool advance(const Produce& produce) {
+    if (!more) return false;
+    if (stored) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(STORES) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    stored = false;
+    more = produce(lds_address(lds) + at * BYTES);
+    at ^= 1;
+    return true;
   }
 };
 
@@ -184,52 +278,66 @@ __device__ __forceinline__ void mat_clear(Acc (&acc)[NA][MB][NN]) {
         for (int r = 0; r < 16; ++r) acc[b][i][j][r] = 0;
 }
 
-// epilogue(m, n, count, v): the sums v[b][0 .. count) of row m from column n on, in runs of four.
-template <int BM, int BN, typename Sum, typename Acc, int NA, int MB, int NN, typename Epilogue>
-__device__ __forceinline__ void mat_finish(const Acc (&acc)[NA][MB][NN], int64_t m0, int64_t n0, int64_t M, int64_t N,
-                                           const Epilogue& epilogue) {
-  const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
+// epilogue(m, n, count, v): the sums v[b][0 .. count) of row m from column n on, in runs of eight. A lane's block holds four
+// adjacent columns of every eight, the lane 32 further on the other four: the two swap halves of two such runs.
+template <typename Waves, int BM, int BN, typename Sum, bool WHOLE, typename Acc, int NA, int MB, int NN, typename Epilogue>
+__device__ __forceinline__ void mat_runs(const Acc (&acc)[NA][MB][NN], int64_t m0, int64_t n0, int64_t M, int64_t N, const Epilogue& epilogue) {
+  const int l = threadIdx.x & 63;
 #pragma unroll
-  for (int i = 0; i < MB; ++i) {
-    const int64_t m = m0 + (wave >> 1) * (BM / 2) + 32 * i + (l & 31);
-    if (m >= M) continue;
+  for (int j = 0; j < NN; ++j)
 #pragma unroll
-    for (int j = 0; j < NN; ++j)
+    for (int q = 0; q < 4; q += 2) {
+      const int64_t n = n0 + Waves::n() * (BN / Waves::N) + 32 * j + 8 * q + 8 * (l >> 5);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int64_t n = n0 + (wave & 1) * (BN / 2) + 32 * j + 8 * q + 4 * (l >> 5);
-        if (n >= N) continue;
-        Sum v[NA][4];
+      for (int i = 0; i < MB; ++i) {
+        const int64_t m = m0 + Waves::m() * (BM / Waves::M) + 32 * i + (l & 31);
+        Sum v[NA][8];
 #pragma unroll
         for (int b = 0; b < NA; ++b)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[b][e] = acc[b][i][j][4 * q + e];
-        epilogue(m, n, static_cast<int>(N - n < 4 ? N - n : 4), v);
+          for (int e = 0; e < 4; ++e) {
+            const auto t = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, static_cast<Sum>(acc[b][i][j][4 * q + e])),
+                                                            __builtin_bit_cast(uint32_t, static_cast<Sum>(acc[b][i][j][4 * q + 4 + e])), false, false);
+            const uint32_t t0 = t[0], t1 = t[1];       // (a bit cast of t[1] itself takes t[0])
+            v[b][e] = __builtin_bit_cast(Sum, t0);
+            v[b][4 + e] = __builtin_bit_cast(Sum, t1);
+          }
+        if (WHOLE) epilogue(m, n, 8, v);
+        else if (m < M && n < N) epilogue(m, n, static_cast<int>(N - n < 8 ? N - n : 8), v);
+        __builtin_amdgcn_sched_barrier(0);             // (mixed, the runs take more registers than there are)
       }
-  }
+    }
+}
+template <typename Waves, int BM, int BN, typename Sum, typename Acc, int NA, int MB, int NN, typename Epilogue>
+__device__ __forceinline__ bool mat_finish(const Acc (&acc)[NA][MB][NN], int64_t m0, int64_t n0, int64_t M, int64_t N,
+                                           const Epilogue& epilogue) {
+  const bool whole = m0 + BM <= M && n0 + BN <= N;     // every lane stores every run
+  if (whole) mat_runs<Waves, BM, BN, Sum, true>(acc, m0, n0, M, N, epilogue);
+  else mat_runs<Waves, BM, BN, Sum, false>(acc, m0, n0, M, N, epilogue);
+  return whole;
 }
 
-// Four (or `count`) adjacent elements as floats, and back.
-template <typename T> __device__ __forceinline__ void load_four(const T* p, int count, float (&v)[4]) {
-  T e[4];
-  if (count == 4) {
+// Eight (or `count`) adjacent elements as floats, and back.
+template <typename T> __device__ __forceinline__ void load_run(const T* p, int count, float (&v)[8]) {
+  T e[8];
+  if (count == 8) {
     __builtin_memcpy(e, p, sizeof(e));
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) e[i] = i < count ? p[i] : T(0);
+    for (int i = 0; i < 8; ++i) e[i] = i < count ? p[i] : T(0);
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = Elem<T>::load(e + i);
+  for (int i = 0; i < 8; ++i) v[i] = Elem<T>::load(e + i);
 }
-template <typename T> __device__ __forceinline__ void store_four(T* p, int count, const float (&v)[4]) {
-  T e[4];
+template <typename T> __device__ __forceinline__ void store_run(T* p, int count, const float (&v)[8]) {
+  T e[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) Elem<T>::store(e + i, v[i]);
-  if (count == 4) {
+  for (int i = 0; i < 8; ++i) Elem<T>::store(e + i, v[i]);
+  if (count == 8) {
     __builtin_memcpy(p, e, sizeof(e));
   } else {
 #pragma unroll
-    for (int i = 0; i < 3; ++i)
+    for (int i = 0; i < 7; ++i)
       if (i < count) p[i] = e[i];
   }
 }
@@ -255,15 +363,117 @@ template <bool EXACT> __device__ __forceinline__ void mat_act_grad(float z, int 
   }
 }
 
-// Tile number of a workgroup: an XCD works on one range of tiles, the tiles of a row of tiles one after another, so
-// that they share x in its L2. false: none is left.
-__device__ __forceinline__ bool mat_tile(int64_t tiles_m, int64_t tiles_n, int64_t& tm, int64_t& tn) {
-  const int64_t tile = xcd_tile(blockIdx.x, gridDim.x);
-  if (tile >= tiles_m * tiles_n) return false;
-  tm = tile / tiles_n;
-  tn = tile - tm * tiles_n;
-  return true;
+// The tiles of a launch: `tiles` for each share of k, `items` in all. An XCD works on one range of them, its
+// workgroups on neighbours. Tiles follow one another along n, in bands of `band` rows of tiles that are walked
+// column by column, so that the 32 tiles that an XCD works on at a time form a block of 8 x 4 or so: the rows of x and w
+// that they share come from its L2.
+struct MatWork {
+  uint32_t tiles_m, tiles_n, tiles, items, band;
+};
+struct MatItem {
+  uint32_t i, end, step;
+  __device__ __forceinline__ explicit MatItem(const MatWork& w) {
+    const uint32_t per = (w.items + 7) >> 3, xcd = blockIdx.x & 7;
+    i = xcd * per + (blockIdx.x >> 3);
+    end = (xcd + 1) * per < w.items ? (xcd + 1) * per : w.items;
+    step = gridDim.x >> 3;
+  }
+  __device__ __forceinline__ bool live() const { return i < end; }
+  __device__ __forceinline__ void next() { i += step; }
+  __device__ __forceinline__ int64_t share(const MatWork& w) const { return i / w.tiles; }
+  __device__ __forceinline__ void place(const MatWork& w, int64_t& m, int64_t& n) const {
+    const uint32_t t = i % w.tiles, band = w.band * w.tiles_n, g = t / band, r = t - g * band;
+    const uint32_t rows = w.tiles_m - g * w.band < w.band ? w.tiles_m - g * w.band : w.band;
+    m = g * w.band + r % rows;
+    n = r / rows;
+  }
+};
+inline int64_t mat_tiles(int64_t M, int64_t N, int bm, int bn) { return (M + bm - 1) / bm * ((N + bn - 1) / bn); }
+inline MatWork mat_work(int64_t M, int64_t N, int bm, int bn, int64_t shares) {
+  const uint32_t tm = static_cast<uint32_t>((M + bm - 1) / bm), tn = static_cast<uint32_t>((N + bn - 1) / bn);
+  return MatWork{tm, tn, tm * tn, static_cast<uint32_t>(tm * tn * shares), tn <= 8 ? 4u : 8u};
 }
-inline unsigned mat_grid(int64_t tiles) { return static_cast<unsigned>((tiles + 7) / 8 * 8); }
+// Workgroups: `each` on each of 256 compute units, a multiple of the 8 XCDs.
+inline unsigned mat_grid(const MatWork& w, int each) {
+  const unsigned n = (w.items + 7) / 8 * 8;
+  return n < 256u * each ? n : 256u * each;
+}
+
+// Columns of a tile of 256 rows: 192 where that leaves less of the last one empty.
+inline int mat_columns(int64_t N) { return (N + 191) / 192 * 192 < (N + 255) / 256 * 256 ? 192 : 256; }
+
+// The tile of a product of M x N sums (`shares` times): of 256, 128 or 64 rows, whichever ends first by the time that a
+// compute unit takes for a stage of its workgroups, one, two or four of them. A stage of 64 K sums took 1, 1.13 and 1.6 in
+// tiles of these sizes (131072 x 1024 by 384, bf16: 129, 147 and 208 us; 131072 x 384 by 2 x 1024: 300, 344 and 432): small
+// ones read more bytes a product from L2 and LDS. fp32 products are slow enough for all sizes to keep up, and tiles of 256
+// rows are not built for them.
+inline int mat_tile_size(int64_t M, int64_t N, int64_t shares, bool fp32, int columns) {
+  const int64_t l = (mat_tiles(M, N, 256, columns) * shares + 255) / 256 * (fp32 ? 1 << 20 : columns);
+  const int64_t m = (mat_tiles(M, N, 128, 128) * shares + 511) / 512 * (fp32 ? 128 : 145);
+  const int64_t s = (mat_tiles(M, N, 64, 64) * shares + 1023) / 1024 * (fp32 ? 64 : 102);
+  return l <= m && l <= s ? 256 : m <= s ? 128 : 64;
+}
+
+template <typename Kernel, typename... Args>
+inline void mat_launch(Kernel kernel, unsigned grid, int threads, size_t lds, hipStream_t stream, Args... args) {
+  if (lds > 65536 && reserve_dynamic_lds(reinterpret_cast<const void*>(kernel), lds) != hipSuccess) return;
+  kernel<<<grid, threads, lds, stream>>>(args...);
+}
+
+// 16 bytes of a run of `len` bytes from `at` on, at any alignment, zeros from its end on.
+__device__ __forceinline__ u32x4 mat_piece(const char* run, int64_t at, int64_t len) {
+  u32x4 u = {0, 0, 0, 0};
+  if (at + 16 <= len) {
+    __builtin_memcpy(&u, run + at, 16);
+  } else if (at < len && len >= 16) {                  // the run's last 16 bytes, shifted down
+    uint64_t w[2];
+    __builtin_memcpy(w, run + len - 16, 16);
+    const int over = static_cast<int>(at + 16 - len) * 8, bits = over & 63;
+    if (over >= 64) { w[0] = w[1]; w[1] = 0; }
+    w[0] = (w[0] >> bits) | (w[1] << 1 << (63 - bits));
+    w[1] >>= bits;
+    __builtin_memcpy(&u, w, 16);
+  } else if (at < len) {                               // a run of fewer than 16 bytes: at is 0
+    uint64_t w[2] = {0, 0};
+    for (int64_t i = 0; i < len; ++i) w[i >> 3] |= static_cast<uint64_t>(static_cast<uint8_t>(run[i])) << ((i & 7) * 8);
+    __builtin_memcpy(&u, w, 16);
+  }
+  return u;
+}
+
+// Matrices that the loads do not take as they are (rows of other lengths, starts or strides than whole 16-byte pieces)
+// are copied in front of a product, their rows filled up with zeros: one launch for all of a call.
+struct MatCopies {
+  static constexpr int MOST = 5;
+  struct { const char* from; char* to; int64_t stride, rows, len; } m[MOST];
+  int n;
+};
+__global__ void mat_copy_kernel(MatCopies c);
+
+// A call's operands: take() gives the matrix that the kernels read, which is the caller's or a copy in the workspace.
+class MatInputs {
+ public:
+  explicit MatInputs(void* workspace) : at_(static_cast<char*>(workspace)), start_(at_) { copies_.n = 0; }
+  // rows x cols elements of `es` bytes, `stride` elements apart; the result's stride is in bytes.
+  MatOperand take(const void* p, int64_t stride, int64_t rows, int64_t cols, int64_t es) {
+    const int64_t bytes = cols * es;
+    if ((reinterpret_cast<uintptr_t>(p) | stride * es | bytes) % 16 == 0 && stride * es < (1 << 22))
+      return MatOperand{static_cast<const char*>(p), stride * es, rows};
+    const int64_t wide = (bytes + 15) / 16 * 16;
+    auto& m = copies_.m[copies_.n++];
+    m.from = static_cast<const char*>(p); m.to = at_; m.stride = stride * es; m.rows = rows; m.len = bytes;
+    const MatOperand o = {at_, wide, rows};
+    at_ += (rows * wide + 255) / 256 * 256;
+    return o;
+  }
+  int64_t used() const { return at_ - start_; }
+  char* rest() const { return at_; }
+  void copy(hipStream_t s) const;
+
+ private:
+  MatCopies copies_;
+  char* at_;
+  char* start_;
+};
 
 }  // namespace fovi

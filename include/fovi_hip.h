@@ -953,7 +953,8 @@ int fovi_dequantize_rows(const int8_t* q, const float* scale, int64_t rows, int6
  * and with weight2 (then without bias and residual) act(that) * the same product with weight2 and weight2_scale.
  * Strides are in elements between rows, elements adjacent, at any alignment. Sums are exact in int32 (up to 131072 inputs).
  * out and residual: out_dtype, F32 or BF16; bias fp32 (may be NULL, as may residual). The workspace
- * (fovi_linear_int8_workspace_bytes, may be 0; 16-byte aligned) holds partial sums where the inputs are split over workgroups.
+ * (fovi_linear_int8_workspace_bytes of the arguments, may be 0; 16-byte aligned) holds copies of
+ * matrices whose rows are not whole, aligned 16-byte pieces.
  */
 enum fovi_gate_act { FOVI_GATE_SILU = 0, FOVI_GATE_GELU = 1 };
 
@@ -979,7 +980,7 @@ typedef struct fovi_linear_int8_args {
   int64_t workspace_bytes;
 } fovi_linear_int8_args;
 
-int64_t fovi_linear_int8_workspace_bytes(int64_t rows, int64_t inputs, int64_t outputs, int32_t gated);
+int64_t fovi_linear_int8_workspace_bytes(const fovi_linear_int8_args* args);
 int fovi_linear_int8(const fovi_linear_int8_args* args, void* stream);
 
 /*
@@ -992,7 +993,8 @@ int fovi_linear_int8(const fovi_linear_int8_args* args, void* stream);
  * saved: gate and up for the backward, of fovi_gated_mlp_saved_bytes (0: the backward forms them again and takes NULL;
  * NULL if no backward follows).
  * backward: dx, dw_down and the pair dw_gate, dw_up, each unless NULL, whole; the residual's gradient is dy.
- * The workspaces are 16-byte aligned.
+ * The workspaces (of the sizes that fovi_gated_mlp_*_workspace_bytes give for the arguments, 16-byte aligned) hold
+ * what lies between the products, and copies of matrices whose rows are not whole, aligned 16-byte pieces.
  */
 typedef struct fovi_gated_mlp_args {
   const void* x;
@@ -1019,9 +1021,9 @@ typedef struct fovi_gated_mlp_args {
 } fovi_gated_mlp_args;
 
 int64_t fovi_gated_mlp_saved_bytes(int64_t rows, int64_t dim, int64_t hidden, int32_t dtype);
-int64_t fovi_gated_mlp_fwd_workspace_bytes(int64_t rows, int64_t dim, int64_t hidden, int32_t dtype);
+int64_t fovi_gated_mlp_fwd_workspace_bytes(const fovi_gated_mlp_args* args);
 int fovi_gated_mlp_fwd(const fovi_gated_mlp_args* args, void* stream);
-int64_t fovi_gated_mlp_bwd_workspace_bytes(int64_t rows, int64_t dim, int64_t hidden, int32_t dtype);
+int64_t fovi_gated_mlp_bwd_workspace_bytes(const fovi_gated_mlp_args* args);
 int fovi_gated_mlp_bwd(const fovi_gated_mlp_args* args, void* stream);
 
 #ifdef __cplusplus

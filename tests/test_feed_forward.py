@@ -217,8 +217,9 @@ def test_writes_its_rows_only(m, c, f, dtype):
     a.w_down_stride, a.residual, a.y, a.y_stride = f, r.data_ptr(), y.data_ptr(), c + 9
     sizes = m, c, f, a.dtype
     saved = torch.empty(max(1, lib.fovi_gated_mlp_saved_bytes(*sizes)), dtype=torch.uint8, device="cuda")
-    work = [torch.full((n + 512,), 3, dtype=torch.uint8, device="cuda") for n in (lib.fovi_gated_mlp_fwd_workspace_bytes(*sizes),
-                                                                                lib.fovi_gated_mlp_bwd_workspace_bytes(*sizes))]
+    a.dy = dy.data_ptr()
+    work = [torch.full((n + 512,), 3, dtype=torch.uint8, device="cuda") for n in (lib.fovi_gated_mlp_fwd_workspace_bytes(a),
+                                                                                lib.fovi_gated_mlp_bwd_workspace_bytes(a))]
     a.saved = saved.data_ptr() if lib.fovi_gated_mlp_saved_bytes(*sizes) else None
     a.workspace, a.workspace_bytes = work[0].data_ptr() + 256, work[0].numel() - 512
     _lib.check(lib.fovi_gated_mlp_fwd(a, _lib.stream_of(x)), "forward")
@@ -226,7 +227,6 @@ def test_writes_its_rows_only(m, c, f, dtype):
     y.fill_(7.0)
     assert (out == 7.0).all()
     grads = [torch.full((t.numel() + 32,), 7.0, dtype=dtype, device="cuda") for t in (x, *w)]
-    a.dy = dy.data_ptr()
     a.dx, a.dw_gate, a.dw_up, a.dw_down = (t.data_ptr() + 16 * es for t in grads)
     a.workspace, a.workspace_bytes = work[1].data_ptr() + 256, work[1].numel() - 512
     _lib.check(lib.fovi_gated_mlp_bwd(a, _lib.stream_of(x)), "backward")
@@ -450,4 +450,4 @@ def test_cpu_tensors_and_c_arguments_are_refused():
     a.rows = 0
     assert lib.fovi_gated_mlp_bwd(a, None) != 0 and b"no rows" in lib.fovi_last_error()
     assert lib.fovi_gated_mlp_saved_bytes(0, 8, 16, _lib.F32) == 0
-    assert lib.fovi_gated_mlp_bwd_workspace_bytes(0, 8, 16, _lib.F32) == 0
+    assert lib.fovi_gated_mlp_fwd_workspace_bytes(a) == 0 and lib.fovi_gated_mlp_bwd_workspace_bytes(a) == 0

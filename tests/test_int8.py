@@ -147,7 +147,7 @@ def test_writes_its_rows_only(m, k, n):
             if two:
                 a.weight2, a.weight2_scale, a.weight2_stride = a.weight, a.weight_scale, k
             a.out, a.out_dtype, a.out_stride = y.data_ptr(), _lib.dtype_code(dtype), n + 9
-            size = _lib.load().fovi_linear_int8_workspace_bytes(m, k, n, int(two))
+            size = _lib.load().fovi_linear_int8_workspace_bytes(a)
             work = torch.empty(max(1, size), dtype=torch.uint8, device="cuda")
             a.workspace, a.workspace_bytes = work.data_ptr(), size
             _lib.check(_lib.load().fovi_linear_int8(a, _lib.stream_of(y)), "product")
