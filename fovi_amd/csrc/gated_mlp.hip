@@ -8,7 +8,7 @@
 // beside dh, in the registers of one kernel, whose epilogue writes dgate, dup and h (bf16; fp32 calls keep gate and up
 // from the forward). The weights' gradients reduce over the tokens: the tokens are split over workgroups, whose
 // partial sums a second launch adds in a fixed order.
-#include "matmul.h"
+#include "matmul_few.h"
 
 namespace fovi {
 
@@ -376,22 +376,34 @@ static void mlp_gated_grad_tiles(const MlpInputs& in, const MatOperand& wd, int6
              M, F, work, epilogue);
 }
 
+static bool mlp_few(const fovi_gated_mlp_args* a) { return a->rows <= kFewRows; }
+
+template <typename T> static MatOperand as_is(const void* p, int64_t stride, int64_t rows) {
+  return MatOperand{static_cast<const char*>(p), stride * static_cast<int64_t>(sizeof(T)), rows};
+}
+
 template <typename T> static void mlp_fwd(const fovi_gated_mlp_args* a, hipStream_t s) {
   const int64_t M = a->rows, C = a->dim, F = a->hidden, Fp = wide(F);
+  T* gate = static_cast<T*>(a->saved);
+  const MlpLinear<T> linear = {static_cast<T*>(a->y), a->y_stride, static_cast<const T*>(a->residual), a->residual_stride};
+  MlpGated<T> gated = {static_cast<T*>(a->workspace), Fp, a->activation, gate, gate + F, 2 * F};
+  if (mlp_few(a)) {
+    few_product<T, 2>(as_is<T>(a->x, a->x_stride, M), as_is<T>(a->w_gate, a->w_gate_stride, F), as_is<T>(a->w_up, a->w_up_stride, F), C, M, F,
+                      gated, s);
+    const MatOperand wd = as_is<T>(a->w_down, a->w_down_stride, C);
+    few_product<T, 1>(as_is<T>(gated.h, Fp, M), wd, wd, F, M, C, linear, s);
+    return;
+  }
   const MlpInputs in(a, a->workspace, false);
   in.in.copy(s);
-  T* h = reinterpret_cast<T*>(in.in.rest());
-  T* gate = static_cast<T*>(a->saved);
-  const MlpGated<T> gated = {h, Fp, a->activation, gate, gate + F, 2 * F};
+  gated.h = reinterpret_cast<T*>(in.in.rest());
   const int size = mat_tile_size(M, 2 * F, 1, sizeof(T) == 4, 256);
   if constexpr (sizeof(T) == 2) {
     if (size == 256) mlp_gated_tiles<T, 256, 128>(in, C, M, F, gated, s);
   }
-  if (size == 256 && sizeof(T) == 2) {
-  } else if (size >= 128) mlp_gated_tiles<T, 128, 64>(in, C, M, F, gated, s);
-  else mlp_gated_tiles<T, 64, 64>(in, C, M, F, gated, s);
-  const MatSegments down = {{MatOperand{reinterpret_cast<char*>(h), Fp * static_cast<int64_t>(sizeof(T)), M}}, {in.wd}, {F, 0}, 1};
-  const MlpLinear<T> linear = {static_cast<T*>(a->y), a->y_stride, static_cast<const T*>(a->residual), a->residual_stride};
+  if (size == 128) mlp_gated_tiles<T, 128, 64>(in, C, M, F, gated, s);
+  else if (size == 64) mlp_gated_tiles<T, 64, 64>(in, C, M, F, gated, s);
+  const MatSegments down = {{as_is<T>(gated.h, Fp, M)}, {in.wd}, {F, 0}, 1};
   mlp_linear<T, false, false>(down, M, C, F, 1, linear, s);
 }
 
@@ -438,7 +450,7 @@ extern "C" int64_t fovi_gated_mlp_saved_bytes(int64_t rows, int64_t dim, int64_t
 
 extern "C" int64_t fovi_gated_mlp_fwd_workspace_bytes(const fovi_gated_mlp_args* a) {
   if (!a || a->rows < 1 || a->dim < 1 || a->hidden < 1) return 0;
-  return MlpInputs(a, nullptr, false).in.used() + a->rows * wide(a->hidden) * mlp_element(a);
+  return (mlp_few(a) ? 0 : MlpInputs(a, nullptr, false).in.used()) + a->rows * wide(a->hidden) * mlp_element(a);
 }
 
 extern "C" int64_t fovi_gated_mlp_bwd_workspace_bytes(const fovi_gated_mlp_args* a) {

@@ -4,7 +4,7 @@
 //   gated: act(gate[m, n]) * up[m, n] of two such products over the same rows
 //
 // The sums are exact (int32 holds 133,000 products of 127 * 127); they become floats once, times the two scales.
-#include "matmul.h"
+#include "matmul_few.h"
 
 namespace fovi {
 
@@ -127,18 +127,25 @@ struct Int8Inputs {
   }
 };
 
+static bool int8_few(const fovi_linear_int8_args* a) { return a->rows <= kFewRows; }
+
 template <typename TO> static void int8_launch(const fovi_linear_int8_args* a, hipStream_t stream) {
   const int64_t M = a->rows, N = a->outputs, K = a->inputs;
-  const Int8Inputs in(a, a->workspace);
-  in.in.copy(stream);
   const Int8Scales scales = {a->x_scale, a->weight_scale, a->weight2_scale};
   TO* out = static_cast<TO*>(a->out);
-  if (a->weight2) {
-    int8_product<2>(in.x, in.w, in.w2, K, M, N, Int8Gated<TO>{scales, a->activation, out, a->out_stride}, stream);
-  } else {
-    const Int8Linear<TO> linear = {scales, a->bias, static_cast<const TO*>(a->residual), a->residual_stride, out, a->out_stride};
-    int8_product<1>(in.x, in.w, in.w, K, M, N, linear, stream);
+  const Int8Gated<TO> gated = {scales, a->activation, out, a->out_stride};
+  const Int8Linear<TO> linear = {scales, a->bias, static_cast<const TO*>(a->residual), a->residual_stride, out, a->out_stride};
+  if (int8_few(a)) {
+    const MatOperand x = {reinterpret_cast<const char*>(a->x), a->x_stride, M}, w = {reinterpret_cast<const char*>(a->weight), a->weight_stride, N},
+                     w2 = {reinterpret_cast<const char*>(a->weight2), a->weight2_stride, N};
+    if (a->weight2) few_product<int8_t, 2>(x, w, w2, K, M, N, gated, stream);
+    else few_product<int8_t, 1>(x, w, w, K, M, N, linear, stream);
+    return;
   }
+  const Int8Inputs in(a, a->workspace);
+  in.in.copy(stream);
+  if (a->weight2) int8_product<2>(in.x, in.w, in.w2, K, M, N, gated, stream);
+  else int8_product<1>(in.x, in.w, in.w, K, M, N, linear, stream);
 }
 
 }  // namespace fovi
@@ -146,7 +153,7 @@ template <typename TO> static void int8_launch(const fovi_linear_int8_args* a, h
 using namespace fovi;
 
 extern "C" int64_t fovi_linear_int8_workspace_bytes(const fovi_linear_int8_args* a) {
-  if (!a || a->rows < 1 || a->inputs < 1 || a->outputs < 1) return 0;
+  if (!a || a->rows < 1 || a->inputs < 1 || a->outputs < 1 || int8_few(a)) return 0;
   return Int8Inputs(a, nullptr).in.used();
 }
 

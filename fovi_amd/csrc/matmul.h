@@ -97,7 +97,9 @@ template <typename T, int NR, bool COL, int WAVES> struct MatLoader {
   uint64_t base;
   int64_t step;
 
-  static __device__ __forceinline__ int piece(int i) { return ((threadIdx.x >> 6) * LOADS + i) * 64 + (threadIdx.x & 63); }
+  // (WAVES 1: every wave loads stages of its own.)
+  static __device__ __forceinline__ int load(int i) { return (WAVES == 1 ? 0 : threadIdx.x >> 6) * LOADS + i; }
+  static __device__ __forceinline__ int piece(int i) { return load(i) * 64 + (threadIdx.x & 63); }
   // The place of a lane's piece in k: its first byte, or (COL) its k row.
   static __device__ __forceinline__ int place(int i) {
     const int id = piece(i), r = id / Tile::PIECES;
@@ -127,7 +129,7 @@ template <typename T, int NR, bool COL, int WAVES> struct MatLoader {
     const int limit = static_cast<int>(COL ? left : left * ES);
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const uint32_t to = lds + ((threadIdx.x >> 6) * LOADS + i) * 1024;
+      const uint32_t to = lds + load(i) * 1024;
       const uint32_t from = whole || place(i) < limit ? off[i] : OUTSIDE;
       // m0, the place in LDS, is read by the load: one wait state behind its writing
       asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
@@ -415,9 +417,14 @@ inline int mat_tile_size(int64_t M, int64_t N, int64_t shares, bool fp32, int co
 }
 
 template <typename Kernel, typename... Args>
-inline void mat_launch(Kernel kernel, unsigned grid, int threads, size_t lds, hipStream_t stream, Args... args) {
+inline void mat_launch(Kernel kernel, dim3 grid, int threads, size_t lds, hipStream_t stream, Args... args) {
   if (lds > 65536 && reserve_dynamic_lds(reinterpret_cast<const void*>(kernel), lds) != hipSuccess) return;
   kernel<<<grid, threads, lds, stream>>>(args...);
+}
+
+// Whether the loads take an operand by rows as it is.
+template <typename T> inline bool mat_whole(const MatOperand& o, int64_t k) {
+  return (reinterpret_cast<uintptr_t>(o.p) | o.stride | k * static_cast<int64_t>(sizeof(T))) % 16 == 0 && o.stride < (1 << 22);
 }
 
 // 16 bytes of a run of `len` bytes from `at` on, at any alignment, zeros from its end on.
@@ -457,8 +464,8 @@ class MatInputs {
   // rows x cols elements of `es` bytes, `stride` elements apart; the result's stride is in bytes.
   MatOperand take(const void* p, int64_t stride, int64_t rows, int64_t cols, int64_t es) {
     const int64_t bytes = cols * es;
-    if ((reinterpret_cast<uintptr_t>(p) | stride * es | bytes) % 16 == 0 && stride * es < (1 << 22))
-      return MatOperand{static_cast<const char*>(p), stride * es, rows};
+    const MatOperand as_is = {static_cast<const char*>(p), stride * es, rows};
+    if (mat_whole<char>(as_is, bytes)) return as_is;
     const int64_t wide = (bytes + 15) / 16 * 16;
     auto& m = copies_.m[copies_.n++];
     m.from = static_cast<const char*>(p); m.to = at_; m.stride = stride * es; m.rows = rows; m.len = bytes;
