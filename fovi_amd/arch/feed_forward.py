@@ -25,17 +25,13 @@ __all__ = ["gated_mlp", "GatedFeedForward", "Int8GatedFeedForward"]
 
 def _args(x, w_gate, w_up, w_down, activation):
     """The arguments that both directions share, with the tensors that they point into."""
-    a = _lib.GatedMlpArgs()
-    xr, rows, a.x_stride = _matrix(x)
-    keep = [xr]
-    for name, w in (("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down)):
-        w, _, stride = _matrix(w)
-        keep.append(w)
-        setattr(a, name, w.data_ptr())
-        setattr(a, name + "_stride", stride)
-    a.x, a.dtype, a.activation = xr.data_ptr(), _lib.dtype_code(x.dtype), activation
-    a.rows, a.dim, a.hidden = rows, x.shape[-1], w_gate.shape[0]
-    return a, keep
+    x, rows, x_stride = _matrix(x)
+    w_gate, _, gate_stride = _matrix(w_gate)
+    w_up, _, up_stride = _matrix(w_up)
+    w_down, _, down_stride = _matrix(w_down)
+    a = _lib.GatedMlpArgs(x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), _lib.dtype_code(x.dtype), activation,
+                          rows, x.shape[-1], w_gate.shape[0], x_stride, gate_stride, up_stride, down_stride)
+    return a, (x, w_gate, w_up, w_down)
 
 
 def _workspace(a, nbytes, device):
@@ -124,30 +120,33 @@ def gated_mlp(x, w_gate, w_up, w_down, activation="silu", residual=None):
     ``activation`` 'silu' or 'gelu' (the exact one); ``residual`` of ``x``'s shape and type, or None. Rows of any stride and
     alignment are read where they are. Differentiable once in everything.
     """
-    _lib.require_device(x, w_gate, w_up, w_down, residual)
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"gated_mlp: expected [..., C] with C >= 1, got {tuple(x.shape)}")
-    c = x.shape[-1]
-    if w_gate.dim() != 2 or w_gate.shape[0] < 1 or w_gate.shape[1] != c or w_up.shape != w_gate.shape \
-            or w_down.shape != (c, w_gate.shape[0]):
-        raise ValueError(f"gated_mlp: weights {tuple(w_gate.shape)}, {tuple(w_up.shape)} and {tuple(w_down.shape)} for {c} channels")
+    tensors = (x, w_gate, w_up, w_down) if residual is None else (x, w_gate, w_up, w_down, residual)
+    _lib.require_device(*tensors)
+    shape = x.shape
+    if len(shape) < 1 or shape[-1] < 1:
+        raise ValueError(f"gated_mlp: expected [..., C] with C >= 1, got {tuple(shape)}")
+    c, weights = shape[-1], w_gate.shape
+    if len(weights) != 2 or weights[0] < 1 or weights[1] != c or w_up.shape != weights or w_down.shape != (c, weights[0]):
+        raise ValueError(f"gated_mlp: weights {tuple(weights)}, {tuple(w_up.shape)} and {tuple(w_down.shape)} for {c} channels")
     if activation not in GATES:
         raise ValueError(f"gated_mlp: unknown activation {activation!r}")
-    if residual is not None and residual.shape != x.shape:
-        raise ValueError(f"gated_mlp: residual of shape {tuple(residual.shape)} for rows {tuple(x.shape)}")
-    tensors = (x, w_gate, w_up, w_down) + (() if residual is None else (residual,))
+    if residual is not None and residual.shape != shape:
+        raise ValueError(f"gated_mlp: residual of shape {tuple(residual.shape)} for rows {tuple(shape)}")
     if _autocast_bf16():
         tensors = tuple(t.to(torch.bfloat16) for t in tensors)
-    x, w_gate, w_up, w_down = tensors[:4]
-    residual = None if residual is None else tensors[4]
-    if x.dtype not in (torch.float32, torch.bfloat16) or any(t.dtype != x.dtype for t in tensors):
-        raise TypeError(f"gated_mlp: unsupported dtypes {', '.join(str(t.dtype) for t in tensors)}")
-    if any(t.device != x.device for t in tensors):
-        raise ValueError("gated_mlp: all tensors must be on one device")
+        x, w_gate, w_up, w_down = tensors[:4]
+        residual = None if residual is None else tensors[4]
+    dtype, device, grad = x.dtype, x.device, False
+    for t in tensors:
+        if t.dtype is not dtype or dtype not in (torch.float32, torch.bfloat16):
+            raise TypeError(f"gated_mlp: unsupported dtypes {', '.join(str(t.dtype) for t in tensors)}")
+        if t.device != device:
+            raise ValueError("gated_mlp: all tensors must be on one device")
+        grad = grad or t.requires_grad
     if x.numel() == 0:
         y = (x @ w_gate.t() * (x @ w_up.t())) @ w_down.t()         # zero gradients for the weights
         return y if residual is None else y + residual
-    if (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)) or _lib.forward_mode():
+    if (grad and torch.is_grad_enabled()) or _lib.forward_mode():
         return _GatedMlpFn.apply(x, w_gate, w_up, w_down, GATES[activation], residual)
     return _forward(x, w_gate, w_up, w_down, GATES[activation], residual, False)[0]
 

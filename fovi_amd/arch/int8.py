@@ -22,8 +22,10 @@ GATES = {"silu": _lib.GATE_SILU, "gelu": _lib.GATE_GELU}
 
 def refuse_gradients(what, *tensors):
     """Raises where a gradient or tangent is asked for."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError(f"{what}: no gradients (call it under torch.no_grad())")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{what}: no gradients (call it under torch.no_grad())")
     if _lib.forward_mode():
         raise ValueError(f"{what}: no forward-mode derivatives")
 
@@ -72,11 +74,13 @@ class Int8Rows(NamedTuple):
 
 def _rows_check(what, rows):
     data, scale = rows
-    _lib.require_device(data, scale)
-    if data.dtype != torch.int8 or scale.dtype != torch.float32:
+    if not (data.is_cuda and scale.is_cuda):
+        _lib.require_device(data, scale)
+    if data.dtype is not torch.int8 or scale.dtype is not torch.float32:
         raise TypeError(f"{what}: expected int8 rows with fp32 scales, got {data.dtype} and {scale.dtype}")
-    if data.dim() < 1 or data.shape[-1] < 1 or scale.shape != data.shape[:-1]:
-        raise ValueError(f"{what}: rows {tuple(data.shape)} with scales {tuple(scale.shape)}")
+    shape = data.shape
+    if len(shape) < 1 or shape[-1] < 1 or scale.shape != shape[:-1]:
+        raise ValueError(f"{what}: rows {tuple(shape)} with scales {tuple(scale.shape)}")
     if scale.device != data.device:
         raise ValueError(f"{what}: scales on {scale.device}, rows on {data.device}")
 
@@ -101,42 +105,46 @@ def quantize_int8(x):
 
 
 def _weight(what, w, k, device):
+    """``(data, stride, scale)`` of weights as the kernels read them."""
     _rows_check(what, w)
-    if w.data.dim() != 2 or w.data.shape[1] != k:
-        raise ValueError(f"{what}: weights {tuple(w.data.shape)} for {k} inputs")
-    if w.data.device != device:
-        raise ValueError(f"{what}: weights on {w.data.device}, x on {device}")
-    data = w.data if w.data.stride(1) == 1 and w.data.stride(0) >= k else w.data.contiguous()
-    return data, w.scale.contiguous()
+    data, scale = w
+    shape = data.shape
+    if len(shape) != 2 or shape[1] != k:
+        raise ValueError(f"{what}: weights {tuple(shape)} for {k} inputs")
+    if data.device != device:
+        raise ValueError(f"{what}: weights on {data.device}, x on {device}")
+    s0, s1 = data.stride()
+    if s1 != 1 or s0 < k:
+        data, s0 = data.contiguous(), k
+    return data, s0, scale if scale.is_contiguous() else scale.contiguous()
 
 
 def _product(what, x, weight, weight2, activation, bias, residual, dtype):
     _rows_check(what, x)
-    if dtype not in (torch.float32, torch.bfloat16):
+    if dtype is not torch.bfloat16 and dtype is not torch.float32:
         raise TypeError(f"{what}: unsupported dtype {dtype}")
-    k, device = x.data.shape[-1], x.data.device
+    data, scale = x
+    shape, device = data.shape, data.device
+    k = shape[-1]
     if k > 131072:
         raise ValueError(f"{what}: {k} inputs, at most 131072 keep the sums exact")
-    w, ws = _weight(what, weight, k, device)
+    w, w_stride, w_scale = _weight(what, weight, k, device)
     n = w.shape[0]
-    shape = x.data.shape[:-1] + (n,)
-    refuse_gradients(what, x.scale, weight.scale, None if weight2 is None else weight2.scale, bias, residual)
-    a = _lib.LinearInt8Args()
-    keep = []
+    shape = shape[:-1] + (n,)
+    refuse_gradients(what, scale, w_scale, None if weight2 is None else weight2.scale, bias, residual)
+    w2, w2_stride, w2_scale, act = None, 0, None, 0
     if weight2 is not None:
-        w2, w2s = _weight(what, weight2, k, device)
+        w2, w2_stride, w2_scale = _weight(what, weight2, k, device)
         if w2.shape != w.shape:
             raise ValueError(f"{what}: weights {tuple(w.shape)} and {tuple(w2.shape)}")
         if activation not in GATES:
             raise ValueError(f"{what}: unknown activation {activation!r}")
-        a.weight2, a.weight2_scale, a.weight2_stride, a.activation = w2.data_ptr(), w2s.data_ptr(), w2.stride(0), GATES[activation]
-        keep += [w2, w2s]
+        act = GATES[activation]
     if bias is not None:
         _lib.require_device(bias)
         if bias.shape != (n,) or bias.device != device:
             raise ValueError(f"{what}: bias {tuple(bias.shape)} on {bias.device} for {n} outputs on {device}")
         bias = bias.float().contiguous()
-        a.bias = bias.data_ptr()
     if residual is not None:
         _lib.require_device(residual)
         if residual.shape != shape or residual.dtype != dtype or residual.device != device:
@@ -145,22 +153,24 @@ def _product(what, x, weight, weight2, activation, bias, residual, dtype):
     out = torch.empty(shape, dtype=dtype, device=device)
     if out.numel() == 0:
         return out
-    data, rows, stride = _matrix(x.data)
-    scale = x.scale.contiguous()
+    data, rows, stride = _matrix(data)
+    if not scale.is_contiguous():
+        scale = scale.contiguous()
+    r_stride = 0
     if residual is not None:
-        residual, _, a.residual_stride = _matrix(residual)
-        a.residual = residual.data_ptr()
-    a.x, a.x_scale, a.rows, a.inputs, a.outputs, a.x_stride = data.data_ptr(), scale.data_ptr(), rows, k, n, stride
-    a.weight, a.weight_scale, a.weight_stride = w.data_ptr(), ws.data_ptr(), w.stride(0)
-    a.out, a.out_dtype, a.out_stride = out.data_ptr(), _lib.dtype_code(dtype), n
+        residual, _, r_stride = _matrix(residual)
+    a = _lib.LinearInt8Args(data.data_ptr(), scale.data_ptr(), rows, k, n, stride, w.data_ptr(), w_scale.data_ptr(), w_stride,
+                            None if w2 is None else w2.data_ptr(), None if w2 is None else w2_scale.data_ptr(), w2_stride, act, _lib.dtype_code(dtype),
+                            None if bias is None else bias.data_ptr(), None if residual is None else residual.data_ptr(), r_stride,
+                            out.data_ptr(), n)
     lib = _lib.load()
     nbytes = lib.fovi_linear_int8_workspace_bytes(a)
+    work = None
     if nbytes:
         work = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        keep.append(work)
         a.workspace, a.workspace_bytes = work.data_ptr(), nbytes
     _lib.check(lib.fovi_linear_int8(a, _lib.stream_of(out)), "fovi_linear_int8")
-    del keep
+    del work
     return out
 
 

@@ -13,6 +13,8 @@ scale each, as the products of ``fovi_amd.arch.int8`` read them.
 """
 from __future__ import annotations
 
+import ctypes as C
+
 import torch
 import torch.nn as nn
 
@@ -175,29 +177,27 @@ class LayerNorm(nn.Module):
         return f"{self.dim}, eps={self.eps}, elementwise_affine={self.weight is not None}"
 
 
+_Pair = C.c_int64 * 2
+
+
 def _rms_args(x, weight, eps, residual):
     """The arguments that both directions share, with the tensors that they point into."""
     c = x.shape[-1]
     xr, n0, n1, s0, s1 = _rows(x)
-    a = _lib.RmsNormArgs()
-    keep = [xr]
+    rr, t0, t1 = None, 0, 0
     if residual is not None:
         rr, m0, m1, t0, t1 = _rows(residual)
-        if (m0, m1) != (n0, n1):
+        if (m0, m1) != (n0, n1):        # rows of both in the same two levels; one splits into any two
             if m0 == 1:
                 t0 = n1 * t1
             elif n0 == 1:
                 n0, n1, s0 = m0, m1, m1 * s1
             else:
                 rr, t0, t1 = residual.contiguous(), n1 * c, c
-        keep.append(rr)
-        a.residual = rr.data_ptr()
-        a.residual_stride[:] = (t0, t1)
-    a.x, a.dtype, a.rows0, a.rows1, a.channels, a.eps = xr.data_ptr(), _lib.dtype_code(x.dtype), n0, n1, c, eps
-    a.x_stride[:] = (s0, s1)
-    if weight is not None:
-        a.weight, a.p_dtype = weight.data_ptr(), _lib.dtype_code(weight.dtype)
-    return a, keep
+    a = _lib.RmsNormArgs(xr.data_ptr(), _lib.dtype_code(x.dtype), 0 if weight is None else _lib.dtype_code(weight.dtype), n0, n1, c,
+                         _Pair(s0, s1), None if rr is None else rr.data_ptr(), _Pair(t0, t1),
+                         None if weight is None else weight.data_ptr(), eps)
+    return a, (xr, rr)
 
 
 def _rms_forward(x, weight, eps, residual, rstd, quantize=False):

@@ -12,12 +12,6 @@
 
 namespace fovi {
 
-struct MatSegments {
-  MatOperand x[2], w[2];
-  int64_t k[2];
-  int n;
-};
-
 // Runs of h, dgate and dup are written whole, with zeros behind the last column: the products that read them go by 16 bytes.
 __device__ __forceinline__ void clear_behind(int count, float (&v)[8]) {
 #pragma unroll
@@ -48,14 +42,6 @@ template <typename T> struct MlpTwoRows {              // `rows` rows to one out
   __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const float (&v)[1][8]) const {
     if (m < rows) store_run(out[0] + m * stride + n, count, v[0]);
     else if (m >= next) store_run(out[1] + (m - next) * stride + n, count, v[0]);
-  }
-};
-
-struct MlpPartial {                                    // the sums of a share of the reduction
-  static constexpr int STORES = 2;
-  float* part; int64_t M, N;
-  __device__ __forceinline__ void operator()(int64_t share, int64_t m, int64_t n, int count, const float (&v)[1][8]) const {
-    store_run(part + (share * M + m) * N + n, count, v[0]);
   }
 };
 
@@ -108,84 +94,6 @@ template <typename T> struct MlpGatedGrad {            // dgate, dup and h from 
     write(m, n, count, g, u, v[0]);
   }
 };
-
-// One product, k in up to two segments (of other operands each), or split in shares of `share`.
-template <typename T, int BM, int BN, bool CX, bool CW, typename Epilogue> struct MlpLinearTile {
-  typedef MatPhase<T, BM, BN, 1, CX, CW> Phase;
-  typedef MatRing<Phase::BYTES, 2 * Phase::MB * Phase::NN * Epilogue::STORES> Ring;
-};
-template <typename T, int BM, int BN, bool CX, bool CW, typename Epilogue>
-__global__ __launch_bounds__((MatUsual<BM, BN>::THREADS), 2) void mlp_linear_kernel(MatSegments s, int64_t M, int64_t N, MatWork work, int64_t share,
-                                                            Epilogue epilogue) {
-  typedef typename MlpLinearTile<T, BM, BN, CX, CW, Epilogue>::Phase Phase;
-  typedef typename MlpLinearTile<T, BM, BN, CX, CW, Epilogue>::Ring Ring;
-  extern __shared__ __attribute__((aligned(1024))) char lds[];
-  MatItem item(work), ahead(work);
-  if (!item.live()) return;
-  auto part = [&](const MatItem& at, int i, int64_t& from) __attribute__((always_inline)) {
-    const int64_t k = i ? s.k[1] : s.k[0];
-    from = at.share(work) * share;
-    return (from + share < k ? from + share : k) - from;
-  };
-  Phase phase;
-  int segment = -1;
-  int64_t left = 0;
-  auto produce = [&](uint32_t to) __attribute__((always_inline)) {
-    while (left <= 0) {
-      if (++segment == s.n) { segment = 0; ahead.next(); }
-      if (!ahead.live()) return false;
-      int64_t from;
-      left = part(ahead, segment, from);
-      const MatOperand w[1] = {segment ? s.w[1] : s.w[0]};
-      int64_t tm, tn;
-      ahead.place(work, tm, tn);
-      phase.open(segment ? s.x[1] : s.x[0], w, tm * BM, tn * BN, from);
-    }
-    phase.start(to, left);
-    left -= Phase::BK;
-    return true;
-  };
-  Ring ring(lds, produce);
-  typename Phase::Step step[2];
-  auto first_step = [&](const char* now) __attribute__((always_inline)) { step[0].read(now, 0); };
-  first_step(ring.now());
-  for (; item.live(); item.next()) {
-    typename Phase::Acc acc[1][Phase::MB][Phase::NN];
-    mat_clear(acc);
-    int64_t stages = 0, from;
-    for (int i = 0; i < s.n; ++i) {
-      const int64_t n = part(item, i, from);
-      stages += n > 0 ? (n + Phase::BK - 1) / Phase::BK : 0;
-    }
-    Phase::run(ring, stages, step, acc, 0, produce, first_step);
-    int64_t tm, tn;
-    item.place(work, tm, tn);
-    if constexpr (__is_same(Epilogue, MlpPartial)) {
-      const int64_t z = item.share(work);
-      ring.stored = mat_finish<typename Phase::Waves, BM, BN, float>(acc, tm * BM, tn * BN, M, N,
-                                [&](int64_t m, int64_t n, int count, const float (&v)[1][8]) { epilogue(z, m, n, count, v); });
-    } else {
-      ring.stored = mat_finish<typename Phase::Waves, BM, BN, float>(acc, tm * BM, tn * BN, M, N, epilogue);
-    }
-  }
-}
-
-// out = the shares' sums added up, through the epilogue.
-template <typename Epilogue>
-__global__ __launch_bounds__(256) void mlp_join_kernel(const float* part, int64_t shares, int64_t M, int64_t N, Epilogue epilogue) {
-  const int64_t per = (N + 7) / 8, i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= M * per) return;
-  const int64_t m = i / per, n = (i - m * per) * 8;
-  const int count = static_cast<int>(N - n < 8 ? N - n : 8);
-  float v[1][8] = {};
-  for (int64_t z = 0; z < shares; ++z) {
-    float t[8];
-    load_run(part + (z * M + m) * N + n, count, t);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[0][e] += t[e];
-  }
-  epilogue(m, n, count, v);
-}
 
 template <typename T, int BM, int BN> struct MlpGatedTile {
   typedef MatPhase<T, BM, BN, 2, false, false> Both;
@@ -280,55 +188,6 @@ __global__ __launch_bounds__(W::THREADS, 2) void mlp_gated_grad_kernel(MatOperan
   }
 }
 
-template <typename T, int BM, int BN, bool CX, bool CW, typename Epilogue>
-static void mlp_linear_tiles(const MatSegments& s, int64_t M, int64_t N, int64_t share, int64_t shares, const Epilogue& epilogue,
-                             hipStream_t stream) {
-  const MatWork work = mat_work(M, N, BM, BN, shares);
-  mat_launch(mlp_linear_kernel<T, BM, BN, CX, CW, Epilogue>, mat_grid(work, 256 / BM), (MatUsual<BM, BN>::THREADS), MlpLinearTile<T, BM, BN, CX, CW, Epilogue>::Ring::LDS,
-             stream, s, M, N, work, share, epilogue);
-}
-template <typename T, bool CX, bool CW, typename Epilogue>
-static void mlp_linear(const MatSegments& s, int64_t M, int64_t N, int64_t share, int64_t shares, const Epilogue& epilogue,
-                       hipStream_t stream) {
-  const int size = mat_tile_size(M, N, shares, sizeof(T) == 4, mat_columns(N));
-  if constexpr (sizeof(T) == 2) {
-    if (size == 256) {
-      if (mat_columns(N) == 192) mlp_linear_tiles<T, 256, 192, CX, CW>(s, M, N, share, shares, epilogue, stream);
-      else mlp_linear_tiles<T, 256, 256, CX, CW>(s, M, N, share, shares, epilogue, stream);
-      return;
-    }
-  }
-  if (size >= 128) mlp_linear_tiles<T, 128, 128, CX, CW>(s, M, N, share, shares, epilogue, stream);
-  else mlp_linear_tiles<T, 64, 64, CX, CW>(s, M, N, share, shares, epilogue, stream);
-}
-
-// Shares of a reduction over the tokens: workgroups for the whole card, at least 512 tokens each.
-static int64_t token_shares(int64_t tokens, int64_t M, int64_t N) {
-  const int64_t most = (tokens + 511) / 512, big = mat_tiles(M, N, 256, 256), small = mat_tiles(M, N, 64, 64);
-  int64_t shares = (256 + big - 1) / big;
-  if (shares > most) {                                 // small tiles, then
-    shares = (1024 + small - 1) / small;
-    if (shares > most) shares = most;
-  }
-  return shares < 1 ? 1 : shares;
-}
-
-// x and w by columns, reduced over the tokens.
-template <typename T, typename Epilogue>
-static void token_product(const MatOperand& x, const MatOperand& w, int64_t tokens, int64_t M, int64_t N, float* part,
-                          const Epilogue& epilogue, hipStream_t stream) {
-  const int64_t shares = token_shares(tokens, M, N);
-  const MatSegments s = {{x}, {w}, {tokens, 0}, 1};
-  if (shares == 1) {
-    mlp_linear<T, true, true>(s, M, N, tokens, 1, epilogue, stream);
-    return;
-  }
-  const int64_t bk = mat_bk<T>(), share = ((tokens + shares - 1) / shares + bk - 1) / bk * bk;
-  const int64_t used = (tokens + share - 1) / share;
-  mlp_linear<T, true, true>(s, M, N, share, used, MlpPartial{part, M, N}, stream);
-  mlp_join_kernel<Epilogue><<<static_cast<unsigned>((M * ((N + 7) / 8) + 255) / 256), 256, 0, stream>>>(part, used, M, N, epilogue);
-}
-
 static int mlp_check(const fovi_gated_mlp_args* a, const char* what) {
   if (!a || !a->x || !a->w_gate || !a->w_up || !a->w_down) { set_error("%s: null pointer", what); return 1; }
   if (a->dtype != FOVI_F32 && a->dtype != FOVI_BF16) { set_error("%s: dtype must be F32 or BF16", what); return 1; }
@@ -404,7 +263,7 @@ template <typename T> static void mlp_fwd(const fovi_gated_mlp_args* a, hipStrea
   if (size == 128) mlp_gated_tiles<T, 128, 64>(in, C, M, F, gated, s);
   else if (size == 64) mlp_gated_tiles<T, 64, 64>(in, C, M, F, gated, s);
   const MatSegments down = {{as_is<T>(gated.h, Fp, M)}, {in.wd}, {F, 0}, 1};
-  mlp_linear<T, false, false>(down, M, C, F, 1, linear, s);
+  mat_linear<T, false, false>(down, M, C, reinterpret_cast<char*>(gated.h) + aligned(M * Fp * sizeof(T)), false, linear, s);
 }
 
 template <typename T> static void mlp_bwd(const fovi_gated_mlp_args* a, hipStream_t s) {
@@ -413,13 +272,13 @@ template <typename T> static void mlp_bwd(const fovi_gated_mlp_args* a, hipStrea
   in.in.copy(s);
   T* grad = reinterpret_cast<T*>(in.in.rest());                     // [M, 2 Fp]: dgate, dup
   T* h = reinterpret_cast<T*>(in.in.rest() + aligned(M * 2 * Fp * es));
-  float* part = reinterpret_cast<float*>(reinterpret_cast<char*>(h) + aligned(M * Fp * es));
+  char* part = reinterpret_cast<char*>(h) + aligned(M * Fp * es);
   const MatOperand wd = columns(in.wd, F, es);
   const T* gate = static_cast<const T*>(a->saved);
   const MlpGatedGrad<T> gated = {grad, grad + Fp, h, 2 * Fp, Fp, a->activation, gate, gate + F, 2 * F};
   if constexpr (sizeof(T) == 4) {
     const MatSegments down = {{in.dy}, {wd}, {C, 0}, 1};
-    mlp_linear<T, false, true>(down, M, F, C, 1, gated, s);
+    mat_linear<T, false, true>(down, M, F, part, false, gated, s);
   } else {
     const int size = mat_tile_size(M, 2 * F, 1, false, 256);
     if (size >= 128) mlp_gated_grad_tiles<T, 128, 64, MatWaves<2, 2>>(in, wd, C, M, F, gated, s);
@@ -429,14 +288,27 @@ template <typename T> static void mlp_bwd(const fovi_gated_mlp_args* a, hipStrea
   if (a->dx) {
     const MatSegments both = {{MatOperand{dgate, 2 * Fp * es, M}, MatOperand{dgate + Fp * es, 2 * Fp * es, M}},
                               {columns(in.wg, C, es), columns(in.wu, C, es)}, {F, F}, 2};
-    mlp_linear<T, false, true>(both, M, C, F, 1, MlpLinear<T>{static_cast<T*>(a->dx), C, nullptr, 0}, s);
+    mat_linear<T, false, true>(both, M, C, part, false, MlpLinear<T>{static_cast<T*>(a->dx), C, nullptr, 0}, s);
   }
-  if (a->dw_gate)
-    token_product<T>(MatOperand{dgate, 2 * Fp * es, 2 * Fp}, columns(in.x, C, es), M, Fp + F, C, part,
-                     MlpTwoRows<T>{{static_cast<T*>(a->dw_gate), static_cast<T*>(a->dw_up)}, F, Fp, C}, s);
-  if (a->dw_down)
-    token_product<T>(columns(in.dy, C, es), MatOperand{reinterpret_cast<char*>(h), Fp * es, Fp}, M, C, F, part,
-                     MlpLinear<T>{static_cast<T*>(a->dw_down), F, nullptr, 0}, s);
+  if (a->dw_gate) {
+    const MatSegments up = {{MatOperand{dgate, 2 * Fp * es, 2 * Fp}}, {columns(in.x, C, es)}, {M, 0}, 1};
+    mat_linear<T, true, true>(up, Fp + F, C, part, true, MlpTwoRows<T>{{static_cast<T*>(a->dw_gate), static_cast<T*>(a->dw_up)}, F, Fp, C}, s);
+  }
+  if (a->dw_down) {
+    const MatSegments down = {{columns(in.dy, C, es)}, {MatOperand{reinterpret_cast<char*>(h), Fp * es, Fp}}, {M, 0}, 1};
+    mat_linear<T, true, true>(down, C, F, part, true, MlpLinear<T>{static_cast<T*>(a->dw_down), F, nullptr, 0}, s);
+  }
+}
+
+// The partial sums of the backward's products, one after the other.
+template <typename T> static int64_t mlp_bwd_part(const fovi_gated_mlp_args* a) {
+  const int64_t M = a->rows, C = a->dim, F = a->hidden;
+  const int64_t parts[4] = {sizeof(T) == 4 ? mat_part_bytes<T>(M, F, C, false) : 0, mat_part_bytes<T>(M, C, F, false),
+                            mat_part_bytes<T>(wide(F) + F, C, M, true), mat_part_bytes<T>(C, F, M, true)};
+  int64_t most = 0;
+  for (int64_t n : parts)
+    if (n > most) most = n;
+  return most;
 }
 
 }  // namespace fovi
@@ -450,14 +322,17 @@ extern "C" int64_t fovi_gated_mlp_saved_bytes(int64_t rows, int64_t dim, int64_t
 
 extern "C" int64_t fovi_gated_mlp_fwd_workspace_bytes(const fovi_gated_mlp_args* a) {
   if (!a || a->rows < 1 || a->dim < 1 || a->hidden < 1) return 0;
-  return (mlp_few(a) ? 0 : MlpInputs(a, nullptr, false).in.used()) + a->rows * wide(a->hidden) * mlp_element(a);
+  const int64_t h = aligned(a->rows * wide(a->hidden) * mlp_element(a));
+  if (mlp_few(a)) return h;
+  return MlpInputs(a, nullptr, false).in.used() + h +
+         (a->dtype == FOVI_F32 ? mat_part_bytes<float>(a->rows, a->dim, a->hidden, false) : mat_part_bytes<uint16_t>(a->rows, a->dim, a->hidden, false));
 }
 
 extern "C" int64_t fovi_gated_mlp_bwd_workspace_bytes(const fovi_gated_mlp_args* a) {
   if (!a || a->rows < 1 || a->dim < 1 || a->hidden < 1) return 0;
-  const int64_t es = mlp_element(a), rows = a->rows, C = a->dim, F = a->hidden, Fp = wide(F);
-  const int64_t up = token_shares(rows, Fp + F, C) * (Fp + F) * C, down = token_shares(rows, C, F) * C * F;
-  return MlpInputs(a, nullptr, true).in.used() + aligned(rows * 2 * Fp * es) + aligned(rows * Fp * es) + (up > down ? up : down) * 4;
+  const int64_t es = mlp_element(a), rows = a->rows, Fp = wide(a->hidden);
+  return MlpInputs(a, nullptr, true).in.used() + aligned(rows * 2 * Fp * es) + aligned(rows * Fp * es) +
+         (a->dtype == FOVI_F32 ? mlp_bwd_part<float>(a) : mlp_bwd_part<uint16_t>(a));
 }
 
 extern "C" int fovi_gated_mlp_fwd(const fovi_gated_mlp_args* a, void* stream) {

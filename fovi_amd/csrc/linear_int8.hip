@@ -54,22 +54,20 @@ template <typename TO> struct Int8Gated {
   }
 };
 
-template <int BM, int BN, int NB, typename Epilogue> struct Int8Tile {
-  typedef MatPhase<int8_t, BM, BN, NB, false, false> Phase;
+template <int BM, int BN, typename Epilogue> struct Int8GatedTile {
+  typedef MatPhase<int8_t, BM, BN, 2, false, false> Phase;
   typedef MatRing<Phase::BYTES, 2 * Phase::MB * Phase::NN * Epilogue::STORES> Ring;
 };
 
-template <int BM, int BN, int NB, typename Epilogue>
-__global__ __launch_bounds__((MatUsual<BM, BN>::THREADS), 2) void int8_kernel(MatOperand x, MatOperand w0, MatOperand w1, int64_t K, int64_t M, int64_t N, MatWork work,
+template <int BM, int BN, typename Epilogue>
+__global__ __launch_bounds__((MatUsual<BM, BN>::THREADS), 2) void int8_gated_kernel(MatOperand x, MatOperand w0, MatOperand w1, int64_t K, int64_t M, int64_t N, MatWork work,
                                                       Epilogue epilogue) {
-  typedef typename Int8Tile<BM, BN, NB, Epilogue>::Phase Phase;
-  typedef typename Int8Tile<BM, BN, NB, Epilogue>::Ring Ring;
+  typedef typename Int8GatedTile<BM, BN, Epilogue>::Phase Phase;
+  typedef typename Int8GatedTile<BM, BN, Epilogue>::Ring Ring;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   MatItem item(work), ahead(work);
   if (!item.live()) return;
-  MatOperand w[NB];
-  w[0] = w0;
-  if (NB == 2) w[NB - 1] = w1;
+  const MatOperand w[2] = {w0, w1};
   Phase phase;
   int64_t left = -1;                                   // of the tile `ahead`; -1: not begun
   auto produce = [&](uint32_t to) __attribute__((always_inline)) {
@@ -91,7 +89,7 @@ __global__ __launch_bounds__((MatUsual<BM, BN>::THREADS), 2) void int8_kernel(Ma
   first_step(ring.now());
   const int64_t stages = (K + Phase::BK - 1) / Phase::BK;
   for (; item.live(); item.next()) {
-    typename Phase::Acc acc[NB][Phase::MB][Phase::NN];
+    typename Phase::Acc acc[2][Phase::MB][Phase::NN];
     mat_clear(acc);
     Phase::run(ring, stages, step, acc, 0, produce, first_step);
     int64_t tm, tn;
@@ -100,21 +98,20 @@ __global__ __launch_bounds__((MatUsual<BM, BN>::THREADS), 2) void int8_kernel(Ma
   }
 }
 
-template <int BM, int BN, int NB, typename Epilogue>
-static void int8_tiles(const MatOperand& x, const MatOperand& w0, const MatOperand& w1, int64_t K, int64_t M, int64_t N,
-                       const Epilogue& epilogue, hipStream_t s) {
+template <int BM, int BN, typename Epilogue>
+static void int8_gated_tiles(const MatOperand& x, const MatOperand& w0, const MatOperand& w1, int64_t K, int64_t M, int64_t N,
+                             const Epilogue& epilogue, hipStream_t s) {
   const MatWork work = mat_work(M, N, BM, BN, 1);
-  mat_launch(int8_kernel<BM, BN, NB, Epilogue>, mat_grid(work, 256 / BM), (MatUsual<BM, BN>::THREADS), Int8Tile<BM, BN, NB, Epilogue>::Ring::LDS, s, x, w0, w1, K, M, N, work,
-             epilogue);
+  mat_launch(int8_gated_kernel<BM, BN, Epilogue>, mat_grid(work, 256 / BM), (MatUsual<BM, BN>::THREADS),
+             Int8GatedTile<BM, BN, Epilogue>::Ring::LDS, s, x, w0, w1, K, M, N, work, epilogue);
 }
-
-template <int NB, typename Epilogue>
-static void int8_product(const MatOperand& x, const MatOperand& w0, const MatOperand& w1, int64_t K, int64_t M, int64_t N,
-                         const Epilogue& epilogue, hipStream_t s) {
-  const int size = mat_tile_size(M, N * NB, 1, false, 256);
-  if (size == 256) int8_tiles<256, 256 / NB, NB>(x, w0, w1, K, M, N, epilogue, s);
-  else if (size == 128) int8_tiles<128, 128 / NB, NB>(x, w0, w1, K, M, N, epilogue, s);
-  else int8_tiles<64, 64, NB>(x, w0, w1, K, M, N, epilogue, s);
+template <typename Epilogue>
+static void int8_gated(const MatOperand& x, const MatOperand& w0, const MatOperand& w1, int64_t K, int64_t M, int64_t N,
+                       const Epilogue& epilogue, hipStream_t s) {
+  const int size = mat_tile_size(M, 2 * N, 1, false, 256);
+  if (size == 256) int8_gated_tiles<256, 128>(x, w0, w1, K, M, N, epilogue, s);
+  else if (size == 128) int8_gated_tiles<128, 64>(x, w0, w1, K, M, N, epilogue, s);
+  else int8_gated_tiles<64, 64>(x, w0, w1, K, M, N, epilogue, s);
 }
 
 struct Int8Inputs {
@@ -144,8 +141,12 @@ template <typename TO> static void int8_launch(const fovi_linear_int8_args* a, h
   }
   const Int8Inputs in(a, a->workspace);
   in.in.copy(stream);
-  if (a->weight2) int8_product<2>(in.x, in.w, in.w2, K, M, N, gated, stream);
-  else int8_product<1>(in.x, in.w, in.w, K, M, N, linear, stream);
+  if (a->weight2) {
+    int8_gated(in.x, in.w, in.w2, K, M, N, gated, stream);
+  } else {
+    const MatSegments s = {{in.x}, {in.w}, {K, 0}, 1};
+    mat_linear<int8_t, false, false>(s, M, N, in.in.rest(), false, linear, stream);
+  }
 }
 
 }  // namespace fovi
@@ -154,7 +155,7 @@ using namespace fovi;
 
 extern "C" int64_t fovi_linear_int8_workspace_bytes(const fovi_linear_int8_args* a) {
   if (!a || a->rows < 1 || a->inputs < 1 || a->outputs < 1 || int8_few(a)) return 0;
-  return Int8Inputs(a, nullptr).in.used();
+  return Int8Inputs(a, nullptr).in.used() + (a->weight2 ? 0 : mat_part_bytes<int8_t>(a->rows, a->outputs, a->inputs, false));
 }
 
 extern "C" int fovi_linear_int8(const fovi_linear_int8_args* a, void* stream) {

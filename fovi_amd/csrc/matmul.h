@@ -93,31 +93,17 @@ template <typename T, int NR, bool COL, int WAVES> struct MatLoader {
   typedef MatTile<T, NR, COL, WAVES> Tile;
   static constexpr int ES = sizeof(T), BK = mat_bk<T>(), LOADS = Tile::LOADS;
   static constexpr uint32_t END = 0x7fffff00u, OUTSIDE = 0x7fffff80u;
-  uint32_t off[LOADS];
-  uint64_t base;
-  int64_t step;
+  uint64_t base;                                       // all of it uniform: the addresses are formed at each load, since
+  int64_t step;                                        // registers are what the largest tiles lack
+  int stride, limit;                                   // limit: the last row of the tile, or (COL) bytes of a k row
 
+  __device__ __forceinline__ MatLoader() {}
   // (WAVES 1: every wave loads stages of its own.)
   static __device__ __forceinline__ int load(int i) { return (WAVES == 1 ? 0 : threadIdx.x >> 6) * LOADS + i; }
-  static __device__ __forceinline__ int piece(int i) { return load(i) * 64 + (threadIdx.x & 63); }
-  // The place of a lane's piece in k: its first byte, or (COL) its k row.
-  static __device__ __forceinline__ int place(int i) {
-    const int id = piece(i), r = id / Tile::PIECES;
-    return COL ? r : Tile::at(r, id % Tile::PIECES) - r * 128;
-  }
   __device__ __forceinline__ void open(const MatOperand& o, int64_t r0, int64_t k0) {
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int id = piece(i), r = id / Tile::PIECES;
-      const int b = Tile::at(r, id % Tile::PIECES) - r * Tile::PIECES * 16;    // the swap is its own inverse
-      const int stride = static_cast<int>(o.stride);
-      if (!COL) {
-        const int last = static_cast<int>(o.extent - 1 - r0 < NR ? o.extent - 1 - r0 : NR);
-        off[i] = static_cast<uint32_t>((r < last ? r : last) * stride + b);
-      } else {
-        off[i] = r0 * ES + b < o.extent * ES ? static_cast<uint32_t>(r * stride + b) : OUTSIDE;
-      }
-    }
+    stride = static_cast<int>(o.stride);
+    limit = COL ? static_cast<int>(o.extent - r0 < NR ? (o.extent - r0) * ES : NR * ES)
+                : static_cast<int>(o.extent - 1 - r0 < NR ? o.extent - 1 - r0 : NR);
     base = reinterpret_cast<uint64_t>(o.p) + (COL ? k0 * o.stride + r0 * ES : r0 * o.stride + k0 * ES);
     step = COL ? BK * o.stride : 128;
   }
@@ -126,14 +112,17 @@ template <typename T, int NR, bool COL, int WAVES> struct MatLoader {
     const i32x4 rsrc = {__builtin_amdgcn_readfirstlane(static_cast<int>(base)), __builtin_amdgcn_readfirstlane(static_cast<int>(base >> 32)),
                         static_cast<int>(END), 0x20000};
     const bool whole = left >= BK;
-    const int limit = static_cast<int>(COL ? left : left * ES);
+    const int end = static_cast<int>(COL ? left : left * ES);
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const uint32_t to = lds + load(i) * 1024;
-      const uint32_t from = whole || place(i) < limit ? off[i] : OUTSIDE;
+      const int id = load(i) * 64 + (threadIdx.x & 63), r = id / Tile::PIECES;
+      const int b = Tile::at(r, id % Tile::PIECES) - r * Tile::PIECES * 16;    // the swap is its own inverse
+      uint32_t from = static_cast<uint32_t>(__mul24(COL || r < limit ? r : limit, stride) + b);
+      if (COL && b >= limit) from = OUTSIDE;
+      if (!whole && (COL ? r : b) >= end) from = OUTSIDE;
       // m0, the place in LDS, is read by the load: one wait state behind its writing
       asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                   :: "s"(__builtin_amdgcn_readfirstlane(to)), "v"(from), "s"(rsrc) : "memory");
+                   :: "s"(__builtin_amdgcn_readfirstlane(lds + load(i) * 1024)), "v"(from), "s"(rsrc) : "memory");
     }
     base += step;
   }
@@ -407,12 +396,12 @@ inline int mat_columns(int64_t N) { return (N + 191) / 192 * 192 < (N + 255) / 2
 // The tile of a product of M x N sums (`shares` times): of 256, 128 or 64 rows, whichever ends first by the time that a
 // compute unit takes for a stage of its workgroups, one, two or four of them. A stage of 64 K sums took 1, 1.13 and 1.6 in
 // tiles of these sizes (131072 x 1024 by 384, bf16: 129, 147 and 208 us; 131072 x 384 by 2 x 1024: 300, 344 and 432): small
-// ones read more bytes a product from L2 and LDS. fp32 products are slow enough for all sizes to keep up, and tiles of 256
-// rows are not built for them.
+// ones read more bytes a product from L2 and LDS. fp32 products are slow enough for tiles of 64 to keep up and, with more
+// waves, to be ahead (2571 x 387 by 2 x 1031: 58 us, and 70 in tiles of 128); tiles of 256 rows are not built for them.
 inline int mat_tile_size(int64_t M, int64_t N, int64_t shares, bool fp32, int columns) {
   const int64_t l = (mat_tiles(M, N, 256, columns) * shares + 255) / 256 * (fp32 ? 1 << 20 : columns);
-  const int64_t m = (mat_tiles(M, N, 128, 128) * shares + 511) / 512 * (fp32 ? 128 : 145);
-  const int64_t s = (mat_tiles(M, N, 64, 64) * shares + 1023) / 1024 * (fp32 ? 64 : 102);
+  const int64_t m = (mat_tiles(M, N, 128, 128) * shares + 511) / 512 * 145;
+  const int64_t s = (mat_tiles(M, N, 64, 64) * shares + 1023) / 1024 * (fp32 ? 61 : 102);
   return l <= m && l <= s ? 256 : m <= s ? 128 : 64;
 }
 
@@ -425,6 +414,169 @@ inline void mat_launch(Kernel kernel, dim3 grid, int threads, size_t lds, hipStr
 // Whether the loads take an operand by rows as it is.
 template <typename T> inline bool mat_whole(const MatOperand& o, int64_t k) {
   return (reinterpret_cast<uintptr_t>(o.p) | o.stride | k * static_cast<int64_t>(sizeof(T))) % 16 == 0 && o.stride < (1 << 22);
+}
+
+// out = x w^T through the epilogue, k in up to two segments of other operands each. With more than one share, every
+// segment is split into shares of `share`, whose sums go to `part` and are added up by a second launch.
+struct MatSegments {
+  MatOperand x[2], w[2];
+  int64_t k[2];
+  int n;
+};
+
+template <typename Sum> struct MatPartial {             // the sums of a share
+  static constexpr int STORES = 2;                      // of 16 bytes for a run of eight
+  Sum* part; int64_t M, N;
+  __device__ __forceinline__ void operator()(int64_t share, int64_t m, int64_t n, int count, const Sum (&v)[1][8]) const {
+    Sum* p = part + (share * M + m) * N + n;
+    if (count == 8) {
+      __builtin_memcpy(p, v[0], 32);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 7; ++i)
+        if (i < count) p[i] = v[0][i];
+    }
+  }
+};
+
+template <typename T, int BM, int BN, bool CX, bool CW, typename Epilogue> struct MatLinearTile {
+  typedef MatPhase<T, BM, BN, 1, CX, CW> Phase;
+  typedef MatRing<Phase::BYTES, 2 * Phase::MB * Phase::NN * Epilogue::STORES> Ring;
+};
+template <typename T, int BM, int BN, bool CX, bool CW, typename Epilogue>
+__global__ __launch_bounds__((MatUsual<BM, BN>::THREADS), 2) void mat_linear_kernel(MatSegments s, int64_t M, int64_t N, MatWork work,
+                                                                                   int64_t share, Epilogue epilogue) {
+  typedef typename MatLinearTile<T, BM, BN, CX, CW, Epilogue>::Phase Phase;
+  typedef typename MatLinearTile<T, BM, BN, CX, CW, Epilogue>::Ring Ring;
+  typedef typename Mat<T>::Sum Sum;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  MatItem item(work), ahead(work);
+  if (!item.live()) return;
+  auto part = [&](const MatItem& at, int i, int64_t& from) __attribute__((always_inline)) {
+    const int64_t k = i ? s.k[1] : s.k[0];
+    from = at.share(work) * share;
+    return (from + share < k ? from + share : k) - from;
+  };
+  Phase phase;
+  int segment = -1;
+  int64_t left = 0;
+  auto produce = [&](uint32_t to) __attribute__((always_inline)) {
+    while (left <= 0) {
+      if (++segment == s.n) { segment = 0; ahead.next(); }
+      if (!ahead.live()) return false;
+      int64_t from;
+      left = part(ahead, segment, from);
+      const MatOperand w[1] = {segment ? s.w[1] : s.w[0]};
+      int64_t tm, tn;
+      ahead.place(work, tm, tn);
+      phase.open(segment ? s.x[1] : s.x[0], w, tm * BM, tn * BN, from);
+    }
+    phase.start(to, left);
+    left -= Phase::BK;
+    return true;
+  };
+  Ring ring(lds, produce);
+  typename Phase::Step step[2];
+  auto first_step = [&](const char* now) __attribute__((always_inline)) { step[0].read(now, 0); };
+  first_step(ring.now());
+  for (; item.live(); item.next()) {
+    typename Phase::Acc acc[1][Phase::MB][Phase::NN];
+    mat_clear(acc);
+    int64_t stages = 0, from;
+    for (int i = 0; i < s.n; ++i) {
+      const int64_t n = part(item, i, from);
+      stages += n > 0 ? (n + Phase::BK - 1) / Phase::BK : 0;
+    }
+    Phase::run(ring, stages, step, acc, 0, produce, first_step);
+    int64_t tm, tn;
+    item.place(work, tm, tn);
+    if constexpr (__is_same(Epilogue, MatPartial<Sum>)) {
+      const int64_t z = item.share(work);
+      ring.stored = mat_finish<typename Phase::Waves, BM, BN, Sum>(
+          acc, tm * BM, tn * BN, M, N, [&](int64_t m, int64_t n, int count, const Sum (&v)[1][8]) { epilogue(z, m, n, count, v); });
+    } else {
+      ring.stored = mat_finish<typename Phase::Waves, BM, BN, Sum>(acc, tm * BM, tn * BN, M, N, epilogue);
+    }
+  }
+}
+
+// The shares' sums added up in order, through the epilogue.
+template <typename Sum, typename Epilogue>
+__global__ __launch_bounds__(256) void mat_join_kernel(const Sum* part, int64_t shares, int64_t M, int64_t N, Epilogue epilogue) {
+  const int64_t per = (N + 7) / 8, i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= M * per) return;
+  const int64_t m = i / per, n = (i - m * per) * 8;
+  const int count = static_cast<int>(N - n < 8 ? N - n : 8);
+  Sum v[1][8] = {};
+  for (int64_t z = 0; z < shares; ++z) {
+    const Sum* p = part + (z * M + m) * N + n;
+    Sum t[8] = {};
+    if (count == 8) {
+      __builtin_memcpy(t, p, 32);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 7; ++e) t[e] = e < count ? p[e] : 0;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[0][e] += t[e];
+  }
+  epilogue(m, n, count, v);
+}
+
+// Shares of k. Over the tokens (long: k in the ten thousands, few sums) as many as give every compute unit a tile of
+// 256 x 256, of 512 tokens or more; else, where even tiles of 64 x 64 leave half of the card without work, as many as
+// fill it, of eight stages or more.
+template <typename T> inline int64_t mat_shares(int64_t M, int64_t N, int64_t k, bool tokens) {
+  const int64_t small = mat_tiles(M, N, 64, 64), most = tokens ? (k + 511) / 512 : k / (8 * mat_bk<T>());
+  int64_t shares = 1;
+  if (tokens) {
+    shares = (256 + mat_tiles(M, N, 256, 256) - 1) / mat_tiles(M, N, 256, 256);
+    if (shares > most) shares = (1024 + small - 1) / small;
+  } else if (small <= 512) {
+    shares = 1024 / small;
+  }
+  if (shares > most) shares = most;
+  return shares < 1 ? 1 : shares;
+}
+template <typename T> inline int64_t mat_part_bytes(int64_t M, int64_t N, int64_t k, bool tokens) {
+  const int64_t shares = mat_shares<T>(M, N, k, tokens);
+  return shares > 1 ? shares * M * N * 4 : 0;
+}
+
+template <typename T, int BM, int BN, bool CX, bool CW, typename Epilogue>
+inline void mat_linear_tiles(const MatSegments& s, int64_t M, int64_t N, int64_t share, int64_t shares, const Epilogue& epilogue,
+                             hipStream_t stream) {
+  const MatWork work = mat_work(M, N, BM, BN, shares);
+  mat_launch(mat_linear_kernel<T, BM, BN, CX, CW, Epilogue>, mat_grid(work, 256 / BM), (MatUsual<BM, BN>::THREADS),
+             MatLinearTile<T, BM, BN, CX, CW, Epilogue>::Ring::LDS, stream, s, M, N, work, share, epilogue);
+}
+template <typename T, bool CX, bool CW, typename Epilogue>
+inline void mat_linear_shares(const MatSegments& s, int64_t M, int64_t N, int64_t share, int64_t shares, const Epilogue& epilogue,
+                              hipStream_t stream) {
+  const int size = mat_tile_size(M, N, shares, sizeof(T) == 4, mat_columns(N));
+  if constexpr (sizeof(T) < 4) {
+    if (size == 256) {
+      if (mat_columns(N) == 192) mat_linear_tiles<T, 256, 192, CX, CW>(s, M, N, share, shares, epilogue, stream);
+      else mat_linear_tiles<T, 256, 256, CX, CW>(s, M, N, share, shares, epilogue, stream);
+      return;
+    }
+  }
+  if (size == 128) mat_linear_tiles<T, 128, 128, CX, CW>(s, M, N, share, shares, epilogue, stream);
+  else mat_linear_tiles<T, 64, 64, CX, CW>(s, M, N, share, shares, epilogue, stream);
+}
+// part: mat_part_bytes of M, N and the longest segment.
+template <typename T, bool CX, bool CW, typename Epilogue>
+inline void mat_linear(const MatSegments& s, int64_t M, int64_t N, void* part, bool tokens, const Epilogue& epilogue, hipStream_t stream) {
+  typedef typename Mat<T>::Sum Sum;
+  const int64_t k = s.n == 2 && s.k[1] > s.k[0] ? s.k[1] : s.k[0], shares = mat_shares<T>(M, N, k, tokens);
+  if (shares == 1) {
+    mat_linear_shares<T, CX, CW>(s, M, N, k, 1, epilogue, stream);
+    return;
+  }
+  const int64_t bk = mat_bk<T>(), share = ((k + shares - 1) / shares + bk - 1) / bk * bk, used = (k + share - 1) / share;
+  Sum* sums = static_cast<Sum*>(part);
+  mat_linear_shares<T, CX, CW>(s, M, N, share, used, MatPartial<Sum>{sums, M, N}, stream);
+  mat_join_kernel<Sum, Epilogue><<<static_cast<unsigned>((M * ((N + 7) / 8) + 255) / 256), 256, 0, stream>>>(sums, used, M, N, epilogue);
 }
 
 // 16 bytes of a run of `len` bytes from `at` on, at any alignment, zeros from its end on.
@@ -452,7 +604,8 @@ __device__ __forceinline__ u32x4 mat_piece(const char* run, int64_t at, int64_t 
 // are copied in front of a product, their rows filled up with zeros: one launch for all of a call.
 struct MatCopies {
   static constexpr int MOST = 5;
-  struct { const char* from; char* to; int64_t stride, rows, len; } m[MOST];
+  struct { const char* from; char* to; int64_t stride, len; } m[MOST];
+  int64_t first[MOST + 1];                             // of each matrix's pieces, in one sequence
   int n;
 };
 __global__ void mat_copy_kernel(MatCopies c);
@@ -460,15 +613,17 @@ __global__ void mat_copy_kernel(MatCopies c);
 // A call's operands: take() gives the matrix that the kernels read, which is the caller's or a copy in the workspace.
 class MatInputs {
  public:
-  explicit MatInputs(void* workspace) : at_(static_cast<char*>(workspace)), start_(at_) { copies_.n = 0; }
+  explicit MatInputs(void* workspace) : at_(static_cast<char*>(workspace)), start_(at_) { copies_.n = 0; copies_.first[0] = 0; }
   // rows x cols elements of `es` bytes, `stride` elements apart; the result's stride is in bytes.
   MatOperand take(const void* p, int64_t stride, int64_t rows, int64_t cols, int64_t es) {
     const int64_t bytes = cols * es;
     const MatOperand as_is = {static_cast<const char*>(p), stride * es, rows};
     if (mat_whole<char>(as_is, bytes)) return as_is;
     const int64_t wide = (bytes + 15) / 16 * 16;
-    auto& m = copies_.m[copies_.n++];
-    m.from = static_cast<const char*>(p); m.to = at_; m.stride = stride * es; m.rows = rows; m.len = bytes;
+    auto& m = copies_.m[copies_.n];
+    m.from = static_cast<const char*>(p); m.to = at_; m.stride = stride * es; m.len = bytes;
+    copies_.first[copies_.n + 1] = copies_.first[copies_.n] + rows * (wide / 16);
+    ++copies_.n;
     const MatOperand o = {at_, wide, rows};
     at_ += (rows * wide + 255) / 256 * 256;
     return o;

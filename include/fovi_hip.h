@@ -954,7 +954,7 @@ int fovi_dequantize_rows(const int8_t* q, const float* scale, int64_t rows, int6
  * Strides are in elements between rows, elements adjacent, at any alignment. Sums are exact in int32 (up to 131072 inputs).
  * out and residual: out_dtype, F32 or BF16; bias fp32 (may be NULL, as may residual). The workspace
  * (fovi_linear_int8_workspace_bytes of the arguments, may be 0; 16-byte aligned) holds copies of
- * matrices whose rows are not whole, aligned 16-byte pieces.
+ * matrices whose rows are not whole, aligned 16-byte pieces, and partial sums where the inputs are split over workgroups.
  */
 enum fovi_gate_act { FOVI_GATE_SILU = 0, FOVI_GATE_GELU = 1 };
 
