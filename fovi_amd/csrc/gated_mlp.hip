@@ -18,38 +18,38 @@ __device__ __forceinline__ void clear_behind(int count, float (&v)[8]) {
   for (int i = 1; i < 8; ++i) v[i] = i < count ? v[i] : 0.0f;
 }
 
-template <typename T> struct MlpLinear {               // out = sums (+ residual)
+template <typename T> struct MlpLinear : NoColumn {               // out = sums (+ residual)
   static constexpr int STORES = sizeof(T) / 2;         // of 16 bytes for a run of eight
+  typedef Run<T> Extra;
   T* out; int64_t stride;
   const T* residual; int64_t residual_stride;
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const float (&v)[1][8]) const {
+  __device__ __forceinline__ Extra load(int64_t m, int64_t n, int count) const {
+    Extra r = {};
+    if (residual) r.load(residual + m * residual_stride + n, count);
+    return r;
+  }
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const float (&v)[1][8], const NoExtra&, const Extra& r) const {
     float y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = v[0][i];
-    if (residual) {
-      float r[8];
-      load_run(residual + m * residual_stride + n, count, r);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] += r[i];
-    }
+    for (int i = 0; i < 8; ++i) y[i] = residual ? v[0][i] + r[i] : v[0][i];
     store_run(out + m * stride + n, count, y);
   }
 };
 
-template <typename T> struct MlpTwoRows {              // `rows` rows to one output, those from `next` on to the other
+template <typename T> struct MlpTwoRows : Plain {              // `rows` rows to one output, those from `next` on to the other
   static constexpr int STORES = 0;                     // rows between the two are not stored
   T* out[2]; int64_t rows, next, stride;
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const float (&v)[1][8]) const {
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const float (&v)[1][8], const NoExtra&, const NoExtra&) const {
     if (m < rows) store_run(out[0] + m * stride + n, count, v[0]);
     else if (m >= next) store_run(out[1] + (m - next) * stride + n, count, v[0]);
   }
 };
 
-template <typename T> struct MlpGated {                // h, and gate and up where a backward will read them
+template <typename T> struct MlpGated : Plain {                // h, and gate and up where a backward will read them
   static constexpr int STORES = sizeof(T) / 2;
   T* h; int64_t stride; int act;
   T* gate; T* up; int64_t saved_stride;
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const float (&v)[2][8]) const {
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const float (&v)[2][8], const NoExtra&, const NoExtra&) const {
     float y[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] = mat_act<sizeof(T) == 4>(v[0][i], act) * v[1][i];
@@ -62,12 +62,12 @@ template <typename T> struct MlpGated {                // h, and gate and up whe
   }
 };
 
-template <typename T> struct MlpGatedGrad {            // dgate, dup and h from gate, up and dh
+// dgate, dup and h of a run of gate, up and dh.
+template <typename T> struct MlpGradRows {
   static constexpr int STORES = 3 * sizeof(T) / 2;
   T* dgate; T* dup; T* h; int64_t stride, h_stride; int act;
-  const T* gate; const T* up; int64_t saved_stride;
-  __device__ __forceinline__ void write(int64_t m, int64_t n, int count, const float (&g)[8], const float (&u)[8],
-                                        const float (&dh)[8]) const {
+  template <typename G, typename U>
+  __device__ __forceinline__ void write(int64_t m, int64_t n, int count, const G& g, const U& u, const float (&dh)[8]) const {
     float a[8], b[8], c[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -84,14 +84,23 @@ template <typename T> struct MlpGatedGrad {            // dgate, dup and h from 
     store_run(dup + m * stride + n, 8, b);
     store_run(h + m * h_stride + n, 8, c);
   }
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const float (&v)[3][8]) const {
-    write(m, n, count, v[0], v[1], v[2]);
+};
+template <typename T> struct MlpGatedGrad : Plain, MlpGradRows<T> {   // of all three sums
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const float (&v)[3][8], const NoExtra&, const NoExtra&) const {
+    this->write(m, n, count, v[0], v[1], v[2]);
   }
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const float (&v)[1][8]) const {
-    float g[8], u[8];
-    load_run(gate + m * saved_stride + n, count, g);
-    load_run(up + m * saved_stride + n, count, u);
-    write(m, n, count, g, u, v[0]);
+};
+template <typename T> struct MlpSavedGrad : NoColumn, MlpGradRows<T> { // of dh's sums and the gate and up of the forward
+  struct Extra { Run<T> gate, up; };
+  const T* gate; const T* up; int64_t saved_stride;
+  __device__ __forceinline__ Extra load(int64_t m, int64_t n, int count) const {
+    Extra x;
+    x.gate.load(gate + m * saved_stride + n, count);
+    x.up.load(up + m * saved_stride + n, count);
+    return x;
+  }
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const float (&v)[1][8], const NoExtra&, const Extra& x) const {
+    this->write(m, n, count, x.gate, x.up, v[0]);
   }
 };
 
@@ -244,8 +253,8 @@ template <typename T> static MatOperand as_is(const void* p, int64_t stride, int
 template <typename T> static void mlp_fwd(const fovi_gated_mlp_args* a, hipStream_t s) {
   const int64_t M = a->rows, C = a->dim, F = a->hidden, Fp = wide(F);
   T* gate = static_cast<T*>(a->saved);
-  const MlpLinear<T> linear = {static_cast<T*>(a->y), a->y_stride, static_cast<const T*>(a->residual), a->residual_stride};
-  MlpGated<T> gated = {static_cast<T*>(a->workspace), Fp, a->activation, gate, gate + F, 2 * F};
+  const MlpLinear<T> linear = {{}, static_cast<T*>(a->y), a->y_stride, static_cast<const T*>(a->residual), a->residual_stride};
+  MlpGated<T> gated = {{}, static_cast<T*>(a->workspace), Fp, a->activation, gate, gate + F, 2 * F};
   if (mlp_few(a)) {
     few_product<T, 2>(as_is<T>(a->x, a->x_stride, M), as_is<T>(a->w_gate, a->w_gate_stride, F), as_is<T>(a->w_up, a->w_up_stride, F), C, M, F,
                       gated, s);
@@ -274,12 +283,13 @@ template <typename T> static void mlp_bwd(const fovi_gated_mlp_args* a, hipStrea
   T* h = reinterpret_cast<T*>(in.in.rest() + aligned(M * 2 * Fp * es));
   char* part = reinterpret_cast<char*>(h) + aligned(M * Fp * es);
   const MatOperand wd = columns(in.wd, F, es);
-  const T* gate = static_cast<const T*>(a->saved);
-  const MlpGatedGrad<T> gated = {grad, grad + Fp, h, 2 * Fp, Fp, a->activation, gate, gate + F, 2 * F};
+  const MlpGradRows<T> rows = {grad, grad + Fp, h, 2 * Fp, Fp, a->activation};
   if constexpr (sizeof(T) == 4) {
+    const T* gate = static_cast<const T*>(a->saved);
     const MatSegments down = {{in.dy}, {wd}, {C, 0}, 1};
-    mat_linear<T, false, true>(down, M, F, part, false, gated, s);
+    mat_linear<T, false, true>(down, M, F, part, false, MlpSavedGrad<T>{{}, rows, gate, gate + F, 2 * F}, s);
   } else {
+    const MlpGatedGrad<T> gated = {{}, rows};
     const int size = mat_tile_size(M, 2 * F, 1, false, 256);
     if (size >= 128) mlp_gated_grad_tiles<T, 128, 64, MatWaves<2, 2>>(in, wd, C, M, F, gated, s);
     else mlp_gated_grad_tiles<T, 64, 64, MatWaves<2, 2>>(in, wd, C, M, F, gated, s);
@@ -288,15 +298,15 @@ template <typename T> static void mlp_bwd(const fovi_gated_mlp_args* a, hipStrea
   if (a->dx) {
     const MatSegments both = {{MatOperand{dgate, 2 * Fp * es, M}, MatOperand{dgate + Fp * es, 2 * Fp * es, M}},
                               {columns(in.wg, C, es), columns(in.wu, C, es)}, {F, F}, 2};
-    mat_linear<T, false, true>(both, M, C, part, false, MlpLinear<T>{static_cast<T*>(a->dx), C, nullptr, 0}, s);
+    mat_linear<T, false, true>(both, M, C, part, false, MlpLinear<T>{{}, static_cast<T*>(a->dx), C, nullptr, 0}, s);
   }
   if (a->dw_gate) {
     const MatSegments up = {{MatOperand{dgate, 2 * Fp * es, 2 * Fp}}, {columns(in.x, C, es)}, {M, 0}, 1};
-    mat_linear<T, true, true>(up, Fp + F, C, part, true, MlpTwoRows<T>{{static_cast<T*>(a->dw_gate), static_cast<T*>(a->dw_up)}, F, Fp, C}, s);
+    mat_linear<T, true, true>(up, Fp + F, C, part, true, MlpTwoRows<T>{{}, {static_cast<T*>(a->dw_gate), static_cast<T*>(a->dw_up)}, F, Fp, C}, s);
   }
   if (a->dw_down) {
     const MatSegments down = {{columns(in.dy, C, es)}, {MatOperand{reinterpret_cast<char*>(h), Fp * es, Fp}}, {M, 0}, 1};
-    mat_linear<T, true, true>(down, C, F, part, true, MlpLinear<T>{static_cast<T*>(a->dw_down), F, nullptr, 0}, s);
+    mat_linear<T, true, true>(down, C, F, part, true, MlpLinear<T>{{}, static_cast<T*>(a->dw_down), F, nullptr, 0}, s);
   }
 }
 

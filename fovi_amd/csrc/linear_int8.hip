@@ -14,24 +14,30 @@ struct Int8Scales {
 
 template <typename TO> struct Int8Linear {
   static constexpr int STORES = sizeof(TO) / 2;        // of 16 bytes for a run of eight
+  struct Column { Run<float> w, bias; };
+  struct Extra { Run<TO> residual; float x; };
   Int8Scales s;
   const float* bias; const TO* residual; int64_t residual_stride;
   TO* out; int64_t stride;
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const int32_t (&v)[1][8]) const {
-    const float sx = s.x[m];
-    float y[8], w[8], t[8];
-    load_run(s.w + n, count, w);
+  __device__ __forceinline__ Column column(int64_t n, int count) const {
+    Column c = {};
+    c.w.load(s.w + n, count);
+    if (bias) c.bias.load(bias + n, count);
+    return c;
+  }
+  __device__ __forceinline__ Extra load(int64_t m, int64_t n, int count) const {
+    Extra e = {};
+    e.x = s.x[m];
+    if (residual) e.residual.load(residual + m * residual_stride + n, count);
+    return e;
+  }
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const int32_t (&v)[1][8], const Column& c, const Extra& e) const {
+    float y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = static_cast<float>(v[0][i]) * sx * w[i];
-    if (bias) {
-      load_run(bias + n, count, t);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] += t[i];
-    }
-    if (residual) {
-      load_run(residual + m * residual_stride + n, count, t);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] += t[i];
+    for (int i = 0; i < 8; ++i) {
+      y[i] = static_cast<float>(v[0][i]) * e.x * c.w[i];
+      if (bias) y[i] += c.bias[i];
+      if (residual) y[i] += e.residual[i];
     }
     store_run(out + m * stride + n, count, y);
   }
@@ -39,17 +45,23 @@ template <typename TO> struct Int8Linear {
 
 template <typename TO> struct Int8Gated {
   static constexpr int STORES = sizeof(TO) / 2;
+  struct Column { Run<float> gate, up; };
+  typedef float Extra;
   Int8Scales s;
   int act;
   TO* out; int64_t stride;
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const int32_t (&v)[2][8]) const {
-    const float sx = s.x[m];
-    float y[8], g[8], u[8];
-    load_run(s.w + n, count, g);
-    load_run(s.w2 + n, count, u);
+  __device__ __forceinline__ Column column(int64_t n, int count) const {
+    Column c;
+    c.gate.load(s.w + n, count);
+    c.up.load(s.w2 + n, count);
+    return c;
+  }
+  __device__ __forceinline__ Extra load(int64_t m, int64_t, int) const { return s.x[m]; }
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const int32_t (&v)[2][8], const Column& c, const Extra& x) const {
+    float y[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      y[i] = mat_act<false>(static_cast<float>(v[0][i]) * sx * g[i], act) * (static_cast<float>(v[1][i]) * sx * u[i]);
+      y[i] = mat_act<false>(static_cast<float>(v[0][i]) * x * c.gate[i], act) * (static_cast<float>(v[1][i]) * x * c.up[i]);
     store_run(out + m * stride + n, count, y);
   }
 };

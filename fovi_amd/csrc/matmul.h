@@ -132,6 +132,18 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)p));
 }
 
+template <typename Acc, int NA, int MB, int NN>
+__device__ __forceinline__ void mat_clear(Acc (&acc)[NA][MB][NN]) {
+#pragma unroll
+  for (int b = 0; b < NA; ++b)
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int j = 0; j < NN; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[b][i][j][r] = 0;
+}
+
 // The waves of a workgroup, WM by WN over its tile.
 template <int WM, int WN> struct MatWaves {
   static constexpr int M = WM, N = WN, ALL = M * N, THREADS = 64 * ALL;
@@ -188,6 +200,9 @@ struct MatPhase {
           for (int j = 0; j < NN; ++j) acc[first + b][i][j] = mat_step(T(), w[b][j], x[i], acc[first + b][i][j]);
     }
   };
+  // fp32 sums are taken by stages and added up: a chain of 32 products and one of the stages, instead of one of all
+  // (2571 x 387, hidden 1031: outputs and gradients 9.8e-7 off in a row, the norm of the difference over the norm, 2.3e-7 so).
+  static constexpr bool STAGED = sizeof(T) == 4;
   // The products of `stages` stages. step[0] holds the first step of the first one; first_step(lds) reads that of the
   // stage behind the last one, if there is one.
   template <int NA, typename Ring, typename Produce, typename FirstStep>
@@ -195,11 +210,14 @@ struct MatPhase {
                                              const Produce& produce, const FirstStep& first_step) {
     for (int64_t t = stages; t > 0; --t) {
       const char* now = ring.now();
+      Acc part[NB][MB][NN];
+      if (STAGED) mat_clear(part);
 #pragma unroll
       for (int s = 0; s < 3; ++s) {
         step[(s + 1) & 1].read(now, s + 1);
         __builtin_amdgcn_sched_barrier(0);
-        step[s & 1].multiply(acc, first);
+        if (STAGED) step[s & 1].multiply(part, 0);
+        else step[s & 1].multiply(acc, first);
         __builtin_amdgcn_sched_barrier(0);
       }
       if (ring.advance(produce)) {
@@ -207,7 +225,17 @@ struct MatPhase {
         else first_step(ring.now());
         __builtin_amdgcn_sched_barrier(0);
       }
-      step[1].multiply(acc, first);
+      if (STAGED) {
+        step[1].multiply(part, 0);
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int j = 0; j < NN; ++j) acc[first + b][i][j] += part[b][i][j];
+      } else {
+        step[1].multiply(acc, first);
+      }
     }
   }
   // The same where the sums leave registers for one step only: its reads are waited for, beside another wave's products.
@@ -257,47 +285,61 @@ template <int BYTES, int STORES> struct MatRing {
   }
 };
 
-template <typename Acc, int NA, int MB, int NN>
-__device__ __forceinline__ void mat_clear(Acc (&acc)[NA][MB][NN]) {
-#pragma unroll
-  for (int b = 0; b < NA; ++b)
-#pragma unroll
-    for (int i = 0; i < MB; ++i)
-#pragma unroll
-      for (int j = 0; j < NN; ++j)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[b][i][j][r] = 0;
-}
-
-// epilogue(m, n, count, v): the sums v[b][0 .. count) of row m from column n on, in runs of eight. A lane's block holds four
-// adjacent columns of every eight, the lane 32 further on the other four: the two swap halves of two such runs.
+// epilogue(m, n, count, v, column, extra): the sums v[b][0 .. count) of row m from column n on, in runs of eight; what
+// epilogue.column(n, count) gave for the columns, and epilogue.load(m, n, count) for the run. These are read a column ahead,
+// and for all runs at once (where the sums and they are too many for the registers, for a column and its runs), not run by
+// run behind the stores of the run before. A lane's block holds four adjacent columns of every eight, the lane 32
+// further on the other four: the two swap halves of two such runs.
 template <typename Waves, int BM, int BN, typename Sum, bool WHOLE, typename Acc, int NA, int MB, int NN, typename Epilogue>
 __device__ __forceinline__ void mat_runs(const Acc (&acc)[NA][MB][NN], int64_t m0, int64_t n0, int64_t M, int64_t N, const Epilogue& epilogue) {
+  constexpr bool FULL = NA * MB * NN * 16 + 2 * NN * MB * static_cast<int>(sizeof(typename Epilogue::Extra)) / 4 > 140;
   const int l = threadIdx.x & 63;
+  const int64_t mw = m0 + Waves::m() * (BM / Waves::M) + (l & 31), nw = n0 + Waves::n() * (BN / Waves::N) + 8 * (l >> 5);
+  typename Epilogue::Extra extra[FULL ? 1 : 2 * NN][MB];
+  auto load = [&](int c, typename Epilogue::Extra (&to)[MB]) __attribute__((always_inline)) {
+    const int64_t n = nw + 16 * c;
 #pragma unroll
-  for (int j = 0; j < NN; ++j)
-#pragma unroll
-    for (int q = 0; q < 4; q += 2) {
-      const int64_t n = n0 + Waves::n() * (BN / Waves::N) + 32 * j + 8 * q + 8 * (l >> 5);
-#pragma unroll
-      for (int i = 0; i < MB; ++i) {
-        const int64_t m = m0 + Waves::m() * (BM / Waves::M) + 32 * i + (l & 31);
-        Sum v[NA][8];
-#pragma unroll
-        for (int b = 0; b < NA; ++b)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const auto t = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, static_cast<Sum>(acc[b][i][j][4 * q + e])),
-                                                            __builtin_bit_cast(uint32_t, static_cast<Sum>(acc[b][i][j][4 * q + 4 + e])), false, false);
-            const uint32_t t0 = t[0], t1 = t[1];       // (a bit cast of t[1] itself takes t[0])
-            v[b][e] = __builtin_bit_cast(Sum, t0);
-            v[b][4 + e] = __builtin_bit_cast(Sum, t1);
-          }
-        if (WHOLE) epilogue(m, n, 8, v);
-        else if (m < M && n < N) epilogue(m, n, static_cast<int>(N - n < 8 ? N - n : 8), v);
-        __builtin_amdgcn_sched_barrier(0);             // (mixed, the runs take more registers than there are)
-      }
+    for (int i = 0; i < MB; ++i) {
+      if (WHOLE) to[i] = epilogue.load(mw + 32 * i, n, 8);
+      else if (mw + 32 * i < M && n < N) to[i] = epilogue.load(mw + 32 * i, n, static_cast<int>(N - n < 8 ? N - n : 8));
     }
+  };
+  if (!FULL) {
+#pragma unroll
+    for (int c = 0; c < 2 * NN; ++c) load(c, extra[FULL ? 0 : c]);
+  }
+  typename Epilogue::Column column[FULL ? 1 : 2];
+  auto load_column = [&](int c) __attribute__((always_inline)) {
+    const int64_t n = nw + 16 * c;
+    if (WHOLE) column[FULL ? 0 : c & 1] = epilogue.column(n, 8);
+    else if (n < N) column[FULL ? 0 : c & 1] = epilogue.column(n, static_cast<int>(N - n < 8 ? N - n : 8));
+  };
+  if (!FULL) load_column(0);
+#pragma unroll
+  for (int c = 0; c < 2 * NN; ++c) {                   // columns of 16
+    if (FULL) { load_column(c); load(c, extra[0]); }
+    else if (c + 1 < 2 * NN) load_column(c + 1);
+    const int j = c / 2, q = c % 2 * 2;
+    const int64_t n = nw + 16 * c;
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+      const int64_t m = mw + 32 * i;
+      Sum v[NA][8];
+#pragma unroll
+      for (int b = 0; b < NA; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const auto t = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, static_cast<Sum>(acc[b][i][j][4 * q + e])),
+                                                          __builtin_bit_cast(uint32_t, static_cast<Sum>(acc[b][i][j][4 * q + 4 + e])), false, false);
+          const uint32_t t0 = t[0], t1 = t[1];         // (a bit cast of t[1] itself takes t[0])
+          v[b][e] = __builtin_bit_cast(Sum, t0);
+          v[b][4 + e] = __builtin_bit_cast(Sum, t1);
+        }
+      if (WHOLE) epilogue(m, n, 8, v, column[FULL ? 0 : c & 1], extra[FULL ? 0 : c][i]);
+      else if (m < M && n < N) epilogue(m, n, static_cast<int>(N - n < 8 ? N - n : 8), v, column[FULL ? 0 : c & 1], extra[FULL ? 0 : c][i]);
+      if (FULL) __builtin_amdgcn_sched_barrier(0);     // (mixed, the runs take more registers than there are)
+    }
+  }
 }
 template <typename Waves, int BM, int BN, typename Sum, typename Acc, int NA, int MB, int NN, typename Epilogue>
 __device__ __forceinline__ bool mat_finish(const Acc (&acc)[NA][MB][NN], int64_t m0, int64_t n0, int64_t M, int64_t N,
@@ -308,18 +350,28 @@ __device__ __forceinline__ bool mat_finish(const Acc (&acc)[NA][MB][NN], int64_t
   return whole;
 }
 
-// Eight (or `count`) adjacent elements as floats, and back.
-template <typename T> __device__ __forceinline__ void load_run(const T* p, int count, float (&v)[8]) {
+// Eight (or `count`) adjacent elements, in registers as they are in memory, and as floats.
+template <typename T> struct Run {
   T e[8];
-  if (count == 8) {
-    __builtin_memcpy(e, p, sizeof(e));
-  } else {
+  __device__ __forceinline__ void load(const T* p, int count) {
+    if (count == 8) {
+      __builtin_memcpy(e, p, sizeof(e));
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = i < count ? p[i] : T(0);
+      for (int i = 0; i < 8; ++i) e[i] = i < count ? p[i] : T(0);
+    }
   }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = Elem<T>::load(e + i);
-}
+  __device__ __forceinline__ float operator[](int i) const { return Elem<T>::load(e + i); }
+};
+struct NoExtra {};
+struct NoColumn {
+  typedef NoExtra Column;
+  __device__ __forceinline__ Column column(int64_t, int) const { return Column(); }
+};
+struct Plain : NoColumn {                              // an epilogue that reads nothing else
+  typedef NoExtra Extra;
+  __device__ __forceinline__ Extra load(int64_t, int64_t, int) const { return Extra(); }
+};
 template <typename T> __device__ __forceinline__ void store_run(T* p, int count, const float (&v)[8]) {
   T e[8];
 #pragma unroll
@@ -424,11 +476,11 @@ struct MatSegments {
   int n;
 };
 
-template <typename Sum> struct MatPartial {             // the sums of a share
+template <typename Sum> struct MatPartial : Plain {             // the sums of a share
   static constexpr int STORES = 2;                      // of 16 bytes for a run of eight
   Sum* part; int64_t M, N;
-  __device__ __forceinline__ void operator()(int64_t share, int64_t m, int64_t n, int count, const Sum (&v)[1][8]) const {
-    Sum* p = part + (share * M + m) * N + n;
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, int count, const Sum (&v)[1][8], const NoExtra&, const NoExtra&) const {
+    Sum* p = part + m * N + n;
     if (count == 8) {
       __builtin_memcpy(p, v[0], 32);
     } else {
@@ -491,9 +543,9 @@ __global__ __launch_bounds__((MatUsual<BM, BN>::THREADS), 2) void mat_linear_ker
     int64_t tm, tn;
     item.place(work, tm, tn);
     if constexpr (__is_same(Epilogue, MatPartial<Sum>)) {
-      const int64_t z = item.share(work);
-      ring.stored = mat_finish<typename Phase::Waves, BM, BN, Sum>(
-          acc, tm * BM, tn * BN, M, N, [&](int64_t m, int64_t n, int count, const Sum (&v)[1][8]) { epilogue(z, m, n, count, v); });
+      MatPartial<Sum> mine = epilogue;
+      mine.part += item.share(work) * M * N;
+      ring.stored = mat_finish<typename Phase::Waves, BM, BN, Sum>(acc, tm * BM, tn * BN, M, N, mine);
     } else {
       ring.stored = mat_finish<typename Phase::Waves, BM, BN, Sum>(acc, tm * BM, tn * BN, M, N, epilogue);
     }
@@ -520,7 +572,7 @@ __global__ __launch_bounds__(256) void mat_join_kernel(const Sum* part, int64_t 
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[0][e] += t[e];
   }
-  epilogue(m, n, count, v);
+  epilogue(m, n, count, v, epilogue.column(n, count), epilogue.load(m, n, count));
 }
 
 // Shares of k. Over the tokens (long: k in the ten thousands, few sums) as many as give every compute unit a tile of
@@ -575,7 +627,7 @@ inline void mat_linear(const MatSegments& s, int64_t M, int64_t N, void* part, b
   }
   const int64_t bk = mat_bk<T>(), share = ((k + shares - 1) / shares + bk - 1) / bk * bk, used = (k + share - 1) / share;
   Sum* sums = static_cast<Sum*>(part);
-  mat_linear_shares<T, CX, CW>(s, M, N, share, used, MatPartial<Sum>{sums, M, N}, stream);
+  mat_linear_shares<T, CX, CW>(s, M, N, share, used, MatPartial<Sum>{{}, sums, M, N}, stream);
   mat_join_kernel<Sum, Epilogue><<<static_cast<unsigned>((M * ((N + 7) / 8) + 255) / 256), 256, 0, stream>>>(sums, used, M, N, epilogue);
 }
 

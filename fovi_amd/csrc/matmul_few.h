@@ -58,6 +58,9 @@ __device__ __forceinline__ void few_finish(char* memory, const typename Few<T>::
     const int m = id / (2 * RB), r = id % (2 * RB);
     const int64_t n = n0 + 8 * r;
     if (m0 + m >= M || n >= N) continue;
+    const int count = static_cast<int>(N - n < 8 ? N - n : 8);
+    const typename Epilogue::Column column = epilogue.column(n, count);
+    const typename Epilogue::Extra extra = epilogue.load(m0 + m, n, count);
     Sum v[NB][8];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
@@ -70,7 +73,7 @@ __device__ __forceinline__ void few_finish(char* memory, const typename Few<T>::
         for (int e = 0; e < 4; ++e) { v[b][e] += lo[e]; v[b][4 + e] += hi[e]; }
       }
     }
-    epilogue(m0 + m, n, static_cast<int>(N - n < 8 ? N - n : 8), v);
+    epilogue(m0 + m, n, count, v, column, extra);
   }
 }
 
