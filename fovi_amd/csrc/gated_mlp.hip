@@ -244,7 +244,9 @@ static void mlp_gated_grad_tiles(const MlpInputs& in, const MatOperand& wd, int6
              M, F, work, epilogue);
 }
 
-static bool mlp_few(const fovi_gated_mlp_args* a) { return a->rows <= kFewRows; }
+static bool mlp_few(const fovi_gated_mlp_args* a) {
+  return few_rows_best(a->rows, a->hidden > a->dim ? a->hidden : a->dim, a->dtype == FOVI_F32);
+}
 
 template <typename T> static MatOperand as_is(const void* p, int64_t stride, int64_t rows) {
   return MatOperand{static_cast<const char*>(p), stride * static_cast<int64_t>(sizeof(T)), rows};

@@ -136,7 +136,7 @@ struct Int8Inputs {
   }
 };
 
-static bool int8_few(const fovi_linear_int8_args* a) { return a->rows <= kFewRows; }
+static bool int8_few(const fovi_linear_int8_args* a) { return few_rows_best(a->rows, a->outputs, a->weight2 != nullptr); }
 
 template <typename TO> static void int8_launch(const fovi_linear_int8_args* a, hipStream_t stream) {
   const int64_t M = a->rows, N = a->outputs, K = a->inputs;

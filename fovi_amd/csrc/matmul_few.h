@@ -1,4 +1,4 @@
-// Products of a few rows (up to 64) with large weights: serving steps. What counts is the weights' way from memory.
+// Products of a few rows with large weights: serving steps. What counts is the weights' way from memory.
 //
 // A wave multiplies 16 rows of w (NB matrices, or RB neighbouring blocks of one) by up to TB blocks of 16 rows of x, over its
 // share of k, with the 16 x 16 matrix instructions (lane l holds row l % 16, the pieces l / 16 of 64 bytes of k). The waves of
@@ -211,7 +211,14 @@ __global__ __launch_bounds__(1024) void few_ring_kernel(MatOperand x, MatOperand
   few_finish<T, NB, RB, TB>(few_ring_memory, acc, m0, n0, M, N, epilogue);
 }
 
-constexpr int kFewRows = 64;
+// Up to 64 rows go here, and up to 256 where tiles of 64 x 64 would leave compute units without work: fewer tiles than compute
+// units, or half as many where a tile has more to do (fp32, two products in int8). Here and by tiles, us: int8 4096 x 1024,
+// 128 rows 5.1 and 10.3, 256 rows 6.5 and 11.5; int8 1024 x 4096, 128 rows 4.7 and 6.6, 192 rows two products 10.6 and 7.6;
+// the block of 384 x 1024, 128 rows, bf16 7.7 and 15.1, fp32 12.7 and 32.6, of 2048 x 5504, bf16 33.9 and 40.1, fp32 151 and
+// 128; int8 4096 x 11008 (344 tiles), 128 rows, 23.8 and 20.8.
+inline bool few_rows_best(int64_t M, int64_t N, bool heavy) {
+  return M <= 64 || (M <= 256 && (M + 63) / 64 * ((N + 63) / 64) <= (heavy ? 128 : 255));
+}
 
 // Waves of a workgroup: four steps of 64 bytes for each, but no more than give the card 4096 waves (as many as are resident
 // at a time), nor fewer than four.
@@ -258,7 +265,7 @@ static void few_product(const MatOperand& x, const MatOperand& w0, const MatOper
   int64_t best = 0;
   int best_rb = 0, best_tb = 0;
   for (int rb = 1; rb <= 3 - NB; ++rb)
-    for (int parts = 1; parts <= blocks; ++parts) {
+    for (int parts = (blocks + 3) / 4; parts <= blocks; ++parts) {
       const int tb = (blocks + parts - 1) / parts;
       const int64_t rounds = ((N + 16 * rb - 1) / (16 * rb) * parts + 255) / 256, cost = rounds * (rb * NB + tb);
       if (!best_rb || cost < best) { best = cost; best_rb = rb; best_tb = tb; }

@@ -79,7 +79,7 @@ def _within(got, want, what):
 NAMES = ("dx", "dw_gate", "dw_up", "dw_down")
 SIZES = [(1, 1, 1), (1, 384, 1024), (2, 8, 24), (3, 5, 7), (16, 64, 64), (17, 33, 129), (31, 2048, 200), (64, 384, 1024), (65, 96, 64),
          (100, 771, 129), (129, 128, 257), (300, 387, 1031), (1000, 64, 96), (2049, 40, 72), (700, 256, 384), (5000, 8, 16),
-         (40, 16, 5504), (33, 1030, 8)]
+         (40, 16, 5504), (33, 1030, 8), (70, 24, 16500), (200, 131, 4100), (256, 640, 96), (200, 100, 67)]
 
 
 @pytest.mark.gpu

@@ -38,7 +38,8 @@ def _act(z, name):
 
 SIZES = [(1, 1, 1), (1, 64, 384), (1, 4096, 100), (2, 16, 16), (3, 17, 5), (16, 1024, 384), (17, 771, 33), (48, 2048, 1003), (64, 128, 129),
          (65, 128, 128), (100, 15, 64), (129, 129, 257), (300, 771, 1537), (1000, 640, 384), (257, 8192, 70), (513, 384, 1024),
-         (64, 12288, 40), (2000, 96, 2752), (1, 65536, 17), (40, 33000, 3)]
+         (64, 12288, 40), (2000, 96, 2752), (1, 65536, 17), (40, 33000, 3), (70, 80, 16500),
+         (200, 33, 4100), (200, 100, 257), (256, 640, 96)]
 
 
 @pytest.mark.gpu
