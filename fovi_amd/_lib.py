@@ -460,6 +460,16 @@ def stream_of(t):
     return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
+def launch(entry, args, t, what):
+    """``entry(*args, stream)`` on the device of ``t`` and its current stream, whichever device is the current one."""
+    index = t.device.index
+    if torch.cuda.current_device() == index:
+        check(entry(*args, stream_of(t)), what)
+        return
+    with torch.cuda.device(index):
+        check(entry(*args, stream_of(t)), what)
+
+
 def check(rc: int, what: str):
     if rc != 0:
         msg = load().fovi_last_error().decode(errors="replace")

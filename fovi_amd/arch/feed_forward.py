@@ -55,7 +55,7 @@ def _forward(x, w_gate, w_up, w_down, activation, residual, keep_for_backward):
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     a.y, a.y_stride = y.data_ptr(), a.dim
     work = _workspace(a, lib.fovi_gated_mlp_fwd_workspace_bytes(a), x.device)
-    _lib.check(lib.fovi_gated_mlp_fwd(a, _lib.stream_of(x)), "fovi_gated_mlp_fwd")
+    _lib.launch(lib.fovi_gated_mlp_fwd, (a,), x, "fovi_gated_mlp_fwd")
     del work, keep
     return y, saved
 
@@ -88,7 +88,7 @@ def _backward(ctx, saved, dy):
         a.dw_down = ddown.data_ptr()
     if need_x or need_gate or need_up or need_down:
         work = _workspace(a, lib.fovi_gated_mlp_bwd_workspace_bytes(a), x.device)
-        _lib.check(lib.fovi_gated_mlp_bwd(a, _lib.stream_of(x)), "fovi_gated_mlp_bwd")
+        _lib.launch(lib.fovi_gated_mlp_bwd, (a,), x, "fovi_gated_mlp_bwd")
         del work
     del keep
     return dx, dgate if need_gate else None, dup if need_up else None, ddown, None, dres

@@ -66,9 +66,8 @@ class Int8Rows(NamedTuple):
         if y.numel():
             data, rows, stride = _matrix(self.data)
             scale = self.scale.contiguous()
-            _lib.check(_lib.load().fovi_dequantize_rows(data.data_ptr(), scale.data_ptr(), rows, data.shape[-1], stride,
-                                                        y.data_ptr(), _lib.dtype_code(dtype), _lib.stream_of(y)),
-                       "fovi_dequantize_rows")
+            _lib.launch(_lib.load().fovi_dequantize_rows, (data.data_ptr(), scale.data_ptr(), rows, data.shape[-1], stride,
+                                                           y.data_ptr(), _lib.dtype_code(dtype)), y, "fovi_dequantize_rows")
         return y
 
 
@@ -98,9 +97,9 @@ def quantize_int8(x):
                  torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device))
     if x.numel():
         xr, rows, stride = _matrix(x)
-        _lib.check(_lib.load().fovi_quantize_rows(xr.data_ptr(), _lib.dtype_code(x.dtype), 1, rows, x.shape[-1],
-                                                  (C.c_int64 * 2)(0, stride), q.data.data_ptr(), q.scale.data_ptr(),
-                                                  _lib.stream_of(x)), "fovi_quantize_rows")
+        _lib.launch(_lib.load().fovi_quantize_rows, (xr.data_ptr(), _lib.dtype_code(x.dtype), 1, rows, x.shape[-1],
+                                                     (C.c_int64 * 2)(0, stride), q.data.data_ptr(), q.scale.data_ptr()),
+                    x, "fovi_quantize_rows")
     return q
 
 
@@ -126,8 +125,8 @@ def _product(what, x, weight, weight2, activation, bias, residual, dtype):
     data, scale = x
     shape, device = data.shape, data.device
     k = shape[-1]
-    if k > 131072:
-        raise ValueError(f"{what}: {k} inputs, at most 131072 keep the sums exact")
+    if k > 131071:
+        raise ValueError(f"{what}: {k} inputs, at most 131071 keep the sums exact")
     w, w_stride, w_scale = _weight(what, weight, k, device)
     n = w.shape[0]
     shape = shape[:-1] + (n,)
@@ -169,7 +168,7 @@ def _product(what, x, weight, weight2, activation, bias, residual, dtype):
     if nbytes:
         work = torch.empty(nbytes, dtype=torch.uint8, device=device)
         a.workspace, a.workspace_bytes = work.data_ptr(), nbytes
-    _lib.check(lib.fovi_linear_int8(a, _lib.stream_of(out)), "fovi_linear_int8")
+    _lib.launch(lib.fovi_linear_int8, (a,), out, "fovi_linear_int8")
     del work
     return out
 

@@ -216,7 +216,7 @@ def _rms_forward(x, weight, eps, residual, rstd, quantize=False):
         a.y = y.data_ptr()
     if rstd is not None:
         a.rstd = rstd.data_ptr()
-    _lib.check(_lib.load().fovi_rms_norm_fwd(a, _lib.stream_of(x)), "fovi_rms_norm_fwd")
+    _lib.launch(_lib.load().fovi_rms_norm_fwd, (a,), x, "fovi_rms_norm_fwd")
     del keep
     return y, total
 
@@ -257,7 +257,7 @@ def _rms_backward(ctx, saved, dy, dtotal=None):
             nbytes = lib.fovi_rms_norm_workspace_bytes(n0 * n1, c)
             work = torch.empty(nbytes, dtype=torch.uint8, device=total.device)
             a.dweight, a.workspace, a.workspace_bytes = dw.data_ptr(), work.data_ptr(), nbytes
-    _lib.check(lib.fovi_rms_norm_bwd(a, _lib.stream_of(total)), "fovi_rms_norm_bwd")
+    _lib.launch(lib.fovi_rms_norm_bwd, (a,), total, "fovi_rms_norm_bwd")
     del keep
     return dx if need_x else None, dw, None, dx if need_r else None
 

@@ -3,7 +3,7 @@
 //   y[m, n] = (sum_k x[m, k] w[n, k]) * sx[m] * sw[n] + bias[n] + residual[m, n]
 //   gated: act(gate[m, n]) * up[m, n] of two such products over the same rows
 //
-// The sums are exact (int32 holds 133,000 products of 127 * 127); they become floats once, times the two scales.
+// The sums are exact (int32 holds 131,071 products of -128 * -128); they become floats once, times the two scales.
 #include "matmul_few.h"
 
 namespace fovi {
@@ -182,8 +182,8 @@ extern "C" int fovi_linear_int8(const fovi_linear_int8_args* a, void* stream) {
     set_error("fovi_linear_int8: unknown activation");
     return 1;
   }
-  if (a->rows < 0 || a->outputs < 0 || a->inputs < 1 || a->inputs > 131072) {
-    set_error("fovi_linear_int8: bad sizes (1 to 131072 inputs)");
+  if (a->rows < 0 || a->outputs < 0 || a->inputs < 1 || a->inputs > 131071) {
+    set_error("fovi_linear_int8: bad sizes (1 to 131071 inputs)");
     return 1;
   }
   if (a->rows == 0 || a->outputs == 0) return 0;

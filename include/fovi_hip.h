@@ -951,7 +951,7 @@ int fovi_dequantize_rows(const int8_t* q, const float* scale, int64_t rows, int6
  * Product of 8-bit rows with 8-bit weights, a scale for each row and for each output:
  *   out[m, n] = (sum_k x[m, k] weight[n, k]) * x_scale[m] * weight_scale[n] + bias[n] + residual[m, n]
  * and with weight2 (then without bias and residual) act(that) * the same product with weight2 and weight2_scale.
- * Strides are in elements between rows, elements adjacent, at any alignment. Sums are exact in int32 (up to 131072 inputs).
+ * Strides are in elements between rows, elements adjacent, at any alignment. Sums are exact in int32 (up to 131071 inputs).
  * out and residual: out_dtype, F32 or BF16; bias fp32 (may be NULL, as may residual). The workspace
  * (fovi_linear_int8_workspace_bytes of the arguments, may be 0; 16-byte aligned) holds copies of
  * matrices whose rows are not whole, aligned 16-byte pieces, and partial sums where the inputs are split over workgroups.

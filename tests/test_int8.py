@@ -81,20 +81,21 @@ def test_gated(m, k, n, activation, dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("m", [3, 70])
-def test_sums_are_exact(m):
-    """Rows of 127 and -127 of the largest length, whose sums pass 2^30, and one pair that cancels to 1."""
+@pytest.mark.parametrize("k", [131071, 131056])
+@pytest.mark.parametrize("m", [3, 70, 300])
+def test_sums_are_exact(m, k):
+    """Rows of -128 and 127 of the largest lengths (the second is of whole 16-byte pieces), whose sums come near 2^31, and one
+    that nearly cancels."""
     from fovi_amd.arch.int8 import Int8Rows, linear_int8
-    k = 131072
-    x = torch.full((m, k), 127, dtype=torch.int8, device="cuda")
-    w = torch.stack([torch.full((k,), v, dtype=torch.int8, device="cuda") for v in (127, -127, 127)])
+    x = torch.full((m, k), -128, dtype=torch.int8, device="cuda")
+    w = torch.stack([torch.full((k,), v, dtype=torch.int8, device="cuda") for v in (-128, 127, 127)])
     w[2, : k // 2] = -127
     x[1, 0], w[2, 0] = 1, 1
     one = torch.ones(m, device="cuda")
     y = linear_int8(Int8Rows(x, one), Int8Rows(w, one[:1].expand(3)), dtype=torch.float32)
     want = (x.double() @ w.double().t()).float()
     assert torch.equal(y, want)
-    assert y[0, 0] == 127.0 * 127 * k
+    assert y[0, 0] == 128.0 * 128 * k
 
 
 @pytest.mark.gpu
@@ -257,8 +258,8 @@ def test_refusals():
         linear_int8(Int8Rows(x.data, x.scale[:3]), w)
     with pytest.raises(ValueError, match="no gradients"):
         linear_int8(x, w, bias=torch.zeros(8, device="cuda", requires_grad=True))
-    with pytest.raises(ValueError, match="at most 131072"):
-        linear_int8(_rows(1, 131073, 1), _rows(1, 131073, 1))
+    with pytest.raises(ValueError, match="at most 131071"):
+        linear_int8(_rows(1, 131072, 1), _rows(1, 131072, 1))
 
 
 def test_cpu_tensors_and_c_arguments_are_refused():
@@ -274,7 +275,7 @@ def test_cpu_tensors_and_c_arguments_are_refused():
     assert lib.fovi_linear_int8(a, None) != 0 and b"out_dtype" in lib.fovi_last_error()
     a.out_dtype, a.rows, a.outputs = _lib.F32, 1, 1
     assert lib.fovi_linear_int8(a, None) != 0 and b"bad sizes" in lib.fovi_last_error()
-    a.inputs = 131073
+    a.inputs = 131072
     assert lib.fovi_linear_int8(a, None) != 0 and b"bad sizes" in lib.fovi_last_error()
     a.inputs, a.weight2 = 8, 16
     assert lib.fovi_linear_int8(a, None) != 0 and b"null pointer" in lib.fovi_last_error()
@@ -282,3 +283,29 @@ def test_cpu_tensors_and_c_arguments_are_refused():
     assert lib.fovi_linear_int8(a, None) != 0 and b"no bias" in lib.fovi_last_error()
     a.bias, a.activation = None, 5
     assert lib.fovi_linear_int8(a, None) != 0 and b"activation" in lib.fovi_last_error()
+
+
+def test_launch_is_on_the_tensors_device(monkeypatch):
+    """An entry point runs with the device of its tensors as the current one, which it leaves as it was."""
+    current, calls = [0], []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(_lib, "stream_of", lambda t: 100 + t.device.index)
+    for index in (0, 1):
+        t = type("T", (), {"device": torch.device("cuda", index)})()
+        _lib.launch(lambda *a: calls.append((current[0],) + a) or 0, (7, 8), t, "entry")
+    assert calls == [(0, 7, 8, 100), (1, 7, 8, 101)] and current == [0]
+    with pytest.raises(RuntimeError, match="entry"):
+        _lib.launch(lambda *a: 1, (), t, "entry")
+    assert current == [0]
