@@ -1,9 +1,10 @@
 """The gated feed-forward block of token rows on the HIP kernels ``fovi_gated_mlp_fwd`` / ``fovi_gated_mlp_bwd``.
 
 ``y = (act(x w_gate^T) * (x w_up^T)) w_down^T``: both first projections, the activation and their product are one
-kernel. The backward of bf16 calls keeps nothing but its inputs: it forms both projections again beside the gradient
-that meets them. Sums are fp32; with bf16 inputs the product of the projections, and in the backward its two
-gradients, are rounded to bf16 (half a step, 2^-8 of each value at most) before the products that they enter. The weights'
+kernel. The backward of bf16 calls with fewer than 768 channels keeps nothing but its inputs: it forms both
+projections again beside the gradient that meets them. Others keep the projections in the inputs' type. Sums are fp32;
+with bf16 inputs the product of the projections, and in the backward its two gradients (and the kept projections), are
+rounded to bf16 (half a step, 2^-8 of each value at most) before the products that they enter. The weights'
 gradients are summed in a fixed order: the same inputs give the same bits.
 
 ``GatedFeedForward`` is the block of a pre-norm model, with the residual's addition and RMS norm in front;

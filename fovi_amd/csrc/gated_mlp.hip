@@ -4,9 +4,9 @@
 //   dh = dy Wd, dgate = dh * up * act'(gate), dup = dh * act(gate)
 //   dx = dgate Wg + dup Wu, dWg = dgate^T x, dWu = dup^T x, dWd = dy^T h
 //
-// Both first projections run over one tile of x, and h is all that leaves them. The backward forms gate and up again
-// beside dh, in the registers of one kernel, whose epilogue writes dgate, dup and h (bf16; fp32 calls keep gate and up
-// from the forward). The weights' gradients reduce over the tokens: the tokens are split over workgroups, whose
+// Both first projections run over one tile of x, and h is all that leaves them, but for gate and up where they are kept
+// for the backward (fp32, wide bf16 rows). The backward forms dh, or gate, up and dh in the registers of one kernel,
+// whose epilogue writes dgate, dup and h. The weights' gradients reduce over the tokens: the tokens are split over workgroups, whose
 // partial sums a second launch adds in a fixed order.
 #include "matmul_few.h"
 
@@ -103,6 +103,7 @@ template <typename T> struct MlpSavedGrad : NoColumn, MlpGradRows<T> { // of dh'
     this->write(m, n, count, x.gate, x.up, v[0]);
   }
 };
+template <typename T> constexpr bool mat_narrow<MlpSavedGrad<T>> = true;
 
 template <typename T, int BM, int BN> struct MlpGatedTile {
   typedef MatPhase<T, BM, BN, 2, false, false> Both;
@@ -244,6 +245,13 @@ static void mlp_gated_grad_tiles(const MlpInputs& in, const MatOperand& wd, int6
              M, F, work, epilogue);
 }
 
+// Whether the forward keeps gate and up for the backward: 4 bytes a pair and row in bf16, where forming them again costs
+// 4 dim operations. Both directions in bf16, us, kept and formed again: 131072 x 384 by 1024 1735 and 1640, 65536 x 512 by
+// 1344 1412 and 1355, 32768 x 768 by 2048 1485 and 1493, 8192 x 1536 by 4096 1270 and 1362, 4572 x 2048 by 5504 1266
+// and 1412. fp32 products are slow enough to keep always.
+constexpr int64_t kKeepDim = 768;
+static bool mlp_keeps(int64_t dim, int32_t dtype) { return dtype == FOVI_F32 || dim >= kKeepDim; }
+static bool mlp_keeps(const fovi_gated_mlp_args* a) { return mlp_keeps(a->dim, a->dtype); }
 static bool mlp_few(const fovi_gated_mlp_args* a) {
   return few_rows_best(a->rows, a->hidden > a->dim ? a->hidden : a->dim, a->dtype == FOVI_F32);
 }
@@ -286,11 +294,11 @@ template <typename T> static void mlp_bwd(const fovi_gated_mlp_args* a, hipStrea
   char* part = reinterpret_cast<char*>(h) + aligned(M * Fp * es);
   const MatOperand wd = columns(in.wd, F, es);
   const MlpGradRows<T> rows = {grad, grad + Fp, h, 2 * Fp, Fp, a->activation};
-  if constexpr (sizeof(T) == 4) {
+  if (mlp_keeps(a)) {
     const T* gate = static_cast<const T*>(a->saved);
     const MatSegments down = {{in.dy}, {wd}, {C, 0}, 1};
     mat_linear<T, false, true>(down, M, F, part, false, MlpSavedGrad<T>{{}, rows, gate, gate + F, 2 * F}, s);
-  } else {
+  } else if constexpr (sizeof(T) == 2) {
     const MlpGatedGrad<T> gated = {{}, rows};
     const int size = mat_tile_size(M, 2 * F, 1, false, 256);
     if (size >= 128) mlp_gated_grad_tiles<T, 128, 64, MatWaves<2, 2>>(in, wd, C, M, F, gated, s);
@@ -315,7 +323,7 @@ template <typename T> static void mlp_bwd(const fovi_gated_mlp_args* a, hipStrea
 // The partial sums of the backward's products, one after the other.
 template <typename T> static int64_t mlp_bwd_part(const fovi_gated_mlp_args* a) {
   const int64_t M = a->rows, C = a->dim, F = a->hidden;
-  const int64_t parts[4] = {sizeof(T) == 4 ? mat_part_bytes<T>(M, F, C, false) : 0, mat_part_bytes<T>(M, C, F, false),
+  const int64_t parts[4] = {mlp_keeps(a) ? mat_part_bytes<T>(M, F, C, false) : 0, mat_part_bytes<T>(M, C, F, false),
                             mat_part_bytes<T>(wide(F) + F, C, M, true), mat_part_bytes<T>(C, F, M, true)};
   int64_t most = 0;
   for (int64_t n : parts)
@@ -328,8 +336,7 @@ template <typename T> static int64_t mlp_bwd_part(const fovi_gated_mlp_args* a) 
 using namespace fovi;
 
 extern "C" int64_t fovi_gated_mlp_saved_bytes(int64_t rows, int64_t dim, int64_t hidden, int32_t dtype) {
-  (void)dim;
-  return dtype == FOVI_F32 && rows > 0 && hidden > 0 ? rows * 2 * hidden * 4 : 0;
+  return mlp_keeps(dim, dtype) && rows > 0 && hidden > 0 ? rows * 2 * hidden * (dtype == FOVI_F32 ? 4 : 2) : 0;
 }
 
 extern "C" int64_t fovi_gated_mlp_fwd_workspace_bytes(const fovi_gated_mlp_args* a) {

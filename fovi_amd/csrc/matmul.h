@@ -602,11 +602,18 @@ inline void mat_linear_tiles(const MatSegments& s, int64_t M, int64_t N, int64_t
   mat_launch(mat_linear_kernel<T, BM, BN, CX, CW, Epilogue>, mat_grid(work, 256 / BM), (MatUsual<BM, BN>::THREADS),
              MatLinearTile<T, BM, BN, CX, CW, Epilogue>::Ring::LDS, stream, s, M, N, work, share, epilogue);
 }
+// Tiles of 256 rows have 128 columns for an epilogue that reads much beside the sums: more of it is then read at once.
+template <typename Epilogue> constexpr bool mat_narrow = false;
 template <typename T, bool CX, bool CW, typename Epilogue>
 inline void mat_linear_shares(const MatSegments& s, int64_t M, int64_t N, int64_t share, int64_t shares, const Epilogue& epilogue,
                               hipStream_t stream) {
-  const int size = mat_tile_size(M, N, shares, sizeof(T) == 4, mat_columns(N));
-  if constexpr (sizeof(T) < 4) {
+  const int size = mat_tile_size(M, N, shares, sizeof(T) == 4, mat_narrow<Epilogue> ? 128 : mat_columns(N));
+  if constexpr (sizeof(T) < 4 && mat_narrow<Epilogue>) {
+    if (size == 256) {
+      mat_linear_tiles<T, 256, 128, CX, CW>(s, M, N, share, shares, epilogue, stream);
+      return;
+    }
+  } else if constexpr (sizeof(T) < 4) {
     if (size == 256) {
       if (mat_columns(N) == 192) mat_linear_tiles<T, 256, 192, CX, CW>(s, M, N, share, shares, epilogue, stream);
       else mat_linear_tiles<T, 256, 256, CX, CW>(s, M, N, share, shares, epilogue, stream);

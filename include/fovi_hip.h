@@ -991,7 +991,7 @@ int fovi_linear_int8(const fovi_linear_int8_args* args, void* stream);
  * Sums are fp32. With BF16 act(gate) * up, and in the backward its gradient's two products, are rounded to it before the
  * products they enter (the matrix unit takes one type).
  * saved: gate and up for the backward, of fovi_gated_mlp_saved_bytes (0: the backward forms them again and takes NULL;
- * NULL if no backward follows).
+ * NULL if no backward follows). With BF16 they are rounded to it, and the backward's values come from the rounded ones.
  * backward: dx, dw_down and the pair dw_gate, dw_up, each unless NULL, whole; the residual's gradient is dy.
  * The workspaces (of the sizes that fovi_gated_mlp_*_workspace_bytes give for the arguments, 16-byte aligned) hold
  * what lies between the products, and copies of matrices whose rows are not whole, aligned 16-byte pieces.
