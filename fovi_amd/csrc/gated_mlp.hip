@@ -8,6 +8,10 @@
 // for the backward (fp32, wide bf16 rows). The backward forms dh, or gate, up and dh in the registers of one kernel,
 // whose epilogue writes dgate, dup and h. The weights' gradients reduce over the tokens: the tokens are split over workgroups, whose
 // partial sums a second launch adds in a fixed order.
+//
+// 131072 rows of 384, hidden 1024, in bf16: gate, up and h 300 us (206 GFLOP), y 137 (103), gate, up and dh 650 (309), dx 257
+// (206), dWg and dWu 246 (206), dWd 167 (103). What bounds them are the loads into LDS and the epilogues: without its loads the
+// first takes 192 us and the third 344, without its stores the third 505. 32 rows of 2048, hidden 5504: 13.2 and 8.3 us (68 MB).
 #include "matmul_few.h"
 
 namespace fovi {
