@@ -114,6 +114,29 @@ def test_values_and_gradients(m, c, f, act, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("c,f", [(1024, 1032), (384, 2056)])
+def test_offsets_past_32_bits(c, f):
+    """Rows, gate and up, and their gradients of more than 2^31 elements. Only the last rows have an incoming gradient, so that
+    every result comes from them."""
+    from fovi_amd.arch.feed_forward import gated_mlp
+    m, last = 2 ** 21 + 70, 70
+    x, w, r, dy = _data(last, c, f, torch.bfloat16)
+    rows = torch.randn(m, c, device="cuda", dtype=torch.bfloat16)
+    rows[-last:] = x
+    grads = torch.zeros(m, c, device="cuda", dtype=torch.bfloat16)
+    grads[-last:] = dy
+    want = _expected(x, w, None, dy, "silu")
+    leaves = [t.requires_grad_(True) for t in [rows] + w]
+    y = gated_mlp(*leaves)
+    _within(y[-last:], want["y"], "y")
+    dx, *dw = torch.autograd.grad(y, leaves, grads)
+    _within(dx[-last:], want["dx"], "dx")
+    assert not dx[:-last].any()
+    for name, g in zip(NAMES[1:], dw):
+        _within(g, want[name], name)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("which", [(0,), (1,), (2,), (3,), (0, 3), (1, 2)])
 def test_parts_of_the_gradients(which, dtype):

@@ -237,6 +237,19 @@ def test_stream_and_capture():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", [(40, 1024, 2 ** 21 + 100), (40, 1023, 2 ** 21 + 4200), (2 ** 21 + 70, 1024, 24), (2 ** 21 + 4200, 1023, 24),
+                                   (70000, 16, 32000)])
+def test_offsets_past_32_bits(m, k, n):
+    """Weights, rows (as they are and copied) and outputs of more than 2^31 elements: the last rows and outputs as a small call
+    gives them (the sums are exact)."""
+    from fovi_amd.arch.int8 import Int8Rows, gated_linear_int8, linear_int8
+    x, w = (Int8Rows(torch.randint(-127, 128, (r, k), dtype=torch.int8, device="cuda"), torch.rand(r, device="cuda")) for r in (m, n))
+    a, b = Int8Rows(x.data[-33:].clone(), x.scale[-33:]), Int8Rows(w.data[-21:].clone(), w.scale[-21:])
+    assert torch.equal(linear_int8(x, w)[-33:, -21:], linear_int8(a, b))
+    assert torch.equal(gated_linear_int8(x, w, w)[-33:, -21:], gated_linear_int8(a, b, b))
+
+
+@pytest.mark.gpu
 def test_refusals():
     from fovi_amd.arch.int8 import Int8Rows, gated_linear_int8, linear_int8
     x, w = _rows(4, 16, 1), _rows(8, 16, 2)

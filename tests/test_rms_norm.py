@@ -444,3 +444,28 @@ def test_capture(rows, c, dtype):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want)), i
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """Rows of more than 2^31 elements in all; only the last have an incoming gradient, so that the weight's comes from them."""
+    from fovi_amd.arch.norm import rms_norm, rms_norm_int8
+    m, c, last = 2 ** 21 + 70, 1024, 70
+    x, r, w, dy, dt = _data((last, c), torch.bfloat16)
+
+    def behind(t, value):
+        rows = torch.full((m, c), value, device="cuda", dtype=torch.bfloat16)
+        rows[-last:] = t
+        return rows
+
+    leaves = [behind(x, 1.0).requires_grad_(True), w.requires_grad_(True), behind(r, 0.5).requires_grad_(True)]
+    y, total = rms_norm(leaves[0], leaves[1], residual=leaves[2])
+    dx, dw, dr = torch.autograd.grad((y, total), leaves, (behind(dy, 0.0), behind(dt, 0.0)))
+    _check(x, r, w, dy, dt, y[-last:], total[-last:], dx[-last:], dw)
+    assert not dx[:-last].any() and torch.equal(dr[-last:], dx[-last:])
+    with torch.no_grad():
+        q, again = rms_norm_int8(leaves[0], leaves[1], residual=leaves[2])
+    assert torch.equal(again, total)
+    values, scale = q.dequantize()[-last:].double(), q.scale[-last:, None].double()
+    y = y[-last:].detach().double()
+    assert ((values - y).abs() <= 0.501 * scale + 1.01 * U[torch.bfloat16] * y.abs()).all()
