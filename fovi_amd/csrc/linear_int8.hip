@@ -64,7 +64,7 @@ template <typename TO> struct Int8Gated {
     float y[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      y[i] = mat_act<false>(static_cast<float>(v[0][i]) * x * c.gate[i], act) * (static_cast<float>(v[1][i]) * x * c.up[i]);
+      y[i] = mat_act<sizeof(TO) == 4>(static_cast<float>(v[0][i]) * x * c.gate[i], act) * (static_cast<float>(v[1][i]) * x * c.up[i]);
     store_run(out + m * stride + n, count, y);
   }
 };

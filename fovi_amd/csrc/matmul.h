@@ -385,7 +385,8 @@ template <typename T> __device__ __forceinline__ void store_run(T* p, int count,
   }
 }
 
-// Activations and their derivatives. EXACT: the library's exponential and division, for fp32 operands.
+// Activations and their derivatives. EXACT: the library's exponential and division, for fp32 results
+// (with the hardware's, silu is 8e-7 off at gates of -10 to -20 and 1.7e-6 at -40).
 template <bool EXACT> __device__ __forceinline__ float mat_sigmoid(float z) {
   if (EXACT) return 1.0f / (1.0f + expf(-z));
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896340736f));

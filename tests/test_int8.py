@@ -81,6 +81,24 @@ def test_gated(m, k, n, activation, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,k", [(5, 16), (40, 21), (300, 32)])
+def test_gate_of_fp32_outputs(m, k):
+    """Gates that are exact, between -40 and 40: what is left is the activation's. The library's exponential is off by 2^-23,
+    the sum below it, the division, the product and the output by 2^-24 each, so 6 * 2^-24 in all. (An exponential of base 2 loses
+    half a step of its argument, which is |gate| 2^-24 of its value.)"""
+    from fovi_amd.arch.int8 import Int8Rows, gated_linear_int8
+    n = 24
+    x, gate, up = (torch.zeros(r, k, dtype=torch.int8) for r in (m, n, n))
+    x[:, 0], x[:, 1] = (torch.arange(m) * 37 % 255 - 127).to(torch.int8), (1 + torch.arange(m) % 127).to(torch.int8)
+    gate[:, 0], up[:, 1] = 1, (1 + torch.arange(n)).to(torch.int8)
+    one = torch.ones(max(m, n), device="cuda")
+    x, gate, up = Int8Rows(x.cuda(), one[:m]), Int8Rows(gate.cuda(), one[:n] * 0.3125), Int8Rows(up.cuda(), one[:n] * 0.125)
+    y = gated_linear_int8(x, gate, up, "silu", torch.float32)
+    want = _act(_sum(x, gate), "silu") * _sum(x, up)
+    _within(y, want, 6 * E * want.abs(), "y")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("k", [131071, 131056])
 @pytest.mark.parametrize("m", [3, 70, 300])
 def test_sums_are_exact(m, k):
