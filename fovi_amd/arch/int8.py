@@ -58,10 +58,11 @@ class Int8Rows(NamedTuple):
     scale: torch.Tensor
 
     def dequantize(self, dtype=torch.float32):
-        """The values that the rows stand for, in fp32 or bf16."""
+        """The values that the rows stand for, in fp32 or bf16. No gradient, and asking for one raises."""
         _rows_check("dequantize", self)
         if dtype not in (torch.float32, torch.bfloat16):
             raise TypeError(f"dequantize: unsupported dtype {dtype}")
+        refuse_gradients("dequantize", self.scale)
         y = torch.empty(self.data.shape, dtype=dtype, device=self.data.device)
         if y.numel():
             data, rows, stride = _matrix(self.data)

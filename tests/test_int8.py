@@ -268,6 +268,22 @@ def test_offsets_past_32_bits(m, k, n):
 
 
 @pytest.mark.gpu
+def test_dequantize_asked_for_gradients():
+    from torch.autograd import forward_ad
+    from fovi_amd.arch.int8 import Int8Rows
+    x = _rows(4, 16, 1)
+    leaf = x.scale.clone().requires_grad_(True)
+    with pytest.raises(ValueError, match="no gradients"):
+        Int8Rows(x.data, leaf).dequantize()
+    with torch.no_grad():
+        assert torch.equal(Int8Rows(x.data, leaf).dequantize(), x.dequantize())
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x.scale, torch.ones_like(x.scale))
+        with pytest.raises(ValueError, match="forward-mode"):
+            Int8Rows(x.data, dual).dequantize()
+
+
+@pytest.mark.gpu
 def test_refusals():
     from fovi_amd.arch.int8 import Int8Rows, gated_linear_int8, linear_int8
     x, w = _rows(4, 16, 1), _rows(8, 16, 2)
