@@ -224,6 +224,9 @@ def _rms_forward(x, weight, eps, residual, rstd, quantize=False):
 def _rms_backward(ctx, saved, dy, dtotal=None):
     total, weight, rstd = saved
     need_x, need_w, need_r = ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[3]
+    if dy is None:                                       # nothing comes through the norm
+        dx = torch.zeros_like(total) if dtotal is None else dtotal.to(total.dtype)
+        return dx if need_x else None, torch.zeros_like(weight) if need_w else None, None, dx if need_r else None
     c = total.shape[-1]
     xr, n0, n1, s0, s1 = _rows(total)
     a = _lib.RmsNormArgs()
@@ -263,10 +266,12 @@ def _rms_backward(ctx, saved, dy, dtotal=None):
 
 
 class _RMSNormFn(torch.autograd.Function):
-    """Forward ``fovi_rms_norm_fwd`` with the rows' statistics kept; backward ``fovi_rms_norm_bwd``."""
+    """Forward ``fovi_rms_norm_fwd`` with the rows' statistics kept; backward ``fovi_rms_norm_bwd``, which reads the
+    gradients that arrive: a block whose ``total`` goes no further has none of it."""
 
     @staticmethod
     def forward(ctx, x, weight, eps, residual):
+        ctx.set_materialize_grads(False)
         rstd = torch.empty(x.numel() // x.shape[-1], dtype=torch.float32, device=x.device)
         y, total = _rms_forward(x, weight, eps, residual, rstd)
         ctx.save_for_backward(total, weight, rstd)

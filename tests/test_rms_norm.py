@@ -119,6 +119,41 @@ def test_parameters_and_parts(c, which):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_gradient_that_does_not_arrive_is_not_read(dtype, monkeypatch):
+    """Only y's gradient: the kernel is given none of total's, and the rows are those of one of zeros. Only total's: it is the rows'
+    gradient, without a kernel, and the weight's is zero. Neither: zeros."""
+    from fovi_amd.arch import norm
+    x, r, w, dy, dt = _data((300, 40), dtype, 13)
+    leaves = [t.requires_grad_(True) for t in (x, r, w)]
+    calls, launch = [], _lib.launch
+    monkeypatch.setattr(_lib, "launch", lambda entry, args, t, what: calls.append((what, args[0].dtotal)) or launch(entry, args, t, what))
+    y, total = norm.rms_norm(x, w, residual=r)
+    want = torch.autograd.grad((y, total), leaves, (dy, torch.zeros_like(dt)), retain_graph=True)
+    assert calls[-1][0] == "fovi_rms_norm_bwd" and calls[-1][1] is not None
+    got = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    assert calls[-1] == ("fovi_rms_norm_bwd", None) and all(torch.equal(a, b) for a, b in zip(got, want))
+    n = len(calls)
+    dx, dr, dw = torch.autograd.grad(total, leaves, dt, retain_graph=True)
+    assert len(calls) == n and torch.equal(dx, dt) and torch.equal(dr, dt) and dw.shape == w.shape and not dw.any()
+
+    class Nothing(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, *args):
+            return args[0].sum()
+
+        @staticmethod
+        def backward(ctx, g):
+            return None, None
+
+    assert not any(g.any() for g in torch.autograd.grad(Nothing.apply(y, total), leaves, retain_graph=True))
+    assert len(calls) == n
+    for g in torch.autograd.grad(total, leaves, dt.requires_grad_(True), create_graph=True):
+        with pytest.raises(RuntimeError, match="differentiated once"):
+            torch.autograd.grad(g.sum(), [dt, x], allow_unused=True, retain_graph=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("layout", ["tokens", "padded", "odd_offset", "channels_first", "four_dims", "expanded", "one_dim"])
 def test_layouts(layout, dtype):
     """Rows where they are, with a residual and gradients of other layouts; the values of the contiguous call."""
