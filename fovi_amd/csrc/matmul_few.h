@@ -36,6 +36,35 @@ __device__ __forceinline__ i32x4s few_step(int8_t, u32x4 w, u32x4 x, i32x4s c) {
   return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, w), __builtin_bit_cast(i32x4, x), c, 0, 0, 0);
 }
 
+// acc += the products of COUNT steps. fp32 sums are taken by such groups (of up to 128 products) and added up, as the tiles take
+// them by stages. In one chain for a wave's share of k, outputs of 32 x 2048 by 5504 were 7.8e-7 off (the norm of the difference
+// over the norm), 2.5e-7 so, at the same speed within 1 %.
+template <typename T, int COUNT, int NW, int TB>
+__device__ __forceinline__ void few_multiply(const u32x4 (&w)[COUNT][NW], const u32x4 (&x)[COUNT][TB], typename Few<T>::Acc (&acc)[NW][TB]) {
+  typedef typename Few<T>::Acc Acc;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      Acc part[TB];
+#pragma unroll
+      for (int t = 0; t < TB; ++t) part[t] = Acc{0, 0, 0, 0};
+#pragma unroll
+      for (int s = 0; s < COUNT; ++s)
+#pragma unroll
+        for (int t = 0; t < TB; ++t) part[t] = few_step(T(), w[s][i], x[s][t], part[t]);
+#pragma unroll
+      for (int t = 0; t < TB; ++t) acc[i][t] += part[t];
+    }
+  } else {
+#pragma unroll
+    for (int s = 0; s < COUNT; ++s)
+#pragma unroll
+      for (int i = 0; i < NW; ++i)
+#pragma unroll
+        for (int t = 0; t < TB; ++t) acc[i][t] = few_step(T(), w[s][i], x[s][t], acc[i][t]);
+  }
+}
+
 constexpr int kFewRow = 20;                            // words of a row of 16 sums in LDS: rows begin in different banks
 template <int NB, int RB, int TB> constexpr int few_lds(int waves) { return waves * NB * RB * TB * 16 * kFewRow * 4; }
 
@@ -116,12 +145,7 @@ __global__ __launch_bounds__(1024) void few_kernel(MatOperand x, MatOperand w0, 
 #pragma unroll
       for (int t = 0; t < TB; ++t) fx[s][t] = load(px[t], at + 64 * s + 16 * (l >> 4));
     }
-#pragma unroll
-    for (int s = 0; s < COUNT; ++s)
-#pragma unroll
-      for (int i = 0; i < NW; ++i)
-#pragma unroll
-        for (int t = 0; t < TB; ++t) acc[i][t] = few_step(T(), fw[s][i], fx[s][t], acc[i][t]);
+    few_multiply<T>(fw, fx, acc);
   };
   auto whole = [](const char* p, int64_t at) __attribute__((always_inline)) {
     u32x4 u;
@@ -200,12 +224,7 @@ __global__ __launch_bounds__(1024) void few_ring_kernel(MatOperand x, MatOperand
     __builtin_amdgcn_sched_barrier(0);
     if (started < to) start(slot);
     slot = slot == 2 ? 0 : slot + 1;
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int i = 0; i < NW; ++i)
-#pragma unroll
-        for (int k = 0; k < TB; ++k) acc[i][k] = few_step(T(), fw[s][i], fx[s][k], acc[i][k]);
+    few_multiply<T>(fw, fx, acc);
   }
   __syncthreads();                                               // the sums take the stages' place
   few_finish<T, NB, RB, TB>(few_ring_memory, acc, m0, n0, M, N, epilogue);

@@ -114,6 +114,37 @@ def test_values_and_gradients(m, c, f, act, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["whole", "odd"])
+@pytest.mark.parametrize("m", [1, 40, 64, 300])
+def test_fp32_sums_are_taken_by_stages(m, layout):
+    """One product of 2^27 in front of 16383 or so of 1, each lost on its own beside it (half a step is 8): sums by stages lose those
+    of its own stage, of 128 at most, a rest of fewer than 16 behind the last one, and the rounding of the result. In the two
+    first products (x [.., C] by up [1, C], behind a gate of 32, whose silu is 32), and in the last one (over F)."""
+    from fovi_amd.arch.feed_forward import gated_mlp
+    k = 16384 if layout == "whole" else 16383
+    lost = 128 + 8 + 8
+
+    def wide(rows, cols):                                            # odd: rows that start anywhere
+        return torch.zeros(rows, cols + 3, device="cuda")[:, 3:] if layout == "odd" else torch.zeros(rows, cols, device="cuda")
+
+    x, wg, wu = wide(m, k), wide(1, k), wide(1, k)
+    wd = torch.full((k, 1), 2.0 ** -5, device="cuda")
+    x.fill_(1.0)
+    wu.fill_(1.0)
+    x[:, 0], wg[:, 0], wu[:, 0] = 2.0 ** 13, 2.0 ** -8, 2.0 ** 14
+    with torch.no_grad():
+        y = gated_mlp(x, wg, wu, wd)
+    assert (y.double() - (2.0 ** 27 + k - 1)).abs().max() <= lost
+
+    x, wg, wu, wd = (torch.ones(m, 4, device="cuda"), torch.zeros(k, 4, device="cuda"), torch.zeros(k, 4, device="cuda"), wide(4, k))
+    wg[:, 0], wu[:, 1], wu[0, 1] = 32.0, 2.0 ** -5, 2.0 ** 22
+    wd.fill_(1.0)
+    with torch.no_grad():
+        y = gated_mlp(x, wg, wu, wd)
+    assert (y.double() - (2.0 ** 27 + k - 1)).abs().max() <= lost
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("c,f", [(1024, 1032), (384, 2056)])
 def test_offsets_past_32_bits(c, f):
     """Rows, gate and up, and their gradients of more than 2^31 elements. Only the last rows have an incoming gradient, so that
