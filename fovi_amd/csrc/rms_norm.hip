@@ -55,6 +55,19 @@ struct Quantum {
   }
 };
 
+// 1 / sqrt(mean of squares + eps). Where the squares' sum has passed fp32's range (values beyond 1.8e19 / sqrt(C)), from
+// scaled_mean(), that of the values times 2^-80: exact for those that count, and finite for any finite row. A row with
+// an infinity stays infinite. All lanes of a row have the same mean, so that they go the same way.
+template <typename ScaledMean>
+__device__ __forceinline__ float rms_rstd(float mean, float eps, const ScaledMean& scaled_mean) {
+  if (mean != INFINITY) return 1.0f / sqrtf(mean + eps);
+  return 0x1p-80f / sqrtf(scaled_mean() + eps * 0x1p-80f * 0x1p-80f);
+}
+__device__ __forceinline__ float scaled_square(float v, float s) {
+  v *= 0x1p-80f;
+  return fmaf(v, v, s);
+}
+
 template <typename T> __device__ __forceinline__ float round_to(float v) { T e; Elem<T>::store(&e, v); return Elem<T>::load(&e); }
 
 template <typename T, int VEC, int LANES, int NV, bool TAIL, bool INT8>
@@ -93,7 +106,14 @@ __global__ __launch_bounds__(256) void rms_fwd_rows_kernel(RmsParams p) {
       for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) s = fmaf(x[k][i], x[k][i], s);
-      rstd = 1.0f / sqrtf(group_sum<LANES>(s, sh) * n + p.eps);
+      rstd = rms_rstd(group_sum<LANES>(s, sh) * n, p.eps, [&]() __attribute__((always_inline)) {
+        float t = 0;
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) t = scaled_square(x[k][i], t);
+        return group_sum<LANES>(t, sh) * n;
+      });
       if (lane == 0 && p.rstd) p.rstd[row] = rstd;
     }
 #pragma unroll
@@ -241,7 +261,11 @@ __global__ __launch_bounds__(256) void rms_fwd_kernel(RmsParams p) {
     const T* from = r ? total : x;                    // each thread reads the places that it wrote
     float rstd = 1.0f;
     if (!INT8 || p.norm) {
-      rstd = 1.0f / sqrtf(block_sum(s, sh) / static_cast<float>(p.C) + p.eps);
+      rstd = rms_rstd(block_sum(s, sh) / static_cast<float>(p.C), p.eps, [&]() __attribute__((always_inline)) {
+        float t = 0;
+        for (int64_t c = threadIdx.x; c < p.C; c += 256) t = scaled_square(Elem<T>::load(from + c), t);
+        return block_sum(t, sh) / static_cast<float>(p.C);
+      });
       if (threadIdx.x == 0 && p.rstd) p.rstd[row] = rstd;
     }
     if (!INT8) {

@@ -246,6 +246,39 @@ def test_extreme_rows_in_8_bits(c):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("top", [4e17, 3e19, 1e30, 1e36])
+@pytest.mark.parametrize("rows,c", [(5, 40), (4099, 1024), (3, 8192), (2, 9001)])
+def test_large_rows(rows, c, top, dtype):
+    """Rows whose sum of squares is past fp32's range, beside others: the norm is that of the formula, in both directions and in
+    8 bits. (Their 1 / sqrt is a normal number, as the bounds assume.)"""
+    from fovi_amd.arch.norm import rms_norm, rms_norm_int8
+    x, r, w, dy, dt = _data((rows, c), dtype, 23)
+    x[1::2] *= top
+    dy[1::2] *= min(top, 1e30)                                       # (g h is summed in fp32 too)
+    dt.zero_()
+    leaves = [t.requires_grad_(True) for t in (x, w, r)]
+    y, total = rms_norm(x, w, residual=r)
+    assert y.isfinite().all() and (y[1].abs().amax() > 0.5)
+    dx, dw, _ = torch.autograd.grad((y, total), leaves, (dy, dt))
+    _check(x, r, w, dy, dt, y, total, dx, dw)
+    with torch.no_grad():
+        q, total = rms_norm_int8(x, w, residual=r)
+    t = total.double().cpu()
+    _eight_bits(t / (t.square().mean(-1, keepdim=True) + 1e-6).sqrt() * w.detach().double().cpu(), q.data, q.scale, c)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("c", [3, 384, 9001])
+def test_the_largest_rows(c):
+    """Rows of the type's largest value: 1 / sqrt of their mean of squares, 2^-128, has 22 bits."""
+    from fovi_amd.arch.norm import rms_norm
+    for dtype in (torch.float32, torch.bfloat16):
+        y = rms_norm(torch.full((2, c), torch.finfo(dtype).max, dtype=dtype, device="cuda"), torch.full((c,), 3.0, device="cuda"), eps=0.0)
+        assert ((y.double() - 3).abs() <= 3 * (2.0 ** -22 + (c / 2 + 8) * E + U[dtype])).all()
+
+
+@pytest.mark.gpu
 def test_infinities_stay_in_their_rows():
     from fovi_amd.arch.norm import rms_norm
     x, r, w, dy, dt = _data((6, 48), torch.float32, 9)
