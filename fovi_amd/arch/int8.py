@@ -190,7 +190,8 @@ def gated_linear_int8(x, gate, up, activation="silu", dtype=torch.bfloat16):
 
 class Int8Linear(nn.Module):
     """An ``nn.Linear`` for serving: its weights in 8 bits, its inputs quantised at every call (``Int8Rows`` are taken as
-    they are), its outputs in the inputs' type (``Int8Rows``: bf16)."""
+    they are). Its outputs are in ``dtype``, by default the inputs' type, or for ``Int8Rows`` the residual's (without one
+    bf16)."""
 
     def __init__(self, linear):
         super().__init__()
@@ -208,11 +209,12 @@ class Int8Linear(nn.Module):
                 setattr(self, n, t.to(getattr(self, n).device))
         return self
 
-    def forward(self, x, residual=None):
-        dtype = torch.bfloat16
+    def forward(self, x, residual=None, dtype=None):
         if not isinstance(x, Int8Rows):
-            dtype = x.dtype
+            dtype = x.dtype if dtype is None else dtype
             x = quantize_int8(x)
+        elif dtype is None:
+            dtype = torch.bfloat16 if residual is None else residual.dtype
         return linear_int8(x, Int8Rows(self.weight, self.weight_scale), self.bias, residual, dtype)
 
     def extra_repr(self):

@@ -224,6 +224,25 @@ def test_module(dtype):
 
 
 @pytest.mark.gpu
+def test_module_output_types():
+    """Rows in 8 bits: the output's type is the residual's, bf16 without one, or what is asked for; other rows: their type, or that."""
+    from fovi_amd.arch.int8 import Int8Linear, Int8Rows, linear_int8, quantize_int8
+    torch.manual_seed(1)
+    mod = Int8Linear(torch.nn.Linear(72, 40, device="cuda"))
+    x, r = torch.randn(5, 72, device="cuda"), torch.randn(5, 40, device="cuda")
+    q, w = quantize_int8(x), Int8Rows(mod.weight, mod.weight_scale)
+    for dtype in (torch.float32, torch.bfloat16):
+        want = linear_int8(q, w, bias=mod.bias, residual=r.to(dtype), dtype=dtype)
+        assert torch.equal(mod(q, residual=r.to(dtype)), want)
+        assert torch.equal(mod(q, residual=r.to(dtype), dtype=dtype), want)
+        assert torch.equal(mod(x, residual=r.to(dtype), dtype=dtype), want)
+        assert torch.equal(mod(q, dtype=dtype), linear_int8(q, w, bias=mod.bias, dtype=dtype))
+    assert mod(q).dtype == torch.bfloat16 and mod(x).dtype == torch.float32
+    with pytest.raises(ValueError, match="residual"):
+        mod(q, residual=r, dtype=torch.bfloat16)
+
+
+@pytest.mark.gpu
 def test_stream_and_capture():
     """The smallest, few-row and tiled calls on another stream and captured, with their workspaces; replayed with new inputs."""
     from fovi_amd.arch.int8 import gated_linear_int8, linear_int8
