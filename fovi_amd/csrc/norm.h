@@ -127,6 +127,14 @@ inline int64_t norm_chunks(int64_t rows, int64_t C) {
   return chunks < 1 ? 1 : chunks;
 }
 
+// Workgroups of `columns` columns each, by `y`: along x no more than 2^20, the rest along z. (A launch whose threads along one
+// dimension pass 2^32 runs without an error, and without the threads in excess: a workgroup for every 8 of 2^27 columns.)
+inline dim3 norm_grid(int64_t C, int columns, int64_t y) {
+  const int64_t n = (C + columns - 1) / columns, most = 1 << 20;
+  return dim3(static_cast<unsigned>(n < most ? n : most), static_cast<unsigned>(y), static_cast<unsigned>((n + most - 1) / most));
+}
+__device__ __forceinline__ int64_t norm_group() { return static_cast<int64_t>(blockIdx.z) * gridDim.x + blockIdx.x; }
+
 // CALL(lanes, pieces, short last piece) of a plan.
 #define FOVI_NORM_TAIL(CALL, L, N) \
   if (f.tail) CALL(L, N, true) else CALL(L, N, false)

@@ -308,7 +308,7 @@ __global__ __launch_bounds__(256) void rms_dx_kernel(RmsParams p) {
 template <typename T>
 __global__ __launch_bounds__(256) void rms_dw_kernel(RmsParams p, int64_t per, float* partial) {
   __shared__ float sw[256];
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * 64 + (threadIdx.x & 63);
+  const int64_t c = norm_group() * 64 + (threadIdx.x & 63);
   const int64_t r0 = blockIdx.y * per, rows = p.rows0 * p.rows1, r1 = r0 + per < rows ? r0 + per : rows;
   float dw = 0;
   if (c < p.C)
@@ -328,7 +328,7 @@ __global__ __launch_bounds__(256) void rms_dw_kernel(RmsParams p, int64_t per, f
 // dweight[c]: the partial sums added up; workgroup: 8 columns by 32 partial rows at a time
 __global__ __launch_bounds__(256) void rms_dw_join_kernel(const float* partial, int64_t chunks, int64_t C, void* dw, int p_bf16) {
   __shared__ float sh[4][8];
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x & 7);
+  const int64_t c = norm_group() * 8 + (threadIdx.x & 7);
   float s = 0;
   if (c < C) {
 #pragma unroll 4
@@ -393,7 +393,7 @@ static int64_t rms_bwd_launch(const RmsParams& p, float* partial, hipStream_t s)
     if (p.dx) rms_dx_kernel<T><<<row_groups(rows), 256, 0, s>>>(p);
     if (!partial) return 0;
     const int64_t chunks = norm_chunks(rows, p.C), per = (rows + chunks - 1) / chunks;
-    rms_dw_kernel<T><<<dim3(static_cast<unsigned>((p.C + 63) / 64), static_cast<unsigned>(chunks)), 256, 0, s>>>(p, per, partial);
+    rms_dw_kernel<T><<<norm_grid(p.C, 64, chunks), 256, 0, s>>>(p, per, partial);
     return chunks;
   }
   const int64_t groups = norm_groups(rows, f, kRmsBlocks);
@@ -481,7 +481,7 @@ extern "C" int fovi_rms_norm_bwd(const fovi_rms_norm_args* a, void* stream) {
     if (check_launch("fovi_rms_norm_bwd")) return 1;
   }
   if (!a->dweight) return 0;
-  rms_dw_join_kernel<<<static_cast<unsigned>((p.C + 7) / 8), 256, 0, s>>>(partial, chunks, p.C, a->dweight, p.p_bf16);
+  rms_dw_join_kernel<<<norm_grid(p.C, 8, 1), 256, 0, s>>>(partial, chunks, p.C, a->dweight, p.p_bf16);
   return check_launch("fovi_rms_norm_bwd");
 }
 

@@ -537,3 +537,17 @@ def test_offsets_past_32_bits():
     values, scale = q.dequantize()[-last:].double(), q.scale[-last:, None].double()
     y = y[-last:].detach().double()
     assert ((values - y).abs() <= 0.501 * scale + 1.01 * U[torch.bfloat16] * y.abs()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("c", [2 ** 27 + 24, 2 ** 30])
+def test_the_widest_weight_gradients(c):
+    """Columns for which a launch along one dimension would have 2^32 threads or more (32 for each in the join, 4 in the sums)."""
+    from fovi_amd.arch.norm import rms_norm
+    x, dy = (torch.zeros(1, c, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    w = torch.ones(c, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    at = torch.tensor([0, 2 ** 23, 2 ** 27 - 1, c - 1], device="cuda")
+    x[0, at], dy[0, at] = 2.0 ** 13, torch.tensor([1.0, 2.0, 3.0, 4.0], device="cuda").bfloat16()
+    (dw,) = torch.autograd.grad(rms_norm(x, w, eps=0.0), w, dy)
+    h = (c / 4) ** 0.5                                     # the root mean square is 2^13 (4 / c)^0.5
+    assert torch.equal(dw[at], (dy[0, at].double() * h).bfloat16()) and dw.count_nonzero() == 4
