@@ -145,6 +145,40 @@ def test_fp32_sums_are_taken_by_stages(m, layout):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,c,f", [(40, 24, 16500), (70, 24, 16500), (70, 17, 16501), (300, 32, 8192), (1025, 8, 5504), (20000, 24, 40),
+                                   (40000, 17, 264)])
+def test_split_sums_are_whole(m, c, f, dtype):
+    """Long reductions, split over workgroups, of small whole numbers: every product and sum is exact in either type (what is
+    rounded to bf16 in between is at most 128; sums stay below 2^24 times what all their parts are multiples of), so that a lost
+    or doubled stage shows whatever its size. Gates of 32 have silu 32 and slope 1."""
+    from fovi_amd.arch.feed_forward import gated_mlp
+    g = torch.Generator().manual_seed(m + f)
+
+    def whole(rows, cols, at):                                       # -1, 0 and 1 in the columns from `at` on
+        t = torch.randint(-1, 2, (rows, cols), generator=g).double()
+        t[:, :at] = 0
+        return t
+
+    x, wu, wd, dy = whole(m, c, 1), whole(f, c, 1), whole(c, f, 0), whole(m, c, 0)
+    wu[:, 4:] = 0                                                    # up is -3 .. 3
+    dy[:, 4:] = 0                                                    # dh is -4 .. 4
+    wg = torch.zeros(f, c, dtype=torch.float64)
+    x[:, 0], wg[:, 0] = 32, 1
+    up, dh = x @ wu.t(), dy @ wd
+    h, dgate, dup = 32 * up, dh * up, dh * 32
+    want = [h @ wd.t(), dgate @ wg + dup @ wu, dgate.t() @ x, dup.t() @ x, dy.t() @ h]
+    for a, b in ((h.abs(), wd.abs().t()), (dup.abs(), wu.abs()), (dgate.abs(), wg), (dgate.abs().t(), x.abs()), (dup.abs().t() / 32, x.abs()),
+                 (dy.abs().t(), h.abs())):
+        assert (a @ b).max() < 2 ** 24
+    leaves = [t.to(dtype).cuda().requires_grad_(True) for t in (x, wg, wu, wd)]
+    y = gated_mlp(*leaves)
+    got = (y,) + torch.autograd.grad(y, leaves, dy.to(dtype).cuda())
+    for name, a, b in zip(("y",) + NAMES, got, want):
+        assert torch.equal(a.detach().cpu(), b.to(dtype)), name
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("c,f", [(1024, 1032), (384, 2056)])
 def test_offsets_past_32_bits(c, f):
     """Rows, gate and up, and their gradients of more than 2^31 elements. Only the last rows have an incoming gradient, so that
