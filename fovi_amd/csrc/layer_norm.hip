@@ -215,7 +215,7 @@ __global__ __launch_bounds__(256) void norm_dx_kernel(NormParams p) {
 template <typename T>
 __global__ __launch_bounds__(256) void norm_dw_kernel(NormParams p, int64_t per, float* partial) {
   __shared__ float sw[256], sb[256];
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * 64 + (threadIdx.x & 63);
+  const int64_t c = norm_group() * 64 + (threadIdx.x & 63);
   const int64_t r0 = blockIdx.y * per, rows = p.rows0 * p.rows1, r1 = r0 + per < rows ? r0 + per : rows;
   float dw = 0, db = 0;
   if (c < p.C)
@@ -241,7 +241,7 @@ __global__ __launch_bounds__(256) void norm_dw_kernel(NormParams p, int64_t per,
 __global__ __launch_bounds__(256) void norm_dw_join_kernel(const float* partial, int64_t chunks, int64_t C, void* dw,
                                                            void* db, int p_bf16) {
   __shared__ float sh[4][8];
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x & 7);
+  const int64_t c = norm_group() * 8 + (threadIdx.x & 7);
   void* out = blockIdx.y ? db : dw;
   if (!out) return;
   float s = 0;
@@ -283,7 +283,7 @@ static int64_t norm_bwd_launch(const NormParams& p, float* partial, hipStream_t 
     if (p.dx) norm_dx_kernel<T><<<static_cast<unsigned>(rows < (1 << 16) ? rows : (1 << 16)), 256, 0, s>>>(p);
     if (!partial) return 0;
     const int64_t chunks = norm_chunks(rows, p.C), per = (rows + chunks - 1) / chunks;
-    norm_dw_kernel<T><<<dim3(static_cast<unsigned>((p.C + 63) / 64), static_cast<unsigned>(chunks)), 256, 0, s>>>(p, per, partial);
+    norm_dw_kernel<T><<<norm_grid(p.C, 64, chunks), 256, 0, s>>>(p, per, partial);
     return chunks;
   }
   const int64_t groups = norm_groups(rows, f, kNormBlocks);
@@ -365,7 +365,6 @@ extern "C" int fovi_layer_norm_bwd(const fovi_layer_norm_args* a, void* stream) 
     if (check_launch("fovi_layer_norm_bwd")) return 1;
   }
   if (!params) return 0;
-  norm_dw_join_kernel<<<dim3(static_cast<unsigned>((p.C + 7) / 8), 2), 256, 0, s>>>(partial, chunks, p.C, a->dweight, a->dbias,
-                                                                                    p.p_bf16);
+  norm_dw_join_kernel<<<norm_grid(p.C, 8, 2), 256, 0, s>>>(partial, chunks, p.C, a->dweight, a->dbias, p.p_bf16);
   return check_launch("fovi_layer_norm_bwd");
 }

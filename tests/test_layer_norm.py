@@ -380,3 +380,19 @@ def test_capture(rows, c, dtype):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want)), i
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("c", [2 ** 27 + 24, 2 ** 30])
+def test_the_widest_weight_gradients(c):
+    """Columns for which a launch along one dimension would have 2^32 threads or more (32 for each in the join, 4 in the sums)."""
+    from fovi_amd.arch.norm import layer_norm
+    x, dy = (torch.zeros(1, c, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    w, b = (torch.ones(c, dtype=torch.bfloat16, device="cuda", requires_grad=True) for _ in range(2))
+    at = torch.tensor([0, 2 ** 23, 2 ** 27 - 1, c - 1], device="cuda")
+    sign = torch.tensor([1.0, -1.0, 1.0, -1.0], device="cuda")
+    x[0, at], dy[0, at] = (2.0 ** 13 * sign).bfloat16(), torch.tensor([1.0, 2.0, 3.0, 4.0], device="cuda").bfloat16()
+    dw, db = torch.autograd.grad(layer_norm(x, w, b, eps=0.0), (w, b), dy)
+    h = (c / 4) ** 0.5                                     # the mean is 0, the deviation 2^13 (4 / c)^0.5
+    assert torch.equal(dw[at], (dy[0, at].double() * sign * h).bfloat16()) and dw.count_nonzero() == 4
+    assert torch.equal(db, dy[0])
