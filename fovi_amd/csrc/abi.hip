@@ -9,6 +9,7 @@ namespace fovi {
 
 static thread_local std::string g_last_error;
 static thread_local const char* g_last_path = "";
+static thread_local int64_t g_refused = 0;             // workgroups of a launch that was left out
 
 void note_path(const char* name) { g_last_path = name; }
 
@@ -21,7 +22,16 @@ void set_error(const char* fmt, ...) {
   g_last_error = buf;
 }
 
-void clear_error() { g_last_error.clear(); }
+void clear_error() {
+  g_last_error.clear();
+  g_refused = 0;
+}
+
+bool launch_fits(int64_t groups, int threads) {
+  if (groups <= 0xffffffffll / threads) return true;
+  g_refused = groups;
+  return false;
+}
 
 hipError_t reserve_dynamic_lds(const void* kernel, size_t bytes) {
   static std::mutex mu;
@@ -38,6 +48,11 @@ hipError_t reserve_dynamic_lds(const void* kernel, size_t bytes) {
 }
 
 int check_launch(const char* what) {
+  if (g_refused) {
+    set_error("%s: %lld workgroups exceed one launch", what, static_cast<long long>(g_refused));
+    g_refused = 0;
+    return 1;
+  }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) {
     set_error("%s: launch failed: %s", what, hipGetErrorString(e));

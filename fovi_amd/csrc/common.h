@@ -16,8 +16,12 @@ namespace fovi {
 void set_error(const char* fmt, ...);
 void clear_error();
 
-// Returns 0, or records the HIP error of the last launch and returns 1.
+// Returns 0, or records the HIP error of the last launch (or that launch_fits refused one) and returns 1.
 int check_launch(const char* what);
+
+// Whether a launch of `groups` workgroups of `threads` along one dimension is whole. HIP runs one of 2^32 threads or more
+// without an error, and without the threads in excess: such a launch is left out, and check_launch reports it.
+bool launch_fits(int64_t groups, int threads);
 
 // hipFuncSetAttribute(MaxDynamicSharedMemorySize) for `kernel` on the current device, called
 // only when `bytes` exceeds what an earlier call reserved (a runtime call per launch costs host

@@ -251,18 +251,21 @@ inline int few_waves(int64_t groups, int64_t bytes) {
 template <typename T, int NB, int RB, int TB, typename Epilogue>
 static void few_launch(const MatOperand& x, const MatOperand& w0, const MatOperand& w1, int64_t K, int64_t M, int64_t N,
                        const Epilogue& epilogue, hipStream_t s) {
-  const dim3 groups(static_cast<unsigned>((N + 16 * RB - 1) / (16 * RB)), static_cast<unsigned>((M + 16 * TB - 1) / (16 * TB)));
-  const int64_t all = static_cast<int64_t>(groups.x) * groups.y;
+  const int64_t across = (N + 16 * RB - 1) / (16 * RB);
+  const dim3 groups(static_cast<unsigned>(across), static_cast<unsigned>((M + 16 * TB - 1) / (16 * TB)));
+  const int64_t all = across * groups.y;
   if (mat_whole<T>(x, K) && mat_whole<T>(w0, K) && mat_whole<T>(w1, K)) {
     // as many waves as LDS holds (two workgroups a compute unit where there are that many), each with two stages or more
     constexpr int each = FewRing<T, NB, RB, TB>::LDS > few_lds<NB, RB, TB>(1) ? FewRing<T, NB, RB, TB>::LDS : few_lds<NB, RB, TB>(1);
     const int64_t most = (all > 256 ? 81920 : 163840) / each, want = (K + 2 * mat_bk<T>() - 1) / (2 * mat_bk<T>());
     const int w = static_cast<int>(want < most ? want : most < 16 ? most : 16);
+    if (!launch_fits(across, 64 * w)) return;
     mat_launch(few_ring_kernel<T, NB, RB, TB, Epilogue>, groups, 64 * w, w * each, s, x, w0, w1, K, static_cast<int>(M), N, epilogue);
     return;
   }
   const int most = 65536 / few_lds<NB, RB, TB>(1), waves = few_waves(all, K * static_cast<int64_t>(sizeof(T)));
   const int w = waves < most ? waves : most;
+  if (!launch_fits(across, 64 * w)) return;
   few_kernel<T, NB, RB, TB, Epilogue><<<groups, 64 * w, few_lds<NB, RB, TB>(w), s>>>(x, w0, w1, K, static_cast<int>(M), N, epilogue);
 }
 

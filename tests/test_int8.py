@@ -351,6 +351,18 @@ def test_cpu_tensors_and_c_arguments_are_refused():
     assert lib.fovi_linear_int8(a, None) != 0 and b"activation" in lib.fovi_last_error()
 
 
+@pytest.mark.parametrize("k,n", [(16, 2 ** 31), (15, 2 ** 31), (1296, 2 ** 31), (1297, 2 ** 31)])
+@pytest.mark.parametrize("two", [False, True])
+def test_launches_past_the_limit_are_refused(k, n, two):
+    """Outputs of one row for which the launch would have 2^32 threads or more. (The host refuses: nothing is read or launched.)"""
+    lib, a = _lib.load(), _lib.LinearInt8Args()
+    a.x = a.x_scale = a.weight = a.weight_scale = a.out = 16
+    if two:
+        a.weight2 = a.weight2_scale = 16
+    a.rows, a.inputs, a.outputs, a.x_stride, a.weight_stride, a.weight2_stride, a.out_stride = 1, k, n, k, k, k, n
+    assert lib.fovi_linear_int8(a, None) != 0 and b"exceed one launch" in lib.fovi_last_error()
+
+
 def test_launch_is_on_the_tensors_device(monkeypatch):
     """An entry point runs with the device of its tensors as the current one, which it leaves as it was."""
     current, calls = [0], []
