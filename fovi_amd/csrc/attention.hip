@@ -65,7 +65,7 @@ extern "C" int fovi_attention_pack_mask(const void* keep, const int64_t* stride,
   clear_error();
   if (!keep || !stride || !words) { set_error("fovi_attention_pack_mask: null pointer"); return 1; }
   if (n0 < 0 || n1 < 0 || n2 < 0 || kv_len < 0) { set_error("fovi_attention_pack_mask: bad sizes"); return 1; }
-  const int64_t per = (kv_len + 31) / 32, most = int64_t(0x7fffffff) * 256;
+  const int64_t per = (kv_len + 31) / 32, most = int64_t(0xffffff) * 256;      // what one launch holds
   if (n0 && n1 && n2 && per && (n0 > most / n1 || n0 * n1 > most / n2 || n0 * n1 * n2 > most / per)) {
     set_error("fovi_attention_pack_mask: mask too large");
     return 1;

@@ -455,14 +455,14 @@ int64_t attn_bwd_workspace(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t
 
 template <typename T, int DP, int KIND>
 static void bwd_dq(const AttnParams& p, hipStream_t s) {
-  const unsigned grid = static_cast<unsigned>((p.B * p.Hk * p.tiles * p.splits + 7) / 8 * 8);
-  attn_dq_kernel<T, DP, KIND><<<grid, 256, 0, s>>>(p);
+  const int64_t grid = (p.B * p.Hk * p.tiles * p.splits + 7) / 8 * 8;
+  if (launch_fits(grid, 256)) attn_dq_kernel<T, DP, KIND><<<static_cast<unsigned>(grid), 256, 0, s>>>(p);
 }
 
 template <typename T, int DP, int KIND>
 static void bwd_dkv(const AttnParams& p, hipStream_t s) {
-  const unsigned grid = static_cast<unsigned>((p.B * p.Hk * p.tiles * p.splits + 7) / 8 * 8);
-  attn_dkv_kernel<T, DP, KIND><<<grid, 256, 0, s>>>(p);
+  const int64_t grid = (p.B * p.Hk * p.tiles * p.splits + 7) / 8 * 8;
+  if (launch_fits(grid, 256)) attn_dkv_kernel<T, DP, KIND><<<static_cast<unsigned>(grid), 256, 0, s>>>(p);
 }
 
 template <typename T, int KIND, bool DQ>
@@ -505,7 +505,7 @@ static int bwd_type(AttnParams& p, hipStream_t s) {
     p.splits = f.q_splits;
     p.chunk = f.q_chunk;
     const int64_t n = (f.q_splits > 1 ? rows : 0) * (p.D / 4) + (f.k_splits > 1 ? p.B * p.Hk * p.Lk : 0) * 2 * (p.D / 4);
-    attn_bwd_join_kernel<T><<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(p);
+    if (launch_fits((n + 255) / 256, 256)) attn_bwd_join_kernel<T><<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(p);
     return check_launch("fovi_attention_bwd");
   }
   return 0;

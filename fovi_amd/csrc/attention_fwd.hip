@@ -475,6 +475,7 @@ int64_t attn_fwd_workspace(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t
 template <typename T, int DP, int KIND>
 static void fwd_launch(const AttnParams& p, const FwdPlan& f, hipStream_t s) {
   const int64_t all = p.B * p.Hk * f.tiles;
+  if (!launch_fits(f.few ? all : (all * f.splits + 7) / 8 * 8, 256)) return;
   if (f.few) {
     const dim3 grid(static_cast<unsigned>(all), static_cast<unsigned>(f.splits));
     if constexpr (sizeof(T) == 4 || KIND != 0) attn_fwd_few_kernel<T, DP, KIND><<<grid, 256, 0, s>>>(p);
@@ -504,6 +505,7 @@ static int fwd_type(AttnParams& p, hipStream_t s) {
   if (check_launch("fovi_attention_fwd")) return 1;
   if (f.splits > 1) {
     const int64_t rows = p.B * p.Hk * p.R;
+    if (!launch_fits(f.splits >= 16 ? rows : (rows + 7) / 8, 256)) return check_launch("fovi_attention_fwd");
     if (f.splits >= 16) attn_fwd_join_kernel<T, 8><<<static_cast<unsigned>(rows), 256, 0, s>>>(p);
     else attn_fwd_join_kernel<T, 1><<<static_cast<unsigned>((rows + 7) / 8), 256, 0, s>>>(p);
     return check_launch("fovi_attention_fwd");

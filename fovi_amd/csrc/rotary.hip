@@ -186,7 +186,7 @@ extern "C" int fovi_rotary(const fovi_rotary_args* a, void* stream) {
   if (per < 1) per = 1;
   p.tokens = static_cast<int>(per);
   const int64_t grid = (tokens + per - 1) / per;
-  if (grid > 0x7fffffff) { set_error("fovi_rotary: too many tokens"); return 1; }
+  if (grid > 0xffffff) { set_error("fovi_rotary: too many tokens"); return 1; }
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (a->dtype == FOVI_BF16) rotary_launch<uint16_t>(p, static_cast<unsigned>(grid), s);
   else rotary_launch<float>(p, static_cast<unsigned>(grid), s);

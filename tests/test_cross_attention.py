@@ -547,6 +547,27 @@ def test_c_layouts_workspaces_and_masks_are_refused():
     assert b"too large" in lib.fovi_last_error()
 
 
+@pytest.mark.parametrize("dtype", [_lib.F32, _lib.BF16])
+def test_launches_past_the_limit_are_refused(dtype):
+    """2^24 workgroups of 256 threads, which one launch does not hold: the host refuses, in both directions."""
+    lib, b = _lib.load(), _lib.AttentionBwdArgs()
+    a = b.fwd
+    for s, names in ((a, ("q", "k", "v", "out", "stats")), (b, ("dout", "dq", "dk", "dv"))):
+        for name in names:
+            setattr(s, name, 4096)
+    a.dtype, a.scale = dtype, 0.125
+    a.batch, a.q_len, a.kv_len, a.heads, a.kv_heads, a.head_dim = 1 << 20, 1, 1, 16, 16, 64
+    for f in (a.q_stride, a.k_stride, a.v_stride, a.out_stride, b.dout_stride, b.dq_stride, b.dk_stride, b.dv_stride):
+        f[:] = (1024, 1024, 64)
+    assert lib.fovi_attention_fwd(a, None) != 0 and b"exceed one launch" in lib.fovi_last_error()
+    a.workspace, a.workspace_bytes = 4096, lib.fovi_attention_bwd_workspace_bytes(1 << 20, 1, 1, 16, 16, 64, dtype)
+    if dtype == _lib.BF16:
+        a.out_rest = 4096
+    assert lib.fovi_attention_bwd(b, None) != 0 and b"exceed one launch" in lib.fovi_last_error(), lib.fovi_last_error()
+    stride = (C.c_int64 * 4)(8, 8, 8, 1)
+    assert lib.fovi_attention_pack_mask(4096, stride, 1 << 32, 1, 1, 8, 4096, None) != 0 and b"too large" in lib.fovi_last_error()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("kind", [_lib.MASK_NONE, _lib.MASK_KEEP, _lib.MASK_BIAS])

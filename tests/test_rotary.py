@@ -230,6 +230,15 @@ def test_c_arguments_are_refused():
     assert lib.fovi_rotary(a, None) != 0 and b"bad sizes" in lib.fovi_last_error()
 
 
+def test_launches_past_the_limit_are_refused():
+    """2^24 workgroups of 256 threads, one for each token of 8192 channels: more than one launch holds."""
+    lib, a = _lib.load(), _lib.RotaryArgs()
+    a.x = a.y = a.positions = a.freqs = 4096
+    a.dtype, a.n_axes, a.batch, a.length, a.heads, a.head_dim = _lib.BF16, 1, 1 << 24, 1, 64, 128
+    a.section_end[:] = [64, 64, 64, 64]
+    assert lib.fovi_rotary(a, None) != 0 and b"too many tokens" in lib.fovi_last_error(), lib.fovi_last_error()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("pairing", ["half", "adjacent"])
