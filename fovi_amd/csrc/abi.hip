@@ -28,7 +28,7 @@ void clear_error() {
 }
 
 bool launch_fits(int64_t groups, int threads) {
-  if (groups <= 0xffffffffll / threads) return true;
+  if (groups <= most_groups(threads)) return true;
   g_refused = groups;
   return false;
 }

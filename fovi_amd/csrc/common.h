@@ -22,6 +22,7 @@ int check_launch(const char* what);
 // Whether a launch of `groups` workgroups of `threads` along one dimension is whole. HIP runs one of 2^32 threads or more
 // without an error, and without the threads in excess: such a launch is left out, and check_launch reports it.
 bool launch_fits(int64_t groups, int threads);
+constexpr int64_t most_groups(int threads) { return 0xffffffffll / threads; }
 
 // hipFuncSetAttribute(MaxDynamicSharedMemorySize) for `kernel` on the current device, called
 // only when `bytes` exceeds what an earlier call reserved (a runtime call per launch costs host

@@ -433,7 +433,7 @@ extern "C" int fovi_local_rf_slots(const fovi_local_rf_args* a, void* stream) {
     return 1;
   }
   if (a->n_out == 0) return 0;
-  if (a->n_out > INT32_MAX) { set_error("fovi_local_rf_slots: n_out too large"); return 1; }
+  if (a->n_out > most_groups(RF_LANES)) { set_error("fovi_local_rf_slots: n_out too large"); return 1; }
   RfParams p;
   p.src_cort = a->src_cortical; p.src_cart = a->src_cart; p.n_src = a->n_src; p.dim = a->dim;
   p.out_cort = a->out_cortical; p.out_cart = a->out_cart; p.n_out = a->n_out;
@@ -473,8 +473,9 @@ extern "C" int fovi_knn_logpolar_candidates(const fovi_knn_logpolar_args* a, voi
   if (reserve_lds(reinterpret_cast<const void*>(&knn_lp_candidates_kernel), lds, "fovi_knn_logpolar_candidates"))
     return 1;
   const unsigned blocks = static_cast<unsigned>((a->n_out + KNN_THREADS - 1) / KNN_THREADS);
-  hipLaunchKernelGGL(knn_lp_candidates_kernel, dim3(blocks), dim3(KNN_THREADS), lds,
-                     static_cast<hipStream_t>(stream), p, a->cap, a->cand_idx, a->cand_sq, a->cand_n);
+  if (launch_fits(blocks, KNN_THREADS))
+    hipLaunchKernelGGL(knn_lp_candidates_kernel, dim3(blocks), dim3(KNN_THREADS), lds,
+                       static_cast<hipStream_t>(stream), p, a->cap, a->cand_idx, a->cand_sq, a->cand_n);
   return check_launch("fovi_knn_logpolar_candidates");
 }
 
@@ -501,8 +502,9 @@ extern "C" int fovi_knn_euclid_candidates(const fovi_knn_euclid_args* a, void* s
   if (reserve_lds(reinterpret_cast<const void*>(&knn_eu_candidates_kernel), lds, "fovi_knn_euclid_candidates"))
     return 1;
   const unsigned blocks = static_cast<unsigned>((a->n_out + KNN_THREADS - 1) / KNN_THREADS);
-  hipLaunchKernelGGL(knn_eu_candidates_kernel, dim3(blocks), dim3(KNN_THREADS), lds,
-                     static_cast<hipStream_t>(stream), p, a->cap, a->cand_idx, a->cand_sq, a->cand_n);
+  if (launch_fits(blocks, KNN_THREADS))
+    hipLaunchKernelGGL(knn_eu_candidates_kernel, dim3(blocks), dim3(KNN_THREADS), lds,
+                       static_cast<hipStream_t>(stream), p, a->cap, a->cand_idx, a->cand_sq, a->cand_n);
   return check_launch("fovi_knn_euclid_candidates");
 }
 
@@ -522,7 +524,8 @@ extern "C" int fovi_knn_select(const fovi_knn_select_args* a, void* stream) {
   const size_t lds = static_cast<size_t>(k) * KNN_THREADS * (sizeof(float) + sizeof(int32_t));
   if (reserve_lds(reinterpret_cast<const void*>(&knn_select_kernel), lds, "fovi_knn_select")) return 1;
   const unsigned blocks = static_cast<unsigned>((a->n_out + KNN_THREADS - 1) / KNN_THREADS);
-  hipLaunchKernelGGL(knn_select_kernel, dim3(blocks), dim3(KNN_THREADS), lds, static_cast<hipStream_t>(stream),
-                     a->n_out, k, a->cap, a->cand_idx, a->cand_d, a->cand_n, a->idx, a->dist);
+  if (launch_fits(blocks, KNN_THREADS))
+    hipLaunchKernelGGL(knn_select_kernel, dim3(blocks), dim3(KNN_THREADS), lds, static_cast<hipStream_t>(stream),
+                       a->n_out, k, a->cap, a->cand_idx, a->cand_d, a->cand_n, a->idx, a->dist);
   return check_launch("fovi_knn_select");
 }

@@ -463,6 +463,7 @@ static int launch_bf16_v2(const KnnParams& p, int out_t, hipStream_t s) {
   const int64_t total = p.B * tiles_per_b * n_tiles_n;
   const int64_t padded = (total + 7) / 8 * 8;
   const size_t lds = v2_lds_bytes(NT, p.V, p.K);
+  if (!launch_fits(padded, 512)) return 0;
   dim3 grid(static_cast<unsigned>(padded));
   if (out_t == FOVI_BF16) {
     (void)reserve_dynamic_lds(reinterpret_cast<const void*>(&knnconv_bf16_v2_kernel<NT, uint16_t>), lds);
@@ -745,6 +746,7 @@ static void launch_bf16_v4_sv(const KnnParams& p, int out_t, hipStream_t s) {
   const int64_t total = p.B * tiles_per_b * n_tiles_n;
   const int64_t padded = (total + 7) / 8 * 8;
   const size_t lds = v4_layout(NT, static_cast<int>(p.V), static_cast<int>(p.K), p.zero_row).total;
+  if (!launch_fits(padded, 512)) return;
   dim3 grid(static_cast<unsigned>(padded));
   if (out_t == FOVI_BF16) {
     (void)reserve_dynamic_lds(reinterpret_cast<const void*>(&knnconv_bf16_v4_kernel<NT, SV, uint16_t>), lds);
@@ -979,6 +981,7 @@ static void launch_bf16_smallc(const KnnParams& p, int out_t, hipStream_t s) {
   const int64_t n_tiles_n = (p.Cout + NT - 1) / NT;
   const int64_t total = p.B * tiles_per_b * n_tiles_n;
   const int64_t padded = (total + 7) / 8 * 8;
+  if (!launch_fits(padded, 512)) return;
   dim3 grid(static_cast<unsigned>(padded));
   if (out_t == FOVI_BF16)
     hipLaunchKernelGGL((knnconv_bf16_smallc_kernel<NT, CP, uint16_t>), grid, dim3(512), 0, s, p, tiles_per_b,
@@ -1215,6 +1218,7 @@ static void launch_dense(const KnnParams& p, const uint16_t* A, int out_t, hipSt
   const int64_t n_tiles_n = (p.Cout + NT - 1) / NT;
   const int64_t total = p.B * tiles_per_b * n_tiles_n;
   const int64_t padded = (total + 7) / 8 * 8;
+  if (!launch_fits(padded, 512)) return;
   dim3 grid(static_cast<unsigned>(padded));
   if (out_t == FOVI_BF16)
     hipLaunchKernelGGL((dense_gemm_kernel<NT, uint16_t>), grid, dim3(512), 0, s, p, A, tiles_per_b, n_tiles_n,
@@ -1226,7 +1230,9 @@ static void launch_dense(const KnnParams& p, const uint16_t* A, int out_t, hipSt
 
 static int launch_two_pass(const KnnParams& p, int cp, uint16_t* A, int out_t, hipStream_t s) {
   const int64_t rows = p.B * p.Nout;
-  dim3 g1(static_cast<unsigned>(((rows + 3) / 4 + 7) / 8 * 8));
+  const int64_t groups = ((rows + 3) / 4 + 7) / 8 * 8;
+  if (!launch_fits(groups, 256)) return check_launch("fovi_knnconv_fwd(slot sums)");
+  dim3 g1(static_cast<unsigned>(groups));
   if (cp == 4) hipLaunchKernelGGL((slotsum_kernel<4>), g1, dim3(256), 0, s, p, A, rows);
   else hipLaunchKernelGGL((slotsum_kernel<8>), g1, dim3(256), 0, s, p, A, rows);
   if (check_launch("fovi_knnconv_fwd(slot sums)")) return 1;
@@ -1243,6 +1249,7 @@ static void launch_bf16(const KnnParams& p, int out_t, hipStream_t s) {
   const int64_t n_tiles_n = (p.Cout + NT - 1) / NT;
   const int64_t total = p.B * tiles_per_b * n_tiles_n;
   const int64_t padded = (total + 7) / 8 * 8;
+  if (!launch_fits(padded, 256)) return;
   dim3 grid(static_cast<unsigned>(padded));
   if (out_t == FOVI_BF16)
     hipLaunchKernelGGL((knnconv_bf16_kernel<NT, VEC, uint16_t>), grid, dim3(256), 0, s, p, tiles_per_b,
@@ -1286,9 +1293,10 @@ extern "C" int fovi_knnconv_pack_weight(const float* w_ref, int64_t c_out, int64
   }
   if (out_dtype == FOVI_F8E4M3 && !w_scale) { set_error("fovi_knnconv_pack_weight: fp8 needs w_scale"); return 1; }
   const int64_t n = c_out * k_pad;
-  hipLaunchKernelGGL(pack_weight_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0,
-                     static_cast<hipStream_t>(stream), w_ref, c_out, c_in, n_ref, w_packed, out_dtype, k_pad,
-                     c_slot, w_scale);
+  if (launch_fits((n + 255) / 256, 256))
+    hipLaunchKernelGGL(pack_weight_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0,
+                       static_cast<hipStream_t>(stream), w_ref, c_out, c_in, n_ref, w_packed, out_dtype, k_pad,
+                       c_slot, w_scale);
   return check_launch("fovi_knnconv_pack_weight");
 }
 
@@ -1399,7 +1407,7 @@ extern "C" int fovi_knnconv_fwd(const fovi_knnconv_args* a, void* stream) {
     const int64_t tiles_per_b = (p.Nout + F32_TM - 1) / F32_TM;
     const int64_t mt = p.B * tiles_per_b;
     const int64_t nt = (p.Cout + F32_TN - 1) / F32_TN;
-    if (mt > 0x7fffffff || nt > 65535) { set_error("fovi_knnconv_fwd: grid too large"); return 1; }
+    if (mt > most_groups(256) || nt > 65535) { set_error("fovi_knnconv_fwd: grid too large"); return 1; }
     dim3 grid(static_cast<unsigned>(mt), static_cast<unsigned>(nt));
     if (a->y_dtype == FOVI_F32)
       hipLaunchKernelGGL((knnconv_f32_kernel<float>), grid, dim3(256), 0, s, p, tiles_per_b);

@@ -214,8 +214,9 @@ int launch_dw(const DwParams& p, int64_t total, int64_t padded, hipStream_t s) {
     set_error("fovi_knnconv_dw: cannot reserve %d bytes of LDS", DwTile<TO, TC>::LDS);
     return 1;
   }
-  hipLaunchKernelGGL((knnconv_dw_kernel<TO, TC>), dim3(static_cast<unsigned>(padded)), dim3(DwTile<TO, TC>::NT),
-                     (DwTile<TO, TC>::LDS), s, p, total, padded);
+  if (launch_fits(padded, DwTile<TO, TC>::NT))
+    hipLaunchKernelGGL((knnconv_dw_kernel<TO, TC>), dim3(static_cast<unsigned>(padded)), dim3(DwTile<TO, TC>::NT),
+                       (DwTile<TO, TC>::LDS), s, p, total, padded);
   return check_launch("fovi_knnconv_dw");
 }
 
@@ -324,7 +325,7 @@ extern "C" int fovi_knnconv_dw(const fovi_knnconv_dw_args* a, void* stream) {
   while (ccs > 0 && (p.V << ccs) > sums) --ccs;
   const int64_t vt = p.V < sums ? p.V : sums, pieces = (p.V + vt - 1) / vt;
   const int64_t blocks = p.Cout * ((p.C + (1 << ccs) - 1) >> ccs);
-  if (blocks > 0x7fffffff || pieces > 65535) {
+  if (blocks > most_groups(256) || pieces > 65535) {
     set_error("fovi_knnconv_dw: c_out=%lld x c_in=%lld x n_ref=%lld too large", (long long)p.Cout, (long long)p.C,
               (long long)p.V);
     return 1;

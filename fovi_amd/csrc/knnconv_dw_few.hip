@@ -326,7 +326,7 @@ int lay_out(const void* in, int64_t B, int64_t C, int64_t N, const int64_t* st, 
   p.sf = rows ? st[1] : st[2]; p.ss = rows ? st[2] : st[1];
   p.of = rows ? 1 : C; p.os = rows ? C : 1;      // row n * C + c
   const int64_t ft = (p.F + 63) / 64, bt = (bp + 63) / 64;
-  if (ft * bt * p.S > 0x7fffffffLL) { set_error("fovi_knnconv_dw_few: too large"); return 1; }
+  if (ft * bt * p.S > most_groups(256)) { set_error("fovi_knnconv_dw_few: too large"); return 1; }
   hipLaunchKernelGGL((images_adjacent_kernel<InT, NS>), dim3(static_cast<unsigned>(ft * bt * p.S)), dim3(256), 0, s, p,
                      static_cast<uint32_t>(ft), static_cast<uint32_t>(bt));
   return check_launch("fovi_knnconv_dw_few(layout)");
@@ -335,7 +335,9 @@ int lay_out(const void* in, int64_t B, int64_t C, int64_t N, const int64_t* st, 
 template <int NS>
 int launch_few(const DwFewParams& p, const FewPlan& f, hipStream_t s) {
   const int groups = (f.n_ct + DF_WAVES - 1) / DF_WAVES;
-  const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(groups) * f.ranges + 7) / 8 * 8), static_cast<unsigned>(f.o_tiles));
+  const int64_t across = (static_cast<int64_t>(groups) * f.ranges + 7) / 8 * 8;
+  if (!launch_fits(across, DF_WAVES * 64)) return check_launch("fovi_knnconv_dw_few");
+  const dim3 grid(static_cast<unsigned>(across), static_cast<unsigned>(f.o_tiles));
   const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(DF_WAVES * 64), 0, s, p, groups, f.ranges); };
   if (f.mb == 1) go(knnconv_dw_few_kernel<1, NS>);
   else if (f.mb == 2) go(knnconv_dw_few_kernel<2, NS>);
@@ -407,7 +409,8 @@ extern "C" int fovi_knnconv_dw_few(const fovi_knnconv_dw_few_args* a, void* stre
   p.slot_ptr = a->slot_ptr; p.nbr = a->nbr_sorted; p.flag = flag; p.part = part;
   if (f.parts == 3 ? launch_few<3>(p, f, s) : launch_few<1>(p, f, s)) return 1;
   const int64_t n = a->c_out * a->c_in * a->n_ref;
-  hipLaunchKernelGGL(knnconv_dw_few_reduce_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, s, p, f.mb,
-                     f.ranges, f.o_tiles, a->dw);
+  if (launch_fits((n + 255) / 256, 256))
+    hipLaunchKernelGGL(knnconv_dw_few_reduce_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, s, p, f.mb,
+                       f.ranges, f.o_tiles, a->dw);
   return check_launch("fovi_knnconv_dw_few(reduce)");
 }

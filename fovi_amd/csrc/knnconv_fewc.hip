@@ -496,6 +496,7 @@ static int launch_fewc_t(const KnnParams& p, const FewcTables& ft, const FewcPla
   const int64_t tiles_per_b = (p.Nout + TM - 1) / TM;
   const int64_t total = p.B * tiles_per_b;
   const int64_t padded = (total + 7) / 8 * 8;
+  if (!launch_fits(padded, NT)) return 0;
   auto* k = &knnconv_fewc_kernel<TM, NT, WM, RB, CB, CP, KC, NP>;
   (void)reserve_dynamic_lds(reinterpret_cast<const void*>(k), pl.lds);
   // staged rows in 16-byte pieces: 16-byte aligned image rows, every span within the pieces

@@ -286,7 +286,7 @@ int launch_vm(const KnnParams& p, const VmTables& t, int n_cg, int vec_out, hipS
   const int64_t n_vb = (p.B + VM_IMAGES - 1) / VM_IMAGES;
   const int64_t total = n_vb * p.Nout * n_cg;
   const int64_t padded = (total + 7) / 8 * 8;
-  if (padded > 0x7fffffff) return 0;
+  if (padded > most_groups(VM_WAVES * 64)) return 0;
   const size_t lds = static_cast<size_t>(VM_WAVES) * 32 * (CB * 32 + 8) * 2;
   hipLaunchKernelGGL((knnconv_fewc_vm_kernel<CP, CB, NCH>), dim3(static_cast<unsigned>(padded)), dim3(VM_WAVES * 64),
                      lds, s, p, t, n_cg, total, padded, vec_out);

@@ -272,6 +272,7 @@ static void launch_fp8_sv(const KnnParams& p, int out_t, hipStream_t s) {
   const int64_t total = p.B * tiles_per_b * n_tiles_n;
   const int64_t padded = (total + 7) / 8 * 8;
   const size_t lds = f8_layout(NT, static_cast<int>(p.V), static_cast<int>(p.K), p.zero_row).total;
+  if (!launch_fits(padded, 512)) return;
   dim3 grid(static_cast<unsigned>(padded));
   if (out_t == FOVI_BF16) {
     (void)reserve_dynamic_lds(reinterpret_cast<const void*>(&knnconv_fp8_kernel<NT, SV, uint16_t>), lds);

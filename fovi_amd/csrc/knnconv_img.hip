@@ -495,7 +495,7 @@ int launch_knnconv_img(const KnnParams& p, const fovi_knnconv_args* a, hipStream
   const int64_t n_ct = (p.Cout + cb * 32 * IM_WAVES - 1) / (cb * 32 * IM_WAVES);
   const int64_t total = n_ct * t.groups * ((p.B + ib - 1) / ib);
   const int64_t padded = (total + 7) / 8 * 8;
-  if (padded > 0x7fffffff || p.V * t.ncb > 0x7fffffff / 64) return 0;
+  if (padded > most_groups(IM_THREADS) || p.V * t.ncb > 0x7fffffff / 64) return 0;
   const int64_t op = dt == FOVI_F32 ? 4 : 8;
   const int vec_out = p.ys1 == 1 && p.ys2 % op == 0 && p.ys0 % op == 0 && p.Cout % op == 0 &&
                       reinterpret_cast<uintptr_t>(p.y) % 16 == 0;
@@ -527,7 +527,7 @@ extern "C" int fovi_knnconv_pack_weight_img(const float* w_ref, int64_t c_out, i
     return 1;
   }
   const int64_t blocks = (total + 255) / 256;
-  if (blocks > 0x7fffffff) { set_error("fovi_knnconv_pack_weight_img: weight too large"); return 1; }
+  if (blocks > most_groups(256)) { set_error("fovi_knnconv_pack_weight_img: weight too large"); return 1; }
   hipLaunchKernelGGL(pack_weight_img_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0,
                      static_cast<hipStream_t>(stream), w_ref, c_out, c_in, n_ref, w_frag, dtype, img_blocks(c_out),
                      total, slot_order, w_scale, flag);

@@ -626,6 +626,7 @@ static void launch_v5_sv(const KnnParams& p, int out_t, hipStream_t s) {
   // 16-byte channels-last bf16 stores: unit channel stride, rows and base 16-byte aligned
   const int vec_out = out_t == FOVI_BF16 && p.ys1 == 1 && p.ys2 % 8 == 0 && p.ys0 % 8 == 0 && p.Cout % 8 == 0 &&
                       reinterpret_cast<uintptr_t>(p.y) % 16 == 0;
+  if (!launch_fits(padded, 256)) return;
   const dim3 grid(static_cast<unsigned>(padded));
   if (out_t == FOVI_BF16)
     launch_v5_kernel<SV, F8, uint16_t, SH>(p, s, lds, grid, ncb, tiles_per_b, n_tiles_n, total, padded, vec_out);
@@ -756,8 +757,9 @@ extern "C" int fovi_knnconv_pack_weight_mfma(const float* w_ref, int64_t c_out, 
     return 1;
   }
   const int64_t ncb = (c_out + V5_NT - 1) / V5_NT * (V5_NT / 32);
-  hipLaunchKernelGGL(pack_weight_mfma_kernel, dim3(static_cast<unsigned>((total + 255) / 256)), dim3(256), 0,
-                     static_cast<hipStream_t>(stream), w_ref, c_out, c_in, n_ref, w_frag, ncb, total, slot_order,
-                     out_dtype == FOVI_F8E4M3 ? w_scale : nullptr);
+  if (launch_fits((total + 255) / 256, 256))
+    hipLaunchKernelGGL(pack_weight_mfma_kernel, dim3(static_cast<unsigned>((total + 255) / 256)), dim3(256), 0,
+                       static_cast<hipStream_t>(stream), w_ref, c_out, c_in, n_ref, w_frag, ncb, total, slot_order,
+                       out_dtype == FOVI_F8E4M3 ? w_scale : nullptr);
   return check_launch("fovi_knnconv_pack_weight_mfma");
 }

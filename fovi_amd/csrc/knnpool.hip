@@ -358,7 +358,7 @@ static void launch_pool(const PoolParams& p, hipStream_t s) {
   const int64_t blocks_per_b = (pts + 255) / 256;
   const int64_t total_blocks = blocks_per_b * p.B;
   const int64_t padded = (total_blocks + 7) / 8 * 8;
-  if (rows && pts <= 0x7fffffffLL && padded <= 0x7fffffffLL) {
+  if (rows && pts <= 0x7fffffffLL && padded <= most_groups(256)) {
     const dim3 grid(static_cast<unsigned>(padded));
     // whole channel groups to unit-stride, 16-byte aligned output rows
     const int vec_out = p.ys1 == 1 && (p.ys2 * sizeof(OutT)) % 16 == 0 && (p.ys0 * sizeof(OutT)) % 16 == 0 &&
@@ -388,7 +388,7 @@ static void launch_pool(const PoolParams& p, hipStream_t s) {
   const int ls = plane_lanes(p.Nout);
   const int64_t n_tiles = (p.Nout + (int64_t(1) << ls) - 1) >> ls;
   const int64_t pblocks = n_tiles * ((p.B * cgroups + (256 >> ls) - 1) / (256 >> ls));
-  if (p.xs2 == 1 && p.K <= POOL_KF && p.Nout >= 16 && p.Nin > 0 && p.B * cgroups <= 0x7fffffffLL && pblocks <= 0x7fffffffLL) {
+  if (p.xs2 == 1 && p.K <= POOL_KF && p.Nout >= 16 && p.Nin > 0 && p.B * cgroups <= 0x7fffffffLL && pblocks <= most_groups(256)) {
     const auto args = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(pblocks)), dim3(256), 0, s, p, ls,
                          static_cast<uint32_t>(n_tiles), static_cast<uint32_t>(cgroups),
@@ -678,8 +678,13 @@ template <typename InT, typename GT>
 static void launch_pool_bwd(const PoolBwdParams& p, bool dx_f32, hipStream_t s) {
   const int64_t n1 = p.B * p.Nout * p.C, n2 = p.B * p.Nin * p.C;
   const int64_t cgroups = (p.C + PL_U - 1) / PL_U;
+  const auto fits = [&](int64_t n) {                 // the plane kernels' workgroups for n points
+    const int ls = plane_lanes(n);
+    return ((n + (int64_t(1) << ls) - 1) >> ls) * ((p.B * cgroups + (256 >> ls) - 1) / (256 >> ls)) <= most_groups(256);
+  };
   if (p.xs2 == 1 && p.gs2 == 1 && p.K <= POOL_KF && p.Nin >= 16 && p.Nout > 0 && n2 > 0 && p.Nout * p.K < 0x7fffffffLL &&
-      p.B * cgroups * ((p.Nin + 31) / 32) <= 0x3fffffffLL && p.B * cgroups * ((p.Nout + 31) / 32) <= 0x3fffffffLL) {
+      p.B * cgroups * ((p.Nin + 31) / 32) <= 0x3fffffffLL && p.B * cgroups * ((p.Nout + 31) / 32) <= 0x3fffffffLL &&
+      fits(p.Nin) && fits(p.Nout)) {
     switch (p.mode) {
       case FOVI_POOL_MAX: launch_pool_bwd_planes<InT, GT, FOVI_POOL_MAX>(p, dx_f32, cgroups, s); break;
       case FOVI_POOL_AVG: launch_pool_bwd_planes<InT, GT, FOVI_POOL_AVG>(p, dx_f32, cgroups, s); break;

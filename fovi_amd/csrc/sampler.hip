@@ -509,6 +509,7 @@ template <typename InT, int MODE, int PAD, bool PAIRS, int VMV>
 static void launch_rings_vm_v(const SamplerParams& p, uint32_t bpv, int64_t n_views, hipStream_t s) {
   const uint32_t groups = static_cast<uint32_t>((n_views + VMV - 1) / VMV);
   const uint32_t total = bpv * groups, padded = (total + 7) / 8 * 8;
+  if (!launch_fits(padded, 256)) return;
   const uint32_t nv = static_cast<uint32_t>(n_views);
   if constexpr (std::is_same<InT, uint16_t>::value) {
     if (p.is1 == 1 && p.is3 == p.C && (p.C == 3 || (p.C == 4 && p.is2 % 2 == 0)) && p.is0 % 2 == 0 &&
@@ -544,6 +545,7 @@ static void launch_rings(const SamplerParams& p, uint32_t bpv, uint32_t total, u
     launch_rings_vm<InT, MODE, PAD, PAIRS>(p, bpv, total / bpv, s);
     return;
   }
+  if (!launch_fits(padded, 256)) return;
   dim3 grid(padded);
   // unit-stride channel planes with 16-byte aligned plane and view starts: whole 16-byte runs
   constexpr int64_t VPL = 16 / sizeof(OutT);
@@ -579,7 +581,6 @@ static void launch_mode(const SamplerParams& p, int64_t n_views, bool pairs, hip
   const int64_t bpv = (p.N + 255) / 256;
   const int64_t total = bpv * n_views;
   const int64_t padded = (total + 7) / 8 * 8;
-  dim3 grid(static_cast<unsigned>(padded));
   if (rings_path(p, n_views)) {
     if (MODE == FOVI_BILINEAR && pairs)
       launch_rings<InT, OutT, MODE, PAD, true>(p, static_cast<uint32_t>(bpv), static_cast<uint32_t>(total),
@@ -589,6 +590,8 @@ static void launch_mode(const SamplerParams& p, int64_t n_views, bool pairs, hip
                                                 static_cast<uint32_t>(padded), s);
     return;
   }
+  if (!launch_fits(padded, 256)) return;
+  dim3 grid(static_cast<unsigned>(padded));
   if (MODE == FOVI_BILINEAR && pairs)
     hipLaunchKernelGGL((sampler_kernel<InT, OutT, MODE, PAD, true>), grid, dim3(256), 0, s, p, bpv, total, padded);
   else
