@@ -9,9 +9,10 @@
 // whose epilogue writes dgate, dup and h. The weights' gradients reduce over the tokens: the tokens are split over workgroups, whose
 // partial sums a second launch adds in a fixed order.
 //
-// 131072 rows of 384, hidden 1024, in bf16: gate, up and h 300 us (206 GFLOP), y 137 (103), gate, up and dh 650 (309), dx 257
-// (206), dWg and dWu 246 (206), dWd 167 (103). What bounds them are the loads into LDS and the epilogues: without its loads the
-// first takes 192 us and the third 344, without its stores the third 505. 32 rows of 2048, hidden 5504: 13.2 and 8.3 us (68 MB).
+// 131072 rows of 384, hidden 1024, in bf16: gate, up and h 281 us (206 GFLOP), y 126 (103), gate, up and dh 615 (309), dx 238
+// (206), dWg and dWu 222 + 10 (206), dWd 141 + 13 (103): 1646 us. What bounds the first and the third is that a compute
+// unit's waves are in the epilogue together: without it they take 180 and 371 us, without their loads 207 and 427. 32 rows
+// of 2048, hidden 5504: 13.0 and 8.0 us (68 MB).
 #include "matmul_few.h"
 
 namespace fovi {

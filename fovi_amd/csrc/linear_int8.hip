@@ -5,8 +5,9 @@
 //
 // The sums are exact (int32 holds 131,071 products of -128 * -128); they become floats once, times the two scales.
 //
-// Bound by the loads of the tiles into LDS where there are many rows (16384 x 1024 by 2 x 2752: 120 us, 1.55 POP/s), by the weights' way
-// from memory where there are few (48 x 4096 by 11008: 12.3 us, 3.7 TB/s).
+// Bound by products and epilogue one after the other where there are many rows (16384 x 1024 by 2 x 2752: 124 us, 1.49 POP/s; 91
+// without the epilogue, 112 without the loads, or without the activation), by the weights' way from memory where there are few
+// (48 x 4096 by 11008: 12.7 us, 3.6 TB/s). fp32 results pay for the library's exponential and division: 143 us for 16384 rows.
 #include "matmul_few.h"
 
 namespace fovi {

@@ -2,8 +2,8 @@
 // reduction axis contiguous ("rows") or strided ("columns"), several products of the same left operand at once, and
 // the caller's own work on the sums (an epilogue) before they are written.
 //
-// out[m, n] = sum_k x[m, k] w[n, k]. A workgroup of four waves takes tiles of BM x BN one after another and walks k in
-// stages of 128 bytes a row (64 bf16, 128 int8, 32 fp32 elements): whole cache lines, since parts of one cost as much
+// out[m, n] = sum_k x[m, k] w[n, k]. A workgroup of four waves (eight for tiles of 256 rows) takes tiles of BM x BN one after another and walks k
+// in stages of 128 bytes a row (64 bf16, 128 int8, 32 fp32 elements): whole cache lines, since parts of one cost as much
 // (loads from L2 into LDS reach 34 TB/s by 128 bytes and 17 by 64). Loads go straight into LDS, a stage ahead of the
 // products and past the end of a tile into the next one, so that a tile's first loads run beside the epilogue of the one
 // before. The matrix instructions of a step run on registers that were read during the step before. There is one
@@ -447,9 +447,9 @@ inline unsigned mat_grid(const MatWork& w, int each) {
 inline int mat_columns(int64_t N) { return (N + 191) / 192 * 192 < (N + 255) / 256 * 256 ? 192 : 256; }
 
 // The tile of a product of M x N sums (`shares` times): of 256, 128 or 64 rows, whichever ends first by the time that a
-// compute unit takes for a stage of its workgroups, one, two or four of them. A stage of 64 K sums took 1, 1.13 and 1.6 in
-// tiles of these sizes (131072 x 1024 by 384, bf16: 129, 147 and 208 us; 131072 x 384 by 2 x 1024: 300, 344 and 432): small
-// ones read more bytes a product from L2 and LDS. fp32 products are slow enough for tiles of 64 to keep up and, with more
+// compute unit takes for a stage of its workgroups, one, two or four of them. A stage of 64 K sums is taken as 1, 1.13
+// and 1.6 in tiles of these sizes (131072 x 1024 by 384, bf16: 123, 131 and 203 us, in short runs 129, 147 and 208; 131072 x
+// 384 by 2 x 1024: 277, 285 and 406, in short runs 300, 344 and 432): small ones read more bytes a product from L2 and LDS. fp32 products are slow enough for tiles of 64 to keep up and, with more
 // waves, to be ahead (2571 x 387 by 2 x 1031: 58 us, and 70 in tiles of 128); tiles of 256 rows are not built for them.
 inline int mat_tile_size(int64_t M, int64_t N, int64_t shares, bool fp32, int columns) {
   const int64_t l = (mat_tiles(M, N, 256, columns) * shares + 255) / 256 * (fp32 ? 1 << 20 : columns);
@@ -604,7 +604,8 @@ inline void mat_linear_tiles(const MatSegments& s, int64_t M, int64_t N, int64_t
              MatLinearTile<T, BM, BN, CX, CW, Epilogue>::Ring::LDS, stream, s, M, N, work, share, epilogue);
 }
 // Tiles of 256 rows have 128 columns for an epilogue that reads much beside the sums: more of it is then read at once
-// (131072 x 1024 by 384, bf16, with gate and up read and three results written: 551 us, and 763 with 256 columns).
+// (131072 x 1024 by 384, bf16, with gate and up read and three results written: 551 us, and 763 with 256 columns). Its tiles
+// of 256 and 128 rows still take more than the 256 registers there are: 37 and 35 of a lane's go through scratch memory.
 template <typename Epilogue> constexpr bool mat_narrow = false;
 template <typename T, bool CX, bool CW, typename Epilogue>
 inline void mat_linear_shares(const MatSegments& s, int64_t M, int64_t N, int64_t share, int64_t shares, const Epilogue& epilogue,

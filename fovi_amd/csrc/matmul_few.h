@@ -7,7 +7,8 @@
 // stages in LDS that each wave has for itself (no barriers, whole cache lines); others straight into the instructions'
 // registers, several steps of loads at a time, at any start and stride (the last, partial piece of a row is put
 // together with care). A register load touches half a line of 16 rows and costs as much as whole ones: 32 x 2048 by 2 x 5504
-// in bf16 takes 13.3 us the first way (45 MB, 3.4 TB/s) and 20.6 the second, 48 x 4096 by 11008 in int8 12.6 (45 MB) and 22.4.
+// in bf16 takes 13.0 us the first way (45 MB, 3.5 TB/s) and took 20.6 the second, 48 x 4096 by 11008 in int8 12.7 (45 MB) and 22.4;
+// rows that start an element off whole pieces, which only the second takes, 53 and 72.
 #pragma once
 
 #include <type_traits>
@@ -270,8 +271,8 @@ static void few_launch(const MatOperand& x, const MatOperand& w0, const MatOpera
 }
 
 // The blocks of w and of x of a workgroup: those with which a compute unit reads least in its rounds of workgroups; on a tie
-// fewer parts of x, since each reads w again. (32 rows by 2048 x 5504 in bf16, which are 128 workgroups: 18.1 us, and 13.1
-// with the rows in two parts.)
+// fewer parts of x, since each reads w again. (32 rows of 5504 by 2048 in bf16: 128 workgroups take 8.7 us, and 7.7 with the rows
+// in two parts.)
 template <typename T, int NB, int RB, typename Epilogue>
 static void few_rows(int tb, const MatOperand& x, const MatOperand& w0, const MatOperand& w1, int64_t K, int64_t M, int64_t N,
                      const Epilogue& epilogue, hipStream_t s) {

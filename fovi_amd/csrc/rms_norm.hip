@@ -10,8 +10,8 @@
 // backward keeps the weight's sums of its rows in registers too; each workgroup leaves one row of them, which a
 // second launch adds in a fixed order. Rows too wide for registers go through kernels of a workgroup per row.
 //
-// 131072 bf16 rows of 384 with a residual: forward 69 us (403 MB, 5.9 TB/s), backward 86 (403 MB, 4.7 TB/s) and 4 for the
-// join; 32768 of 1024 to 8 bits 49 us (235 MB, 4.8 TB/s), 7421 fp32 rows of 771 12 and 16 us.
+// 131072 bf16 rows of 384 with a residual: forward 68 us (403 MB, 5.9 TB/s), backward 83 (403 MB, 4.9 TB/s) and 5 for the
+// join; 32768 of 1024 to 8 bits 48 us (235 MB, 4.9 TB/s), 7421 fp32 rows of 771 11 and 16 us.
 #include "norm.h"
 
 namespace fovi {
